@@ -277,6 +277,101 @@ typedef struct BellTernaryFFNDesc {
 
 int bell_swiglu_fwd_ternary(const BellTernaryFFNDesc* desc, void* stream);
 
+/* ------------------------------------------------------------------ MXFP4 */
+
+/*
+ * Microscaled 4-bit floats (OCP Microscaling Formats 1.0, MXFP4): blocks of 32
+ * values along the contraction share a power-of-two scale,
+ *   a = max |v|,  s = 2^max(floor(log2 a) - 2, -127),
+ *   Q(v) = s * (v / s rounded to nearest even on 0, .5, 1, 1.5, 2, 3, 4, 6,
+ *          saturating at 6);
+ * a block that holds an infinity or a NaN becomes NaN throughout.  No
+ * counterpart in the reference, whose only compressed weights are ternary
+ * (bonsai-test/bitlinear.py:34-69).
+ *
+ * Quantised rows and tiles are opaque byte arrays in the tensor core's own
+ * operand layout (csrc/bell_mx.cuh).  Tile size B is 64 or 128.
+ */
+
+/* Bytes of T quantised rows of `features` values for tile size B, and of R*K
+ * quantised tiles (0 for arguments that no entry point takes). */
+size_t bell_mx_rows_bytes(int64_t T, int32_t features, int32_t B);
+size_t bell_mx_tiles_bytes(int32_t R, int32_t K, int32_t B);
+
+/* Quantise src [T, features] (bf16 or f32, rows ld_src elements apart, a
+ * multiple of 16 bytes) into dst, bell_mx_rows_bytes() bytes; and back, exact
+ * in either type. */
+int bell_mx_quantize_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* src, int64_t ld_src,
+                          void* dst, void* stream);
+int bell_mx_dequantize_rows(int64_t T, int32_t features, int32_t B, const void* src, int32_t dtype, void* dst,
+                            int64_t ld_dst, void* stream);
+
+/* Quantise the tiles of a Block-ELL weight (values bf16 or f32 as `dtype`
+ * says, either layout; scale blocks run along B_in) into chunks,
+ * bell_mx_tiles_bytes() bytes, and list its live slots in plan,
+ * bell_plan_bytes(0, 0, 0, R, K) bytes.  Dead slots (-1) are left out of the
+ * plan; any other index outside [0, C) too, and sets BELL_STATUS_COLIDX. */
+int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, int32_t* status, void* stream);
+
+/* Quantised tiles back to bf16, [tiles, B, B] as [B_out, B_in]: output tile i
+ * is tile index[i] (i when index is NULL) of the tiles0 tiles at chunks0
+ * followed by the tiles1 at chunks1 (the gathered tiles of a transposed,
+ * stacked weight). */
+int bell_mx_unpack_tiles(const void* chunks0, int64_t tiles0, const void* chunks1, int64_t tiles1, int32_t B,
+                         const int64_t* index, int64_t tiles, void* values, void* stream);
+
+/* One quantised Block-ELL weight: what bell_mx_pack_ell wrote. */
+typedef struct BellMxEll {
+  const void* chunks;
+  const void* plan;
+  int32_t R, C, K, B;
+} BellMxEll;
+
+/* out = Q(x) Q(W)^T (+ residual): fp32 sums, one rounding. */
+typedef struct BellMxLinearDesc {
+  int64_t T;
+  int32_t out_dtype;           /* BELL_DTYPE_BF16 / BELL_DTYPE_F32           */
+  int32_t max_ctas;            /* cap on the persistent grid (0 = all SMs)   */
+  void* x;                     /* quantised rows, C*B features               */
+  const void* x_src;           /* optional: rows to quantise into x first    */
+  int64_t ld_src;              /* row stride of x_src in elements            */
+  int32_t src_dtype;           /* BELL_DTYPE_BF16 / BELL_DTYPE_F32           */
+  int32_t reserved;
+  const void* residual;        /* optional [T, R*B], out's type              */
+  void* out;                   /* [T, R*B]                                   */
+  BellMxEll w;
+  int32_t* status;
+} BellMxLinearDesc;
+
+int bell_linear_mx(const BellMxLinearDesc* desc, void* stream);
+
+/*
+ * Gated feed-forward: out = Q(h) Wd^T (+ residual), h = silu(Q(x) Wg^T) *
+ * (Q(x) Wu^T) in fp32.  Both projections, the SiLU, the product and the
+ * quantisation of h are one kernel; the down projection is bell_linear_mx's.
+ * h receives the quantised rows (bell_mx_rows_bytes(T, d_ff, B) bytes);
+ * gate_pre and up_out, both or neither, the projections in bf16 [T, d_ff].
+ */
+typedef struct BellMxFFNDesc {
+  int64_t T;
+  int32_t out_dtype;
+  int32_t max_ctas;
+  void* x;                     /* quantised rows, d_model features           */
+  const void* x_src;           /* optional: rows to quantise into x first    */
+  int64_t ld_src;              /* row stride of x_src in elements            */
+  int32_t src_dtype;           /* BELL_DTYPE_BF16 / BELL_DTYPE_F32           */
+  int32_t reserved;
+  const void* residual;        /* optional [T, d_model], out's type          */
+  void* h;
+  void* gate_pre;
+  void* up_out;
+  void* out;                   /* [T, d_model]                               */
+  BellMxEll gate, up, down;
+  int32_t* status;
+} BellMxFFNDesc;
+
+int bell_swiglu_fwd_mx(const BellMxFFNDesc* desc, void* stream);
+
 /* ------------------------------------------------------------------- loop */
 
 /*

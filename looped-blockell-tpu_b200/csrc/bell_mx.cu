@@ -1,0 +1,555 @@
+// bell_mx.cu — Block-ELL products of MXFP4 rows and tiles on tcgen05
+// (kind::mxf4: e2m1 operands, one ue8m0 scale for 32 values, fp32 sums): the
+// linear, and the gated feed-forward's gate and up projections with SiLU*up
+// and the re-quantisation of h in the epilogue.
+//
+// y[t, rB + o] = sum over live slots k of row r, i < B, of
+//                Q(x)[t, c(r,k) B + i] Q(W)[r, k, i, o]
+//
+// A job is one accumulator: 128 tokens x one block-row of one matrix.  A unit
+// is one job (linear) or a gate job and an up job (gated).  One step of a job
+// brings one activation chunk and one weight chunk (codes and scales, bulk
+// copies; layouts in bell_mx.cuh), copies both scale images into TMEM and
+// issues B/64 MMAs of 128 x B x 64.
+//
+// Warps: 0-3 producers (step g of the CTA belongs to producer g % 4), 4-11
+// epilogue (TMEM lane quadrant w % 4, column half (w - 4) / 4), 12 issuer and
+// TMEM owner.  Accumulators form a ring of kAccs, so the issuer runs ahead of
+// the epilogue by a job or two.  The TMEM scale columns belong to the stage:
+// a stage is refilled only after its MMAs have completed, so the scales of
+// MMAs in flight are never overwritten.  Token-major, because a lane of the
+// epilogue then holds 32 consecutive features of its token: one scale block,
+// quantised without talking to another lane and stored as 16 bytes.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <string>
+
+#include "bell_mx.cuh"
+
+namespace bell {
+namespace mx {
+
+static constexpr int kProducers = 4;
+static constexpr int kEpiWarps = 8;
+static constexpr int kIssuer = kProducers + kEpiWarps;  // 12
+static constexpr int kThreads = 32 * (kIssuer + 1);
+
+template <int B>
+struct Geo {
+  static constexpr int A = row_chunk(B), W = tile_chunk(B);
+  static constexpr int STAGE = A + W;            // 17408 / 7168 bytes, multiples of 256
+  static constexpr int NS = B == 128 ? 12 : 16;  // a multiple of kProducers
+  static constexpr int ACCS = B == 128 ? 3 : 4;
+  static constexpr int SF_COL = ACCS * B;        // 8 scale columns per stage from here
+  static constexpr int SMEM = NS * STAGE + 1024 + 1024;
+  static_assert(NS % kProducers == 0, "a stage belongs to one producer");
+  static_assert(SF_COL + NS * 8 <= 512, "TMEM columns");
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct Params {
+  int64_t T;
+  int32_t mtiles, R, C, K0, K1;
+  const uint8_t* x;               // rows of chunks, C column blocks
+  const uint8_t *w0, *w1;         // tiles
+  Plan p0, p1;
+  uint8_t* h;                     // gated: [mtiles, R] chunks
+  __nv_bfloat16 *gate, *up;       // gated, optional [T, R*B]
+  void* out;                      // linear [T, R*B]
+  const void* residual;           // linear, optional, out's type
+  int32_t out_f32;
+  int32_t* status;
+  uint64_t timeout_ns;
+};
+
+enum : uint32_t { kFirst = 1u, kLast = 2u, kTile = 4u };
+
+struct Smem {
+  uint8_t* stages;
+  uint64_t *full, *empty, *acc_full, *acc_empty, *drain;
+  uint32_t *info, *tmem_slot;
+  volatile int* abort_flag;
+};
+
+template <int B>
+__device__ __forceinline__ Smem carve(uint8_t* raw) {
+  using G = Geo<B>;
+  Smem s;
+  s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ctl = s.stages + G::NS * G::STAGE;
+  s.full = reinterpret_cast<uint64_t*>(ctl);
+  s.empty = s.full + G::NS;
+  s.acc_full = s.empty + G::NS;
+  s.acc_empty = s.acc_full + G::ACCS;
+  s.drain = s.acc_empty + G::ACCS;
+  s.info = reinterpret_cast<uint32_t*>(s.drain + 1);
+  s.tmem_slot = s.info + G::NS;
+  s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
+  return s;
+}
+
+// ---------------------------------------------------------------- producer
+
+template <int B, bool GATED>
+__device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl) {
+  using G = Geo<B>;
+  const int lane = threadIdx.x & 31;
+  const int units = p.mtiles * p.R;
+  const uint64_t keep = policy_evict_last(), pass = policy_evict_normal();
+  uint32_t g = 0;       // steps of the CTA so far
+  uint32_t mine = 0;    // fills of this producer
+  bool ok = true;
+  auto fetch = [&](int u, int mat, int& n) -> uint32_t {  // a job's first 32 entries, and their number
+    const int r = u % p.R;
+    const Plan& pl = mat ? p.p1 : p.p0;
+    n = __ldg(pl.counts + r);
+    const int K = mat ? p.K1 : p.K0;
+    return lane < K ? __ldg(pl.entries + int64_t(r) * K + lane) : 0u;
+  };
+  int u = blockIdx.x, mat = 0, n_next = 0;
+  uint32_t e_next = u < units ? fetch(u, 0, n_next) : 0u;
+  while (u < units && ok) {
+    const int m = u / p.R, r = u - m * p.R;
+    const int K = mat ? p.K1 : p.K0;
+    const uint8_t* w = mat ? p.w1 : p.w0;
+    const uint32_t* entries = (mat ? p.p1 : p.p0).entries + int64_t(r) * K;
+    const int n = n_next;
+    uint32_t e = e_next;
+    // the next job's entries travel while this one's steps are issued
+    int u2 = u, mat2 = 0;
+    if (GATED && mat == 0)
+      mat2 = 1;
+    else
+      u2 = u + int(gridDim.x);
+    if (u2 < units) e_next = fetch(u2, mat2, n_next);
+    const int steps = n > 0 ? n : 1;  // a row without live slots: one empty stage
+    for (int j = 0; j < steps; ++j, ++g) {
+      if (j && (j & 31) == 0) e = j + lane < n ? __ldg(entries + j + lane) : 0u;
+      const uint32_t ent = __shfl_sync(0xffffffffu, e, j & 31);
+      if (int(g % kProducers) != pid) continue;
+      const int slot = int(g % G::NS);
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[slot], ((g / G::NS) & 1u) ^ 1u, ctl))) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
+        const bool tile = j < n;
+        s.info[slot] = (j == 0 ? kFirst : 0u) | (j == steps - 1 ? kLast : 0u) | (tile ? kTile : 0u);
+        if (tile) {
+          const int c = int(ent & 0xFFFFu), k = int(ent >> 16);
+          uint8_t* st = s.stages + slot * G::STAGE;
+          mbar_arrive_expect_tx(&s.full[slot], G::STAGE);
+          bulk_load(st, p.x + (int64_t(m) * p.C + c) * G::A, G::A, &s.full[slot], pass);
+          bulk_load(st + G::A, w + (int64_t(r) * K + k) * G::W, G::W, &s.full[slot], keep);
+        } else {
+          mbar_arrive(&s.full[slot]);
+        }
+      }
+      __syncwarp();
+      mine = g + 1;
+    }
+    u = u2;
+    mat = mat2;
+  }
+  if (!ok && mine && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
+    for (int i = 0; i < G::NS / kProducers; ++i) {
+      if (mine < uint32_t(1 + i * kProducers)) break;
+      const uint32_t gi = mine - 1 - i * kProducers;
+      const uint32_t a = smem_u32(&s.full[gi % G::NS]);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(a, (gi / G::NS) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ issuer
+
+template <int B, bool GATED>
+__device__ void issue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
+  using G = Geo<B>;
+  const bool leader = elect_one();
+  const int units = p.mtiles * p.R;
+  const int mine = int(blockIdx.x) < units ? (units - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x) : 0;
+  const int64_t jobs = int64_t(mine) * (GATED ? 2 : 1);
+  const uint64_t a0 = sdesc_plain(smem_u32(s.stages), 128, 256);
+  const uint64_t sf0 = sdesc_plain(smem_u32(s.stages), 16, 128);
+  uint32_t g = 0, acc = 0, use = 0;
+  bool ok = true;
+  for (int64_t job = 0; job < jobs && ok; ++job) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_empty[acc], (use & 1u) ^ 1u, ctl));
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t d = tmem + acc * B;
+    for (bool last = false; !last; ++g) {
+      const uint32_t slot = g % G::NS;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.full[slot], (g / G::NS) & 1u, ctl));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t info = s.info[slot];
+      last = (info & kLast) != 0;
+      if (leader) {
+        if (info & kTile) {
+          const uint64_t st = uint64_t(slot) * (G::STAGE >> 4);
+          const uint64_t ad = a0 + st, bd = ad + (G::A >> 4);
+          const uint32_t sfa = tmem + G::SF_COL + slot * 8, sfb = sfa + 4;
+          copy_scales(sfa, sf0 + st + ((G::A - kScaleBytes) >> 4));
+          copy_scales(sfb, sf0 + st + ((G::STAGE - kScaleBytes) >> 4));
+#pragma unroll
+          for (int kk = 0; kk < B / 64; ++kk)
+            mma_mxf4(d, ad + kk * (kRows * 32 >> 4), bd + kk * (B * 32 >> 4), idesc_mxf4(kRows, B, kk * 2), sfa, sfb,
+                     kk > 0 || !(info & kFirst));
+        }
+        mma_commit(&s.empty[slot]);
+      }
+      __syncwarp();
+    }
+    if (!ok) break;
+    if (leader) mma_commit(&s.acc_full[acc]);
+    __syncwarp();
+    if (++acc == G::ACCS) {
+      acc = 0;
+      ++use;
+    }
+  }
+  if (leader) {  // every MMA has completed before TMEM is released
+    mma_commit(s.drain);
+    const uint32_t a = smem_u32(s.drain);
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(a, 0) && globaltimer_ns() - t0 < 100000000ull) {
+    }
+  }
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------- epilogue
+
+// h = silu(g) u = g u / (1 + e^-g) in fp32 (about 1e-6 relative): the hardware
+// tanh form of the bf16 kernels (2^-11) would move one in a few hundred of
+// h's 4-bit codes to a neighbour.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+template <int B, bool GATED>
+__device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
+  using G = Geo<B>;
+  constexpr int NB = B / 64;  // scale blocks (32 features) of this warp
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
+  const int q = w & 3, half = w >> 2;
+  const int units = p.mtiles * p.R;
+  const int64_t ld = int64_t(p.R) * B;
+  const uint32_t lanes = uint32_t(q * 32) << 16;
+  uint32_t acc = 0, use = 0;
+  auto next = [&] {
+    if (++acc == G::ACCS) {
+      acc = 0;
+      ++use;
+    }
+  };
+  for (int u = blockIdx.x; u < units; u += int(gridDim.x)) {
+    const int m = u / p.R, r = u - m * p.R;
+    const int n = q * 32 + lane;
+    const int64_t t = int64_t(m) * kRows + n;
+    const bool live0 = __ldg(p.p0.counts + r) > 0;
+    if constexpr (GATED) {
+      const bool live1 = __ldg(p.p1.counts + r) > 0;
+      const uint32_t a0 = acc;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
+      next();
+      const uint32_t a1 = acc;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
+      next();
+      tc_fence_after();
+      uint8_t* ch = p.h + (int64_t(m) * p.R + r) * G::A;
+      uint32_t bytes = 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int j = half * NB + b;
+        uint32_t gr[32], ur[32];
+        tmem_ld32x2_sync(tmem + lanes + a0 * B + j * 32, gr, tmem + lanes + a1 * B + j * 32, ur);
+        if (b == NB - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&s.acc_empty[a0]);
+            mbar_arrive(&s.acc_empty[a1]);
+          }
+        }
+        float h[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (!live0) gr[i] = 0u;  // a projection without a live slot is zero
+          if (!live1) ur[i] = 0u;
+          h[i] = silu_mul(__uint_as_float(gr[i]), __uint_as_float(ur[i]));
+        }
+        if (t < p.T) {
+          const int64_t at = t * ld + int64_t(r) * B + j * 32;
+          if (p.gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a[4], c[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                a[e] = pack_bf16x2(__uint_as_float(gr[8 * i + 2 * e]), __uint_as_float(gr[8 * i + 2 * e + 1]));
+                c[e] = pack_bf16x2(__uint_as_float(ur[8 * i + 2 * e]), __uint_as_float(ur[8 * i + 2 * e + 1]));
+              }
+              st_global_v4(p.gate + at + 8 * i, a[0], a[1], a[2], a[3]);
+              st_global_v4(p.up + at + 8 * i, c[0], c[1], c[2], c[3]);
+            }
+          }
+        }
+        uint32_t byte;
+        const uint4 c = quantize32(h, byte);
+        bytes |= byte << (8 * b);
+        if (t < p.T) st_global_v4(ch + code_off(n, j, kRows * 32), c.x, c.y, c.z, c.w);
+      }
+      if (t < p.T) {
+        uint8_t* sp = ch + kRows * B / 2 + scale_off(n, half * NB);
+        if constexpr (NB == 2)
+          *reinterpret_cast<uint16_t*>(sp) = uint16_t(bytes);
+        else
+          *sp = uint8_t(bytes);
+      }
+    } else {
+      const uint32_t a0 = acc;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
+      next();
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int j = half * NB + b;
+        uint32_t a[32];
+        tmem_ld32_sync(tmem + lanes + a0 * B + j * 32, a);
+        if (b == NB - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.acc_empty[a0]);
+        }
+        if (t >= p.T) continue;
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
+        const int64_t at = t * ld + int64_t(r) * B + j * 32;
+        if (p.out_f32) {
+          float* o = static_cast<float*>(p.out) + at;
+          const float* rs = static_cast<const float*>(p.residual);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (rs) {
+              const uint4 v = ld_global_v4(rs + at + 4 * i);
+              f[4 * i] += __uint_as_float(v.x);
+              f[4 * i + 1] += __uint_as_float(v.y);
+              f[4 * i + 2] += __uint_as_float(v.z);
+              f[4 * i + 3] += __uint_as_float(v.w);
+            }
+            st_global_v4(o + 4 * i, __float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
+                         __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+          }
+        } else {
+          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
+          const __nv_bfloat16* rs = static_cast<const __nv_bfloat16*>(p.residual);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (rs) {
+              const uint4 v = ld_global_v4(rs + at + 8 * i);
+              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 x2 = unpack_bf16x2(vw[e]);
+                f[8 * i + 2 * e] += x2.x;
+                f[8 * i + 2 * e + 1] += x2.y;
+              }
+            }
+            st_global_v4(o + 8 * i, pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                         pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int B, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
+  using G = Geo<B>;
+  extern __shared__ uint8_t smem_raw[];
+  const Smem s = carve<B>(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < G::NS; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < G::ACCS; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], kEpiWarps);
+    }
+    mbar_init(s.drain, 1);
+    *s.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kIssuer) {
+    tmem_alloc(s.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s.tmem_slot;
+  const Ctl ctl{s.abort_flag, p.status, p.timeout_ns};
+  griddep_launch();
+  griddep_wait();  // the rows come from the kernel before
+  if (warp < kProducers)
+    produce<B, GATED>(p, s, warp, ctl);
+  else if (warp < kIssuer)
+    epilogue<B, GATED>(p, s, tmem, ctl);
+  else
+    issue<B, GATED>(p, s, tmem, ctl);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssuer) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int B, bool GATED>
+static int launch(const Params& p, int32_t max_ctas, bool dependent, cudaStream_t s) {
+  auto kern = bell_mx_kernel<B, GATED>;
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), Geo<B>::SMEM)) return rc;
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  int64_t grid = int64_t(p.mtiles) * p.R;
+  if (grid > sms) grid = sms;
+  if (max_ctas > 0 && grid > max_ctas) grid = max_ctas;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Geo<B>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(BELL_ERR_LAUNCH, std::string("MXFP4 kernel: ") + cudaGetErrorString(e));
+  }
+  return BELL_OK;
+}
+
+static int check_ell(const BellMxEll& e, const char* name) {
+  if (!e.chunks || !e.plan) return fail(BELL_ERR_ARG, std::string(name) + ": NULL chunks/plan");
+  if (e.B != 64 && e.B != 128) return fail(BELL_ERR_SHAPE, std::string(name) + ": tile size B must be 64 or 128");
+  if (e.R < 1 || e.C < 1 || e.K < 1 || e.R > (1 << 23) || e.C > 65535 || e.K > 65535)
+    return fail(BELL_ERR_SHAPE, std::string(name) + ": R, C, K must be >= 1, R <= 2^23 and C, K <= 65535");
+  if (!aligned16(e.chunks) || !aligned16(e.plan))
+    return fail(BELL_ERR_ALIGN, std::string(name) + ": chunks and plan must be 16-byte aligned");
+  return BELL_OK;
+}
+
+static int check_size(int64_t T, int32_t R) {
+  if (T < 0 || T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "T must be in [0, 2^31 - 256)");
+  if ((T + kRows - 1) / kRows * R > INT_MAX / 4) return fail(BELL_ERR_SHAPE, "T x block-rows too large");
+  return BELL_OK;
+}
+
+static Params base_params(int64_t T, const BellMxEll& w0, const BellMxEll* w1, const void* x, int32_t* status) {
+  Params p{};
+  p.T = T;
+  p.mtiles = int32_t((T + kRows - 1) / kRows);
+  p.R = w0.R;
+  p.C = w0.C;
+  p.K0 = w0.K;
+  p.x = static_cast<const uint8_t*>(x);
+  p.w0 = static_cast<const uint8_t*>(w0.chunks);
+  p.p0 = plan_of(w0.plan, w0.R, w0.K);
+  if (w1) {
+    p.K1 = w1->K;
+    p.w1 = static_cast<const uint8_t*>(w1->chunks);
+    p.p1 = plan_of(w1->plan, w1->R, w1->K);
+  }
+  p.status = status;
+  p.timeout_ns = wait_budget_ns();
+  return p;
+}
+
+// Quantise the caller's rows first where it gave any.
+template <class D>
+static int quantize_source(const D* d, const BellMxEll& w, void* stream) {
+  if (!d->x_src) return BELL_OK;
+  return bell_mx_quantize_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->ld_src, d->x, stream);
+}
+
+static int linear(int64_t T, const void* x, const BellMxEll& w, const void* residual, void* out, int32_t out_dtype,
+                  int32_t max_ctas, int32_t* status, bool dependent, cudaStream_t s) {
+  Params p = base_params(T, w, nullptr, x, status);
+  p.out = out;
+  p.residual = residual;
+  p.out_f32 = out_dtype == BELL_DTYPE_F32;
+  return w.B == 128 ? launch<128, false>(p, max_ctas, dependent, s) : launch<64, false>(p, max_ctas, dependent, s);
+}
+
+}  // namespace mx
+}  // namespace bell
+
+using namespace bell;
+
+extern "C" {
+
+int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
+  if (!d) return fail(BELL_ERR_ARG, "descriptor is NULL");
+  if (int rc = mx::check_ell(d->w, "weight")) return rc;
+  if (int rc = mx::check_size(d->T, d->w.R)) return rc;
+  if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
+    return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
+  if (d->T > 0 && (!d->x || !d->out)) return fail(BELL_ERR_ARG, "x and out must be non-NULL");
+  if (!aligned16(d->x) || !aligned16(d->out) || !aligned16(d->residual))
+    return fail(BELL_ERR_ALIGN, "x, out and residual must be 16-byte aligned");
+  if (d->max_ctas < 0) return fail(BELL_ERR_ARG, "max_ctas must be >= 0");
+  if (int rc = require_sm100()) return rc;
+  if (d->T == 0) return BELL_OK;
+  int32_t* status = d->status ? d->status : default_status_ptr();
+  if (!status) return BELL_ERR_LAUNCH;
+  if (int rc = mx::quantize_source(d, d->w, stream)) return rc;
+  return mx::linear(d->T, d->x, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, status, true,
+                    static_cast<cudaStream_t>(stream));
+}
+
+int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
+  if (!d) return fail(BELL_ERR_ARG, "descriptor is NULL");
+  if (int rc = mx::check_ell(d->gate, "gate")) return rc;
+  if (int rc = mx::check_ell(d->up, "up")) return rc;
+  if (int rc = mx::check_ell(d->down, "down")) return rc;
+  const BellMxEll &g = d->gate, &u = d->up, &w = d->down;
+  if (g.B != u.B || g.B != w.B) return fail(BELL_ERR_SHAPE, "gate, up and down must share the tile size");
+  if (g.R != u.R || g.C != u.C) return fail(BELL_ERR_SHAPE, "gate and up must have the same R and C");
+  if (w.C != g.R || w.R != g.C) return fail(BELL_ERR_SHAPE, "down must map d_ff back to d_model");
+  if (int rc = mx::check_size(d->T, g.R > w.R ? g.R : w.R)) return rc;
+  if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
+    return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
+  if (d->T > 0 && (!d->x || !d->h || !d->out)) return fail(BELL_ERR_ARG, "x, h and out must be non-NULL");
+  if (!d->gate_pre != !d->up_out) return fail(BELL_ERR_ARG, "gate_pre and up_out come together");
+  if (!aligned16(d->x) || !aligned16(d->h) || !aligned16(d->out) || !aligned16(d->residual) ||
+      !aligned16(d->gate_pre) || !aligned16(d->up_out))
+    return fail(BELL_ERR_ALIGN, "buffers must be 16-byte aligned");
+  if (d->max_ctas < 0) return fail(BELL_ERR_ARG, "max_ctas must be >= 0");
+  if (int rc = require_sm100()) return rc;
+  if (d->T == 0) return BELL_OK;
+  int32_t* status = d->status ? d->status : default_status_ptr();
+  if (!status) return BELL_ERR_LAUNCH;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int rc = mx::quantize_source(d, g, stream)) return rc;
+  mx::Params p = mx::base_params(d->T, g, &u, d->x, status);
+  p.h = static_cast<uint8_t*>(d->h);
+  p.gate = static_cast<__nv_bfloat16*>(d->gate_pre);
+  p.up = static_cast<__nv_bfloat16*>(d->up_out);
+  if (int rc = g.B == 128 ? mx::launch<128, true>(p, d->max_ctas, true, s) : mx::launch<64, true>(p, d->max_ctas, true, s))
+    return rc;
+  return mx::linear(d->T, d->h, w, d->residual, d->out, d->out_dtype, d->max_ctas, status, true, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,157 @@
+// bell_mx.cuh — the MXFP4 layouts (e2m1 codes with one e8m0 scale for 32
+// values along the contraction) and the device helpers that read and write them.
+//
+// Everything is stored in the form the tensor core consumes, so that operands
+// move with untiled bulk copies and no kernel shuffles nibbles:
+//
+//   atom   N rows x 64 values (32 bytes a row) as 8-row x 16-byte core
+//          matrices: byte b of row n at (n/8)*256 + (b/16)*128 + (n%8)*16 + b%16
+//          (K-major without swizzle: LBO 128, SBO 256).  Value 2i of a row is
+//          the low nibble of byte i.  One atom is the K = 64 of one MMA.
+//   scales 512 bytes: scale j (0..3) of row n at (n%32)*16 + (n/32)*4 + j,
+//          the image of tcgen05.cp.32x128b (four 32-bit TMEM columns of 32
+//          lanes).
+//   chunk  B/64 atoms, then the scales: the activations' [128 tokens x B]
+//          piece or the weights' [B outputs x B inputs] tile.
+//
+// Rows:  chunk (m, c) at (m * C + c) * row_chunk(B): tokens 128m.. of column
+//        block c.  Rows past the last token are never written nor used.
+// Tiles: chunk (r, k) at (r * K + k) * tile_chunk(B).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "bell_host.h"
+#include "bell_ptx.cuh"
+
+namespace bell {
+namespace mx {
+
+static constexpr int kRows = 128;       // tokens of a chunk (MMA M)
+static constexpr int kBlock = 32;       // values of one scale
+static constexpr int kScaleBytes = 512;
+
+__host__ __device__ constexpr int row_chunk(int B) { return kRows * B / 2 + kScaleBytes; }
+__host__ __device__ constexpr int tile_chunk(int B) { return B * B / 2 + kScaleBytes; }
+
+// Offset of the 16 bytes holding scale block j (32 values) of row n of a
+// chunk whose atoms are `atom` bytes (32 x rows).
+__host__ __device__ constexpr int code_off(int n, int j, int atom) {
+  return (j >> 1) * atom + (n >> 3) * 256 + (j & 1) * 128 + (n & 7) * 16;
+}
+__host__ __device__ constexpr int scale_off(int n, int j) { return (n & 31) * 16 + (n >> 5) * 4 + j; }
+
+// Scale byte of a block whose largest magnitude has the fp32 bits `top`:
+// exponent floor(log2 top) - 2, not below 2^-127; 255 when it is not finite.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  const uint32_t e = top >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+// 1 / scale, exact (2^127 .. 2^-125); a non-finite block has no finite codes,
+// any multiplier does.
+__device__ __forceinline__ float scale_inverse(uint32_t byte) {
+  return __uint_as_float((byte == 255u ? 127u : 254u - byte) << 23);
+}
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7FC00000u : (byte ? byte << 23 : 0x00400000u));
+}
+
+// Eight e2m1 codes, round to nearest even, saturating at 6; v[0] lowest.
+__device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// One scale block: codes of v[0..31] and the scale byte.
+__device__ __forceinline__ uint4 quantize32(const float (&v)[32], uint32_t& byte) {
+  uint32_t top = 0;  // magnitudes as integers: NaN > inf > every finite value
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  byte = scale_byte(top);
+  const float inv = scale_inverse(byte);
+  float s[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = v[i] * inv;
+  return make_uint4(pack_e2m1(s), pack_e2m1(s + 8), pack_e2m1(s + 16), pack_e2m1(s + 24));
+}
+
+// Eight codes -> values times the scale.
+__device__ __forceinline__ void unpack_e2m1(uint32_t w, float scale, float* v) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+    v[2 * i] = f.x * scale;
+    v[2 * i + 1] = f.y * scale;
+  }
+}
+
+// ------------------------------------------------------------------ tcgen05
+
+// Shared-memory matrix descriptor without swizzle.
+__device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) |
+         (uint64_t((sbo >> 4) & 0x3FFFu) << 32) | (uint64_t(1) << 46);
+}
+
+// kind::mxf4 instruction descriptor: e2m1 x e2m1 -> f32, ue8m0 scales; both
+// operands K-major; sf selects scale bytes (0: the first two of a 32-bit
+// column, 2: the last two) for both.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (1u << 23) | (uint32_t(M >> 7) << 27) |
+         (sf << 29);
+}
+
+// D[tmem] (+)= A x B over K = 64, A and B from shared memory, scales in TMEM.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                         uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// Scales: 32 x 16 bytes of shared memory into four TMEM columns, repeated in
+// each quarter of the lanes.  Runs in order with this thread's later MMAs.
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+// ------------------------------------------------------------- weight plan
+
+// Live slots of each block-row in ascending slot order: entry = column |
+// slot << 16, and their number.  [R, K] entries, then [R] counts, each part
+// padded to 16 bytes (bell_plan_bytes(0, 0, 0, R, K) bytes).
+struct Plan {
+  const uint32_t* entries;
+  const int32_t* counts;
+};
+inline Plan plan_of(const void* plan, int32_t R, int32_t K) {
+  const PlanLayout L = plan_layout(0, 0, 0, R, K);
+  const char* p = static_cast<const char*>(plan);
+  return {reinterpret_cast<const uint32_t*>(p + L.d_entries), reinterpret_cast<const int32_t*>(p + L.d_counts)};
+}
+
+}  // namespace mx
+}  // namespace bell

@@ -1,0 +1,336 @@
+// bell_mx_quant.cu — MXFP4 quantisation and its inverse: activation rows,
+// Block-ELL tiles, and the plan of a weight's live slots (layouts: bell_mx.cuh).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <string>
+
+#include "bell_mx.cuh"
+
+namespace bell {
+namespace mx {
+
+static constexpr int kThr = 256;
+
+// 32 consecutive values of a row, 16-byte loads.
+__device__ __forceinline__ void load32(const __nv_bfloat16* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = ld_global_nc_v4(p + 8 * i);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(u[j]);
+      v[8 * i + 2 * j] = f.x;
+      v[8 * i + 2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void load32(const float* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 w = ld_global_nc_v4(p + 4 * i);
+    v[4 * i] = __uint_as_float(w.x);
+    v[4 * i + 1] = __uint_as_float(w.y);
+    v[4 * i + 2] = __uint_as_float(w.z);
+    v[4 * i + 3] = __uint_as_float(w.w);
+  }
+}
+// Q(v) is a 2-bit significand times a power of two: exact in bf16 and fp32.
+__device__ __forceinline__ void store32(__nv_bfloat16* p, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_global_v4(p + 8 * i, pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                 pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+}
+__device__ __forceinline__ void store32(float* p, const float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    st_global_v4(p + 4 * i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                 __float_as_uint(v[4 * i + 3]));
+}
+
+// A warp takes 8 rows x 4 scale blocks: lane -> row l & 7, block l >> 3.  Its
+// 16-byte code stores fill whole core matrices (128 bytes each).
+struct RowsArgs {
+  int64_t T;
+  int32_t features, C, B;
+  int64_t groups;   // ceil(T / 8) * ceil(features / 128)
+  int32_t col_groups;
+};
+
+__device__ __forceinline__ bool locate(const RowsArgs& a, int64_t w, int lane, int64_t& t, int32_t& f, int64_t& chunk,
+                                       int& n, int& j) {
+  const int64_t rg = w / a.col_groups;
+  const int32_t cg = int32_t(w - rg * a.col_groups);
+  t = rg * 8 + (lane & 7);
+  f = cg * 128 + (lane >> 3) * kBlock;
+  n = int(t & (kRows - 1));
+  const int32_t c = f / a.B;
+  j = (f - c * a.B) / kBlock;
+  chunk = ((t / kRows) * a.C + c) * row_chunk(a.B);
+  return t < a.T && f < a.features;
+}
+
+template <class E>
+__global__ void __launch_bounds__(kThr) bell_mx_quantize_kernel(RowsArgs a, const E* __restrict__ src, int64_t ld,
+                                                               uint8_t* __restrict__ dst) {
+  griddep_launch();
+  const int lane = threadIdx.x & 31;
+  for (int64_t w = (int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5; w < a.groups; w += int64_t(gridDim.x) * (kThr / 32)) {
+    int64_t t, chunk;
+    int32_t f;
+    int n, j;
+    const bool ok = locate(a, w, lane, t, f, chunk, n, j);
+    uint32_t byte = 0;
+    if (ok) {
+      float v[32];
+      load32(src + t * ld + f, v);
+      const uint4 q = quantize32(v, byte);
+      st_global_v4(dst + chunk + code_off(n, j, kRows * 32), q.x, q.y, q.z, q.w);
+    }
+    // the scales of one row and column block are adjacent bytes: two (B = 64)
+    // or four (B = 128) lanes' bytes leave as one store
+    uint32_t word = byte | (__shfl_xor_sync(0xffffffffu, byte, 8) << 8);
+    if (a.B == 128) word |= __shfl_xor_sync(0xffffffffu, word, 16) << 16;
+    if (ok && j == 0) {
+      uint8_t* p = dst + chunk + a.B * (kRows / 2) + scale_off(n, 0);
+      if (a.B == 128)
+        *reinterpret_cast<uint32_t*>(p) = word;
+      else
+        *reinterpret_cast<uint16_t*>(p) = uint16_t(word);
+    }
+  }
+}
+
+template <class E>
+__global__ void __launch_bounds__(kThr) bell_mx_dequantize_kernel(RowsArgs a, const uint8_t* __restrict__ src,
+                                                                 E* __restrict__ dst, int64_t ld) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t w = (int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5; w < a.groups; w += int64_t(gridDim.x) * (kThr / 32)) {
+    int64_t t, chunk;
+    int32_t f;
+    int n, j;
+    if (!locate(a, w, lane, t, f, chunk, n, j)) continue;
+    const uint4 q = ld_global_nc_v4(src + chunk + code_off(n, j, kRows * 32));
+    const float s = scale_value(src[chunk + a.B * (kRows / 2) + scale_off(n, j)]);
+    float v[32];
+    unpack_e2m1(q.x, s, v);
+    unpack_e2m1(q.y, s, v + 8);
+    unpack_e2m1(q.z, s, v + 16);
+    unpack_e2m1(q.w, s, v + 24);
+    store32(dst + t * ld + f, v);
+  }
+}
+
+// One thread per scale block of a tile: output o, block j of its inputs.
+// [B_in, B_out] tiles are read a row of outputs at a time (lane = output), so
+// the 32 values of a thread are strided and a warp's loads contiguous.
+template <class E>
+__global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const E* __restrict__ values, int64_t tiles, int32_t B,
+                                                           int32_t in_out, uint8_t* __restrict__ chunks) {
+  const int per_tile = B * (B / kBlock);
+  for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
+    const int64_t tile = i / per_tile;
+    const int e = int(i - tile * per_tile);
+    const E* v0 = values + tile * B * B;
+    int o, j;
+    float v[32];
+    if (in_out) {
+      o = e % B;
+      j = e / B;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = float(v0[(j * kBlock + k) * B + o]);
+    } else {
+      j = e % (B / kBlock);
+      o = e / (B / kBlock);
+      load32(v0 + o * B + j * kBlock, v);
+    }
+    uint32_t byte;
+    const uint4 q = quantize32(v, byte);
+    uint8_t* ch = chunks + tile * tile_chunk(B);
+    st_global_v4(ch + code_off(o, j, B * 32), q.x, q.y, q.z, q.w);
+    ch[B * B / 2 + scale_off(o, j)] = uint8_t(byte);
+  }
+}
+
+// Tiles back to bf16 [B_out, B_in], out tile i from tile index[i] (or i) of
+// the n0 tiles at c0 followed by those at c1.
+__global__ void __launch_bounds__(kThr) bell_mx_unpack_kernel(const uint8_t* __restrict__ c0, int64_t n0,
+                                                             const uint8_t* __restrict__ c1, int64_t n1,
+                                                             const int64_t* __restrict__ index, int64_t tiles,
+                                                             int32_t B, __nv_bfloat16* __restrict__ values) {
+  const int blocks = B / kBlock, per_tile = B * blocks;
+  for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
+    const int64_t tile = i / per_tile;
+    const int e = int(i - tile * per_tile), j = e % blocks, o = e / blocks;
+    const int64_t from = index ? index[tile] : tile;
+    if (from < 0 || from >= n0 + n1) continue;
+    const uint8_t* ch = from < n0 ? c0 + from * tile_chunk(B) : c1 + (from - n0) * tile_chunk(B);
+    const uint4 q = ld_global_nc_v4(ch + code_off(o, j, B * 32));
+    const float s = scale_value(ch[B * B / 2 + scale_off(o, j)]);
+    float v[32];
+    unpack_e2m1(q.x, s, v);
+    unpack_e2m1(q.y, s, v + 8);
+    unpack_e2m1(q.z, s, v + 16);
+    unpack_e2m1(q.w, s, v + 24);
+    store32(values + tile * B * B + o * B + j * kBlock, v);
+  }
+}
+
+// One warp per block-row: the live slots, compacted in slot order.
+__global__ void __launch_bounds__(kThr) bell_mx_plan_kernel(const int32_t* __restrict__ cols, int32_t R, int32_t C,
+                                                           int32_t K, uint32_t* __restrict__ entries,
+                                                           int32_t* __restrict__ counts, int32_t* status) {
+  const int lane = threadIdx.x & 31;
+  const int r = int((int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5);
+  if (r >= R) return;
+  int n = 0, bad = 0;
+  for (int k0 = 0; k0 < K; k0 += 32) {
+    const int k = k0 + lane;
+    const int c = k < K ? cols[int64_t(r) * K + k] : -1;
+    const bool live = c >= 0 && c < C;
+    bad |= c < -1 || c >= C;
+    const uint32_t m = __ballot_sync(0xffffffffu, live);
+    if (live) entries[int64_t(r) * K + n + __popc(m & ((1u << lane) - 1u))] = uint32_t(c) | (uint32_t(k) << 16);
+    n += __popc(m);
+  }
+  if (lane == 0) counts[r] = n;
+  if (bad) atomicOr(status, BELL_STATUS_COLIDX);
+}
+
+// Grid of grid-stride kernels: enough blocks for every SM's 2048 threads.
+static int grid_for(int64_t threads, unsigned* grid) {
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  const int64_t need = (threads + kThr - 1) / kThr, most = int64_t(sms) * 8 * 4;
+  *grid = unsigned(need < most ? need : most);
+  return BELL_OK;
+}
+
+static int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks,
+                      int64_t ld) {
+  if (B != 64 && B != 128) return fail(BELL_ERR_SHAPE, "MXFP4 rows: tile size B must be 64 or 128");
+  if (T < 0 || T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "MXFP4 rows: T must be in [0, 2^31 - 256)");
+  if (features < 1 || features % B) return fail(BELL_ERR_SHAPE, "MXFP4 rows: features must be a multiple of B");
+  if (dtype != BELL_DTYPE_BF16 && dtype != BELL_DTYPE_F32) return fail(BELL_ERR_DTYPE, "MXFP4 rows: dtype must be bf16 or f32");
+  if (T > 0 && (!rows || !chunks)) return fail(BELL_ERR_ARG, "MXFP4 rows: NULL buffer");
+  if (ld < features || (ld * (dtype == BELL_DTYPE_BF16 ? 2 : 4)) % 16)
+    return fail(BELL_ERR_ALIGN, "MXFP4 rows: the row stride must cover the features and be a multiple of 16 bytes");
+  if (!aligned16(rows) || !aligned16(chunks)) return fail(BELL_ERR_ALIGN, "MXFP4 rows: buffers must be 16-byte aligned");
+  return require_sm100();
+}
+
+static RowsArgs rows_args(int64_t T, int32_t features, int32_t B) {
+  RowsArgs a{};
+  a.T = T;
+  a.features = features;
+  a.C = features / B;
+  a.B = B;
+  a.col_groups = (features + 127) / 128;
+  a.groups = (T + 7) / 8 * a.col_groups;
+  return a;
+}
+
+}  // namespace mx
+}  // namespace bell
+
+using namespace bell;
+
+extern "C" {
+
+size_t bell_mx_rows_bytes(int64_t T, int32_t features, int32_t B) {
+  if (T <= 0 || features <= 0 || (B != 64 && B != 128)) return 0;
+  return size_t((T + mx::kRows - 1) / mx::kRows) * size_t(features / B) * size_t(mx::row_chunk(B));
+}
+
+size_t bell_mx_tiles_bytes(int32_t R, int32_t K, int32_t B) {
+  if (R <= 0 || K <= 0 || (B != 64 && B != 128)) return 0;
+  return size_t(R) * size_t(K) * size_t(mx::tile_chunk(B));
+}
+
+int bell_mx_quantize_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* src, int64_t ld_src,
+                          void* dst, void* stream) {
+  if (int rc = mx::check_rows(T, features, B, dtype, src, dst, ld_src)) return rc;
+  if (T == 0) return BELL_OK;
+  const mx::RowsArgs a = mx::rows_args(T, features, B);
+  unsigned grid;
+  if (int rc = mx::grid_for(a.groups * 32, &grid)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == BELL_DTYPE_BF16)
+    mx::bell_mx_quantize_kernel<<<grid, mx::kThr, 0, s>>>(a, static_cast<const __nv_bfloat16*>(src), ld_src,
+                                                          static_cast<uint8_t*>(dst));
+  else
+    mx::bell_mx_quantize_kernel<<<grid, mx::kThr, 0, s>>>(a, static_cast<const float*>(src), ld_src,
+                                                          static_cast<uint8_t*>(dst));
+  return check_launch("bell_mx_quantize_rows");
+}
+
+int bell_mx_dequantize_rows(int64_t T, int32_t features, int32_t B, const void* src, int32_t dtype, void* dst,
+                            int64_t ld_dst, void* stream) {
+  if (int rc = mx::check_rows(T, features, B, dtype, dst, src, ld_dst)) return rc;
+  if (T == 0) return BELL_OK;
+  const mx::RowsArgs a = mx::rows_args(T, features, B);
+  unsigned grid;
+  if (int rc = mx::grid_for(a.groups * 32, &grid)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const uint8_t* q = static_cast<const uint8_t*>(src);
+  if (dtype == BELL_DTYPE_BF16)
+    mx::bell_mx_dequantize_kernel<<<grid, mx::kThr, 0, s>>>(a, q, static_cast<__nv_bfloat16*>(dst), ld_dst);
+  else
+    mx::bell_mx_dequantize_kernel<<<grid, mx::kThr, 0, s>>>(a, q, static_cast<float*>(dst), ld_dst);
+  return check_launch("bell_mx_dequantize_rows");
+}
+
+int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, int32_t* status, void* stream) {
+  if (!w || !w->values || !w->col_indices || !chunks || !plan) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: NULL argument");
+  if (w->B != 64 && w->B != 128) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: tile size B must be 64 or 128");
+  if (w->R < 1 || w->C < 1 || w->K < 1) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R, C, K must be >= 1");
+  if (w->C > 65535 || w->K > 65535) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: C and K must be <= 65535");
+  if (dtype != BELL_DTYPE_BF16 && dtype != BELL_DTYPE_F32)
+    return fail(BELL_ERR_DTYPE, "bell_mx_pack_ell: dtype must be bf16 or f32");
+  if (w->layout != BELL_TILE_IN_OUT && w->layout != BELL_TILE_OUT_IN)
+    return fail(BELL_ERR_ARG, "bell_mx_pack_ell: unknown tile layout");
+  if (!aligned16(w->values) || !aligned16(chunks) || !aligned16(plan))
+    return fail(BELL_ERR_ALIGN, "bell_mx_pack_ell: values, chunks and plan must be 16-byte aligned");
+  if (int rc = require_sm100()) return rc;
+  int32_t* st = status ? status : default_status_ptr();
+  if (!st) return BELL_ERR_LAUNCH;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = int64_t(w->R) * w->K;
+  unsigned grid;
+  if (int rc = mx::grid_for(tiles * w->B * (w->B / mx::kBlock), &grid)) return rc;
+  const int32_t in_out = w->layout == BELL_TILE_IN_OUT;
+  uint8_t* dst = static_cast<uint8_t*>(chunks);
+  if (dtype == BELL_DTYPE_BF16)
+    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const __nv_bfloat16*>(w->values), tiles, w->B, in_out, dst);
+  else
+    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const float*>(w->values), tiles, w->B, in_out, dst);
+  if (int rc = check_launch("bell_mx_pack_kernel")) return rc;
+  const mx::Plan p = mx::plan_of(plan, w->R, w->K);
+  mx::bell_mx_plan_kernel<<<(w->R + mx::kThr / 32 - 1) / (mx::kThr / 32), mx::kThr, 0, s>>>(
+      w->col_indices, w->R, w->C, w->K, const_cast<uint32_t*>(p.entries), const_cast<int32_t*>(p.counts), st);
+  return check_launch("bell_mx_plan_kernel");
+}
+
+int bell_mx_unpack_tiles(const void* chunks0, int64_t tiles0, const void* chunks1, int64_t tiles1, int32_t B,
+                         const int64_t* index, int64_t tiles, void* values, void* stream) {
+  if (B != 64 && B != 128) return fail(BELL_ERR_SHAPE, "bell_mx_unpack_tiles: tile size B must be 64 or 128");
+  if (tiles0 < 0 || tiles1 < 0 || tiles < 0 || (!index && tiles > tiles0 + tiles1))
+    return fail(BELL_ERR_SHAPE, "bell_mx_unpack_tiles: bad tile counts");
+  if (tiles > 0 && ((tiles0 && !chunks0) || (tiles1 && !chunks1) || !values))
+    return fail(BELL_ERR_ARG, "bell_mx_unpack_tiles: NULL buffer");
+  if (!aligned16(chunks0) || !aligned16(chunks1) || !aligned16(values))
+    return fail(BELL_ERR_ALIGN, "bell_mx_unpack_tiles: buffers must be 16-byte aligned");
+  if (int rc = require_sm100()) return rc;
+  if (tiles == 0) return BELL_OK;
+  unsigned grid;
+  if (int rc = mx::grid_for(tiles * B * (B / mx::kBlock), &grid)) return rc;
+  mx::bell_mx_unpack_kernel<<<grid, mx::kThr, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(chunks0), tiles0, static_cast<const uint8_t*>(chunks1), tiles1, index, tiles, B,
+      static_cast<__nv_bfloat16*>(values));
+  return check_launch("bell_mx_unpack_kernel");
+}
+
+}  // extern "C"

@@ -2,7 +2,7 @@
 libbell_b200.so.  The reference's ``looped_blockell/kernels/__init__.py`` is an
 empty placeholder; this package fills it with the fused SwiGLU forward, the
 single Block-ELL projection, the SwiGLU backward (``backward``), the ternary
-path, the loop ops and host-buffer (pipelined) entry points, and registers the reference's native op names under
+path, the MXFP4 path (``mxfp4``), the loop ops and host-buffer (pipelined) entry points, and registers the reference's native op names under
 ``torch.ops.titan`` on import (``torch_ops``; skipped when those names are
 already defined in the process).
 """
@@ -14,6 +14,8 @@ from .loop import (diagonal_injection, inject_rmsnorm, looped_ffn, persistent_ml
 from .backward import (block_ell_sddmm, block_ell_swiglu, block_ell_swiglu_bwd, down_silu_bwd,  # noqa: F401
                        silu_mul_bwd, transpose_ell, transposed_topology)
 from .convert import dense_to_block_ell  # noqa: F401
+from .mxfp4 import (MXBlockELL, MXRows, make_mxfp4, mxfp4_dequantize, mxfp4_linear, mxfp4_linear_ad,  # noqa: F401
+                    mxfp4_quantize, mxfp4_swiglu, mxfp4_swiglu_fwd)
 from .stream import block_ell_swiglu_fwd_host, looped_ffn_host, pipeline_tokens  # noqa: F401
 from . import torch_ops as _torch_ops
 

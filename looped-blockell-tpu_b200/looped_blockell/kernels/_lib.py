@@ -91,6 +91,25 @@ class BellDenseToEllDesc(C.Structure):
                 ("values", C.c_void_p), ("col_indices", C.c_void_p), ("norms", C.c_void_p)]
 
 
+class BellMxEll(C.Structure):
+    _fields_ = [("chunks", C.c_void_p), ("plan", C.c_void_p), ("R", C.c_int32), ("C", C.c_int32), ("K", C.c_int32),
+                ("B", C.c_int32)]
+
+
+class BellMxLinearDesc(C.Structure):
+    _fields_ = [("T", C.c_int64), ("out_dtype", C.c_int32), ("max_ctas", C.c_int32), ("x", C.c_void_p),
+                ("x_src", C.c_void_p), ("ld_src", C.c_int64), ("src_dtype", C.c_int32), ("reserved", C.c_int32),
+                ("residual", C.c_void_p), ("out", C.c_void_p), ("w", BellMxEll), ("status", C.c_void_p)]
+
+
+class BellMxFFNDesc(C.Structure):
+    _fields_ = [("T", C.c_int64), ("out_dtype", C.c_int32), ("max_ctas", C.c_int32), ("x", C.c_void_p),
+                ("x_src", C.c_void_p), ("ld_src", C.c_int64), ("src_dtype", C.c_int32), ("reserved", C.c_int32),
+                ("residual", C.c_void_p), ("h", C.c_void_p), ("gate_pre", C.c_void_p), ("up_out", C.c_void_p),
+                ("out", C.c_void_p), ("gate", BellMxEll), ("up", BellMxEll), ("down", BellMxEll),
+                ("status", C.c_void_p)]
+
+
 # every exported symbol of include/bell.h: name -> (restype, argtypes)
 SIGNATURES = {
     "bell_abi_version": (C.c_int, []),
@@ -118,6 +137,17 @@ SIGNATURES = {
     "bell_f32x_linear_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "bell_linear_f32x": (C.c_int, [C.POINTER(BellLinearDesc), C.c_void_p, C.c_void_p]),
     "bell_swiglu_fwd_ternary": (C.c_int, [C.POINTER(BellTernaryFFNDesc), C.c_void_p]),
+    "bell_mx_rows_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    "bell_mx_tiles_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "bell_mx_quantize_rows": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_void_p]),
+    "bell_mx_dequantize_rows": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
+                                          C.c_int64, C.c_void_p]),
+    "bell_mx_pack_ell": (C.c_int, [C.POINTER(BellEll), C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "bell_mx_unpack_tiles": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64,
+                                       C.c_void_p, C.c_void_p]),
+    "bell_linear_mx": (C.c_int, [C.POINTER(BellMxLinearDesc), C.c_void_p]),
+    "bell_swiglu_fwd_mx": (C.c_int, [C.POINTER(BellMxFFNDesc), C.c_void_p]),
     "bell_loop_fwd_bf16": (C.c_int, [C.POINTER(BellLoopDesc), C.c_void_p]),
     "bell_loop_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "bell_diag_injection_bf16": (C.c_int, [C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -1,0 +1,248 @@
+"""MXFP4 Block-ELL on the B200 against the float64 definition.
+
+Tolerances, derived: Q is exact (every code and scale is compared).  A product
+of two quantised values is exact in fp32, so a linear's error is that of its
+sum: at most 64 additions inside an MMA and one per MMA after it, each losing
+at most one unit of 2^-23 of the running sum of magnitudes, plus one rounding
+of the output (half a step: bf16 2^-8, fp32 2^-24 of the value).
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import rand_cols
+from oracle import mxfp4_oracle as M
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {BF16: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def _K():
+    from looped_blockell import kernels
+    return kernels
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def rows(rng, T, n, dtype=BF16, spread=2.0):
+    """Rows whose magnitudes spread over several octaves."""
+    x = rng.standard_normal((T, n)) * np.exp2(rng.uniform(-spread, spread, (T, n)))
+    return torch.from_numpy(x.astype(np.float32)).to(dtype).cuda()
+
+
+def weight(rng, R, C, K, B, dead=0, dtype=BF16, layout=0, dup=False, dead_row=None):
+    cols = rand_cols(rng, R, C, K, dead, dup)
+    if dead_row is not None:
+        cols[dead_row] = -1
+    v = torch.from_numpy((rng.standard_normal((R, K, B, B)) * 0.02).astype(np.float32)).to(dtype).cuda()
+    ct = torch.from_numpy(cols).cuda()
+    return v, ct, M.dense(M.quantize_tiles(f64(v), layout), cols, C, layout)
+
+
+def sum_bound(xq, w, n_mma):
+    return (64 + n_mma) * 2.0 ** -23 * (np.abs(xq) @ np.abs(w).T)
+
+
+def check_linear(y, xq, w, n_mma, res=None):
+    ref = xq @ w.T
+    bound = sum_bound(xq, w, n_mma)
+    if res is not None:
+        bound = bound + 2.0 ** -23 * (np.abs(ref) + np.abs(res))
+        ref = ref + res
+    err = np.abs(f64(y) - ref)
+    assert (err <= bound + HALF_STEP[y.dtype] * (np.abs(ref) + bound)).all(), float((err - bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,n,tile", [(1, 128, 128), (1, 64, 64), (7, 192, 64), (128, 256, 128), (130, 320, 64),
+                                      (333, 1152, 128)])
+def test_quantize_rows_equals_the_definition(T, n, tile, dtype):
+    K = _K()
+    x = rows(np.random.default_rng(T + n), T, n, dtype)
+    q = K.mxfp4_quantize(x, tile=tile)
+    ref = M.quantize(f64(x))
+    for out_dtype in (BF16, F32):  # Q(x) is exact in either
+        np.testing.assert_array_equal(f64(K.mxfp4_dequantize(q, out_dtype)), ref)
+
+
+def test_quantize_every_rounding_case_and_extreme_scales():
+    K = _K()
+    # every tie, both neighbours of each, both signs, at scales over the whole fp32 range
+    edges = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9375])
+    vals = np.concatenate([edges, np.nextafter(edges.astype(np.float32), np.float32(0)),
+                           np.nextafter(edges.astype(np.float32), np.float32(8)), -edges]).astype(np.float32)
+    lead = np.float32(4.0)  # the block's largest magnitude is in [4, 8): s = 1
+    blocks = [np.concatenate([[lead], vals[i:i + 31], np.zeros(31 - len(vals[i:i + 31]))]) for i in range(0, len(vals), 31)]
+    base = np.stack(blocks).astype(np.float32)
+    out = []
+    for e in (-145, -130, -128, -126, -100, -1, 0, 1, 90, 124):
+        with np.errstate(over="ignore"):
+            out.append(np.ldexp(base, e).astype(np.float32))
+    out.append(np.zeros((2, 32), np.float32))
+    x = np.concatenate([o for o in out if np.isfinite(o).all()])
+    x = np.concatenate([x, np.zeros((-len(x) % 2, 32), np.float32)]).reshape(-1, 64)
+    q = K.mxfp4_quantize(torch.from_numpy(x).cuda(), tile=64)
+    np.testing.assert_array_equal(f64(q.dequantize(F32)), M.quantize(x))
+
+
+def test_quantize_non_finite_blocks_only():
+    K = _K()
+    x = np.random.default_rng(0).standard_normal((3, 128)).astype(np.float32)
+    x[0, 5], x[1, 40], x[2, 127] = np.nan, np.inf, -np.inf
+    got = f64(K.mxfp4_quantize(torch.from_numpy(x).cuda()).dequantize(F32))
+    bad = np.zeros((3, 4), bool)
+    bad[0, 0] = bad[1, 1] = bad[2, 3] = True
+    np.testing.assert_array_equal(np.isnan(got).reshape(3, 4, 32), np.repeat(bad[..., None], 32, -1))
+    ok = ~np.isnan(got)
+    np.testing.assert_array_equal(got[ok], M.quantize(x)[ok])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quantize_strided_and_misaligned_rows(dtype):
+    K = _K()
+    wide = rows(np.random.default_rng(3), 40, 512, dtype)
+    for x in (wide[:, 128:384], wide[::3, :256], wide[:, 1:257], wide.t()[:128, :].t()[:, :128], wide[5:6, 64:192]):
+        np.testing.assert_array_equal(f64(K.mxfp4_quantize(x).dequantize(F32)), M.quantize(f64(x)))
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B", [64, 128])
+def test_make_mxfp4_tiles(B, dtype, layout):
+    K = _K()
+    rng = np.random.default_rng(B + layout)
+    v, cols, _ = weight(rng, 3, 4, 2, B, dead=1, dtype=dtype)
+    w = K.make_mxfp4(v, cols, 4, layout)
+    for back in (0, 1):
+        ref = M.quantize_tiles(f64(v), layout)
+        np.testing.assert_array_equal(f64(w.dequantize(back)), ref if back == layout else np.swapaxes(ref, -1, -2))
+
+
+@pytest.mark.parametrize("T,R,C,Kk,B,dead", [
+    (1, 1, 1, 1, 128, 0), (1, 1, 1, 1, 64, 0), (5, 3, 4, 2, 64, 1), (128, 2, 3, 3, 128, 0), (129, 2, 40, 35, 64, 3),
+    (257, 5, 36, 33, 128, 7), (300, 160, 2, 2, 64, 11), (1000, 40, 9, 4, 128, 5)])
+@pytest.mark.parametrize("dtype,residual", [(BF16, False), (BF16, True), (F32, True)])
+def test_linear(T, R, C, Kk, B, dead, dtype, residual):
+    K = _K()
+    rng = np.random.default_rng(T + R)
+    v, cols, w = weight(rng, R, C, Kk, B, dead, dead_row=R - 1 if dead else None)
+    x = rows(rng, T, C * B, dtype)
+    res = rows(rng, T, R * B, dtype) if residual else None
+    mw = K.make_mxfp4(v, cols, C)
+    y = K.mxfp4_linear(x, mw, residual=res)
+    assert y.dtype == dtype and y.shape == (T, R * B)
+    check_linear(y, M.quantize(f64(x)), w, Kk * B // 64, None if res is None else f64(res))
+    y2 = K.mxfp4_linear(K.mxfp4_quantize(x, tile=B), mw, residual=res, out_dtype=dtype)
+    assert torch.equal(y, y2)  # quantised before or on the way: the same bits
+    assert K.read_status() == 0
+
+
+def check_ffn(K, x, g, u, d, wg, wu, wd, residual):
+    """Every stage against the definition at the GPU's own operands of that stage."""
+    B = g.B
+    out, ws = K.mxfp4_swiglu_fwd(x, g, u, d, add_residual=residual, return_intermediates=True)
+    xq, hq = f64(ws["q_x"].dequantize(F32)), f64(ws["q_h"].dequantize(F32))
+    np.testing.assert_array_equal(xq, M.quantize(f64(x)))
+    n = g.K * B // 64
+    bg, bu = sum_bound(xq, wg, n), sum_bound(xq, wu, u.K * B // 64)
+    gd, ud = xq @ wg.T, xq @ wu.T
+    for name, ref, bound in (("gate", gd, bg), ("up", ud, bu)):
+        assert (np.abs(f64(ws[name]) - ref) <= bound + HALF_STEP[BF16] * (np.abs(ref) + bound)).all(), name
+    # h's codes: those of some h within the fp32 error of g, u, e^-g and the divide (2^-18)
+    h = M.silu_mul(gd, ud)
+    sig = 1 / (1 + np.exp(-gd))
+    tol = 1.1 * np.abs(ud) * bg + np.abs(gd * sig) * bu + 2.0 ** -18 * np.abs(h) + 1.1 * bg * bu
+    T, F = h.shape
+    lo, hi = h - tol, h + tol
+    mag = np.abs(h).reshape(T, -1, 32)
+    top_lo, top_hi = (np.maximum(mag + s * tol.reshape(T, -1, 32), 0).max(-1, keepdims=True) for s in (-1, 1))
+    s_lo, s_hi = (M.scales(np.repeat(t, 32, -1)) for t in (top_lo, top_hi))
+    q = hq.reshape(T, -1, 32)
+    fits = np.zeros((T, F // 32), bool)
+    for s in (s_lo, s_hi):  # the block's scale may be either, where its largest value is next to a power of two
+        a, b = (M.e2m1(v.reshape(T, -1, 32) / s[..., :1]) * s[..., :1] for v in (lo, hi))
+        fits |= ((q >= a) & (q <= b)).all(-1)
+    assert fits.all(), int((~fits).sum())
+    check_linear(out, hq, wd, d.K * B // 64, f64(x) if residual else None)
+    assert K.read_status() == 0
+    return out
+
+
+@pytest.mark.parametrize("T,d,F,B,Kg,Kd,dead", [
+    (1, 128, 256, 64, 1, 1, 0), (1, 256, 512, 128, 2, 4, 0), (3, 192, 320, 64, 2, 3, 2), (128, 256, 512, 64, 4, 8, 3),
+    (131, 384, 640, 128, 2, 5, 2), (700, 512, 2560, 64, 3, 20, 9), (515, 640, 3200, 128, 3, 12, 4)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_swiglu_stages(T, d, F, B, Kg, Kd, dead, residual):
+    K = _K()
+    rng = np.random.default_rng(T + d)
+    vg, cg, wg = weight(rng, F // B, d // B, Kg, B, dead, dead_row=0 if dead else None)
+    vu, cu, wu = weight(rng, F // B, d // B, Kg, B, dead)
+    vd, cd, wd = weight(rng, d // B, F // B, Kd, B, dead, dead_row=0 if dead > 2 else None)
+    x = rows(rng, T, d, spread=1.0)
+    out = check_ffn(K, x, K.make_mxfp4(vg, cg, d // B), K.make_mxfp4(vu, cu, d // B), K.make_mxfp4(vd, cd, F // B), wg,
+                    wu, wd, residual)
+    out2 = K.mxfp4_swiglu_fwd(x, K.make_mxfp4(vg, cg, d // B), K.make_mxfp4(vu, cu, d // B),
+                              K.make_mxfp4(vd, cd, F // B), add_residual=residual)
+    assert torch.equal(out, out2)
+
+
+def rel(a, b):
+    return np.linalg.norm(a - b) / np.linalg.norm(b)
+
+
+# Counted for the backward: bf16 roundings (2^-8 of a value each) of g or u, d_h, d_g or d_u and the result, and the
+# sigmoid's 2^-11: at most 5 x 2^-8 of the norm.
+GRAD_TOL = 5 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("T,R,C,Kk,B,dead,layout,dtype", [
+    (1, 2, 3, 2, 64, 0, 0, BF16), (130, 4, 6, 3, 64, 2, 1, BF16), (257, 3, 4, 2, 128, 1, 0, F32), (64, 3, 4, 3, 128, 0, 1, BF16)])
+def test_linear_gradients(T, R, C, Kk, B, dead, layout, dtype):
+    K = _K()
+    rng = np.random.default_rng(T)
+    v, cols, w = weight(rng, R, C, Kk, B, dead, dtype=dtype, layout=layout)
+    x, dy = rows(rng, T, C * B), rows(rng, T, R * B)
+    res = rows(rng, T, R * B)
+    for t in (x, v, res):
+        t.requires_grad_(True)
+    y = K.mxfp4_linear_ad(x, v, cols, residual=res, layout=layout)
+    y.backward(dy)
+    xq = M.quantize(f64(x))
+    check_linear(y, xq, w, Kk * B // 64, f64(res))
+    assert x.grad.dtype == BF16 and v.grad.dtype == dtype
+    assert rel(f64(x.grad), f64(dy) @ w) <= GRAD_TOL
+    assert rel(f64(v.grad), M.tile_grads(f64(dy).T @ xq, f64(cols).astype(int), B, layout)) <= GRAD_TOL
+    assert torch.equal(res.grad, dy)
+    if dead:
+        assert (v.grad[cols < 0] == 0).all()
+
+
+@pytest.mark.parametrize("T,d,F,B,Kg,Kd,dead,layout,dtype", [
+    (1, 128, 256, 64, 1, 2, 0, 0, BF16), (200, 256, 512, 64, 2, 4, 3, 0, BF16), (257, 256, 512, 128, 2, 3, 1, 1, BF16),
+    (130, 384, 640, 128, 2, 4, 0, 0, F32)])
+def test_swiglu_gradients(T, d, F, B, Kg, Kd, dead, layout, dtype):
+    K = _K()
+    rng = np.random.default_rng(T + 1)
+    mats = [weight(rng, F // B, d // B, Kg, B, dead, dtype, layout), weight(rng, F // B, d // B, Kg, B, dead, dtype, layout),
+            weight(rng, d // B, F // B, Kd, B, dead, dtype, layout)]
+    x, dy = rows(rng, T, d, spread=1.0), rows(rng, T, d)
+    leaves = [x] + [m[0] for m in mats]
+    for t in leaves:
+        t.requires_grad_(True)
+    args = [a for v, c, _ in mats for a in (v, c)]
+    y = K.mxfp4_swiglu(x, *args, add_residual=True, layout=layout)
+    y.backward(dy)
+    packed = [K.make_mxfp4(v.detach(), c, n, layout) for (v, c, _), n in zip(mats, (d // B, d // B, F // B))]
+    out, ws = K.mxfp4_swiglu_fwd(x.detach(), *packed, add_residual=True, return_intermediates=True)
+    assert torch.equal(out, y)
+    refs = M.swiglu_backward(M.quantize(f64(x)), *(m[2] for m in mats), f64(ws["q_h"].dequantize(F32)), f64(dy), True)
+    assert rel(f64(x.grad), refs[0]) <= GRAD_TOL
+    for (v, c, _), ref in zip(mats, refs[1:]):
+        assert v.grad.dtype == dtype
+        assert rel(f64(v.grad), M.tile_grads(ref, f64(c).astype(int), B, layout)) <= GRAD_TOL
+    assert K.read_status() == 0

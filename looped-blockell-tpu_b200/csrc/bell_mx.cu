@@ -7,12 +7,14 @@
 //                Q(x)[t, c(r,k) B + i] Q(W)[r, k, i, o]
 //
 // A job is one accumulator: 128 tokens x one block-row of one matrix.  A unit
-// is one job (linear) or a gate job and an up job (gated).  One step of a job
-// brings one activation chunk and one weight chunk (codes and scales, bulk
-// copies; layouts in bell_mx.cuh), copies both scale images into TMEM and
-// issues B/64 MMAs of 128 x B x 64.
+// is one job (linear) or a gate job and an up job (gated).  A slot of a job
+// takes one activation chunk and one weight chunk (codes and scales, bulk
+// copies; layouts in bell_mx.cuh); its scale images are copied into TMEM and
+// B/64 MMAs of 128 x B x 64 issued.  A pipeline stage holds SLOTS slots: the
+// issuer's wait, commit and bookkeeping cost about 300 cycles, more than a
+// slot's MMAs (B = 128: 128 cycles at the fp4 rate).
 //
-// Warps: 0-3 producers (step g of the CTA belongs to producer g % 4), 4-11
+// Warps: 0-3 producers (stage use g of the CTA belongs to producer g % 4), 4-11
 // epilogue (TMEM lane quadrant w % 4, column half (w - 4) / 4), 12 issuer and
 // TMEM owner.  Accumulators form a ring of kAccs, so the issuer runs ahead of
 // the epilogue by a job or two.  The TMEM scale columns belong to the stage:
@@ -39,13 +41,17 @@ static constexpr int kThreads = 32 * (kIssuer + 1);
 template <int B>
 struct Geo {
   static constexpr int A = row_chunk(B), W = tile_chunk(B);
-  static constexpr int STAGE = A + W;            // 17408 / 7168 bytes, multiples of 256
-  static constexpr int NS = B == 128 ? 12 : 16;  // a multiple of kProducers
+  static constexpr int SLOT = A + W;             // 17408 / 7168 bytes, multiples of 256
+  static constexpr int SLOTS = B == 128 ? 2 : 4;
+  static constexpr int STAGE = SLOTS * SLOT;
+  static constexpr int NS = B == 128 ? 6 : 7;
   static constexpr int ACCS = B == 128 ? 3 : 4;
-  static constexpr int SF_COL = ACCS * B;        // 8 scale columns per stage from here
+  static constexpr int SF_COL = ACCS * B;        // 8 scale columns per slot of a stage from here
   static constexpr int SMEM = NS * STAGE + 1024 + 1024;
-  static_assert(NS % kProducers == 0, "a stage belongs to one producer");
-  static_assert(SF_COL + NS * 8 <= 512, "TMEM columns");
+  // a producer's wait for stage use g - NS must not meet the parity of use
+  // g - 2 NS: that one is released before the producer's own use g - P - NS
+  static_assert(NS > kProducers, "mbarrier parity");
+  static_assert(SF_COL + NS * SLOTS * 8 <= 512, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -64,12 +70,10 @@ struct Params {
   uint64_t timeout_ns;
 };
 
-enum : uint32_t { kFirst = 1u, kLast = 2u, kTile = 4u };
-
 struct Smem {
   uint8_t* stages;
   uint64_t *full, *empty, *acc_full, *acc_empty, *drain;
-  uint32_t *info, *tmem_slot;
+  uint32_t* tmem_slot;
   volatile int* abort_flag;
 };
 
@@ -84,8 +88,7 @@ __device__ __forceinline__ Smem carve(uint8_t* raw) {
   s.acc_full = s.empty + G::NS;
   s.acc_empty = s.acc_full + G::ACCS;
   s.drain = s.acc_empty + G::ACCS;
-  s.info = reinterpret_cast<uint32_t*>(s.drain + 1);
-  s.tmem_slot = s.info + G::NS;
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.drain + 1);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
   return s;
 }
@@ -98,8 +101,8 @@ __device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl)
   const int lane = threadIdx.x & 31;
   const int units = p.mtiles * p.R;
   const uint64_t keep = policy_evict_last(), pass = policy_evict_normal();
-  uint32_t g = 0;       // steps of the CTA so far
-  uint32_t mine = 0;    // fills of this producer
+  uint32_t g = 0;       // stage uses of the CTA so far
+  uint32_t mine = 0;    // 1 + the last one that this producer filled
   bool ok = true;
   auto fetch = [&](int u, int mat, int& n) -> uint32_t {  // a job's first 32 entries, and their number
     const int r = u % p.R;
@@ -117,17 +120,18 @@ __device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl)
     const uint32_t* entries = (mat ? p.p1 : p.p0).entries + int64_t(r) * K;
     const int n = n_next;
     uint32_t e = e_next;
-    // the next job's entries travel while this one's steps are issued
+    // the next job's entries travel while this one's copies are issued
     int u2 = u, mat2 = 0;
     if (GATED && mat == 0)
       mat2 = 1;
     else
       u2 = u + int(gridDim.x);
     if (u2 < units) e_next = fetch(u2, mat2, n_next);
-    const int steps = n > 0 ? n : 1;  // a row without live slots: one empty stage
-    for (int j = 0; j < steps; ++j, ++g) {
+    for (int j = 0; j < n; j += G::SLOTS, ++g) {
       if (j && (j & 31) == 0) e = j + lane < n ? __ldg(entries + j + lane) : 0u;
-      const uint32_t ent = __shfl_sync(0xffffffffu, e, j & 31);
+      uint32_t ent[G::SLOTS];
+#pragma unroll
+      for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, e, (j + i) & 31);
       if (int(g % kProducers) != pid) continue;
       const int slot = int(g % G::NS);
       if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[slot], ((g / G::NS) & 1u) ^ 1u, ctl))) {
@@ -135,16 +139,16 @@ __device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl)
         break;
       }
       if (elect_one()) {
-        const bool tile = j < n;
-        s.info[slot] = (j == 0 ? kFirst : 0u) | (j == steps - 1 ? kLast : 0u) | (tile ? kTile : 0u);
-        if (tile) {
-          const int c = int(ent & 0xFFFFu), k = int(ent >> 16);
-          uint8_t* st = s.stages + slot * G::STAGE;
-          mbar_arrive_expect_tx(&s.full[slot], G::STAGE);
-          bulk_load(st, p.x + (int64_t(m) * p.C + c) * G::A, G::A, &s.full[slot], pass);
-          bulk_load(st + G::A, w + (int64_t(r) * K + k) * G::W, G::W, &s.full[slot], keep);
-        } else {
-          mbar_arrive(&s.full[slot]);
+        uint8_t* st = s.stages + slot * G::STAGE;
+        const int cnt = min(G::SLOTS, n - j);
+        mbar_arrive_expect_tx(&s.full[slot], cnt * G::SLOT);
+#pragma unroll
+        for (int i = 0; i < G::SLOTS; ++i) {
+          if (i < cnt) {
+            const int c = int(ent[i] & 0xFFFFu), k = int(ent[i] >> 16);
+            bulk_load(st + i * G::SLOT, p.x + (int64_t(m) * p.C + c) * G::A, G::A, &s.full[slot], pass);
+            bulk_load(st + i * G::SLOT + G::A, w + (int64_t(r) * K + k) * G::W, G::W, &s.full[slot], keep);
+          }
         }
       }
       __syncwarp();
@@ -154,7 +158,7 @@ __device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl)
     mat = mat2;
   }
   if (!ok && mine && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
-    for (int i = 0; i < G::NS / kProducers; ++i) {
+    for (int i = 0; i <= G::NS / kProducers; ++i) {
       if (mine < uint32_t(1 + i * kProducers)) break;
       const uint32_t gi = mine - 1 - i * kProducers;
       const uint32_t a = smem_u32(&s.full[gi % G::NS]);
@@ -172,42 +176,53 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& 
   using G = Geo<B>;
   const bool leader = elect_one();
   const int units = p.mtiles * p.R;
-  const int mine = int(blockIdx.x) < units ? (units - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x) : 0;
-  const int64_t jobs = int64_t(mine) * (GATED ? 2 : 1);
-  const uint64_t a0 = sdesc_plain(smem_u32(s.stages), 128, 256);
-  const uint64_t sf0 = sdesc_plain(smem_u32(s.stages), 16, 128);
-  uint32_t g = 0, acc = 0, use = 0;
+  const uint32_t a0 = sdesc_lo(smem_u32(s.stages), 128), sf0 = sdesc_lo(smem_u32(s.stages), 16);
+  uint32_t stage = 0, phase = 0, acc = 0, use = 0;
   bool ok = true;
-  for (int64_t job = 0; job < jobs && ok; ++job) {
+  int u = blockIdx.x, mat = 0;
+  int n_next = u < units ? __ldg(p.p0.counts + u % p.R) : 0;
+  while (u < units && ok) {
+    int n = n_next;  // live slots of this job; the next job's are read ahead
+    if (GATED && mat == 0) {
+      mat = 1;
+    } else {
+      mat = 0;
+      u += int(gridDim.x);
+    }
+    if (u < units) n_next = __ldg((mat ? p.p1 : p.p0).counts + u % p.R);
     ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_empty[acc], (use & 1u) ^ 1u, ctl));
     if (!ok) break;
     tc_fence_after();
     const uint32_t d = tmem + acc * B;
-    for (bool last = false; !last; ++g) {
-      const uint32_t slot = g % G::NS;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s.full[slot], (g / G::NS) & 1u, ctl));
+    for (uint32_t more = 0; n > 0; n -= G::SLOTS, more = 1) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, ctl));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t info = s.info[slot];
-      last = (info & kLast) != 0;
       if (leader) {
-        if (info & kTile) {
-          const uint64_t st = uint64_t(slot) * (G::STAGE >> 4);
-          const uint64_t ad = a0 + st, bd = ad + (G::A >> 4);
-          const uint32_t sfa = tmem + G::SF_COL + slot * 8, sfb = sfa + 4;
-          copy_scales(sfa, sf0 + st + ((G::A - kScaleBytes) >> 4));
-          copy_scales(sfb, sf0 + st + ((G::STAGE - kScaleBytes) >> 4));
+        const uint32_t st = stage * uint32_t(G::STAGE >> 4);
+        const uint32_t sf = tmem + G::SF_COL + stage * (G::SLOTS * 8);
 #pragma unroll
-          for (int kk = 0; kk < B / 64; ++kk)
-            mma_mxf4(d, ad + kk * (kRows * 32 >> 4), bd + kk * (B * 32 >> 4), idesc_mxf4(kRows, B, kk * 2), sfa, sfb,
-                     kk > 0 || !(info & kFirst));
+        for (int i = 0; i < G::SLOTS; ++i) {
+          if (i < n) {
+            const uint32_t at = st + i * (G::SLOT >> 4);
+            copy_scales(sf + i * 8, sf0 + at + ((G::A - kScaleBytes) >> 4));
+            copy_scales(sf + i * 8 + 4, sf0 + at + ((G::SLOT - kScaleBytes) >> 4));
+#pragma unroll
+            for (int kk = 0; kk < B / 64; ++kk)
+              mma_mxf4(d, a0 + at + kk * (kRows * 32 >> 4), a0 + at + ((G::A + kk * B * 32) >> 4),
+                       idesc_mxf4(kRows, B, kk * 2), sf + i * 8, sf + i * 8 + 4, i > 0 || kk > 0 ? 1u : more);
+          }
         }
-        mma_commit(&s.empty[slot]);
+        mma_commit(&s.empty[stage]);
       }
       __syncwarp();
+      if (++stage == G::NS) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
     if (!ok) break;
-    if (leader) mma_commit(&s.acc_full[acc]);
+    if (leader) mma_commit(&s.acc_full[acc]);  // a job without live slots: nothing to wait for
     __syncwarp();
     if (++acc == G::ACCS) {
       acc = 0;

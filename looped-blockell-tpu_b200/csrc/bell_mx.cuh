@@ -107,11 +107,15 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t w, float scale, float* v) {
 
 // ------------------------------------------------------------------ tcgen05
 
-// Shared-memory matrix descriptor without swizzle.
-__device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) |
-         (uint64_t((sbo >> 4) & 0x3FFFu) << 32) | (uint64_t(1) << 46);
+// Shared-memory matrix descriptors without swizzle, as two words: the low one
+// (start address and LBO, in 16-byte units) moves with the stage, the high one
+// (SBO and the version) is a constant.  They are joined inside the
+// instructions' asm, so that no 64-bit arithmetic is done on descriptors.
+__device__ __forceinline__ uint32_t sdesc_lo(uint32_t saddr, uint32_t lbo) {
+  return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
 }
+static constexpr uint32_t kOperandHi = (256u >> 4) | (1u << 14);  // 8-row groups 256 bytes apart
+static constexpr uint32_t kScaleHi = (128u >> 4) | (1u << 14);    // 8 x 16 bytes after 8 x 16 bytes
 
 // kind::mxf4 instruction descriptor: e2m1 x e2m1 -> f32, ue8m0 scales; both
 // operands K-major; sf selects scale bytes (0: the first two of a 32-bit
@@ -121,21 +125,28 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, uint32_t sf) {
          (sf << 29);
 }
 
-// D[tmem] (+)= A x B over K = 64, A and B from shared memory, scales in TMEM.
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+// D[tmem] (+)= A x B over K = 64, A and B from shared memory (low descriptor
+// words), scales in TMEM.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sfa,
                                          uint32_t sfb, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      "mov.b64 da, {%1, %7};\n\t"
+      "mov.b64 db, {%2, %7};\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(kOperandHi)
       : "memory");
 }
 
 // Scales: 32 x 16 bytes of shared memory into four TMEM columns, repeated in
 // each quarter of the lanes.  Runs in order with this thread's later MMAs.
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t desc) {
+  asm volatile(
+      "{\n\t.reg .b64 ds;\n\t"
+      "mov.b64 ds, {%1, %2};\n\t"
+      "tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], ds;\n\t}\n" ::"r"(tmem), "r"(desc), "r"(kScaleHi)
+      : "memory");
 }
 
 // ------------------------------------------------------------- weight plan

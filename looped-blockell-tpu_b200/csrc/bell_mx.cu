@@ -10,18 +10,25 @@
 // is one job (linear) or a gate job and an up job (gated).  A slot of a job
 // takes one activation chunk and one weight chunk (codes and scales, bulk
 // copies; layouts in bell_mx.cuh); its scale images are copied into TMEM and
-// B/64 MMAs of 128 x B x 64 issued.  A pipeline stage holds SLOTS slots: the
-// issuer's wait, commit and bookkeeping cost about 300 cycles, more than a
-// slot's MMAs (B = 128: 128 cycles at the fp4 rate).
+// B/64 MMAs of 128 x B x 64 issued.  A pipeline stage holds up to SLOTS slots
+// of a job, and a job takes ceil(K / SLOTS) stages whatever its live slots (a
+// dead row's are empty), so that every warp knows the order of the stages
+// without reading the plan first.
 //
-// Warps: 0-3 producers (stage use g of the CTA belongs to producer g % 4), 4-11
-// epilogue (TMEM lane quadrant w % 4, column half (w - 4) / 4), 12 issuer and
-// TMEM owner.  Accumulators form a ring of kAccs, so the issuer runs ahead of
-// the epilogue by a job or two.  The TMEM scale columns belong to the stage:
-// a stage is refilled only after its MMAs have completed, so the scales of
-// MMAs in flight are never overwritten.  Token-major, because a lane of the
-// epilogue then holds 32 consecutive features of its token: one scale block,
-// quantised without talking to another lane and stored as 16 bytes.
+// The issuing warp's wait, commit and bookkeeping cost about 300 cycles a
+// stage, more than a slot's MMAs (B = 128: 128 cycles at the fp4 rate).  Hence
+// the multi-slot stages, and two issuers: job j of the CTA belongs to issuer
+// j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
+//
+// Warps: 0-3 producers (ring w / 2; stage use h of a ring belongs to its
+// producer h & 1), 4-11 epilogue (TMEM lane quadrant w % 4, column half
+// (w - 4) / 4), 12 and 13 issuers (12 owns TMEM).  Accumulators form a ring of
+// ACCS in job order, so the issuers run ahead of the epilogue.  The TMEM scale
+// columns belong to the stage: a stage is refilled only after its MMAs have
+// completed, so the scales of MMAs in flight are never overwritten.
+// Token-major, because a lane of the epilogue then holds 32 consecutive
+// features of its token: one scale block, quantised without talking to another
+// lane and stored as 16 bytes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,10 +40,10 @@
 namespace bell {
 namespace mx {
 
-static constexpr int kProducers = 4;
+static constexpr int kProducers = 4;  // two to a ring
 static constexpr int kEpiWarps = 8;
-static constexpr int kIssuer = kProducers + kEpiWarps;  // 12
-static constexpr int kThreads = 32 * (kIssuer + 1);
+static constexpr int kIssuer = kProducers + kEpiWarps;  // 12, 13
+static constexpr int kThreads = 32 * (kIssuer + 2);
 
 template <int B>
 struct Geo {
@@ -44,13 +51,14 @@ struct Geo {
   static constexpr int SLOT = A + W;             // 17408 / 7168 bytes, multiples of 256
   static constexpr int SLOTS = B == 128 ? 2 : 4;
   static constexpr int STAGE = SLOTS * SLOT;
-  static constexpr int NS = B == 128 ? 6 : 7;
+  static constexpr int NR = B == 128 ? 3 : 4;    // stages of a ring
+  static constexpr int NS = 2 * NR;
   static constexpr int ACCS = B == 128 ? 3 : 4;
   static constexpr int SF_COL = ACCS * B;        // 8 scale columns per slot of a stage from here
   static constexpr int SMEM = NS * STAGE + 1024 + 1024;
-  // a producer's wait for stage use g - NS must not meet the parity of use
-  // g - 2 NS: that one is released before the producer's own use g - P - NS
-  static_assert(NS > kProducers, "mbarrier parity");
+  // a producer's wait for the release of use h - NR must not meet the parity of
+  // use h - 2 NR: that one is released before h - 2 - NR, which it waited for
+  static_assert(NR > 2, "mbarrier parity");
   static_assert(SF_COL + NS * SLOTS * 8 <= 512, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -73,7 +81,7 @@ struct Params {
 struct Smem {
   uint8_t* stages;
   uint64_t *full, *empty, *acc_full, *acc_empty, *drain;
-  uint32_t* tmem_slot;
+  uint32_t *count, *tmem_slot;  // live slots of each stage
   volatile int* abort_flag;
 };
 
@@ -88,82 +96,103 @@ __device__ __forceinline__ Smem carve(uint8_t* raw) {
   s.acc_full = s.empty + G::NS;
   s.acc_empty = s.acc_full + G::ACCS;
   s.drain = s.acc_empty + G::ACCS;
-  s.tmem_slot = reinterpret_cast<uint32_t*>(s.drain + 1);
+  s.count = reinterpret_cast<uint32_t*>(s.drain + 2);
+  s.tmem_slot = s.count + G::NS;
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
   return s;
+}
+
+// The CTA's units are blockIdx.x + i * gridDim.x; ring k's job i is unit i of
+// matrix k (gated) or unit 2i + k (linear).
+template <bool GATED>
+__device__ __forceinline__ int ring_jobs(const Params& p, int k) {
+  const int units = p.mtiles * p.R, first = int(blockIdx.x), grid = int(gridDim.x);
+  const int mine = first < units ? (units - first + grid - 1) / grid : 0;
+  return GATED ? mine : (mine - k + 1) / 2;
+}
+template <bool GATED>
+__device__ __forceinline__ int job_unit(int i, int k) {
+  return int(blockIdx.x) + (GATED ? i : 2 * i + k) * int(gridDim.x);
 }
 
 // ---------------------------------------------------------------- producer
 
 template <int B, bool GATED>
-__device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl) {
+__device__ void produce(const Params& p, const Smem& s, int ring, int sub, const Ctl& ctl) {
   using G = Geo<B>;
   const int lane = threadIdx.x & 31;
-  const int units = p.mtiles * p.R;
   const uint64_t keep = policy_evict_last(), pass = policy_evict_normal();
-  uint32_t g = 0;       // stage uses of the CTA so far
-  uint32_t mine = 0;    // 1 + the last one that this producer filled
-  bool ok = true;
-  auto fetch = [&](int u, int mat, int& n) -> uint32_t {  // a job's first 32 entries, and their number
-    const int r = u % p.R;
-    const Plan& pl = mat ? p.p1 : p.p0;
-    n = __ldg(pl.counts + r);
-    const int K = mat ? p.K1 : p.K0;
-    return lane < K ? __ldg(pl.entries + int64_t(r) * K + lane) : 0u;
+  const int mat = GATED ? ring : 0;
+  const int K = mat ? p.K1 : p.K0;
+  const uint8_t* w = mat ? p.w1 : p.w0;
+  const uint32_t* entries = (mat ? p.p1 : p.p0).entries;
+  const int per_job = (K + G::SLOTS - 1) / G::SLOTS;
+  const int jobs = ring_jobs<GATED>(p, ring);
+  uint64_t* full = s.full + ring * G::NR;
+  uint64_t* empty = s.empty + ring * G::NR;
+  int job = sub / per_job, part = sub % per_job;  // of the next use
+  int m = 0, r = 0;
+  // this producer's next use's entries travel while the one before is issued
+  auto fetch = [&]() -> uint32_t {
+    const int u = job_unit<GATED>(job, ring);
+    m = u / p.R;
+    r = u - m * p.R;
+    const int k = part * G::SLOTS + lane;
+    return lane < G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
   };
-  int u = blockIdx.x, mat = 0, n_next = 0;
-  uint32_t e_next = u < units ? fetch(u, 0, n_next) : 0u;
-  while (u < units && ok) {
-    const int m = u / p.R, r = u - m * p.R;
-    const int K = mat ? p.K1 : p.K0;
-    const uint8_t* w = mat ? p.w1 : p.w0;
-    const uint32_t* entries = (mat ? p.p1 : p.p0).entries + int64_t(r) * K;
-    const int n = n_next;
-    uint32_t e = e_next;
-    // the next job's entries travel while this one's copies are issued
-    int u2 = u, mat2 = 0;
-    if (GATED && mat == 0)
-      mat2 = 1;
-    else
-      u2 = u + int(gridDim.x);
-    if (u2 < units) e_next = fetch(u2, mat2, n_next);
-    for (int j = 0; j < n; j += G::SLOTS, ++g) {
-      if (j && (j & 31) == 0) e = j + lane < n ? __ldg(entries + j + lane) : 0u;
-      uint32_t ent[G::SLOTS];
+  uint32_t e_next = job < jobs ? fetch() : kNoSlot;
+  uint32_t stage = uint32_t(sub), phase = 0;
+  bool ok = true;
+  int64_t filled = 0;
+  while (job < jobs) {
+    const uint32_t e = e_next;
+    const uint8_t* xm = p.x + int64_t(m) * p.C * G::A;
+    const uint8_t* wr = w + int64_t(r) * K * G::W;
+    part += 2;
+    while (part >= per_job) {
+      part -= per_job;
+      ++job;
+    }
+    if (job < jobs) e_next = fetch();
+    ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, ctl));
+    if (!ok) break;
+    const int cnt = __popc(__ballot_sync(0xffffffffu, e != kNoSlot));
+    uint8_t* st = s.stages + (ring * G::NR + int(stage)) * G::STAGE;
+    uint32_t ent[G::SLOTS];
 #pragma unroll
-      for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, e, (j + i) & 31);
-      if (int(g % kProducers) != pid) continue;
-      const int slot = int(g % G::NS);
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.empty[slot], ((g / G::NS) & 1u) ^ 1u, ctl))) {
-        ok = false;
-        break;
-      }
-      if (elect_one()) {
-        uint8_t* st = s.stages + slot * G::STAGE;
-        const int cnt = min(G::SLOTS, n - j);
-        mbar_arrive_expect_tx(&s.full[slot], cnt * G::SLOT);
+    for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, e, i);
+    if (elect_one()) {
+      s.count[ring * G::NR + stage] = uint32_t(cnt);
+      if (cnt)
+        mbar_arrive_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::SLOT));
+      else
+        mbar_arrive(&full[stage]);
 #pragma unroll
-        for (int i = 0; i < G::SLOTS; ++i) {
-          if (i < cnt) {
-            const int c = int(ent[i] & 0xFFFFu), k = int(ent[i] >> 16);
-            bulk_load(st + i * G::SLOT, p.x + (int64_t(m) * p.C + c) * G::A, G::A, &s.full[slot], pass);
-            bulk_load(st + i * G::SLOT + G::A, w + (int64_t(r) * K + k) * G::W, G::W, &s.full[slot], keep);
-          }
+      for (int i = 0; i < G::SLOTS; ++i) {
+        if (i < cnt) {
+          bulk_load(st + i * G::SLOT, xm + int64_t(ent[i] & 0xFFFFu) * G::A, G::A, &full[stage], pass);
+          bulk_load(st + i * G::SLOT + G::A, wr + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
         }
       }
-      __syncwarp();
-      mine = g + 1;
     }
-    u = u2;
-    mat = mat2;
+    __syncwarp();
+    ++filled;
+    stage += 2;
+    if (stage >= uint32_t(G::NR)) {
+      stage -= G::NR;
+      phase ^= 1u;
+    }
   }
-  if (!ok && mine && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
-    for (int i = 0; i <= G::NS / kProducers; ++i) {
-      if (mine < uint32_t(1 + i * kProducers)) break;
-      const uint32_t gi = mine - 1 - i * kProducers;
-      const uint32_t a = smem_u32(&s.full[gi % G::NS]);
+  if (!ok && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
+    for (int i = 0; i < G::NR && filled > 0; ++i, --filled) {
+      if (stage < 2u) {
+        stage += G::NR;
+        phase ^= 1u;
+      }
+      stage -= 2;
+      const uint32_t a = smem_u32(&full[stage]);
       const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(a, (gi / G::NS) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
+      while (!mbar_try_wait(a, phase) && globaltimer_ns() - t0 < 100000000ull) {
       }
     }
   }
@@ -172,66 +201,66 @@ __device__ void produce(const Params& p, const Smem& s, int pid, const Ctl& ctl)
 // ------------------------------------------------------------------ issuer
 
 template <int B, bool GATED>
-__device__ void issue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
+__device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, const Ctl& ctl) {
   using G = Geo<B>;
   const bool leader = elect_one();
-  const int units = p.mtiles * p.R;
-  const uint32_t a0 = sdesc_lo(smem_u32(s.stages), 128), sf0 = sdesc_lo(smem_u32(s.stages), 16);
-  uint32_t stage = 0, phase = 0, acc = 0, use = 0;
+  const uint32_t a0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 128);
+  const uint32_t sf0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 16);
+  const int K = GATED && ring ? p.K1 : p.K0;
+  const int per_job = (K + G::SLOTS - 1) / G::SLOTS;
+  const int jobs = ring_jobs<GATED>(p, ring);
+  uint64_t* full = s.full + ring * G::NR;
+  uint64_t* empty = s.empty + ring * G::NR;
+  uint32_t stage = 0, phase = 0;
+  uint32_t acc = uint32_t(ring), use = 0;  // job 2i + ring of the CTA: accumulator (2i + ring) % ACCS
   bool ok = true;
-  int u = blockIdx.x, mat = 0;
-  int n_next = u < units ? __ldg(p.p0.counts + u % p.R) : 0;
-  while (u < units && ok) {
-    int n = n_next;  // live slots of this job; the next job's are read ahead
-    if (GATED && mat == 0) {
-      mat = 1;
-    } else {
-      mat = 0;
-      u += int(gridDim.x);
-    }
-    if (u < units) n_next = __ldg((mat ? p.p1 : p.p0).counts + u % p.R);
+  for (int i = 0; i < jobs && ok; ++i) {
     ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_empty[acc], (use & 1u) ^ 1u, ctl));
     if (!ok) break;
     tc_fence_after();
     const uint32_t d = tmem + acc * B;
-    for (uint32_t more = 0; n > 0; n -= G::SLOTS, more = 1) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, ctl));
+    uint32_t more = 0;
+    for (int part = 0; part < per_job; ++part) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, ctl));
       if (!ok) break;
       tc_fence_after();
+      const int n = int(s.count[ring * G::NR + stage]);
       if (leader) {
         const uint32_t st = stage * uint32_t(G::STAGE >> 4);
-        const uint32_t sf = tmem + G::SF_COL + stage * (G::SLOTS * 8);
+        const uint32_t sf = tmem + G::SF_COL + (ring * G::NR + stage) * (G::SLOTS * 8);
 #pragma unroll
-        for (int i = 0; i < G::SLOTS; ++i) {
-          if (i < n) {
-            const uint32_t at = st + i * (G::SLOT >> 4);
-            copy_scales(sf + i * 8, sf0 + at + ((G::A - kScaleBytes) >> 4));
-            copy_scales(sf + i * 8 + 4, sf0 + at + ((G::SLOT - kScaleBytes) >> 4));
+        for (int j = 0; j < G::SLOTS; ++j) {
+          if (j < n) {
+            const uint32_t at = st + j * (G::SLOT >> 4);
+            copy_scales(sf + j * 8, sf0 + at + ((G::A - kScaleBytes) >> 4));
+            copy_scales(sf + j * 8 + 4, sf0 + at + ((G::SLOT - kScaleBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < B / 64; ++kk)
               mma_mxf4(d, a0 + at + kk * (kRows * 32 >> 4), a0 + at + ((G::A + kk * B * 32) >> 4),
-                       idesc_mxf4(kRows, B, kk * 2), sf + i * 8, sf + i * 8 + 4, i > 0 || kk > 0 ? 1u : more);
+                       idesc_mxf4(kRows, B, kk * 2), sf + j * 8, sf + j * 8 + 4, j > 0 || kk > 0 ? 1u : more);
           }
         }
-        mma_commit(&s.empty[stage]);
+        mma_commit(&empty[stage]);
       }
       __syncwarp();
-      if (++stage == G::NS) {
+      more = 1;
+      if (++stage == G::NR) {
         stage = 0;
         phase ^= 1;
       }
     }
     if (!ok) break;
-    if (leader) mma_commit(&s.acc_full[acc]);  // a job without live slots: nothing to wait for
+    if (leader) mma_commit(&s.acc_full[acc]);
     __syncwarp();
-    if (++acc == G::ACCS) {
-      acc = 0;
+    acc += 2;
+    if (acc >= uint32_t(G::ACCS)) {
+      acc -= G::ACCS;
       ++use;
     }
   }
   if (leader) {  // every MMA has completed before TMEM is released
-    mma_commit(s.drain);
-    const uint32_t a = smem_u32(s.drain);
+    mma_commit(&s.drain[ring]);
+    const uint32_t a = smem_u32(&s.drain[ring]);
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(a, 0) && globaltimer_ns() - t0 < 100000000ull) {
     }
@@ -262,13 +291,19 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       ++use;
     }
   };
+  int c0 = 0, c1 = 0;  // live slots of the next unit's rows, read a unit ahead
+  auto counts = [&](int u) {
+    c0 = __ldg(p.p0.counts + u % p.R);
+    if (GATED) c1 = __ldg(p.p1.counts + u % p.R);
+  };
+  if (int(blockIdx.x) < units) counts(blockIdx.x);
   for (int u = blockIdx.x; u < units; u += int(gridDim.x)) {
     const int m = u / p.R, r = u - m * p.R;
     const int n = q * 32 + lane;
     const int64_t t = int64_t(m) * kRows + n;
-    const bool live0 = __ldg(p.p0.counts + r) > 0;
+    const bool live0 = c0 > 0, live1 = c1 > 0;
+    if (u + int(gridDim.x) < units) counts(u + int(gridDim.x));
     if constexpr (GATED) {
-      const bool live1 = __ldg(p.p1.counts + r) > 0;
       const uint32_t a0 = acc;
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
       next();
@@ -400,7 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
       mbar_init(&s.acc_full[i], 1);
       mbar_init(&s.acc_empty[i], kEpiWarps);
     }
-    mbar_init(s.drain, 1);
+    mbar_init(&s.drain[0], 1);
+    mbar_init(&s.drain[1], 1);
     *s.abort_flag = 0;
     fence_mbar_init();
   }
@@ -416,11 +452,11 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   griddep_launch();
   griddep_wait();  // the rows come from the kernel before
   if (warp < kProducers)
-    produce<B, GATED>(p, s, warp, ctl);
+    produce<B, GATED>(p, s, warp >> 1, warp & 1, ctl);
   else if (warp < kIssuer)
     epilogue<B, GATED>(p, s, tmem, ctl);
   else
-    issue<B, GATED>(p, s, tmem, ctl);
+    issue<B, GATED>(p, s, tmem, warp - kIssuer, ctl);
   tc_fence_before();
   __syncthreads();
   if (warp == kIssuer) {

@@ -151,9 +151,11 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t desc) {
 
 // ------------------------------------------------------------- weight plan
 
-// Live slots of each block-row in ascending slot order: entry = column |
-// slot << 16, and their number.  [R, K] entries, then [R] counts, each part
-// padded to 16 bytes (bell_plan_bytes(0, 0, 0, R, K) bytes).
+// Live slots of each block-row in ascending slot order (entry = column |
+// slot << 16), then kNoSlot up to K; and their number.  [R, K] entries, then
+// [R] counts, each part padded to 16 bytes (bell_plan_bytes(0, 0, 0, R, K)
+// bytes).
+static constexpr uint32_t kNoSlot = 0xFFFFFFFFu;  // column and slot are at most 65534
 struct Plan {
   const uint32_t* entries;
   const int32_t* counts;

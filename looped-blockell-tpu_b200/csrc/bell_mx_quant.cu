@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(kThr) bell_mx_plan_kernel(const int32_t* __res
     if (live) entries[int64_t(r) * K + n + __popc(m & ((1u << lane) - 1u))] = uint32_t(c) | (uint32_t(k) << 16);
     n += __popc(m);
   }
+  for (int k = n + lane; k < K; k += 32) entries[int64_t(r) * K + k] = kNoSlot;
   if (lane == 0) counts[r] = n;
   if (bad) atomicOr(status, BELL_STATUS_COLIDX);
 }
@@ -287,7 +288,8 @@ int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, 
   if (!w || !w->values || !w->col_indices || !chunks || !plan) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: NULL argument");
   if (w->B != 64 && w->B != 128) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: tile size B must be 64 or 128");
   if (w->R < 1 || w->C < 1 || w->K < 1) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R, C, K must be >= 1");
-  if (w->C > 65535 || w->K > 65535) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: C and K must be <= 65535");
+  if (w->R > (1 << 23) || w->C > 65535 || w->K > 65535)
+    return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R must be <= 2^23, C and K <= 65535");
   if (dtype != BELL_DTYPE_BF16 && dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "bell_mx_pack_ell: dtype must be bf16 or f32");
   if (w->layout != BELL_TILE_IN_OUT && w->layout != BELL_TILE_OUT_IN)

@@ -270,10 +270,20 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
 
 // ---------------------------------------------------------------- epilogue
 
-// h = silu(g) u = g u / (1 + e^-g) in fp32 (about 1e-6 relative): the hardware
-// tanh form of the bf16 kernels (2^-11) would move one in a few hundred of
-// h's 4-bit codes to a neighbour.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// h = silu(g) u = g u / (1 + e^-g) in fp32, two at a time (about 1e-6
+// relative): the hardware tanh form of the bf16 kernels (2^-11) would move one
+// in a few hundred of h's 4-bit codes to a neighbour.  Subnormal intermediates
+// are flushed: e^-g below 2^-126 next to 1, and 1 / (1 + e^-g) below 2^-126.
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+  const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 a = add2(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
+  return mul2(mul2(g, r), u);
+}
 
 template <int B, bool GATED>
 __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
@@ -326,12 +336,20 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
             mbar_arrive(&s.acc_empty[a1]);
           }
         }
+        if (!live0 || !live1) {  // a projection without a live slot is zero
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!live0) gr[i] = 0u;
+            if (!live1) ur[i] = 0u;
+          }
+        }
         float h[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!live0) gr[i] = 0u;  // a projection without a live slot is zero
-          if (!live1) ur[i] = 0u;
-          h[i] = silu_mul(__uint_as_float(gr[i]), __uint_as_float(ur[i]));
+        for (int i = 0; i < 32; i += 2) {
+          const float2 v = silu_mul2(make_float2(__uint_as_float(gr[i]), __uint_as_float(gr[i + 1])),
+                                     make_float2(__uint_as_float(ur[i]), __uint_as_float(ur[i + 1])));
+          h[i] = v.x;
+          h[i + 1] = v.y;
         }
         if (t < p.T) {
           const int64_t at = t * ld + int64_t(r) * B + j * 32;

@@ -73,16 +73,50 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
   return r;
 }
 
+// Two fp32 products or sums in one instruction, each rounded as alone.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// Largest magnitude of three; NaN if one is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // One scale block: codes of v[0..31] and the scale byte.
 __device__ __forceinline__ uint4 quantize32(const float (&v)[32], uint32_t& byte) {
-  uint32_t top = 0;  // magnitudes as integers: NaN > inf > every finite value
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  byte = scale_byte(top);
+  for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = max_abs3(m[j], v[i + 2 * j], v[i + 2 * j + 1]);
+  }
+  const float top = max_abs3(max_abs3(m[0], m[1], m[2]), m[3], 0.f);
+  byte = scale_byte(__float_as_uint(top) & 0x7FFFFFFFu);
   const float inv = scale_inverse(byte);
   float s[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = v[i] * inv;
+  for (int i = 0; i < 32; i += 2) {
+    const float2 t = mul2(make_float2(v[i], v[i + 1]), make_float2(inv, inv));
+    s[i] = t.x;
+    s[i + 1] = t.y;
+  }
   return make_uint4(pack_e2m1(s), pack_e2m1(s + 8), pack_e2m1(s + 16), pack_e2m1(s + 24));
 }
 

@@ -21,9 +21,11 @@
 // j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
 //
 // Warps: 0-3 producers (ring w / 2; stage use h of a ring belongs to its
-// producer h & 1), 4-11 epilogue (TMEM lane quadrant w % 4, column half
-// (w - 4) / 4), 12 and 13 issuers (12 owns TMEM).  Accumulators form a ring of
-// ACCS in job order, so the issuers run ahead of the epilogue.  The TMEM scale
+// producer h & 1), 4-19 epilogue (a warp takes the TMEM lane quadrant w % 4 and
+// one 32-column block of a unit; at B = 64, two blocks, two groups of eight
+// warps take the CTA's units in turn), 20 and 21 issuers (20 owns TMEM).
+// Accumulators form a ring of ACCS in job order, so the issuers run ahead of the
+// epilogue.  The TMEM scale
 // columns belong to the stage: a stage is refilled only after its MMAs have
 // completed, so the scales of MMAs in flight are never overwritten.
 // Token-major, because a lane of the epilogue then holds 32 consecutive
@@ -41,8 +43,8 @@ namespace bell {
 namespace mx {
 
 static constexpr int kProducers = 4;  // two to a ring
-static constexpr int kEpiWarps = 8;
-static constexpr int kIssuer = kProducers + kEpiWarps;  // 12, 13
+static constexpr int kEpiWarps = 16;
+static constexpr int kIssuer = kProducers + kEpiWarps;  // 20, 21
 static constexpr int kThreads = 32 * (kIssuer + 2);
 
 template <int B>
@@ -288,47 +290,43 @@ __device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
 template <int B, bool GATED>
 __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
   using G = Geo<B>;
-  constexpr int NB = B / 64;  // scale blocks (32 features) of this warp
+  constexpr int NB = B / 32;             // scale blocks (32 features) of a unit
+  constexpr int GROUPS = kEpiWarps / (4 * NB);
+  constexpr int JOBS = GATED ? 2 : 1;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
-  const int q = w & 3, half = w >> 2;
+  const int q = w & 3, j = (w >> 2) % NB, group = (w >> 2) / NB;
   const int units = p.mtiles * p.R;
   const int64_t ld = int64_t(p.R) * B;
   const uint32_t lanes = uint32_t(q * 32) << 16;
-  uint32_t acc = 0, use = 0;
-  auto next = [&] {
-    if (++acc == G::ACCS) {
-      acc = 0;
-      ++use;
-    }
-  };
+  const int step = GROUPS * int(gridDim.x);
+  uint32_t acc = uint32_t(group * JOBS), use = 0;  // accumulator of this unit's first job
   int c0 = 0, c1 = 0;  // live slots of the next unit's rows, read a unit ahead
   auto counts = [&](int u) {
     c0 = __ldg(p.p0.counts + u % p.R);
     if (GATED) c1 = __ldg(p.p1.counts + u % p.R);
   };
-  if (int(blockIdx.x) < units) counts(blockIdx.x);
-  for (int u = blockIdx.x; u < units; u += int(gridDim.x)) {
+  int u = int(blockIdx.x) + group * int(gridDim.x);
+  if (u < units) counts(u);
+  for (; u < units; u += step) {
     const int m = u / p.R, r = u - m * p.R;
     const int n = q * 32 + lane;
     const int64_t t = int64_t(m) * kRows + n;
     const bool live0 = c0 > 0, live1 = c1 > 0;
-    if (u + int(gridDim.x) < units) counts(u + int(gridDim.x));
+    if (u + step < units) counts(u + step);
+    const int64_t at = t * ld + int64_t(r) * B + j * 32;
     if constexpr (GATED) {
-      const uint32_t a0 = acc;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
-      next();
-      const uint32_t a1 = acc;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
-      next();
+      const uint32_t a0 = acc, a1 = acc + 1 == uint32_t(G::ACCS) ? 0u : acc + 1;
+      const uint32_t use1 = a1 ? use : use + 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
       tc_fence_after();
-      uint8_t* ch = p.h + (int64_t(m) * p.R + r) * G::A;
-      uint32_t bytes = 0;
+      float h[32];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int j = half * NB + b;
-        uint32_t gr[32], ur[32];
-        tmem_ld32x2_sync(tmem + lanes + a0 * B + j * 32, gr, tmem + lanes + a1 * B + j * 32, ur);
-        if (b == NB - 1) {
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t col = tmem + lanes + uint32_t(j * 32 + half * 16);
+        uint32_t gr[16], ur[16];
+        tmem_ld16x2_sync(col + a0 * B, gr, col + a1 * B, ur);
+        if (half) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -338,67 +336,51 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         }
         if (!live0 || !live1) {  // a projection without a live slot is zero
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < 16; ++i) {
             if (!live0) gr[i] = 0u;
             if (!live1) ur[i] = 0u;
           }
         }
-        float h[32];
+        if (p.gate && t < p.T) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 v = silu_mul2(make_float2(__uint_as_float(gr[i]), __uint_as_float(gr[i + 1])),
-                                     make_float2(__uint_as_float(ur[i]), __uint_as_float(ur[i + 1])));
-          h[i] = v.x;
-          h[i + 1] = v.y;
-        }
-        if (t < p.T) {
-          const int64_t at = t * ld + int64_t(r) * B + j * 32;
-          if (p.gate) {
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a[4], c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a[4], c[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                a[e] = pack_bf16x2(__uint_as_float(gr[8 * i + 2 * e]), __uint_as_float(gr[8 * i + 2 * e + 1]));
-                c[e] = pack_bf16x2(__uint_as_float(ur[8 * i + 2 * e]), __uint_as_float(ur[8 * i + 2 * e + 1]));
-              }
-              st_global_v4(p.gate + at + 8 * i, a[0], a[1], a[2], a[3]);
-              st_global_v4(p.up + at + 8 * i, c[0], c[1], c[2], c[3]);
+            for (int e = 0; e < 4; ++e) {
+              a[e] = pack_bf16x2(__uint_as_float(gr[8 * i + 2 * e]), __uint_as_float(gr[8 * i + 2 * e + 1]));
+              c[e] = pack_bf16x2(__uint_as_float(ur[8 * i + 2 * e]), __uint_as_float(ur[8 * i + 2 * e + 1]));
             }
+            st_global_v4(p.gate + at + half * 16 + 8 * i, a[0], a[1], a[2], a[3]);
+            st_global_v4(p.up + at + half * 16 + 8 * i, c[0], c[1], c[2], c[3]);
           }
         }
-        uint32_t byte;
-        const uint4 c = quantize32(h, byte);
-        bytes |= byte << (8 * b);
-        if (t < p.T) st_global_v4(ch + code_off(n, j, kRows * 32), c.x, c.y, c.z, c.w);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float2 v = silu_mul2(make_float2(__uint_as_float(gr[i]), __uint_as_float(gr[i + 1])),
+                                     make_float2(__uint_as_float(ur[i]), __uint_as_float(ur[i + 1])));
+          h[half * 16 + i] = v.x;
+          h[half * 16 + i + 1] = v.y;
+        }
       }
+      uint32_t byte;
+      const uint4 c = quantize32(h, byte);
       if (t < p.T) {
-        uint8_t* sp = ch + kRows * B / 2 + scale_off(n, half * NB);
-        if constexpr (NB == 2)
-          *reinterpret_cast<uint16_t*>(sp) = uint16_t(bytes);
-        else
-          *sp = uint8_t(bytes);
+        uint8_t* ch = p.h + (int64_t(m) * p.R + r) * G::A;
+        st_global_v4(ch + code_off(n, j, kRows * 32), c.x, c.y, c.z, c.w);
+        ch[kRows * B / 2 + scale_off(n, j)] = uint8_t(byte);
       }
     } else {
-      const uint32_t a0 = acc;
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
-      next();
       tc_fence_after();
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int j = half * NB + b;
-        uint32_t a[32];
-        tmem_ld32_sync(tmem + lanes + a0 * B + j * 32, a);
-        if (b == NB - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.acc_empty[a0]);
-        }
-        if (t >= p.T) continue;
+      uint32_t a[32];
+      tmem_ld32_sync(tmem + lanes + acc * B + j * 32, a);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.acc_empty[acc]);
+      if (t < p.T) {
         float f[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
-        const int64_t at = t * ld + int64_t(r) * B + j * 32;
         if (p.out_f32) {
           float* o = static_cast<float*>(p.out) + at;
           const float* rs = static_cast<const float*>(p.residual);
@@ -435,6 +417,11 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         }
       }
     }
+    acc += GROUPS * JOBS;
+    while (acc >= uint32_t(G::ACCS)) {
+      acc -= G::ACCS;
+      ++use;
+    }
   }
 }
 
@@ -451,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
     }
     for (int i = 0; i < G::ACCS; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], kEpiWarps);
+      mbar_init(&s.acc_empty[i], B / 32 * 4);  // the epilogue warps of a unit
     }
     mbar_init(&s.drain[0], 1);
     mbar_init(&s.drain[1], 1);

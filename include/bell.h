@@ -372,6 +372,73 @@ typedef struct BellMxFFNDesc {
 
 int bell_swiglu_fwd_mx(const BellMxFFNDesc* desc, void* stream);
 
+/*
+ * Straight-through backward of bell_linear_mx (without the residual, whose
+ * gradient is grad_out): dx = dy Q(W) and the tile gradients dW = dy^T Q(x)
+ * on the live slots (zero in dead ones), in bf16 products with fp32 sums.
+ * The transposed topology [C, K_t]: cols_t lists, for each column block, the
+ * block-rows that use it (-1 pads), index_t those tiles' positions r * K + k.
+ */
+typedef struct BellMxLinearBwdDesc {
+  int64_t T;
+  const void* grad_out;        /* bf16 [T, R*B]                              */
+  const void* x;               /* quantised rows of the forward              */
+  BellMxEll w;
+  const int32_t* col_indices;  /* [R, K]                                     */
+  const int32_t* cols_t;
+  const int64_t* index_t;
+  int32_t K_t;
+  int32_t layout;              /* of dw                                      */
+  void* dx;                    /* optional bf16 [T, C*B]                     */
+  void* dw;                    /* optional [R, K, B, B]                      */
+  int32_t grad_dtype;          /* of dw: BELL_DTYPE_BF16 / BELL_DTYPE_F32    */
+  int32_t reserved;
+  void* workspace;
+  int32_t* status;
+} BellMxLinearBwdDesc;
+
+size_t bell_linear_bwd_mx_workspace_bytes(const BellMxLinearBwdDesc* desc);
+int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
+
+/*
+ * Straight-through backward of bell_swiglu_fwd_mx: gate_pre and up_out are its
+ * bf16 projections, x and h its quantised rows.  cols_t_down / index_t_down:
+ * transposed topology of down [d_ff/B, K_t_down]; cols_t_gate_up /
+ * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
+ * of up, and its tiles, counted after gate's).  Results that are NULL are not
+ * computed.  With add_residual, dx includes grad_out.
+ */
+typedef struct BellMxFFNBwdDesc {
+  int64_t T;
+  int32_t add_residual;
+  int32_t layout;              /* of the tile gradients                      */
+  const void* grad_out;        /* bf16 [T, d_model]                          */
+  const void* gate_pre;        /* bf16 [T, d_ff]                             */
+  const void* up_out;
+  const void* x;               /* quantised rows                             */
+  const void* h;
+  BellMxEll gate, up, down;
+  const int32_t* cols_gate;    /* [R, K] of each weight                      */
+  const int32_t* cols_up;
+  const int32_t* cols_down;
+  const int32_t* cols_t_down;
+  const int64_t* index_t_down;
+  const int32_t* cols_t_gate_up;
+  const int64_t* index_t_gate_up;
+  int32_t K_t_down, K_t_gate_up;
+  void* dx;                    /* optional bf16 [T, d_model]                 */
+  void* d_gate;                /* optional tile gradients, each of its type  */
+  void* d_up;
+  void* d_down;
+  int32_t gate_dtype, up_dtype, down_dtype;
+  int32_t reserved;
+  void* workspace;
+  int32_t* status;
+} BellMxFFNBwdDesc;
+
+size_t bell_swiglu_bwd_mx_workspace_bytes(const BellMxFFNBwdDesc* desc);
+int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* desc, void* stream);
+
 /* ------------------------------------------------------------------- loop */
 
 /*

@@ -1,5 +1,5 @@
 // bell_mx_quant.cu — MXFP4 quantisation and its inverse: activation rows,
-// Block-ELL tiles, and the plan of a weight's live slots (layouts: bell_mx.cuh).
+// Block-ELL tiles and the plan of their live slots (layouts: bell_mx.cuh).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -124,34 +124,85 @@ __global__ void __launch_bounds__(kThr) bell_mx_dequantize_kernel(RowsArgs a, co
   }
 }
 
-// One thread per scale block of a tile: output o, block j of its inputs.
-// [B_in, B_out] tiles are read a row of outputs at a time (lane = output), so
-// the 32 values of a thread are strided and a warp's loads contiguous.
+// One warp per block-row: the live slots, compacted in slot order.
+__device__ __forceinline__ void plan_row(const int32_t* __restrict__ cols, int r, int32_t C, int32_t K,
+                                         uint32_t* __restrict__ entries, int32_t* __restrict__ counts,
+                                         int32_t* status) {
+  const int lane = threadIdx.x & 31;
+  int n = 0, bad = 0;
+  for (int k0 = 0; k0 < K; k0 += 32) {
+    const int k = k0 + lane;
+    const int c = k < K ? cols[int64_t(r) * K + k] : -1;
+    const bool live = c >= 0 && c < C;
+    bad |= c < -1 || c >= C;
+    const uint32_t m = __ballot_sync(0xffffffffu, live);
+    if (live) entries[int64_t(r) * K + n + __popc(m & ((1u << lane) - 1u))] = uint32_t(c) | (uint32_t(k) << 16);
+    n += __popc(m);
+  }
+  for (int k = n + lane; k < K; k += 32) entries[int64_t(r) * K + k] = kNoSlot;
+  if (lane == 0) counts[r] = n;
+  if (bad) atomicOr(status, BELL_STATUS_COLIDX);
+}
+
+struct PackArgs {
+  int64_t tiles;
+  int32_t B, in_out;
+  const int32_t* cols;
+  int32_t R, C, K;
+  uint32_t* entries;
+  int32_t* counts;
+  int32_t* status;
+  unsigned plan_blocks;  // blocks of the grid that write the plan, a warp to a block-row
+};
+
+__device__ __forceinline__ void put_block(uint8_t* chunk, int B, int o, int j, const float (&v)[32]) {
+  uint32_t byte;
+  const uint4 q = quantize32(v, byte);
+  st_global_v4(chunk + code_off(o, j, B * 32), q.x, q.y, q.z, q.w);
+  chunk[B * B / 2 + scale_off(o, j)] = uint8_t(byte);
+}
+
+__device__ __forceinline__ float2 load_pair(const __nv_bfloat16* p) {
+  return unpack_bf16x2(__ldg(reinterpret_cast<const unsigned*>(p)));
+}
+__device__ __forceinline__ float2 load_pair(const float* p) { return __ldg(reinterpret_cast<const float2*>(p)); }
+
+// A thread takes the scale blocks j of two outputs of a tile.  [B_in, B_out]
+// tiles are read a row of outputs at a time (lane = output pair): the 32 values
+// of a block are strided and a warp's loads contiguous.
 template <class E>
-__global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const E* __restrict__ values, int64_t tiles, int32_t B,
-                                                           int32_t in_out, uint8_t* __restrict__ chunks) {
-  const int per_tile = B * (B / kBlock);
-  for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
+__global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const E* __restrict__ values, PackArgs a,
+                                                           uint8_t* __restrict__ chunks) {
+  if (blockIdx.x < a.plan_blocks) {
+    const int r = int(blockIdx.x) * (kThr / 32) + int(threadIdx.x >> 5);
+    if (r < a.R) plan_row(a.cols, r, a.C, a.K, a.entries, a.counts, a.status);
+    return;
+  }
+  const int B = a.B, blocks = B / kBlock, per_tile = B / 2 * blocks;
+  const int64_t stride = int64_t(gridDim.x - a.plan_blocks) * kThr;
+  for (int64_t i = int64_t(blockIdx.x - a.plan_blocks) * kThr + threadIdx.x; i < a.tiles * per_tile; i += stride) {
     const int64_t tile = i / per_tile;
     const int e = int(i - tile * per_tile);
     const E* v0 = values + tile * B * B;
-    int o, j;
-    float v[32];
-    if (in_out) {
-      o = e % B;
-      j = e / B;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] = float(v0[(j * kBlock + k) * B + o]);
-    } else {
-      j = e % (B / kBlock);
-      o = e / (B / kBlock);
-      load32(v0 + o * B + j * kBlock, v);
-    }
-    uint32_t byte;
-    const uint4 q = quantize32(v, byte);
     uint8_t* ch = chunks + tile * tile_chunk(B);
-    st_global_v4(ch + code_off(o, j, B * 32), q.x, q.y, q.z, q.w);
-    ch[B * B / 2 + scale_off(o, j)] = uint8_t(byte);
+    float v[32], w[32];
+    if (a.in_out) {
+      const int o = e % (B / 2) * 2, j = e / (B / 2);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float2 f = load_pair(v0 + (j * kBlock + k) * B + o);
+        v[k] = f.x;
+        w[k] = f.y;
+      }
+      put_block(ch, B, o, j, v);
+      put_block(ch, B, o + 1, j, w);
+    } else {
+      const int j = e % blocks, o = e / blocks * 2;
+      load32(v0 + o * B + j * kBlock, v);
+      load32(v0 + (o + 1) * B + j * kBlock, w);
+      put_block(ch, B, o, j, v);
+      put_block(ch, B, o + 1, j, w);
+    }
   }
 }
 
@@ -177,28 +228,6 @@ __global__ void __launch_bounds__(kThr) bell_mx_unpack_kernel(const uint8_t* __r
     unpack_e2m1(q.w, s, v + 24);
     store32(values + tile * B * B + o * B + j * kBlock, v);
   }
-}
-
-// One warp per block-row: the live slots, compacted in slot order.
-__global__ void __launch_bounds__(kThr) bell_mx_plan_kernel(const int32_t* __restrict__ cols, int32_t R, int32_t C,
-                                                           int32_t K, uint32_t* __restrict__ entries,
-                                                           int32_t* __restrict__ counts, int32_t* status) {
-  const int lane = threadIdx.x & 31;
-  const int r = int((int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5);
-  if (r >= R) return;
-  int n = 0, bad = 0;
-  for (int k0 = 0; k0 < K; k0 += 32) {
-    const int k = k0 + lane;
-    const int c = k < K ? cols[int64_t(r) * K + k] : -1;
-    const bool live = c >= 0 && c < C;
-    bad |= c < -1 || c >= C;
-    const uint32_t m = __ballot_sync(0xffffffffu, live);
-    if (live) entries[int64_t(r) * K + n + __popc(m & ((1u << lane) - 1u))] = uint32_t(c) | (uint32_t(k) << 16);
-    n += __popc(m);
-  }
-  for (int k = n + lane; k < K; k += 32) entries[int64_t(r) * K + k] = kNoSlot;
-  if (lane == 0) counts[r] = n;
-  if (bad) atomicOr(status, BELL_STATUS_COLIDX);
 }
 
 // Grid of grid-stride kernels: enough blocks for every SM's 2048 threads.
@@ -302,18 +331,27 @@ int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t tiles = int64_t(w->R) * w->K;
   unsigned grid;
-  if (int rc = mx::grid_for(tiles * w->B * (w->B / mx::kBlock), &grid)) return rc;
-  const int32_t in_out = w->layout == BELL_TILE_IN_OUT;
+  if (int rc = mx::grid_for(tiles * (w->B / 2) * (w->B / mx::kBlock), &grid)) return rc;
+  const mx::Plan p = mx::plan_of(plan, w->R, w->K);
+  mx::PackArgs a{};
+  a.tiles = tiles;
+  a.B = w->B;
+  a.in_out = w->layout == BELL_TILE_IN_OUT;
+  a.cols = w->col_indices;
+  a.R = w->R;
+  a.C = w->C;
+  a.K = w->K;
+  a.entries = const_cast<uint32_t*>(p.entries);
+  a.counts = const_cast<int32_t*>(p.counts);
+  a.status = st;
+  a.plan_blocks = unsigned((w->R + mx::kThr / 32 - 1) / (mx::kThr / 32));
+  grid += a.plan_blocks;
   uint8_t* dst = static_cast<uint8_t*>(chunks);
   if (dtype == BELL_DTYPE_BF16)
-    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const __nv_bfloat16*>(w->values), tiles, w->B, in_out, dst);
+    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const __nv_bfloat16*>(w->values), a, dst);
   else
-    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const float*>(w->values), tiles, w->B, in_out, dst);
-  if (int rc = check_launch("bell_mx_pack_kernel")) return rc;
-  const mx::Plan p = mx::plan_of(plan, w->R, w->K);
-  mx::bell_mx_plan_kernel<<<(w->R + mx::kThr / 32 - 1) / (mx::kThr / 32), mx::kThr, 0, s>>>(
-      w->col_indices, w->R, w->C, w->K, const_cast<uint32_t*>(p.entries), const_cast<int32_t*>(p.counts), st);
-  return check_launch("bell_mx_plan_kernel");
+    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const float*>(w->values), a, dst);
+  return check_launch("bell_mx_pack_kernel");
 }
 
 int bell_mx_unpack_tiles(const void* chunks0, int64_t tiles0, const void* chunks1, int64_t tiles1, int32_t B,

@@ -110,6 +110,25 @@ class BellMxFFNDesc(C.Structure):
                 ("status", C.c_void_p)]
 
 
+class BellMxLinearBwdDesc(C.Structure):
+    _fields_ = [("T", C.c_int64), ("grad_out", C.c_void_p), ("x", C.c_void_p), ("w", BellMxEll),
+                ("col_indices", C.c_void_p), ("cols_t", C.c_void_p), ("index_t", C.c_void_p), ("K_t", C.c_int32),
+                ("layout", C.c_int32), ("dx", C.c_void_p), ("dw", C.c_void_p), ("grad_dtype", C.c_int32),
+                ("reserved", C.c_int32), ("workspace", C.c_void_p), ("status", C.c_void_p)]
+
+
+class BellMxFFNBwdDesc(C.Structure):
+    _fields_ = [("T", C.c_int64), ("add_residual", C.c_int32), ("layout", C.c_int32), ("grad_out", C.c_void_p),
+                ("gate_pre", C.c_void_p), ("up_out", C.c_void_p), ("x", C.c_void_p), ("h", C.c_void_p),
+                ("gate", BellMxEll), ("up", BellMxEll), ("down", BellMxEll), ("cols_gate", C.c_void_p),
+                ("cols_up", C.c_void_p), ("cols_down", C.c_void_p), ("cols_t_down", C.c_void_p),
+                ("index_t_down", C.c_void_p), ("cols_t_gate_up", C.c_void_p), ("index_t_gate_up", C.c_void_p),
+                ("K_t_down", C.c_int32), ("K_t_gate_up", C.c_int32), ("dx", C.c_void_p), ("d_gate", C.c_void_p),
+                ("d_up", C.c_void_p), ("d_down", C.c_void_p), ("gate_dtype", C.c_int32), ("up_dtype", C.c_int32),
+                ("down_dtype", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
 # every exported symbol of include/bell.h: name -> (restype, argtypes)
 SIGNATURES = {
     "bell_abi_version": (C.c_int, []),
@@ -148,6 +167,10 @@ SIGNATURES = {
                                        C.c_void_p, C.c_void_p]),
     "bell_linear_mx": (C.c_int, [C.POINTER(BellMxLinearDesc), C.c_void_p]),
     "bell_swiglu_fwd_mx": (C.c_int, [C.POINTER(BellMxFFNDesc), C.c_void_p]),
+    "bell_linear_bwd_mx": (C.c_int, [C.POINTER(BellMxLinearBwdDesc), C.c_void_p]),
+    "bell_linear_bwd_mx_workspace_bytes": (C.c_size_t, [C.POINTER(BellMxLinearBwdDesc)]),
+    "bell_swiglu_bwd_mx": (C.c_int, [C.POINTER(BellMxFFNBwdDesc), C.c_void_p]),
+    "bell_swiglu_bwd_mx_workspace_bytes": (C.c_size_t, [C.POINTER(BellMxFFNBwdDesc)]),
     "bell_loop_fwd_bf16": (C.c_int, [C.POINTER(BellLoopDesc), C.c_void_p]),
     "bell_loop_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "bell_diag_injection_bf16": (C.c_int, [C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -34,11 +34,28 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .backward import block_ell_sddmm, down_silu_bwd, silu_mul_bwd, transposed_topology
-from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _prep_ell, _stream, block_ell_linear, plan_bytes
+from .backward import transposed_topology
+from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _prep_ell, plan_bytes
 
-_DTYPES = {torch.bfloat16: _lib.BELL_DTYPE_BF16, torch.float32: _lib.BELL_DTYPE_F32}
+_BF16, _F32 = _lib.BELL_DTYPE_BF16, _lib.BELL_DTYPE_F32
+_DTYPES = {torch.bfloat16: _BF16, torch.float32: _F32}
 _ROWS = 128  # tokens of one chunk of quantised rows
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """Library entry point `name` on the current stream of `dev`."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _bytes(n: int, dev: torch.device) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=dev)
 
 
 def _check_tile(tile: int) -> None:
@@ -66,8 +83,7 @@ class MXRows:
 @dataclass
 class MXBlockELL:
     """A quantised Block-ELL weight (``make_mxfp4``)."""
-    data: torch.Tensor         # uint8: the quantised tiles, operand layout
-    plan: torch.Tensor         # uint8: live slots of each block-row
+    data: torch.Tensor         # uint8: the quantised tiles, operand layout, then the plan of the live slots
     col_indices: torch.Tensor  # int32 [R, K]
     R: int
     K: int
@@ -75,7 +91,8 @@ class MXBlockELL:
     B: int
 
     def __post_init__(self):
-        self._abi = _lib.BellMxEll(self.data.data_ptr(), self.plan.data_ptr(), self.R, self.C, self.K, self.B)
+        at = self.data.data_ptr()
+        self._abi = _lib.BellMxEll(at, at + _tiles_bytes(self.R, self.K, self.B), self.R, self.C, self.K, self.B)
 
     @property
     def in_features(self) -> int:
@@ -87,8 +104,14 @@ class MXBlockELL:
 
     def dequantize(self, layout: int = TILE_IN_OUT) -> torch.Tensor:
         """The quantised values as bf16 tiles ``[R, K, B, B]`` (dead slots too)."""
-        v = _unpack((self,), None, self.R * self.K).view(self.R, self.K, self.B, self.B)
+        n, dev = self.R * self.K, self.data.device
+        v = torch.empty((self.R, self.K, self.B, self.B), dtype=torch.bfloat16, device=dev)
+        _call("bell_mx_unpack_tiles", dev, self._abi.chunks, n, None, 0, self.B, None, n, v.data_ptr())
         return v if layout == TILE_OUT_IN else v.transpose(-1, -2).contiguous()
+
+
+def _tiles_bytes(R: int, K: int, B: int) -> int:
+    return R * K * (B * B // 2 + 512)
 
 
 def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
@@ -101,10 +124,8 @@ def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
         raise RuntimeError(f"{name} must be bf16 or fp32")
     per16 = 16 // x.element_size()
     T, f = x.shape
-    if x.is_contiguous() and f % per16 == 0:
-        ok = x.data_ptr() % 16 == 0
-    else:
-        ok = x.stride(1) == 1 and (T < 2 or (x.stride(0) >= f and x.stride(0) % per16 == 0)) and x.data_ptr() % 16 == 0
+    ok = x.data_ptr() % 16 == 0 and x.stride(1) == 1 and \
+        (x.stride(0) >= f and x.stride(0) % per16 == 0 or T < 2 and f % per16 == 0)
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
@@ -120,10 +141,9 @@ def mxfp4_quantize(x: torch.Tensor, tile: int = 128) -> MXRows:
     T, f = x.shape
     if f % tile or f == 0:
         raise RuntimeError(f"features={f} is not a multiple of the tile size {tile}")
-    data = torch.empty(_rows_bytes(T, f, tile), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().bell_mx_quantize_rows(T, f, tile, _DTYPES[x.dtype], x.data_ptr(), _ld(x),
-                                                     data.data_ptr(), _stream()), "mxfp4_quantize")
+    dev = x.device
+    data = _bytes(_rows_bytes(T, f, tile), dev)
+    _call("bell_mx_quantize_rows", dev, T, f, tile, _DTYPES[x.dtype], x.data_ptr(), _ld(x), data.data_ptr())
     return MXRows(data, T, f, tile)
 
 
@@ -132,20 +152,22 @@ def mxfp4_dequantize(q: MXRows, dtype: torch.dtype = torch.bfloat16, out: Option
     _check_rows(q)
     if dtype not in _DTYPES:
         raise RuntimeError("dtype must be bf16 or fp32")
+    dev = q.data.device
     if out is None:
-        out = torch.empty((q.T, q.features), dtype=dtype, device=q.data.device)
+        out = torch.empty((q.T, q.features), dtype=dtype, device=dev)
     else:
-        _check_out("out", out, (q.T, q.features), dtype, q.data.device)
-    with torch.cuda.device(q.data.device):
-        _lib.check(_lib.load().bell_mx_dequantize_rows(q.T, q.features, q.tile, q.data.data_ptr(), _DTYPES[dtype],
-                                                       out.data_ptr(), q.features, _stream()), "mxfp4_dequantize")
+        _check_out("out", out, (q.T, q.features), dtype, dev)
+    _call("bell_mx_dequantize_rows", dev, q.T, q.features, q.tile, q.data.data_ptr(), _DTYPES[dtype], out.data_ptr(),
+          q.features)
     return out
 
 
 def _check_rows(q: MXRows) -> None:
-    _check_cuda("quantised rows", q.data)
-    if q.data.numel() < _rows_bytes(q.T, q.features, q.tile) or q.data.dtype != torch.uint8 or \
-            not q.data.is_contiguous():
+    data = q.data
+    _check_cuda("quantised rows", data)
+    _check_tile(q.tile)
+    if q.T < 0 or q.features < 1 or q.features % q.tile or data.dtype != torch.uint8 or not data.is_contiguous() or \
+            data.numel() < _rows_bytes(q.T, q.features, q.tile):
         raise RuntimeError("MXRows.data does not hold T x features quantised values")
 
 
@@ -153,78 +175,50 @@ def make_mxfp4(values: torch.Tensor, col_indices: torch.Tensor, C_blocks: int, l
     """Quantise the tiles of a Block-ELL weight (``values [R, K, B, B]`` bf16 or
     fp32, B 64 or 128) and list its live slots.  A column index of -1 is a dead
     slot; one outside [0, C_blocks) is dropped and sets the status word."""
-    if values.dtype not in _DTYPES:
+    dtype = values.dtype
+    if dtype not in _DTYPES:
         raise RuntimeError("tiles must be bf16 or fp32")
-    v, cols = _prep_ell("weight", values, col_indices, values.dtype)
+    v, cols = _prep_ell("weight", values, col_indices, dtype)
     R, K, B, B2 = v.shape
     _check_tile(B)
     if B2 != B or tuple(cols.shape) != (R, K):
         raise RuntimeError(f"values {tuple(v.shape)} and col_indices {tuple(cols.shape)} do not fit")
-    if cols.device != v.device:
+    dev = v.device
+    if cols.device != dev:
         raise RuntimeError("values and col_indices must be on one device")
-    data = torch.empty(R * K * (B * B // 2 + 512), dtype=torch.uint8, device=v.device)
-    plan = torch.empty(plan_bytes(0, 0, 0, R, K), dtype=torch.uint8, device=v.device)
+    n = _tiles_bytes(R, K, B)
+    data = _bytes(n + plan_bytes(0, 0, 0, R, K), dev)
     w = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, int(C_blocks), K, B, layout, 0)
-    with torch.cuda.device(v.device):
-        _lib.check(_lib.load().bell_mx_pack_ell(C.byref(w), _DTYPES[v.dtype], data.data_ptr(), plan.data_ptr(), None,
-                                                _stream()), "make_mxfp4")
-    return MXBlockELL(data, plan, cols, R, K, int(C_blocks), B)
+    _call("bell_mx_pack_ell", dev, C.byref(w), _DTYPES[dtype], data.data_ptr(), data.data_ptr() + n, None)
+    return MXBlockELL(data, cols, R, K, int(C_blocks), B)
 
 
-def _unpack(weights, index: Optional[torch.Tensor], n: int) -> torch.Tensor:
-    """bf16 tiles ``[n, B_out, B_in]`` of one or two stacked weights, gathered by ``index``."""
-    w0 = weights[0]
-    w1 = weights[1] if len(weights) > 1 else None
-    out = torch.empty((n, w0.B, w0.B), dtype=torch.bfloat16, device=w0.data.device)
-    with torch.cuda.device(w0.data.device):
-        _lib.check(_lib.load().bell_mx_unpack_tiles(
-            w0.data.data_ptr(), w0.R * w0.K, w1.data.data_ptr() if w1 is not None else None,
-            w1.R * w1.K if w1 is not None else 0, w0.B, index.data_ptr() if index is not None else None, n,
-            out.data_ptr(), _stream()), "mxfp4 unpack")
-    return out
+def _check_weight(w: MXBlockELL, dev: torch.device) -> None:
+    if w.data.device != dev:
+        raise RuntimeError(f"weight is on {w.data.device}, x on {dev}")
 
 
-def _same_device(dev, *weights) -> None:
-    for w in weights:
-        if w.data.device != dev:
-            raise RuntimeError(f"weight is on {w.data.device}, x on {dev}")
-
-
-def _source(desc, x, tile: int, features: int):
-    """Point ``desc`` at the rows of x (quantised already, or to be quantised
-    into a workspace); returns (T, device, output dtype, the rows' buffer)."""
+def _source(x, tile: int, features: int):
+    """The rows a product reads: (T, device, output dtype, address of rows to
+    quantise or None, their stride and type), for x quantised already or not."""
     if isinstance(x, MXRows):
         _check_rows(x)
         if x.tile != tile or x.features != features:
             raise RuntimeError(f"quantised rows of {x.features} features, tile {x.tile}; the weight needs {features}, "
                                f"tile {tile}")
-        desc.x = x.data.data_ptr()
-        return x.T, x.data.device, torch.bfloat16, x.data
-    T, f = x.shape
-    if f != features:
-        raise RuntimeError(f"x has {f} features, the weight {features}")
-    buf = torch.empty(_rows_bytes(T, f, tile), dtype=torch.uint8, device=x.device)
-    desc.x, desc.x_src, desc.ld_src, desc.src_dtype = buf.data_ptr(), x.data_ptr(), _ld(x), _DTYPES[x.dtype]
-    return T, x.device, x.dtype, buf
+        return x.T, x.data.device, torch.bfloat16, None, 0, 0
+    if x.shape[1] != features:
+        raise RuntimeError(f"x has {x.shape[1]} features, the weight {features}")
+    return x.shape[0], x.device, x.dtype, x.data_ptr(), _ld(x), _DTYPES[x.dtype]
 
 
-def _out_and_residual(desc, T, features, dtype, dev, out, out_dtype, residual):
-    out_dtype = out_dtype or dtype
-    if out_dtype not in _DTYPES:
-        raise RuntimeError("out_dtype must be bf16 or fp32")
-    if out is None:
-        out = torch.empty((T, features), dtype=out_dtype, device=dev)
-    else:
-        _check_out("out", out, (T, features), out_dtype, dev)
-    if residual is not None:
-        _check_cuda("residual", residual)
-        if tuple(residual.shape) != (T, features) or residual.dtype != out_dtype or residual.device != dev:
-            raise RuntimeError(f"residual must be {out_dtype} {(T, features)} on {dev}, as the output")
-        if not residual.is_contiguous() or residual.data_ptr() % 16:
-            residual = residual.clone(memory_format=torch.contiguous_format)
-        desc.residual = residual.data_ptr()
-    desc.T, desc.out, desc.out_dtype = T, out.data_ptr(), _DTYPES[out_dtype]
-    return out, residual
+def _check_residual(residual, shape, dtype, dev) -> torch.Tensor:
+    _check_cuda("residual", residual)
+    if tuple(residual.shape) != shape or residual.dtype != dtype or residual.device != dev:
+        raise RuntimeError(f"residual must be {dtype} {shape} on {dev}, as the output")
+    if not residual.is_contiguous() or residual.data_ptr() % 16:
+        residual = residual.clone(memory_format=torch.contiguous_format)
+    return residual
 
 
 def mxfp4_linear(x: Union[torch.Tensor, MXRows], w: MXBlockELL, residual: Optional[torch.Tensor] = None,
@@ -242,13 +236,22 @@ def mxfp4_linear(x: Union[torch.Tensor, MXRows], w: MXBlockELL, residual: Option
 def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0):
     if not isinstance(x, MXRows):
         x = _rows_2d("x", x)
-    d = _lib.BellMxLinearDesc()
-    T, dev, dtype, rows = _source(d, x, w.B, w.C * w.B)
-    _same_device(dev, w)
-    out, residual = _out_and_residual(d, T, w.R * w.B, dtype, dev, out, out_dtype, residual)
-    d.w, d.max_ctas = w._abi, int(max_ctas)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().bell_linear_mx(C.byref(d), _stream()), "mxfp4_linear")
+    in_f, out_f = w.C * w.B, w.R * w.B
+    T, dev, dtype, src, ld, src_type = _source(x, w.B, in_f)
+    _check_weight(w, dev)
+    dtype = out_dtype or dtype
+    if dtype not in _DTYPES:
+        raise RuntimeError("out_dtype must be bf16 or fp32")
+    if out is None:
+        out = torch.empty((T, out_f), dtype=dtype, device=dev)
+    else:
+        _check_out("out", out, (T, out_f), dtype, dev)
+    if residual is not None:
+        residual = _check_residual(residual, (T, out_f), dtype, dev)
+    rows = x.data if src is None else _bytes(_rows_bytes(T, in_f, w.B), dev)
+    d = _lib.BellMxLinearDesc(T, _DTYPES[dtype], int(max_ctas), rows.data_ptr(), src, ld, src_type, 0,
+                              None if residual is None else residual.data_ptr(), out.data_ptr(), w._abi, None)
+    _call("bell_linear_mx", dev, C.byref(d))
     return out, rows
 
 
@@ -262,81 +265,88 @@ def mxfp4_swiglu_fwd(x: Union[torch.Tensor, MXRows], gate: MXBlockELL, up: MXBlo
     ``add_residual``).  ``return_intermediates`` returns ``(out, ws)``, ``ws``
     with the quantised rows ``q_x`` and ``q_h`` (``MXRows``) and the bf16
     projections ``gate`` and ``up``."""
-    if not isinstance(x, MXRows):
+    quantised = isinstance(x, MXRows)
+    if not quantised:
         x = _rows_2d("x", x)
-    if gate.R != up.R or gate.C != up.C or gate.B != up.B:
+    B, R, Cm = gate.B, gate.R, gate.C
+    if R != up.R or Cm != up.C or B != up.B:
         raise RuntimeError("gate and up must have the same R, C and tile size")
-    if down.B != gate.B or down.C != gate.R or down.R != gate.C:
+    if down.B != B or down.C != R or down.R != Cm:
         raise RuntimeError("down must map d_ff back to d_model at the tile size of gate and up")
-    d = _lib.BellMxFFNDesc()
-    B, F = gate.B, gate.R * gate.B
-    T, dev, dtype, rows = _source(d, x, B, gate.C * B)
-    _same_device(dev, gate, up, down)
-    if add_residual and residual is None:
-        if isinstance(x, MXRows):
-            raise RuntimeError("add_residual on quantised rows needs the residual")
-        residual = x
-    out, residual = _out_and_residual(d, T, down.R * B, dtype, dev, None, None, residual if add_residual else None)
-    h = torch.empty(_rows_bytes(T, F, B), dtype=torch.uint8, device=dev)
-    d.h = h.data_ptr()
+    D, F = Cm * B, R * B
+    T, dev, dtype, src, ld, src_type = _source(x, B, D)
+    for w in (gate, up, down):
+        _check_weight(w, dev)
+    if not add_residual:
+        residual = None
+    else:
+        if residual is None:
+            if quantised:
+                raise RuntimeError("add_residual on quantised rows needs the residual")
+            residual = x
+        residual = _check_residual(residual, (T, D), dtype, dev)
+    out = torch.empty((T, D), dtype=dtype, device=dev)
+    n_x, n_h = 0 if quantised else _rows_bytes(T, D, B), _rows_bytes(T, F, B)
+    ws = _bytes(n_x + n_h, dev)  # the quantised rows of x, then of h
+    at = ws.data_ptr()
     g = u = None
     if return_intermediates:
         g, u = (torch.empty((T, F), dtype=torch.bfloat16, device=dev) for _ in range(2))
-        d.gate_pre, d.up_out = g.data_ptr(), u.data_ptr()
-    d.gate, d.up, d.down, d.max_ctas = gate._abi, up._abi, down._abi, int(max_ctas)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().bell_swiglu_fwd_mx(C.byref(d), _stream()), "mxfp4_swiglu_fwd")
+    d = _lib.BellMxFFNDesc(T, _DTYPES[dtype], int(max_ctas), x.data.data_ptr() if quantised else at, src, ld, src_type, 0,
+                           None if residual is None else residual.data_ptr(), at + n_x,
+                           None if g is None else g.data_ptr(), None if u is None else u.data_ptr(), out.data_ptr(),
+                           gate._abi, up._abi, down._abi, None)
+    _call("bell_swiglu_fwd_mx", dev, C.byref(d))
     if return_intermediates:
-        return out, dict(q_x=MXRows(rows, T, gate.C * B, B), q_h=MXRows(h, T, F, B), gate=g, up=u)
+        return out, dict(q_x=x if quantised else MXRows(ws[:n_x], T, D, B), q_h=MXRows(ws[n_x:], T, F, B), gate=g, up=u)
     return out
 
 
 # ----------------------------------------------------------------- training
 
 
-def _transposed(weights, cols, C_blocks: int):
-    """bf16 tiles and columns of the transpose of the stacked quantised weights.
-    The tiles come out [B_out, B_in], which the transpose reads as [B_in, B_out]."""
-    cols_t, index = transposed_topology(cols, C_blocks)
-    B = weights[0].B
-    return _unpack(weights, index.reshape(-1), index.numel()).view(*index.shape, B, B), cols_t
-
-
-def _like_master(grad: torch.Tensor, bf16: Optional[torch.Tensor], master: torch.Tensor) -> torch.Tensor:
-    return bf16 if bf16 is not None else grad.to(master.dtype)
-
-
-def _tile_grad(a, b, cols, B, layout, dtype):
-    """Tile gradient in the master's dtype (the bf16 copy is written by the same launch)."""
-    R, K = cols.shape
-    half = torch.empty((R, K, B, B), dtype=torch.bfloat16, device=a.device) if dtype == torch.bfloat16 else None
-    full = block_ell_sddmm(a, b, cols, B, layout, out_bf16=half)
-    return full if half is None else half
+def _grad(need: bool, cols: torch.Tensor, B: int, dtype: torch.dtype):
+    """Buffer of a tile gradient (bf16 for bf16 tiles, else fp32), its address and type."""
+    if not need:
+        return None, None, _BF16
+    kind = torch.bfloat16 if dtype == torch.bfloat16 else torch.float32
+    g = torch.empty((*cols.shape, B, B), dtype=kind, device=cols.device)
+    return g, g.data_ptr(), _DTYPES[kind]
 
 
 class MXLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, values, cols, residual, layout):
         w = make_mxfp4(values, cols, x.shape[1] // values.shape[2], layout)
-        x2 = _rows_2d("x", x)
-        y, rows = _linear(x2, w, residual)
-        ctx.w, ctx.rows, ctx.layout = w, MXRows(rows, x.shape[0], x.shape[1], w.B), layout
-        ctx.save_for_backward(cols)
+        y, rows = _linear(x, w, residual)
+        ctx.w, ctx.layout = w, layout
+        ctx.save_for_backward(cols, w.data, rows)
         ctx.dtypes = (x.dtype, values.dtype)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        w, (cols,) = ctx.w, ctx.saved_tensors
+        w, (cols, _, rows) = ctx.w, ctx.saved_tensors
         x_dtype, v_dtype = ctx.dtypes
         dyb = dy.to(torch.bfloat16).contiguous()
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            vt, ct = _transposed((w,), [cols], w.C)
-            dx = block_ell_linear(dyb, vt, ct, layout=TILE_IN_OUT).to(x_dtype)
-        if ctx.needs_input_grad[1]:
-            dw = _tile_grad(ctx.rows.dequantize(), dyb, w.col_indices, w.B, ctx.layout, v_dtype)
-        return dx, dw, None, dy if ctx.needs_input_grad[3] else None, None
+        T, dev = dyb.shape[0], dyb.device
+        need = ctx.needs_input_grad
+        dx = dx_at = cols_t = index_t = None
+        K_t = 1
+        if need[0]:
+            cols_t, index_t = transposed_topology([cols], w.C)
+            K_t = cols_t.shape[1]
+            dx = torch.empty((T, w.C * w.B), dtype=torch.bfloat16, device=dev)
+            dx_at = dx.data_ptr()
+        dw, dw_at, kind = _grad(need[1], w.col_indices, w.B, v_dtype)
+        d = _lib.BellMxLinearBwdDesc(T, dyb.data_ptr(), rows.data_ptr(), w._abi, w.col_indices.data_ptr(),
+                                     None if cols_t is None else cols_t.data_ptr(),
+                                     None if index_t is None else index_t.data_ptr(), K_t, ctx.layout, dx_at, dw_at,
+                                     kind, 0, None, None)
+        ws = _bytes(_lib.load().bell_linear_bwd_mx_workspace_bytes(C.byref(d)), dev)
+        d.workspace = ws.data_ptr()
+        _call("bell_linear_bwd_mx", dev, C.byref(d))
+        return (None if dx is None else dx.to(x_dtype)), dw, None, dy if need[3] else None, None
 
 
 def mxfp4_linear_ad(x: torch.Tensor, values: torch.Tensor, cols: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -355,49 +365,41 @@ def mxfp4_linear_ad(x: torch.Tensor, values: torch.Tensor, cols: torch.Tensor, r
 class MXSwiGLUFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, v_gate, ci_gate, v_up, ci_up, v_down, ci_down, add_residual, layout):
-        B = v_gate.shape[2]
-        C_model, R_ff = x.shape[1] // B, v_gate.shape[0]
+        C_model, R_ff = x.shape[1] // v_gate.shape[2], v_gate.shape[0]
         gate, up = make_mxfp4(v_gate, ci_gate, C_model, layout), make_mxfp4(v_up, ci_up, C_model, layout)
         down = make_mxfp4(v_down, ci_down, R_ff, layout)
         out, ws = mxfp4_swiglu_fwd(x, gate, up, down, add_residual=add_residual, return_intermediates=True)
-        ctx.weights, ctx.q = (gate, up, down), (ws["q_x"], ws["q_h"])
-        ctx.save_for_backward(ws["gate"], ws["up"], ci_gate, ci_up, ci_down)
+        ctx.weights = (gate, up, down)
+        ctx.save_for_backward(ws["gate"], ws["up"], ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down, gate.data,
+                              up.data, down.data)
         ctx.add_residual, ctx.layout = bool(add_residual), layout
         ctx.dtypes = (x.dtype, v_gate.dtype, v_up.dtype, v_down.dtype)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        g, u, ci_gate, ci_up, ci_down = ctx.saved_tensors
-        (gate, up, down), (q_x, q_h), layout = ctx.weights, ctx.q, ctx.layout
-        x_dtype, *v_dtypes = ctx.dtypes
-        B, F = gate.B, gate.R * gate.B
+        g, u, q_x, q_h, ci_gate, ci_up, ci_down, *_ = ctx.saved_tensors
+        gate, up, down = ctx.weights
         dy = grad_out.to(torch.bfloat16).contiguous()
-        T = dy.shape[0]
+        T, dev = dy.shape[0], dy.device
         need = ctx.needs_input_grad
-        dx = d_gate = d_up = d_down = dgu = None
-        if need[0] or need[1] or need[3]:
-            if T > 0:
-                vt, ct = _transposed((down,), [ci_down], gate.R)
-                # as the bf16 backward: one kernel for d_h and the SiLU backward at tile 64, two at 128
-                if B == 64:
-                    dgu = down_silu_bwd(dy, vt, ct, TILE_IN_OUT, g, u)
-                else:
-                    dgu = silu_mul_bwd(block_ell_linear(dy, vt, ct, layout=TILE_IN_OUT), g, u)
-            else:
-                dgu = torch.empty((0, 2 * F), dtype=torch.bfloat16, device=dy.device)
-        if need[0]:
-            vt, ct = _transposed((gate, up), [ci_gate, ci_up], gate.C)
-            dx = block_ell_linear(dgu, vt, ct, residual=dy if ctx.add_residual else None, layout=TILE_IN_OUT).to(x_dtype)
-        if need[1] or need[3]:
-            xq = q_x.dequantize()
-            if need[1]:
-                d_gate = _tile_grad(xq, dgu[:, :F], gate.col_indices, B, layout, v_dtypes[0])
-            if need[3]:
-                d_up = _tile_grad(xq, dgu[:, F:], up.col_indices, B, layout, v_dtypes[1])
-        if need[5]:
-            d_down = _tile_grad(q_h.dequantize(), dy, down.col_indices, B, layout, v_dtypes[2])
-        return dx, d_gate, None, d_up, None, d_down, None, None, None
+        td_cols, td_index = transposed_topology([ci_down], gate.R)
+        tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
+        dx = torch.empty_like(dy) if need[0] else None
+        cols = (gate.col_indices, up.col_indices, down.col_indices)
+        grads = [_grad(n, c, gate.B, t) for n, c, t in zip((need[1], need[3], need[5]), cols, ctx.dtypes[1:])]
+        d = _lib.BellMxFFNBwdDesc(
+            T, int(ctx.add_residual), ctx.layout, dy.data_ptr(), g.data_ptr(), u.data_ptr(), q_x.data_ptr(),
+            q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
+            td_cols.data_ptr(), td_index.data_ptr(), tg_cols.data_ptr(), tg_index.data_ptr(), td_cols.shape[1],
+            tg_cols.shape[1], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
+            grads[1][2], grads[2][2], 0, None, None)
+        ws = _bytes(_lib.load().bell_swiglu_bwd_mx_workspace_bytes(C.byref(d)), dev)
+        d.workspace = ws.data_ptr()
+        _call("bell_swiglu_bwd_mx", dev, C.byref(d))
+        if dx is not None:
+            dx = dx.to(ctx.dtypes[0])
+        return dx, grads[0][0], None, grads[1][0], None, grads[2][0], None, None, None
 
 
 def mxfp4_swiglu(x: torch.Tensor, v_gate: torch.Tensor, ci_gate: torch.Tensor, v_up: torch.Tensor, ci_up: torch.Tensor,

@@ -154,3 +154,29 @@ def test_python_refuses_what_is_not_on_a_gpu_or_does_not_fit():
         K.mxfp4_swiglu(x, v[0], c, v, c, v, c)
     with pytest.raises(RuntimeError, match="not a multiple"):
         K.mxfp4_swiglu(x[:, :100], v, c, v, c, v, c)
+
+
+def test_backward_refusals():
+    L = _L()
+    lib = L.load()
+    assert lib.bell_linear_bwd_mx(None, None) == -8 and lib.bell_swiglu_bwd_mx(None, None) == -8
+    assert lib.bell_linear_bwd_mx_workspace_bytes(None) == 0 and lib.bell_swiglu_bwd_mx_workspace_bytes(None) == 0
+    d = L.BellMxLinearBwdDesc()
+    d.T, d.grad_out, d.x, d.w = 4, 1024, 1024, _mx(L, 2, 3)
+    d.workspace = 1024
+    d.dx = 1024
+    assert lib.bell_linear_bwd_mx(C.byref(d), None) == -8 and "transposed" in L.last_error()
+    d.dx, d.dw, d.col_indices, d.grad_dtype = None, 1024, 1024, 5
+    assert lib.bell_linear_bwd_mx(C.byref(d), None) == -8
+    d.grad_dtype, d.workspace = 0, None
+    assert lib.bell_linear_bwd_mx(C.byref(d), None) == -3
+    d.K_t = 1
+    # unpacked transpose [3, 1] tiles + plan + Q(x) + fp32 sums of [2, 2] tiles, each padded to 256 bytes
+    assert lib.bell_linear_bwd_mx_workspace_bytes(C.byref(d)) == 3 * 64 * 64 * 2 + 256 + 4 * 192 * 2 + 4 * 64 * 64 * 4
+    f = L.BellMxFFNBwdDesc()
+    f.T, f.gate, f.up, f.down = 4, _mx(L, 4, 2), _mx(L, 4, 2), _mx(L, 2, 4)
+    f.grad_out = f.gate_pre = f.up_out = f.x = f.h = f.workspace = 1024
+    assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -8 and "topologies" in L.last_error()
+    assert lib.bell_swiglu_bwd_mx_workspace_bytes(C.byref(f)) == 0
+    f.up = _mx(L, 4, 3)
+    assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -2

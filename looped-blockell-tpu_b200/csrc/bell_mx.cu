@@ -25,7 +25,12 @@
 // one 32-column block of a unit; at B = 64, two blocks, two groups of eight
 // warps take the CTA's units in turn), 20 and 21 issuers (20 owns TMEM).
 // Accumulators form a ring of ACCS in job order, so the issuers run ahead of the
-// epilogue.  The TMEM scale
+// epilogue.
+//
+// Few units (a linear of few tokens): split mode.  A cluster of `split` CTAs
+// shares one unit, each ring of each CTA takes an equal range of the stages
+// into an accumulator of its own, and the partial sums meet in distributed
+// shared memory, in a fixed order.  The TMEM scale
 // columns belong to the stage: a stage is refilled only after its MMAs have
 // completed, so the scales of MMAs in flight are never overwritten.
 // Token-major, because a lane of the epilogue then holds 32 consecutive
@@ -34,6 +39,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <atomic>
 #include <climits>
 #include <string>
 
@@ -76,6 +83,8 @@ struct Params {
   void* out;                      // linear [T, R*B]
   const void* residual;           // linear, optional, out's type
   int32_t out_f32;
+  int32_t split;                  // linear: CTAs sharing a unit (0: persistent, whole units)
+  int32_t early;                  // weights, plan and residual were complete before the kernel ahead
   int32_t* status;
   uint64_t timeout_ns;
 };
@@ -105,15 +114,26 @@ __device__ __forceinline__ Smem carve(uint8_t* raw) {
 }
 
 // The CTA's units are blockIdx.x + i * gridDim.x; ring k's job i is unit i of
-// matrix k (gated) or unit 2i + k (linear).
-template <bool GATED>
-__device__ __forceinline__ int ring_jobs(const Params& p, int k) {
-  const int units = p.mtiles * p.R, first = int(blockIdx.x), grid = int(gridDim.x);
-  const int mine = first < units ? (units - first + grid - 1) / grid : 0;
-  return GATED ? mine : (mine - k + 1) / 2;
+// matrix k (gated) or unit 2i + k (linear).  In split mode a ring has one job,
+// stages [first, first + stages) of the cluster's unit.
+struct RingWork {
+  int jobs, first, stages;
+};
+template <int B, bool GATED>
+__device__ __forceinline__ RingWork ring_work(const Params& p, int k) {
+  const int K = GATED && k ? p.K1 : p.K0;
+  const int all = (K + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS;
+  if (!GATED && p.split) {
+    const int part = int(blockIdx.x) % p.split * 2 + k, each = (all + 2 * p.split - 1) / (2 * p.split);
+    return {1, part * each, max(0, min(each, all - part * each))};
+  }
+  const int units = p.mtiles * p.R, grid = int(gridDim.x);
+  const int mine = int(blockIdx.x) < units ? (units - int(blockIdx.x) + grid - 1) / grid : 0;
+  return {GATED ? mine : (mine - k + 1) / 2, 0, all};
 }
 template <bool GATED>
-__device__ __forceinline__ int job_unit(int i, int k) {
+__device__ __forceinline__ int job_unit(const Params& p, int i, int k) {
+  if (!GATED && p.split) return int(blockIdx.x) / p.split;
   return int(blockIdx.x) + (GATED ? i : 2 * i + k) * int(gridDim.x);
 }
 
@@ -128,62 +148,105 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   const int K = mat ? p.K1 : p.K0;
   const uint8_t* w = mat ? p.w1 : p.w0;
   const uint32_t* entries = (mat ? p.p1 : p.p0).entries;
-  const int per_job = (K + G::SLOTS - 1) / G::SLOTS;
-  const int jobs = ring_jobs<GATED>(p, ring);
+  const RingWork rw = ring_work<B, GATED>(p, ring);
   uint64_t* full = s.full + ring * G::NR;
   uint64_t* empty = s.empty + ring * G::NR;
-  int job = sub / per_job, part = sub % per_job;  // of the next use
-  int m = 0, r = 0;
-  // this producer's next use's entries travel while the one before is issued
-  auto fetch = [&]() -> uint32_t {
-    const int u = job_unit<GATED>(job, ring);
-    m = u / p.R;
-    r = u - m * p.R;
-    const int k = part * G::SLOTS + lane;
-    return lane < G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
-  };
-  uint32_t e_next = job < jobs ? fetch() : kNoSlot;
-  uint32_t stage = uint32_t(sub), phase = 0;
-  bool ok = true;
-  int64_t filled = 0;
-  while (job < jobs) {
-    const uint32_t e = e_next;
-    const uint8_t* xm = p.x + int64_t(m) * p.C * G::A;
-    const uint8_t* wr = w + int64_t(r) * K * G::W;
-    part += 2;
-    while (part >= per_job) {
-      part -= per_job;
+  uint32_t* count = s.count + ring * G::NR;
+  uint8_t* stages = s.stages + ring * (G::NR * G::STAGE);
+  int job = 0, part = sub, left = rw.stages > 0 ? rw.jobs : 0;  // of the next use
+  auto settle = [&] {
+    while (part >= rw.stages && job < left) {
+      part -= rw.stages;
       ++job;
     }
-    if (job < jobs) e_next = fetch();
-    ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, ctl));
-    if (!ok) break;
-    const int cnt = __popc(__ballot_sync(0xffffffffu, e != kNoSlot));
-    uint8_t* st = s.stages + (ring * G::NR + int(stage)) * G::STAGE;
+  };
+  settle();
+  // A use's entries (lane i: slot i of the stage) and where its chunks are.
+  struct Use {
+    uint32_t e;
+    const uint8_t *x, *w;
+  };
+  auto fetch = [&]() -> Use {
+    const int u = job_unit<GATED>(p, job, ring);
+    const int m = u / p.R, r = u - m * p.R;
+    const int k = (rw.first + part) * G::SLOTS + lane;
+    const uint32_t e = lane < G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
+    return {e, p.x + int64_t(m) * p.C * G::A, w + int64_t(r) * K * G::W};
+  };
+  auto advance = [&] {
+    part += 2;
+    settle();
+  };
+  auto copies = [&](const Use& use, uint32_t stage, bool weights, bool rows) {
+    const int cnt = __popc(__ballot_sync(0xffffffffu, use.e != kNoSlot));
     uint32_t ent[G::SLOTS];
 #pragma unroll
-    for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, e, i);
+    for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, use.e, i);
     if (elect_one()) {
-      s.count[ring * G::NR + stage] = uint32_t(cnt);
-      if (cnt)
-        mbar_arrive_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::SLOT));
-      else
-        mbar_arrive(&full[stage]);
+      uint8_t* st = stages + stage * uint32_t(G::STAGE);
+      if (weights) {
+        count[stage] = uint32_t(cnt);
+        if (cnt)
+          mbar_arrive_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::SLOT));
+        else
+          mbar_arrive(&full[stage]);
+      }
 #pragma unroll
       for (int i = 0; i < G::SLOTS; ++i) {
         if (i < cnt) {
-          bulk_load(st + i * G::SLOT, xm + int64_t(ent[i] & 0xFFFFu) * G::A, G::A, &full[stage], pass);
-          bulk_load(st + i * G::SLOT + G::A, wr + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
+          if (rows) bulk_load(st + i * G::SLOT, use.x + int64_t(ent[i] & 0xFFFFu) * G::A, G::A, &full[stage], pass);
+          if (weights)
+            bulk_load(st + i * G::SLOT + G::A, use.w + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
         }
       }
     }
     __syncwarp();
+  };
+  uint32_t stage = uint32_t(sub), phase = 0;
+  int64_t filled = 0;
+  auto turn = [&] {
     ++filled;
     stage += 2;
     if (stage >= uint32_t(G::NR)) {
       stage -= G::NR;
       phase ^= 1u;
     }
+  };
+  // The ring's first filling: the weights need not wait for the kernel ahead,
+  // which makes the rows.
+  if (p.early) {
+    Use first[(G::NR + 1) / 2];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < (G::NR + 1) / 2; ++i) {
+      if (sub + 2 * i < G::NR && job < left) {
+        first[i] = fetch();
+        advance();
+        copies(first[i], uint32_t(sub + 2 * i), true, false);
+        n = i + 1;
+      }
+    }
+    griddep_wait();
+#pragma unroll
+    for (int i = 0; i < (G::NR + 1) / 2; ++i) {
+      if (i < n) {
+        copies(first[i], uint32_t(sub + 2 * i), false, true);
+        turn();
+      }
+    }
+  }
+  // from here each use's entries travel while the one before is issued
+  Use next{kNoSlot, nullptr, nullptr};
+  if (job < left) next = fetch();
+  bool ok = true;
+  while (job < left) {
+    const Use use = next;
+    advance();
+    if (job < left) next = fetch();
+    ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, ctl));
+    if (!ok) break;
+    copies(use, stage, true, true);
+    turn();
   }
   if (!ok && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
     for (int i = 0; i < G::NR && filled > 0; ++i, --filled) {
@@ -208,21 +271,19 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
   const bool leader = elect_one();
   const uint32_t a0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 128);
   const uint32_t sf0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 16);
-  const int K = GATED && ring ? p.K1 : p.K0;
-  const int per_job = (K + G::SLOTS - 1) / G::SLOTS;
-  const int jobs = ring_jobs<GATED>(p, ring);
+  const RingWork rw = ring_work<B, GATED>(p, ring);
   uint64_t* full = s.full + ring * G::NR;
   uint64_t* empty = s.empty + ring * G::NR;
   uint32_t stage = 0, phase = 0;
   uint32_t acc = uint32_t(ring), use = 0;  // job 2i + ring of the CTA: accumulator (2i + ring) % ACCS
   bool ok = true;
-  for (int i = 0; i < jobs && ok; ++i) {
+  for (int i = 0; i < rw.jobs && ok; ++i) {
     ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_empty[acc], (use & 1u) ^ 1u, ctl));
     if (!ok) break;
     tc_fence_after();
     const uint32_t d = tmem + acc * B;
     uint32_t more = 0;
-    for (int part = 0; part < per_job; ++part) {
+    for (int part = 0; part < rw.stages; ++part) {
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, ctl));
       if (!ok) break;
       tc_fence_after();
@@ -285,6 +346,113 @@ __device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
   return mul2(mul2(g, r), u);
+}
+
+// Eight outputs of a linear at element `at`: the residual, one rounding, the store.
+__device__ __forceinline__ void put8(const Params& p, int64_t at, const float* v) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = v[i];
+  if (p.out_f32) {
+    if (p.residual) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const uint4 r = ld_global_v4(static_cast<const float*>(p.residual) + at + i);
+        f[i] += __uint_as_float(r.x);
+        f[i + 1] += __uint_as_float(r.y);
+        f[i + 2] += __uint_as_float(r.z);
+        f[i + 3] += __uint_as_float(r.w);
+      }
+    }
+    float* o = static_cast<float*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      st_global_v4(o + i, __float_as_uint(f[i]), __float_as_uint(f[i + 1]), __float_as_uint(f[i + 2]),
+                   __float_as_uint(f[i + 3]));
+  } else {
+    if (p.residual) {
+      const uint4 r = ld_global_v4(static_cast<const __nv_bfloat16*>(p.residual) + at);
+      const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x2 = unpack_bf16x2(rw[i]);
+        f[2 * i] += x2.x;
+        f[2 * i + 1] += x2.y;
+      }
+    }
+    st_global_v4(static_cast<__nv_bfloat16*>(p.out) + at, pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                 pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+}
+
+// Split mode.  Each CTA leaves the sum of its two accumulators in the ring's
+// shared memory (free: every copy into it has been consumed), rows of B + 4
+// floats; then CTA `rank` of the cluster adds columns [rank * B / split, ...)
+// of all of them, in rank order.
+template <int B>
+struct Partial {
+  static constexpr int LD = B + 4;
+  static_assert(kRows * LD * 4 <= Geo<B>::NS * Geo<B>::STAGE, "the partial sums fit the ring");
+};
+
+template <int B>
+__device__ void split_partial(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
+  using G = Geo<B>;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
+  const int q = w & 3, j = w >> 2;
+  if (j >= B / 32) return;  // one unit: the second group of B = 64 has none
+  const int u = int(blockIdx.x) / p.split, m = u / p.R, r = u - m * p.R;
+  const int n = q * 32 + lane;
+  const int live = __ldg(p.p0.counts + r);
+  float f[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[k], 0, ctl))) return;
+    tc_fence_after();
+    uint32_t a[32];
+    tmem_ld32_sync(tmem + (uint32_t(q * 32) << 16) + uint32_t(k * B + j * 32), a);
+    const RingWork rw = ring_work<B, false>(p, k);
+    if (rw.stages > 0 && live > rw.first * G::SLOTS) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] += __uint_as_float(a[i]);
+    }
+  }
+  if (int64_t(m) * kRows + n >= p.T) return;
+  float* row = reinterpret_cast<float*>(s.stages) + n * Partial<B>::LD + j * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+}
+
+template <int B>
+__device__ void split_join(const Params& p, const Smem& s) {
+  const int u = int(blockIdx.x) / p.split, rank = int(blockIdx.x) % p.split, m = u / p.R, r = u - m * p.R;
+  const int rows = int(min(int64_t(kRows), p.T - int64_t(m) * kRows));
+  const int cols = B / p.split, per_row = cols / 8;
+  const uint32_t base = smem_u32(s.stages);
+  for (int i = threadIdx.x; i < rows * per_row; i += kThreads) {
+    const int n = i / per_row, c = rank * cols + (i - n * per_row) * 8;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    for (int k = 0; k < p.split; ++k) {
+      const uint32_t from = mapa_shared(base + uint32_t(n * Partial<B>::LD + c) * 4u, uint32_t(k));
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        float4 v;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(from + e * 4)
+                     : "memory");
+        f[e] += v.x;
+        f[e + 1] += v.y;
+        f[e + 2] += v.z;
+        f[e + 3] += v.w;
+      }
+    }
+    put8(p, (int64_t(m) * kRows + n) * (int64_t(p.R) * B) + int64_t(r) * B + c, f);
+  }
 }
 
 template <int B, bool GATED>
@@ -381,40 +549,8 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         float f[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
-        if (p.out_f32) {
-          float* o = static_cast<float*>(p.out) + at;
-          const float* rs = static_cast<const float*>(p.residual);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (rs) {
-              const uint4 v = ld_global_v4(rs + at + 4 * i);
-              f[4 * i] += __uint_as_float(v.x);
-              f[4 * i + 1] += __uint_as_float(v.y);
-              f[4 * i + 2] += __uint_as_float(v.z);
-              f[4 * i + 3] += __uint_as_float(v.w);
-            }
-            st_global_v4(o + 4 * i, __float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
-                         __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
-          }
-        } else {
-          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
-          const __nv_bfloat16* rs = static_cast<const __nv_bfloat16*>(p.residual);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (rs) {
-              const uint4 v = ld_global_v4(rs + at + 8 * i);
-              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 x2 = unpack_bf16x2(vw[e]);
-                f[8 * i + 2 * e] += x2.x;
-                f[8 * i + 2 * e + 1] += x2.y;
-              }
-            }
-            st_global_v4(o + 8 * i, pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                         pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
-          }
-        }
+        for (int i = 0; i < 32; i += 8) put8(p, at + i, f + i);
       }
     }
     acc += GROUPS * JOBS;
@@ -455,40 +591,73 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   const uint32_t tmem = *s.tmem_slot;
   const Ctl ctl{s.abort_flag, p.status, p.timeout_ns};
   griddep_launch();
-  griddep_wait();  // the rows come from the kernel before
-  if (warp < kProducers)
+  // Rows, and possibly weights, come from the kernel ahead.  With p.early only
+  // the rows do, and the producers start the weights before they wait.
+  if (!p.early || warp >= kProducers) griddep_wait();
+  const bool split = !GATED && p.split;
+  if (warp < kProducers) {
     produce<B, GATED>(p, s, warp >> 1, warp & 1, ctl);
-  else if (warp < kIssuer)
-    epilogue<B, GATED>(p, s, tmem, ctl);
-  else
+  } else if (warp < kIssuer) {
+    if constexpr (!GATED) {
+      if (split) split_partial<B>(p, s, tmem, ctl);
+    }
+    if (!split) epilogue<B, GATED>(p, s, tmem, ctl);
+  } else {
     issue<B, GATED>(p, s, tmem, warp - kIssuer, ctl);
+  }
   tc_fence_before();
   __syncthreads();
+  if constexpr (!GATED) {
+    if (split) {
+      cluster_sync();  // every partial sum is in place
+      split_join<B>(p, s);
+      cluster_sync();  // and has been read before its CTA leaves
+    }
+  }
   if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
+// CTAs that share a unit of a linear: where whole units would leave more than
+// half of the SMs without one, as many as fit (a power of two, at most the
+// portable cluster of 8), while every ring gets a stage.
+static int split_of(int64_t units, int stages, int sms) {
+  if (units * 2 > sms) return 0;
+  int split = 1;
+  while (split < 8 && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
+  return split;
+}
+
 template <int B, bool GATED>
-static int launch(const Params& p, int32_t max_ctas, bool dependent, cudaStream_t s) {
+static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   auto kern = bell_mx_kernel<B, GATED>;
-  if (int rc = set_smem(reinterpret_cast<const void*>(kern), Geo<B>::SMEM)) return rc;
-  int sms = 0;
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
+  int dev = 0, sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  int64_t grid = int64_t(p.mtiles) * p.R;
-  if (grid > sms) grid = sms;
-  if (max_ctas > 0 && grid > max_ctas) grid = max_ctas;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(BELL_ERR_LAUNCH, "cudaGetDevice");
+  if (!(ready.load() >> dev & 1)) {
+    if (int rc = set_smem(reinterpret_cast<const void*>(kern), Geo<B>::SMEM)) return rc;
+    ready.fetch_or(uint64_t(1) << dev);
+  }
+  if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
+  const int64_t units = int64_t(p.mtiles) * p.R;
+  p.split = GATED ? 0 : split_of(units, (p.K0 + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS, sms);
+  const int64_t grid = p.split ? units * p.split : std::min<int64_t>(units, sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Geo<B>::SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(p.split);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = p.split ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -541,12 +710,13 @@ static int quantize_source(const D* d, const BellMxEll& w, void* stream) {
 }
 
 static int linear(int64_t T, const void* x, const BellMxEll& w, const void* residual, void* out, int32_t out_dtype,
-                  int32_t max_ctas, int32_t* status, bool dependent, cudaStream_t s) {
+                  int32_t max_ctas, int32_t* status, bool early, cudaStream_t s) {
   Params p = base_params(T, w, nullptr, x, status);
   p.out = out;
   p.residual = residual;
   p.out_f32 = out_dtype == BELL_DTYPE_F32;
-  return w.B == 128 ? launch<128, false>(p, max_ctas, dependent, s) : launch<64, false>(p, max_ctas, dependent, s);
+  p.early = early;
+  return w.B == 128 ? launch<128, false>(p, max_ctas, s) : launch<64, false>(p, max_ctas, s);
 }
 
 }  // namespace mx
@@ -571,7 +741,9 @@ int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
   int32_t* status = d->status ? d->status : default_status_ptr();
   if (!status) return BELL_ERR_LAUNCH;
   if (int rc = mx::quantize_source(d, d->w, stream)) return rc;
-  return mx::linear(d->T, d->x, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, status, true,
+  // early: the quantisation ahead of the product is a plain launch, so all that
+  // came before it is complete when the product starts
+  return mx::linear(d->T, d->x, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, status, d->x_src != nullptr,
                     static_cast<cudaStream_t>(stream));
 }
 
@@ -603,9 +775,9 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   p.h = static_cast<uint8_t*>(d->h);
   p.gate = static_cast<__nv_bfloat16*>(d->gate_pre);
   p.up = static_cast<__nv_bfloat16*>(d->up_out);
-  if (int rc = g.B == 128 ? mx::launch<128, true>(p, d->max_ctas, true, s) : mx::launch<64, true>(p, d->max_ctas, true, s))
-    return rc;
-  return mx::linear(d->T, d->h, w, d->residual, d->out, d->out_dtype, d->max_ctas, status, true, s);
+  p.early = d->x_src != nullptr;
+  if (int rc = g.B == 128 ? mx::launch<128, true>(p, d->max_ctas, s) : mx::launch<64, true>(p, d->max_ctas, s)) return rc;
+  return mx::linear(d->T, d->h, w, d->residual, d->out, d->out_dtype, d->max_ctas, status, d->x_src != nullptr, s);
 }
 
 }  // extern "C"

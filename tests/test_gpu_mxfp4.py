@@ -125,7 +125,8 @@ def test_make_mxfp4_tiles(B, dtype, layout):
 
 @pytest.mark.parametrize("T,R,C,Kk,B,dead", [
     (1, 1, 1, 1, 128, 0), (1, 1, 1, 1, 64, 0), (5, 3, 4, 2, 64, 1), (128, 2, 3, 3, 128, 0), (129, 2, 40, 35, 64, 3),
-    (257, 5, 36, 33, 128, 7), (300, 160, 2, 2, 64, 11), (1000, 40, 9, 4, 128, 5)])
+    (257, 5, 36, 33, 128, 7), (300, 160, 2, 2, 64, 11), (1000, 40, 9, 4, 128, 5),
+    (1, 32, 128, 32, 128, 0), (2, 70, 20, 17, 64, 9), (130, 9, 32, 32, 128, 20), (33, 1, 64, 61, 64, 3)])
 @pytest.mark.parametrize("dtype,residual", [(BF16, False), (BF16, True), (F32, True)])
 def test_linear(T, R, C, Kk, B, dead, dtype, residual):
     K = _K()

@@ -327,10 +327,6 @@ typedef struct BellMxEll {
   int32_t R, C, K, B;
 } BellMxEll;
 
-/* Up to this many rows, a product is one launch and quantises the rows itself:
- * x may then be NULL (with x_src). */
-#define BELL_MX_FEW_ROWS 32
-
 /* out = Q(x) Q(W)^T (+ residual): fp32 sums, one rounding. */
 typedef struct BellMxLinearDesc {
   int64_t T;

@@ -45,7 +45,6 @@
 #include <string>
 
 #include "bell_mx.cuh"
-#include "bell_mx_gemm.h"
 
 namespace bell {
 namespace mx {
@@ -333,6 +332,21 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
 }
 
 // ---------------------------------------------------------------- epilogue
+
+// h = silu(g) u = g u / (1 + e^-g) in fp32, two at a time (about 1e-6
+// relative): the hardware tanh form of the bf16 kernels (2^-11) would move one
+// in a few hundred of h's 4-bit codes to a neighbour.  Subnormal intermediates
+// are flushed: e^-g below 2^-126 next to 1, and 1 / (1 + e^-g) below 2^-126.
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+  const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 a = add2(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
+  return mul2(mul2(g, r), u);
+}
 
 // Eight outputs of a linear at element `at`: the residual, one rounding, the store.
 __device__ __forceinline__ void put8(const Params& p, int64_t at, const float* v) {
@@ -688,21 +702,11 @@ static Params base_params(int64_t T, const BellMxEll& w0, const BellMxEll* w1, c
   return p;
 }
 
-// Quantise the caller's rows into x where it gave both, and say where the
-// product's rows are.
+// Quantise the caller's rows first where it gave any.
 template <class D>
-static int row_source(const D* d, const BellMxEll& w, RowSource* src, void* stream) {
-  *src = RowSource{d->x, d->x_src, d->ld_src, d->src_dtype == BELL_DTYPE_F32};
-  if (d->x && d->x_src)
-    return bell_mx_quantize_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->ld_src, d->x, stream);
-  return d->x ? BELL_OK : check_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->x_src, d->ld_src);
-}
-
-template <class D>
-static int check_source(const D* d) {
-  if (d->T > 0 && !d->x && !(d->x_src && d->T <= BELL_MX_FEW_ROWS))
-    return fail(BELL_ERR_ARG, "x may be NULL only with x_src and T <= BELL_MX_FEW_ROWS");
-  return BELL_OK;
+static int quantize_source(const D* d, const BellMxEll& w, void* stream) {
+  if (!d->x_src) return BELL_OK;
+  return bell_mx_quantize_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->ld_src, d->x, stream);
 }
 
 static int linear(int64_t T, const void* x, const BellMxEll& w, const void* residual, void* out, int32_t out_dtype,
@@ -728,8 +732,7 @@ int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
   if (int rc = mx::check_size(d->T, d->w.R)) return rc;
   if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
-  if (int rc = mx::check_source(d)) return rc;
-  if (d->T > 0 && !d->out) return fail(BELL_ERR_ARG, "out must be non-NULL");
+  if (d->T > 0 && (!d->x || !d->out)) return fail(BELL_ERR_ARG, "x and out must be non-NULL");
   if (!aligned16(d->x) || !aligned16(d->out) || !aligned16(d->residual))
     return fail(BELL_ERR_ALIGN, "x, out and residual must be 16-byte aligned");
   if (d->max_ctas < 0) return fail(BELL_ERR_ARG, "max_ctas must be >= 0");
@@ -737,15 +740,11 @@ int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
   if (d->T == 0) return BELL_OK;
   int32_t* status = d->status ? d->status : default_status_ptr();
   if (!status) return BELL_ERR_LAUNCH;
-  mx::RowSource src;
-  if (int rc = mx::row_source(d, d->w, &src, stream)) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->T <= BELL_MX_FEW_ROWS)
-    return mx::few_linear(d->T, src, d->w, d->residual, d->out, d->out_dtype == BELL_DTYPE_F32, d->max_ctas, s);
+  if (int rc = mx::quantize_source(d, d->w, stream)) return rc;
   // early: the quantisation ahead of the product is a plain launch, so all that
   // came before it is complete when the product starts
   return mx::linear(d->T, d->x, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, status, d->x_src != nullptr,
-                    s);
+                    static_cast<cudaStream_t>(stream));
 }
 
 int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
@@ -760,8 +759,7 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   if (int rc = mx::check_size(d->T, g.R > w.R ? g.R : w.R)) return rc;
   if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
-  if (int rc = mx::check_source(d)) return rc;
-  if (d->T > 0 && (!d->h || !d->out)) return fail(BELL_ERR_ARG, "h and out must be non-NULL");
+  if (d->T > 0 && (!d->x || !d->h || !d->out)) return fail(BELL_ERR_ARG, "x, h and out must be non-NULL");
   if (!d->gate_pre != !d->up_out) return fail(BELL_ERR_ARG, "gate_pre and up_out come together");
   if (!aligned16(d->x) || !aligned16(d->h) || !aligned16(d->out) || !aligned16(d->residual) ||
       !aligned16(d->gate_pre) || !aligned16(d->up_out))
@@ -772,11 +770,7 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   int32_t* status = d->status ? d->status : default_status_ptr();
   if (!status) return BELL_ERR_LAUNCH;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  mx::RowSource src;
-  if (int rc = mx::row_source(d, g, &src, stream)) return rc;
-  if (d->T <= BELL_MX_FEW_ROWS)
-    return mx::few_swiglu(d->T, src, g, u, w, d->h, d->gate_pre, d->up_out, d->residual, d->out,
-                          d->out_dtype == BELL_DTYPE_F32, d->max_ctas, s);
+  if (int rc = mx::quantize_source(d, g, stream)) return rc;
   mx::Params p = mx::base_params(d->T, g, &u, d->x, status);
   p.h = static_cast<uint8_t*>(d->h);
   p.gate = static_cast<__nv_bfloat16*>(d->gate_pre);

@@ -19,7 +19,6 @@
 // Tiles: chunk (r, k) at (r * K + k) * tile_chunk(B).
 #pragma once
 
-#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -138,45 +137,6 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t w, float scale, float* v) {
     v[2 * i] = f.x * scale;
     v[2 * i + 1] = f.y * scale;
   }
-}
-
-// 32 consecutive values of a row, 16-byte loads.
-__device__ __forceinline__ void load32(const __nv_bfloat16* p, float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 w = ld_global_nc_v4(p + 8 * i);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack_bf16x2(u[j]);
-      v[8 * i + 2 * j] = f.x;
-      v[8 * i + 2 * j + 1] = f.y;
-    }
-  }
-}
-__device__ __forceinline__ void load32(const float* p, float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 w = ld_global_nc_v4(p + 4 * i);
-    v[4 * i] = __uint_as_float(w.x);
-    v[4 * i + 1] = __uint_as_float(w.y);
-    v[4 * i + 2] = __uint_as_float(w.z);
-    v[4 * i + 3] = __uint_as_float(w.w);
-  }
-}
-// h = silu(g) u = g u / (1 + e^-g) in fp32, two at a time (about 1e-6
-// relative): the hardware tanh form of the bf16 kernels (2^-11) would move one
-// in a few hundred of h's 4-bit codes to a neighbour.  Subnormal intermediates
-// are flushed: e^-g below 2^-126 next to 1, and 1 / (1 + e^-g) below 2^-126.
-__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
-  const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  float2 e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-  const float2 a = add2(e, make_float2(1.f, 1.f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
-  return mul2(mul2(g, r), u);
 }
 
 // ------------------------------------------------------------------ tcgen05

@@ -233,7 +233,7 @@ def mxfp4_linear(x: Union[torch.Tensor, MXRows], w: MXBlockELL, residual: Option
     return _linear(x, w, residual, out_dtype, out, max_ctas)[0]
 
 
-def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0, keep_rows=False):
+def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0):
     if not isinstance(x, MXRows):
         x = _rows_2d("x", x)
     in_f, out_f = w.C * w.B, w.R * w.B
@@ -248,11 +248,8 @@ def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0, keep_rows
         _check_out("out", out, (T, out_f), dtype, dev)
     if residual is not None:
         residual = _check_residual(residual, (T, out_f), dtype, dev)
-    if src is None:
-        rows = x.data
-    else:  # a few rows are quantised by the product itself
-        rows = _bytes(_rows_bytes(T, in_f, w.B), dev) if keep_rows or T > _lib.BELL_MX_FEW_ROWS else None
-    d = _lib.BellMxLinearDesc(T, _DTYPES[dtype], int(max_ctas), None if rows is None else rows.data_ptr(), src, ld, src_type, 0,
+    rows = x.data if src is None else _bytes(_rows_bytes(T, in_f, w.B), dev)
+    d = _lib.BellMxLinearDesc(T, _DTYPES[dtype], int(max_ctas), rows.data_ptr(), src, ld, src_type, 0,
                               None if residual is None else residual.data_ptr(), out.data_ptr(), w._abi, None)
     _call("bell_linear_mx", dev, C.byref(d))
     return out, rows
@@ -289,14 +286,13 @@ def mxfp4_swiglu_fwd(x: Union[torch.Tensor, MXRows], gate: MXBlockELL, up: MXBlo
             residual = x
         residual = _check_residual(residual, (T, D), dtype, dev)
     out = torch.empty((T, D), dtype=dtype, device=dev)
-    direct = not quantised and not return_intermediates and T <= _lib.BELL_MX_FEW_ROWS
-    n_x, n_h = 0 if quantised or direct else _rows_bytes(T, D, B), _rows_bytes(T, F, B)
+    n_x, n_h = 0 if quantised else _rows_bytes(T, D, B), _rows_bytes(T, F, B)
     ws = _bytes(n_x + n_h, dev)  # the quantised rows of x, then of h
     at = ws.data_ptr()
     g = u = None
     if return_intermediates:
         g, u = (torch.empty((T, F), dtype=torch.bfloat16, device=dev) for _ in range(2))
-    d = _lib.BellMxFFNDesc(T, _DTYPES[dtype], int(max_ctas), x.data.data_ptr() if quantised else None if direct else at, src, ld, src_type, 0,
+    d = _lib.BellMxFFNDesc(T, _DTYPES[dtype], int(max_ctas), x.data.data_ptr() if quantised else at, src, ld, src_type, 0,
                            None if residual is None else residual.data_ptr(), at + n_x,
                            None if g is None else g.data_ptr(), None if u is None else u.data_ptr(), out.data_ptr(),
                            gate._abi, up._abi, down._abi, None)
@@ -322,7 +318,7 @@ class MXLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, values, cols, residual, layout):
         w = make_mxfp4(values, cols, x.shape[1] // values.shape[2], layout)
-        y, rows = _linear(x, w, residual, keep_rows=True)
+        y, rows = _linear(x, w, residual)
         ctx.w, ctx.layout = w, layout
         ctx.save_for_backward(cols, w.data, rows)
         ctx.dtypes = (x.dtype, values.dtype)

@@ -327,6 +327,10 @@ typedef struct BellMxEll {
   int32_t R, C, K, B;
 } BellMxEll;
 
+/* Rows that a product quantises itself: for T up to this, x may be NULL (with
+ * x_src), which saves a launch. */
+#define BELL_MX_DIRECT_ROWS 32
+
 /* out = Q(x) Q(W)^T (+ residual): fp32 sums, one rounding. */
 typedef struct BellMxLinearDesc {
   int64_t T;

@@ -76,6 +76,9 @@ struct Params {
   int64_t T;
   int32_t mtiles, R, C, K0, K1;
   const uint8_t* x;               // rows of chunks, C column blocks
+  const void* src;                // or, x null: T <= BELL_MX_DIRECT_ROWS rows, quantised here
+  int64_t ld_src;
+  int32_t src_f32;
   const uint8_t *w0, *w1;         // tiles
   Plan p0, p1;
   uint8_t* h;                     // gated: [mtiles, R] chunks
@@ -137,6 +140,60 @@ __device__ __forceinline__ int job_unit(const Params& p, int i, int k) {
   return int(blockIdx.x) + (GATED ? i : 2 * i + k) * int(gridDim.x);
 }
 
+// ------------------------------------------------------------- direct rows
+//
+// Few rows come as they are (no chunks in memory, and no launch to write them):
+// each CTA quantises the columns that its slots take, into the stages.  The
+// epilogue's warps, idle until the first accumulator, do so for the rings'
+// first filling, all slots and row groups at once; the producers for the uses
+// after it.
+
+// Rows [n0, n0 + N), N = 8 or 16, of the chunk of column block c: a lane takes a
+// scale block of a row, as in the quantisation kernel.
+template <int B>
+struct DirectRows {
+  static constexpr int N = 32 * kBlock / B;
+  static __device__ __forceinline__ void put(const Params& p, int c, int n0, uint8_t* chunk) {
+    const int lane = threadIdx.x & 31;
+    const int j = (lane >> 3) & (B / kBlock - 1), n = n0 + (lane & 7) + (B == 64 ? (lane >> 4) * 8 : 0);
+    if (n >= int(p.T)) return;
+    float v[32];
+    const int64_t at = n * p.ld_src + int64_t(c) * B + j * kBlock;
+    if (p.src_f32)
+      load32(static_cast<const float*>(p.src) + at, v);
+    else
+      load32(static_cast<const __nv_bfloat16*>(p.src) + at, v);
+    uint32_t byte;
+    *reinterpret_cast<uint4*>(chunk + code_off(n, j, kRows * 32)) = quantize32(v, byte);
+    chunk[kRows * B / 2 + scale_off(n, j)] = uint8_t(byte);
+  }
+};
+
+// The epilogue warps and the producers, once, after the first filling's rows.
+__device__ __forceinline__ void direct_barrier() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * (kProducers + kEpiWarps)) : "memory");
+}
+
+template <int B, bool GATED>
+__device__ void direct_first(const Params& p, const Smem& s) {
+  using G = Geo<B>;
+  const int w = (threadIdx.x >> 5) - kProducers;
+  const int groups = (int(p.T) + DirectRows<B>::N - 1) / DirectRows<B>::N;
+  for (int item = w; item < G::NS * G::SLOTS * groups; item += kEpiWarps) {
+    const int n0 = item % groups * DirectRows<B>::N, at = item / groups;
+    const int i = at % G::SLOTS, use = at / G::SLOTS % G::NR, ring = at / (G::SLOTS * G::NR);
+    const RingWork rw = ring_work<B, GATED>(p, ring);
+    const int job = rw.stages > 0 ? use / rw.stages : rw.jobs;
+    if (job >= rw.jobs) continue;
+    const int u = job_unit<GATED>(p, job, ring), r = u % p.R;
+    const int mat = GATED ? ring : 0, K = mat ? p.K1 : p.K0, k = (rw.first + use - job * rw.stages) * G::SLOTS + i;
+    const uint32_t e = k < K ? __ldg((mat ? p.p1 : p.p0).entries + int64_t(r) * K + k) : kNoSlot;
+    if (e != kNoSlot) DirectRows<B>::put(p, int(e & 0xFFFFu), n0, s.stages + (ring * G::NR + use) * G::STAGE + i * G::SLOT);
+  }
+  fence_proxy_async_smem();
+  direct_barrier();
+}
+
 // ---------------------------------------------------------------- producer
 
 template <int B, bool GATED>
@@ -182,8 +239,29 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     uint32_t ent[G::SLOTS];
 #pragma unroll
     for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, use.e, i);
+    uint8_t* st = stages + stage * uint32_t(G::STAGE);
+    if (!p.x) {  // direct rows: this warp's, or with `rows` false already on their way
+      if (elect_one()) {
+        count[stage] = uint32_t(cnt);
+        mbar_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::W));
+#pragma unroll
+        for (int i = 0; i < G::SLOTS; ++i)
+          if (i < cnt)
+            bulk_load(st + i * G::SLOT + G::A, use.w + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
+      }
+      __syncwarp();
+      if (!rows) return;
+#pragma unroll
+      for (int i = 0; i < G::SLOTS; ++i)
+        for (int n0 = 0; i < cnt && n0 < int(p.T); n0 += DirectRows<B>::N)
+          DirectRows<B>::put(p, int(ent[i] & 0xFFFFu), n0, st + i * G::SLOT);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (elect_one()) mbar_arrive(&full[stage]);
+      __syncwarp();
+      return;
+    }
     if (elect_one()) {
-      uint8_t* st = stages + stage * uint32_t(G::STAGE);
       if (weights) {
         count[stage] = uint32_t(cnt);
         if (cnt)
@@ -212,9 +290,9 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
       phase ^= 1u;
     }
   };
-  // The ring's first filling: the weights need not wait for the kernel ahead,
-  // which makes the rows.
-  if (p.early) {
+  // The ring's first filling: the weights need not wait for the rows, which the
+  // kernel ahead or the epilogue's warps make.
+  if (p.early || !p.x) {
     Use first[(G::NR + 1) / 2];
     int n = 0;
 #pragma unroll
@@ -226,14 +304,21 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
         n = i + 1;
       }
     }
-    griddep_wait();
+    if (p.x)
+      griddep_wait();
+    else
+      direct_barrier();
 #pragma unroll
     for (int i = 0; i < (G::NR + 1) / 2; ++i) {
       if (i < n) {
-        copies(first[i], uint32_t(sub + 2 * i), false, true);
+        if (p.x)
+          copies(first[i], uint32_t(sub + 2 * i), false, true);
+        else if (elect_one())
+          mbar_arrive(&full[sub + 2 * i]);
         turn();
       }
     }
+    __syncwarp();
   }
   // from here each use's entries travel while the one before is issued
   Use next{kNoSlot, nullptr, nullptr};
@@ -598,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   if (warp < kProducers) {
     produce<B, GATED>(p, s, warp >> 1, warp & 1, ctl);
   } else if (warp < kIssuer) {
+    if (!p.x) direct_first<B, GATED>(p, s);
     if constexpr (!GATED) {
       if (split) split_partial<B>(p, s, tmem, ctl);
     }
@@ -656,8 +742,9 @@ static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(p.split);
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.split ? 2 : 1;
+  // direct rows may come from any kernel ahead: a plain launch waits for it
+  cfg.attrs = attr + (p.x ? 0 : 1);
+  cfg.numAttrs = (p.x ? 1 : 0) + (p.split ? 1 : 0);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -702,20 +789,29 @@ static Params base_params(int64_t T, const BellMxEll& w0, const BellMxEll* w1, c
   return p;
 }
 
-// Quantise the caller's rows first where it gave any.
+// Quantise the caller's rows first where it gave any and wants them in x.
 template <class D>
-static int quantize_source(const D* d, const BellMxEll& w, void* stream) {
+static int quantize_source(const D* d, const BellMxEll& w, Params* p, void* stream) {
   if (!d->x_src) return BELL_OK;
-  return bell_mx_quantize_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->ld_src, d->x, stream);
+  if (d->x) return bell_mx_quantize_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->ld_src, d->x, stream);
+  p->src = d->x_src;
+  p->ld_src = d->ld_src;
+  p->src_f32 = d->src_dtype == BELL_DTYPE_F32;
+  return check_rows(d->T, w.C * w.B, w.B, d->src_dtype, d->x_src, d->x_src, d->ld_src);
 }
 
-static int linear(int64_t T, const void* x, const BellMxEll& w, const void* residual, void* out, int32_t out_dtype,
-                  int32_t max_ctas, int32_t* status, bool early, cudaStream_t s) {
-  Params p = base_params(T, w, nullptr, x, status);
+template <class D>
+static int check_source(const D* d) {
+  if (d->T > 0 && !d->x && !(d->x_src && d->T <= BELL_MX_DIRECT_ROWS))
+    return fail(BELL_ERR_ARG, "x may be NULL only with x_src and T <= BELL_MX_DIRECT_ROWS");
+  return BELL_OK;
+}
+
+static int linear(Params p, const BellMxEll& w, const void* residual, void* out, int32_t out_dtype, int32_t max_ctas,
+                  cudaStream_t s) {
   p.out = out;
   p.residual = residual;
   p.out_f32 = out_dtype == BELL_DTYPE_F32;
-  p.early = early;
   return w.B == 128 ? launch<128, false>(p, max_ctas, s) : launch<64, false>(p, max_ctas, s);
 }
 
@@ -732,7 +828,8 @@ int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
   if (int rc = mx::check_size(d->T, d->w.R)) return rc;
   if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
-  if (d->T > 0 && (!d->x || !d->out)) return fail(BELL_ERR_ARG, "x and out must be non-NULL");
+  if (int rc = mx::check_source(d)) return rc;
+  if (d->T > 0 && !d->out) return fail(BELL_ERR_ARG, "out must be non-NULL");
   if (!aligned16(d->x) || !aligned16(d->out) || !aligned16(d->residual))
     return fail(BELL_ERR_ALIGN, "x, out and residual must be 16-byte aligned");
   if (d->max_ctas < 0) return fail(BELL_ERR_ARG, "max_ctas must be >= 0");
@@ -740,11 +837,12 @@ int bell_linear_mx(const BellMxLinearDesc* d, void* stream) {
   if (d->T == 0) return BELL_OK;
   int32_t* status = d->status ? d->status : default_status_ptr();
   if (!status) return BELL_ERR_LAUNCH;
-  if (int rc = mx::quantize_source(d, d->w, stream)) return rc;
+  mx::Params p = mx::base_params(d->T, d->w, nullptr, d->x, status);
+  if (int rc = mx::quantize_source(d, d->w, &p, stream)) return rc;
   // early: the quantisation ahead of the product is a plain launch, so all that
   // came before it is complete when the product starts
-  return mx::linear(d->T, d->x, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, status, d->x_src != nullptr,
-                    static_cast<cudaStream_t>(stream));
+  p.early = d->x && d->x_src;
+  return mx::linear(p, d->w, d->residual, d->out, d->out_dtype, d->max_ctas, static_cast<cudaStream_t>(stream));
 }
 
 int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
@@ -759,7 +857,8 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   if (int rc = mx::check_size(d->T, g.R > w.R ? g.R : w.R)) return rc;
   if (d->out_dtype != BELL_DTYPE_BF16 && d->out_dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "out_dtype must be bf16 or f32");
-  if (d->T > 0 && (!d->x || !d->h || !d->out)) return fail(BELL_ERR_ARG, "x, h and out must be non-NULL");
+  if (int rc = mx::check_source(d)) return rc;
+  if (d->T > 0 && (!d->h || !d->out)) return fail(BELL_ERR_ARG, "h and out must be non-NULL");
   if (!d->gate_pre != !d->up_out) return fail(BELL_ERR_ARG, "gate_pre and up_out come together");
   if (!aligned16(d->x) || !aligned16(d->h) || !aligned16(d->out) || !aligned16(d->residual) ||
       !aligned16(d->gate_pre) || !aligned16(d->up_out))
@@ -770,14 +869,16 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   int32_t* status = d->status ? d->status : default_status_ptr();
   if (!status) return BELL_ERR_LAUNCH;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int rc = mx::quantize_source(d, g, stream)) return rc;
   mx::Params p = mx::base_params(d->T, g, &u, d->x, status);
+  if (int rc = mx::quantize_source(d, g, &p, stream)) return rc;
   p.h = static_cast<uint8_t*>(d->h);
   p.gate = static_cast<__nv_bfloat16*>(d->gate_pre);
   p.up = static_cast<__nv_bfloat16*>(d->up_out);
-  p.early = d->x_src != nullptr;
+  p.early = d->x && d->x_src;
   if (int rc = g.B == 128 ? mx::launch<128, true>(p, d->max_ctas, s) : mx::launch<64, true>(p, d->max_ctas, s)) return rc;
-  return mx::linear(d->T, d->h, w, d->residual, d->out, d->out_dtype, d->max_ctas, status, d->x_src != nullptr, s);
+  mx::Params q = mx::base_params(d->T, w, nullptr, d->h, status);
+  q.early = d->x_src != nullptr;  // a plain launch (the quantisation, or gate/up from the caller's rows) came before
+  return mx::linear(q, w, d->residual, d->out, d->out_dtype, d->max_ctas, s);
 }
 
 }  // extern "C"

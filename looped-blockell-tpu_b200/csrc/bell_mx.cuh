@@ -19,6 +19,7 @@
 // Tiles: chunk (r, k) at (r * K + k) * tile_chunk(B).
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -71,6 +72,11 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float* v) {
       : "=r"(r)
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
+}
+
+// Raise the transaction count of the current phase without arriving.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // Two fp32 products or sums in one instruction, each rounded as alone.
@@ -139,6 +145,30 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t w, float scale, float* v) {
   }
 }
 
+// 32 consecutive values of a row, 16-byte loads.
+__device__ __forceinline__ void load32(const __nv_bfloat16* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = ld_global_nc_v4(p + 8 * i);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(u[j]);
+      v[8 * i + 2 * j] = f.x;
+      v[8 * i + 2 * j + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void load32(const float* p, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 w = ld_global_nc_v4(p + 4 * i);
+    v[4 * i] = __uint_as_float(w.x);
+    v[4 * i + 1] = __uint_as_float(w.y);
+    v[4 * i + 2] = __uint_as_float(w.z);
+    v[4 * i + 3] = __uint_as_float(w.w);
+  }
+}
 // ------------------------------------------------------------------ tcgen05
 
 // Shared-memory matrix descriptors without swizzle, as two words: the low one
@@ -210,6 +240,9 @@ inline Plan plan_of(const void* plan, int32_t R, int32_t K) {
   const char* p = static_cast<const char*>(plan);
   return {reinterpret_cast<const uint32_t*>(p + L.d_entries), reinterpret_cast<const int32_t*>(p + L.d_counts)};
 }
+
+// Argument checks of rows [T, features], ld elements apart (bell_mx_quant.cu).
+int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks, int64_t ld);
 
 }  // namespace mx
 }  // namespace bell

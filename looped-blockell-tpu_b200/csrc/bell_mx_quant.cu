@@ -13,30 +13,6 @@ namespace mx {
 
 static constexpr int kThr = 256;
 
-// 32 consecutive values of a row, 16-byte loads.
-__device__ __forceinline__ void load32(const __nv_bfloat16* p, float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4 w = ld_global_nc_v4(p + 8 * i);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack_bf16x2(u[j]);
-      v[8 * i + 2 * j] = f.x;
-      v[8 * i + 2 * j + 1] = f.y;
-    }
-  }
-}
-__device__ __forceinline__ void load32(const float* p, float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 w = ld_global_nc_v4(p + 4 * i);
-    v[4 * i] = __uint_as_float(w.x);
-    v[4 * i + 1] = __uint_as_float(w.y);
-    v[4 * i + 2] = __uint_as_float(w.z);
-    v[4 * i + 3] = __uint_as_float(w.w);
-  }
-}
 // Q(v) is a 2-bit significand times a power of two: exact in bf16 and fp32.
 __device__ __forceinline__ void store32(__nv_bfloat16* p, const float (&v)[32]) {
 #pragma unroll
@@ -239,7 +215,7 @@ static int grid_for(int64_t threads, unsigned* grid) {
   return BELL_OK;
 }
 
-static int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks,
+int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks,
                       int64_t ld) {
   if (B != 64 && B != 128) return fail(BELL_ERR_SHAPE, "MXFP4 rows: tile size B must be 64 or 128");
   if (T < 0 || T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "MXFP4 rows: T must be in [0, 2^31 - 256)");

@@ -18,6 +18,7 @@ BELL_TILE_IN_OUT = 0
 BELL_TILE_OUT_IN = 1
 BELL_DTYPE_BF16 = 0
 BELL_DTYPE_F32 = 1
+BELL_MX_DIRECT_ROWS = 32
 BELL_STATUS_COLIDX = 1
 BELL_STATUS_TIMEOUT = 2
 

@@ -126,7 +126,8 @@ def test_make_mxfp4_tiles(B, dtype, layout):
 @pytest.mark.parametrize("T,R,C,Kk,B,dead", [
     (1, 1, 1, 1, 128, 0), (1, 1, 1, 1, 64, 0), (5, 3, 4, 2, 64, 1), (128, 2, 3, 3, 128, 0), (129, 2, 40, 35, 64, 3),
     (257, 5, 36, 33, 128, 7), (300, 160, 2, 2, 64, 11), (1000, 40, 9, 4, 128, 5),
-    (1, 32, 128, 32, 128, 0), (2, 70, 20, 17, 64, 9), (130, 9, 32, 32, 128, 20), (33, 1, 64, 61, 64, 3)])
+    (1, 32, 128, 32, 128, 0), (2, 70, 20, 17, 64, 9), (130, 9, 32, 32, 128, 20), (33, 1, 64, 61, 64, 3),
+    (8, 3, 5, 5, 128, 2), (9, 6, 9, 9, 64, 4), (25, 2, 17, 13, 128, 0), (32, 4, 3, 2, 64, 0), (17, 170, 40, 39, 64, 9)])
 @pytest.mark.parametrize("dtype,residual", [(BF16, False), (BF16, True), (F32, True)])
 def test_linear(T, R, C, Kk, B, dead, dtype, residual):
     K = _K()
@@ -175,7 +176,8 @@ def check_ffn(K, x, g, u, d, wg, wu, wd, residual):
 
 
 @pytest.mark.parametrize("T,d,F,B,Kg,Kd,dead", [
-    (1, 128, 256, 64, 1, 1, 0), (1, 256, 512, 128, 2, 4, 0), (3, 192, 320, 64, 2, 3, 2), (128, 256, 512, 64, 4, 8, 3),
+    (1, 128, 256, 64, 1, 1, 0), (1, 256, 512, 128, 2, 4, 0), (3, 192, 320, 64, 2, 3, 2), (8, 1280, 1536, 128, 9, 11, 3),
+    (17, 640, 896, 64, 9, 13, 5), (32, 512, 20480, 128, 3, 2, 0), (33, 384, 512, 128, 3, 3, 1), (2, 1280, 20480, 64, 18, 40, 30), (128, 256, 512, 64, 4, 8, 3),
     (131, 384, 640, 128, 2, 5, 2), (700, 512, 2560, 64, 3, 20, 9), (515, 640, 3200, 128, 3, 12, 4)])
 @pytest.mark.parametrize("residual", [False, True])
 def test_swiglu_stages(T, d, F, B, Kg, Kd, dead, residual):

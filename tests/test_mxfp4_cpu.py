@@ -122,6 +122,7 @@ def test_linear_and_ffn_refusals():
     assert lin(T=-1) == -2 and lin(T=1 << 31) == -2 and lin(T=(1 << 31) - 300, w=_mx(L, 64, 3)) == -2
     assert lin(out_dtype=9) == -1 and lin(x=None) == -8 and lin(out=1025) == -3 and lin(residual=1026) == -3
     assert lin(max_ctas=-1) == -8
+    assert lin(x=None, x_src=1024, ld_src=192, T=L.BELL_MX_DIRECT_ROWS + 1) == -8 and "DIRECT_ROWS" in L.last_error()
 
     def ffn(**kw):
         d = L.BellMxFFNDesc()

@@ -306,12 +306,15 @@ int bell_mx_quantize_rows(int64_t T, int32_t features, int32_t B, int32_t dtype,
 int bell_mx_dequantize_rows(int64_t T, int32_t features, int32_t B, const void* src, int32_t dtype, void* dst,
                             int64_t ld_dst, void* stream);
 
-/* Quantise the tiles of a Block-ELL weight (values bf16 or f32 as `dtype`
- * says, either layout; scale blocks run along B_in) into chunks,
- * bell_mx_tiles_bytes() bytes, and list its live slots in plan,
- * bell_plan_bytes(0, 0, 0, R, K) bytes.  Dead slots (-1) are left out of the
- * plan; any other index outside [0, C) too, and sets BELL_STATUS_COLIDX. */
-int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, int32_t* status, void* stream);
+/* Quantise the tiles of n Block-ELL weights, at most BELL_MX_PACK_MAX, in one
+ * launch (values bf16 or f32 as `dtype` says, either layout; scale blocks run
+ * along B_in): weight i into chunks[i], bell_mx_tiles_bytes() bytes, and its
+ * live slots into plans[i], bell_plan_bytes(0, 0, 0, R, K) bytes.  The two
+ * arrays are host memory.  Dead slots (-1) are left out of the plan; any other
+ * index outside [0, C) too, and sets BELL_STATUS_COLIDX. */
+#define BELL_MX_PACK_MAX 3
+int bell_mx_pack_ell(const BellEll* weights, int32_t n, int32_t dtype, void* const* chunks, void* const* plans,
+                     int32_t* status, void* stream);
 
 /* Quantised tiles back to bf16, [tiles, B, B] as [B_out, B_in]: output tile i
  * is tile index[i] (i when index is NULL) of the tiles0 tiles at chunks0

@@ -241,6 +241,43 @@ inline Plan plan_of(const void* plan, int32_t R, int32_t K) {
   return {reinterpret_cast<const uint32_t*>(p + L.d_entries), reinterpret_cast<const int32_t*>(p + L.d_counts)};
 }
 
+// Gathered tiles to bf16 [tiles, B_out, B_in]: tile index[i] (or i) of the n0
+// tiles at c0 followed by the n1 at c1.
+struct TileGather {
+  const void* c0;
+  int64_t n0;
+  const void* c1;
+  int64_t n1;
+  const int64_t* index;
+  int64_t tiles;
+  void* values;
+};
+struct RowsTo {  // quantised rows to bf16 [T, features]
+  const void* src;
+  int32_t features;
+  void* dst;
+};
+struct Zeros {
+  float* at;
+  int64_t floats;  // a multiple of 4
+};
+// Everything that a backward unpacks or clears before its products, one launch.
+struct ExpandArgs {
+  int64_t T;
+  int32_t B;
+  TileGather gather[2];
+  RowsTo rows[2];
+  Zeros zero[3];
+};
+int expand(const ExpandArgs& e, cudaStream_t s);
+// n[i] fp32 sums (a multiple of 8) rounded to bf16.
+struct RoundArgs {
+  const float* src[3];
+  void* dst[3];
+  int64_t n[3];
+};
+int round_sums(const RoundArgs& a, cudaStream_t s);
+
 // Argument checks of rows [T, features], ld elements apart (bell_mx_quant.cu).
 int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks, int64_t ld);
 

@@ -3,14 +3,16 @@
 // whose values are exact in bf16.  Each entry point is the sequence of launches
 // on the caller's stream and one workspace:
 //
-//   W_down^T  gathered and unpacked; [d_gate | d_up] from d_h = dy Q(W_down)
-//             and the SiLU backward (one kernel at B = 64, two at B = 128, as
-//             the bf16 backward measured faster)
-//   [W_gate ; W_up]^T likewise; dx = [d_gate | d_up] Q([W_gate ; W_up]) (+ dy)
-//   Q(x), Q(h) unpacked; the three tile gradients, summed in fp32
+//   unpack    the gathered tiles of W_down^T and [W_gate ; W_up]^T, Q(x) and
+//             (at B = 64) Q(h), and zeros for the tile gradients: one launch
+//   [d_gate | d_up] from d_h = dy Q(W_down) and the SiLU backward (one kernel at
+//             B = 64, two at B = 128, as the bf16 backward measured faster)
+//   dx = [d_gate | d_up] Q([W_gate ; W_up]) (+ dy)
+//   the three tile gradients, summed in fp32; one launch rounds them to bf16
 //
-// The unpacked operands live in the workspace only while their product runs:
-// they add 2 bytes a value to the traffic and nothing to what training keeps.
+// The unpacked operands live in the workspace only during the call: they add 2
+// bytes a value to the traffic and nothing to what training keeps.  At B = 128
+// Q(h) takes the place of d_h once that has been read.
 #include <algorithm>
 #include <string>
 
@@ -21,45 +23,72 @@ namespace mx {
 
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Offsets of the workspace.
+// Offsets of the workspace: the unpacked transposes (of down, and of gate and
+// up or the one weight), a plan, the unpacked rows, d_h and Q(h), fp32 sums
+// whose result is bf16, [d_gate | d_up].
 struct BwdWs {
-  size_t tiles, plan, rows, mid, grads, dgu, total;
+  size_t tiles_down, tiles, plan, rows, mid, grads[3], dgu, total;
 };
 
-// tiles: the larger of the unpacked transposes; rows: unpacked rows; mid: d_h,
-// then Q(h); grads: fp32 sums whose result is bf16; dgu: [d_gate | d_up].
-static BwdWs bwd_ws(size_t tiles, size_t plan, size_t rows, size_t mid, size_t grads, size_t dgu) {
-  BwdWs w{};
-  w.tiles = 0;
-  w.plan = up256(tiles);
-  w.rows = w.plan + up256(plan);
-  w.mid = w.rows + up256(rows);
-  w.grads = w.mid + up256(mid);
-  w.dgu = w.grads + up256(grads);
-  w.total = w.dgu + up256(dgu);
-  return w;
+struct Layout {
+  size_t at = 0;
+  size_t take(size_t n) {
+    const size_t from = at;
+    at += up256(n);
+    return from;
+  }
+};
+
+static size_t sums_bytes(const BellMxEll& w, bool wanted, int32_t dtype) {
+  return wanted && dtype == BELL_DTYPE_BF16 ? size_t(w.R) * w.K * w.B * w.B * 4 : 0;
 }
 
 static BwdWs linear_ws(const BellMxLinearBwdDesc& d) {
-  const size_t BB = size_t(d.w.B) * d.w.B;
-  return bwd_ws(size_t(d.w.C) * d.K_t * BB * 2, bell_plan_bytes(0, 0, 0, d.w.C, d.K_t),
-                size_t(d.T) * d.w.C * d.w.B * 2, 0, d.grad_dtype == BELL_DTYPE_BF16 ? size_t(d.w.R) * d.w.K * BB * 4 : 0, 0);
+  BwdWs o{};
+  Layout l;
+  o.tiles = l.take(d.dx ? size_t(d.w.C) * d.K_t * d.w.B * d.w.B * 2 : 0);
+  o.plan = l.take(d.dx ? bell_plan_bytes(0, 0, 0, d.w.C, d.K_t) : 0);
+  o.rows = l.take(d.dw ? size_t(d.T) * d.w.C * d.w.B * 2 : 0);
+  o.grads[0] = l.take(sums_bytes(d.w, d.dw != nullptr, d.grad_dtype));
+  o.total = std::max<size_t>(l.at, 256);
+  return o;
 }
 
 static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
-  const BellMxEll &g = d.gate, &u = d.up, &w = d.down;
-  const size_t BB = size_t(g.B) * g.B, F = size_t(g.R) * g.B;
-  const size_t tiles = std::max(size_t(g.R) * d.K_t_down, size_t(g.C) * d.K_t_gate_up) * BB * 2;
-  const size_t plan = std::max(bell_plan_bytes(0, 0, 0, g.R, d.K_t_down), bell_plan_bytes(0, 0, 0, g.C, d.K_t_gate_up));
-  size_t most = 0;
-  if (d.gate_dtype == BELL_DTYPE_BF16) most = std::max(most, size_t(g.R) * g.K);
-  if (d.up_dtype == BELL_DTYPE_BF16) most = std::max(most, size_t(u.R) * u.K);
-  if (d.down_dtype == BELL_DTYPE_BF16) most = std::max(most, size_t(w.R) * w.K);
-  return bwd_ws(tiles, plan, size_t(d.T) * g.C * g.B * 2, size_t(d.T) * F * 2, most * BB * 4, size_t(d.T) * 2 * F * 2);
+  const BellMxEll& g = d.gate;
+  const size_t BB = size_t(g.B) * g.B, F = size_t(g.R) * g.B, T = size_t(d.T);
+  BwdWs o{};
+  Layout l;
+  o.tiles_down = l.take(size_t(g.R) * d.K_t_down * BB * 2);
+  o.tiles = l.take(size_t(g.C) * d.K_t_gate_up * BB * 2);
+  o.plan = l.take(std::max(bell_plan_bytes(0, 0, 0, g.R, d.K_t_down), bell_plan_bytes(0, 0, 0, g.C, d.K_t_gate_up)));
+  o.rows = l.take(T * g.C * g.B * 2);
+  o.mid = l.take(T * F * 2);
+  o.grads[0] = l.take(sums_bytes(d.gate, d.d_gate != nullptr, d.gate_dtype));
+  o.grads[1] = l.take(sums_bytes(d.up, d.d_up != nullptr, d.up_dtype));
+  o.grads[2] = l.take(sums_bytes(d.down, d.d_down != nullptr, d.down_dtype));
+  o.dgu = l.take(T * 2 * F * 2);
+  o.total = l.at;
+  return o;
+}
+
+// One tile gradient's place: its fp32 sums (the result itself, or workspace) and
+// its bf16 result.
+struct Grad {
+  float* sums = nullptr;
+  void* rounded = nullptr;
+  int64_t n = 0;
+};
+static Grad grad_of(const BellMxEll& w, void* out, int32_t dtype, char* ws) {
+  if (!out) return Grad{};
+  const bool half = dtype == BELL_DTYPE_BF16;
+  return Grad{half ? reinterpret_cast<float*>(ws) : static_cast<float*>(out), half ? out : nullptr,
+              int64_t(w.R) * w.K * w.B * w.B};
 }
 
 static int tile_grad(int64_t T, const void* a, const void* b, int64_t ldb, const int32_t* cols, const BellMxEll& w,
-                     int32_t layout, void* out, int32_t dtype, void* sums, int32_t* status, void* stream) {
+                     int32_t layout, const Grad& g, int32_t* status, void* stream) {
+  if (!g.sums) return BELL_OK;
   BellSddmmDesc s{};
   s.T = T;
   s.a = a;
@@ -72,19 +101,20 @@ static int tile_grad(int64_t T, const void* a, const void* b, int64_t ldb, const
   s.K = w.K;
   s.B = w.B;
   s.layout = layout;
-  s.grad = static_cast<float*>(dtype == BELL_DTYPE_BF16 ? sums : out);
-  s.grad_bf16 = dtype == BELL_DTYPE_BF16 ? out : nullptr;
+  s.accumulate = 1;  // onto the zeros written with the unpacked operands
+  s.grad = g.sums;
   s.status = status;
   return bell_sddmm_bf16(&s, stream);
 }
 
-// Transposed weight in bf16: rows = column blocks of the (stacked) weight.
-// Tiles are unpacked [B_out, B_in], which their transpose reads as [B_in, B_out].
-static int transposed(const BellMxEll& w0, const BellMxEll* w1, const int32_t* cols_t, const int64_t* index, int32_t K_t,
-                      int32_t C_t, void* tiles, BellEll* out, void* stream) {
-  *out = BellEll{tiles, cols_t, w0.C, C_t, K_t, w0.B, BELL_TILE_IN_OUT, 0};
-  return bell_mx_unpack_tiles(w0.chunks, int64_t(w0.R) * w0.K, w1 ? w1->chunks : nullptr, w1 ? int64_t(w1->R) * w1->K : 0,
-                              w0.B, index, int64_t(w0.C) * K_t, tiles, stream);
+static int round_all(const Grad (&g)[3], cudaStream_t s) {
+  RoundArgs a{};
+  for (int i = 0; i < 3; ++i) {
+    a.src[i] = g[i].sums;
+    a.dst[i] = g[i].rounded;
+    a.n[i] = g[i].rounded ? g[i].n : 0;
+  }
+  return round_sums(a, s);
 }
 
 static int product(int64_t T, const void* x, const BellEll& w, const void* residual, void* out, void* plan,
@@ -134,17 +164,27 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   if (!d->workspace || !aligned16(d->workspace)) return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned");
   if (int rc = require_sm100()) return rc;
   char* ws = static_cast<char*>(d->workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const mx::BwdWs o = mx::linear_ws(*d);
-  if (d->dx && d->T > 0) {
-    BellEll wt;
-    if (int rc = mx::transposed(w, nullptr, d->cols_t, d->index_t, d->K_t, w.R, ws + o.tiles, &wt, stream)) return rc;
+  const bool want_dx = d->dx && d->T > 0;
+  const int32_t in_f = w.C * w.B;
+  const mx::Grad grads[3] = {mx::grad_of(w, d->dw, d->grad_dtype, ws + o.grads[0]), {}, {}};
+  mx::ExpandArgs e{};
+  e.T = d->T;
+  e.B = w.B;
+  if (want_dx)
+    e.gather[0] = {w.chunks, int64_t(w.R) * w.K, nullptr, 0, d->index_t, int64_t(w.C) * d->K_t, ws + o.tiles};
+  if (d->dw && d->T > 0) e.rows[0] = {d->x, in_f, ws + o.rows};
+  e.zero[0] = {grads[0].sums, grads[0].n};
+  if (int rc = mx::expand(e, s)) return rc;
+  if (want_dx) {
+    const BellEll wt{ws + o.tiles, d->cols_t, w.C, w.R, d->K_t, w.B, BELL_TILE_IN_OUT, 0};
     if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, ws + o.plan, d->status, stream)) return rc;
   }
-  if (!d->dw) return BELL_OK;
-  const int32_t in_f = w.C * w.B;
-  if (int rc = bell_mx_dequantize_rows(d->T, in_f, w.B, d->x, BELL_DTYPE_BF16, ws + o.rows, in_f, stream)) return rc;
-  return mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, d->dw,
-                       d->grad_dtype, ws + o.grads, d->status, stream);
+  if (int rc = mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, grads[0],
+                             d->status, stream))
+    return rc;
+  return mx::round_all(grads, s);
 }
 
 size_t bell_swiglu_bwd_mx_workspace_bytes(const BellMxFFNBwdDesc* d) {
@@ -175,16 +215,33 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   if (!d->workspace || !aligned16(d->workspace)) return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned");
   if (int rc = require_sm100()) return rc;
   char* ws = static_cast<char*>(d->workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const mx::BwdWs o = mx::swiglu_ws(*d);
   const int32_t F = g.R * g.B, D = g.C * g.B;
-  char* dgu = ws + o.dgu;
-  BellEll wt;
-  if (d->T > 0 && (d->dx || d->d_gate || d->d_up)) {
-    if (int rc = mx::transposed(w, nullptr, d->cols_t_down, d->index_t_down, d->K_t_down, w.R, ws + o.tiles, &wt, stream))
-      return rc;
+  const int64_t T = d->T;
+  const bool want_dgu = T > 0 && (d->dx || d->d_gate || d->d_up), want_dx = T > 0 && d->dx;
+  char *dgu = ws + o.dgu, *mid = ws + o.mid;
+  const mx::Grad grads[3] = {mx::grad_of(g, d->d_gate, d->gate_dtype, ws + o.grads[0]),
+                             mx::grad_of(u, d->d_up, d->up_dtype, ws + o.grads[1]),
+                             mx::grad_of(w, d->d_down, d->down_dtype, ws + o.grads[2])};
+  mx::ExpandArgs e{};
+  e.T = T;
+  e.B = g.B;
+  if (want_dgu)
+    e.gather[0] = {w.chunks, int64_t(w.R) * w.K, nullptr, 0, d->index_t_down, int64_t(g.R) * d->K_t_down,
+                   ws + o.tiles_down};
+  if (want_dx)
+    e.gather[1] = {g.chunks, int64_t(g.R) * g.K, u.chunks, int64_t(u.R) * u.K, d->index_t_gate_up,
+                   int64_t(g.C) * d->K_t_gate_up, ws + o.tiles};
+  if (T > 0 && (d->d_gate || d->d_up)) e.rows[0] = {d->x, D, ws + o.rows};
+  if (T > 0 && d->d_down && g.B == 64) e.rows[1] = {d->h, F, mid};
+  for (int i = 0; i < 3; ++i) e.zero[i] = {grads[i].sums, grads[i].n};
+  if (int rc = mx::expand(e, s)) return rc;
+  if (want_dgu) {
+    const BellEll wt{ws + o.tiles_down, d->cols_t_down, g.R, w.R, d->K_t_down, g.B, BELL_TILE_IN_OUT, 0};
     if (g.B == 64) {
       BellDownBwdDesc b{};
-      b.T = d->T;
+      b.T = T;
       b.grad_out = d->grad_out;
       b.gate_pre = d->gate_pre;
       b.up_out = d->up_out;
@@ -194,37 +251,25 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
       b.status = d->status;
       if (int rc = bell_down_silu_bwd_bf16(&b, stream)) return rc;
     } else {
-      if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, ws + o.mid, ws + o.plan, d->status, stream)) return rc;
-      if (int rc = bell_silu_mul_bwd_bf16(d->T, F, ws + o.mid, d->gate_pre, d->up_out, dgu, dgu + size_t(F) * 2,
-                                          int64_t(F) * 2, stream))
+      if (int rc = mx::product(T, d->grad_out, wt, nullptr, mid, ws + o.plan, d->status, stream)) return rc;
+      if (int rc = bell_silu_mul_bwd_bf16(T, F, mid, d->gate_pre, d->up_out, dgu, dgu + size_t(F) * 2, int64_t(F) * 2, stream))
         return rc;
     }
   }
-  if (d->T > 0 && d->dx) {
-    if (int rc = mx::transposed(g, &u, d->cols_t_gate_up, d->index_t_gate_up, d->K_t_gate_up, 2 * g.R, ws + o.tiles, &wt,
-                                stream))
-      return rc;
-    if (int rc = mx::product(d->T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, ws + o.plan, d->status, stream))
+  if (want_dx) {
+    const BellEll wt{ws + o.tiles, d->cols_t_gate_up, g.C, 2 * g.R, d->K_t_gate_up, g.B, BELL_TILE_IN_OUT, 0};
+    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, ws + o.plan, d->status, stream))
       return rc;
   }
-  if (d->d_gate || d->d_up) {
-    if (int rc = bell_mx_dequantize_rows(d->T, D, g.B, d->x, BELL_DTYPE_BF16, ws + o.rows, D, stream)) return rc;
-    if (d->d_gate)
-      if (int rc = mx::tile_grad(d->T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, d->d_gate,
-                                 d->gate_dtype, ws + o.grads, d->status, stream))
-        return rc;
-    if (d->d_up)
-      if (int rc = mx::tile_grad(d->T, ws + o.rows, dgu + size_t(F) * 2, int64_t(F) * 2, d->cols_up, u, d->layout, d->d_up,
-                                 d->up_dtype, ws + o.grads, d->status, stream))
-        return rc;
-  }
-  if (d->d_down) {
-    if (int rc = bell_mx_dequantize_rows(d->T, F, g.B, d->h, BELL_DTYPE_BF16, ws + o.mid, F, stream)) return rc;
-    if (int rc = mx::tile_grad(d->T, ws + o.mid, d->grad_out, D, d->cols_down, w, d->layout, d->d_down, d->down_dtype,
-                               ws + o.grads, d->status, stream))
-      return rc;
-  }
-  return BELL_OK;
+  if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads[0], d->status, stream))
+    return rc;
+  if (int rc = mx::tile_grad(T, ws + o.rows, dgu + size_t(F) * 2, int64_t(F) * 2, d->cols_up, u, d->layout, grads[1],
+                             d->status, stream))
+    return rc;
+  if (T > 0 && d->d_down && g.B == 128)
+    if (int rc = bell_mx_dequantize_rows(T, F, g.B, d->h, BELL_DTYPE_BF16, mid, F, stream)) return rc;
+  if (int rc = mx::tile_grad(T, mid, d->grad_out, D, d->cols_down, w, d->layout, grads[2], d->status, stream)) return rc;
+  return mx::round_all(grads, s);
 }
 
 }  // extern "C"

@@ -3,7 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <climits>
+#include <algorithm>
 #include <string>
 
 #include "bell_mx.cuh"
@@ -80,24 +80,33 @@ __global__ void __launch_bounds__(kThr) bell_mx_quantize_kernel(RowsArgs a, cons
   }
 }
 
+__device__ __forceinline__ void unpack32(uint4 q, float s, float (&v)[32]) {
+  unpack_e2m1(q.x, s, v);
+  unpack_e2m1(q.y, s, v + 8);
+  unpack_e2m1(q.z, s, v + 16);
+  unpack_e2m1(q.w, s, v + 24);
+}
+
 template <class E>
-__global__ void __launch_bounds__(kThr) bell_mx_dequantize_kernel(RowsArgs a, const uint8_t* __restrict__ src,
-                                                                 E* __restrict__ dst, int64_t ld) {
+__device__ __forceinline__ void dequantize_rows(const RowsArgs& a, const uint8_t* __restrict__ src, E* __restrict__ dst,
+                                                int64_t ld) {
   const int lane = threadIdx.x & 31;
   for (int64_t w = (int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5; w < a.groups; w += int64_t(gridDim.x) * (kThr / 32)) {
     int64_t t, chunk;
     int32_t f;
     int n, j;
     if (!locate(a, w, lane, t, f, chunk, n, j)) continue;
-    const uint4 q = ld_global_nc_v4(src + chunk + code_off(n, j, kRows * 32));
-    const float s = scale_value(src[chunk + a.B * (kRows / 2) + scale_off(n, j)]);
     float v[32];
-    unpack_e2m1(q.x, s, v);
-    unpack_e2m1(q.y, s, v + 8);
-    unpack_e2m1(q.z, s, v + 16);
-    unpack_e2m1(q.w, s, v + 24);
+    unpack32(ld_global_nc_v4(src + chunk + code_off(n, j, kRows * 32)),
+             scale_value(src[chunk + a.B * (kRows / 2) + scale_off(n, j)]), v);
     store32(dst + t * ld + f, v);
   }
+}
+
+template <class E>
+__global__ void __launch_bounds__(kThr) bell_mx_dequantize_kernel(RowsArgs a, const uint8_t* __restrict__ src,
+                                                                 E* __restrict__ dst, int64_t ld) {
+  dequantize_rows(a, src, dst, ld);
 }
 
 // One warp per block-row: the live slots, compacted in slot order.
@@ -120,15 +129,21 @@ __device__ __forceinline__ void plan_row(const int32_t* __restrict__ cols, int r
   if (bad) atomicOr(status, BELL_STATUS_COLIDX);
 }
 
-struct PackArgs {
+struct PackWeight {
+  const void* values;
   int64_t tiles;
   int32_t B, in_out;
   const int32_t* cols;
   int32_t R, C, K;
+  uint8_t* chunks;
   uint32_t* entries;
   int32_t* counts;
+  unsigned plan_end;  // blocks [.., plan_end) of the grid write the plan, a warp to a block-row
+};
+struct PackArgs {
+  PackWeight w[BELL_MX_PACK_MAX];
+  int32_t n;
   int32_t* status;
-  unsigned plan_blocks;  // blocks of the grid that write the plan, a warp to a block-row
 };
 
 __device__ __forceinline__ void put_block(uint8_t* chunk, int B, int o, int j, const float (&v)[32]) {
@@ -147,63 +162,93 @@ __device__ __forceinline__ float2 load_pair(const float* p) { return __ldg(reint
 // tiles are read a row of outputs at a time (lane = output pair): the 32 values
 // of a block are strided and a warp's loads contiguous.
 template <class E>
-__global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const E* __restrict__ values, PackArgs a,
-                                                           uint8_t* __restrict__ chunks) {
-  if (blockIdx.x < a.plan_blocks) {
-    const int r = int(blockIdx.x) * (kThr / 32) + int(threadIdx.x >> 5);
-    if (r < a.R) plan_row(a.cols, r, a.C, a.K, a.entries, a.counts, a.status);
+__global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const PackArgs a) {
+  const unsigned plans = a.w[a.n - 1].plan_end;
+  if (blockIdx.x < plans) {
+    int i = 0;
+    while (blockIdx.x >= a.w[i].plan_end) ++i;
+    const PackWeight& w = a.w[i];
+    const int r = int(blockIdx.x - (i ? a.w[i - 1].plan_end : 0u)) * (kThr / 32) + int(threadIdx.x >> 5);
+    if (r < w.R) plan_row(w.cols, r, w.C, w.K, w.entries, w.counts, a.status);
     return;
   }
-  const int B = a.B, blocks = B / kBlock, per_tile = B / 2 * blocks;
-  const int64_t stride = int64_t(gridDim.x - a.plan_blocks) * kThr;
-  for (int64_t i = int64_t(blockIdx.x - a.plan_blocks) * kThr + threadIdx.x; i < a.tiles * per_tile; i += stride) {
-    const int64_t tile = i / per_tile;
-    const int e = int(i - tile * per_tile);
-    const E* v0 = values + tile * B * B;
-    uint8_t* ch = chunks + tile * tile_chunk(B);
-    float v[32], w[32];
-    if (a.in_out) {
-      const int o = e % (B / 2) * 2, j = e / (B / 2);
+  for (int i = 0; i < a.n; ++i) {
+    const PackWeight& p = a.w[i];
+    const int B = p.B, blocks = B / kBlock, per_tile = B / 2 * blocks;
+    const int64_t stride = int64_t(gridDim.x - plans) * kThr, n = p.tiles * per_tile;
+    for (int64_t at = int64_t(blockIdx.x - plans) * kThr + threadIdx.x; at < n; at += stride) {
+      const int64_t tile = at / per_tile;
+      const int e = int(at - tile * per_tile);
+      const E* v0 = static_cast<const E*>(p.values) + tile * B * B;
+      uint8_t* ch = p.chunks + tile * tile_chunk(B);
+      float v[32], w[32];
+      if (p.in_out) {
+        const int o = e % (B / 2) * 2, j = e / (B / 2);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float2 f = load_pair(v0 + (j * kBlock + k) * B + o);
-        v[k] = f.x;
-        w[k] = f.y;
+        for (int k = 0; k < 32; ++k) {
+          const float2 f = load_pair(v0 + (j * kBlock + k) * B + o);
+          v[k] = f.x;
+          w[k] = f.y;
+        }
+        put_block(ch, B, o, j, v);
+        put_block(ch, B, o + 1, j, w);
+      } else {
+        const int j = e % blocks, o = e / blocks * 2;
+        load32(v0 + o * B + j * kBlock, v);
+        load32(v0 + (o + 1) * B + j * kBlock, w);
+        put_block(ch, B, o, j, v);
+        put_block(ch, B, o + 1, j, w);
       }
-      put_block(ch, B, o, j, v);
-      put_block(ch, B, o + 1, j, w);
-    } else {
-      const int j = e % blocks, o = e / blocks * 2;
-      load32(v0 + o * B + j * kBlock, v);
-      load32(v0 + (o + 1) * B + j * kBlock, w);
-      put_block(ch, B, o, j, v);
-      put_block(ch, B, o + 1, j, w);
     }
   }
 }
 
-// Tiles back to bf16 [B_out, B_in], out tile i from tile index[i] (or i) of
-// the n0 tiles at c0 followed by those at c1.
-__global__ void __launch_bounds__(kThr) bell_mx_unpack_kernel(const uint8_t* __restrict__ c0, int64_t n0,
-                                                             const uint8_t* __restrict__ c1, int64_t n1,
-                                                             const int64_t* __restrict__ index, int64_t tiles,
-                                                             int32_t B, __nv_bfloat16* __restrict__ values) {
+// Tiles back to bf16 [B_out, B_in].
+__device__ __forceinline__ void unpack_tiles(const TileGather& g, int32_t B) {
   const int blocks = B / kBlock, per_tile = B * blocks;
-  for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
+  __nv_bfloat16* values = static_cast<__nv_bfloat16*>(g.values);
+  for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < g.tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
     const int64_t tile = i / per_tile;
     const int e = int(i - tile * per_tile), j = e % blocks, o = e / blocks;
-    const int64_t from = index ? index[tile] : tile;
-    if (from < 0 || from >= n0 + n1) continue;
-    const uint8_t* ch = from < n0 ? c0 + from * tile_chunk(B) : c1 + (from - n0) * tile_chunk(B);
-    const uint4 q = ld_global_nc_v4(ch + code_off(o, j, B * 32));
-    const float s = scale_value(ch[B * B / 2 + scale_off(o, j)]);
+    const int64_t from = g.index ? g.index[tile] : tile;
+    if (from < 0 || from >= g.n0 + g.n1) continue;
+    const uint8_t* ch = static_cast<const uint8_t*>(from < g.n0 ? g.c0 : g.c1) + (from < g.n0 ? from : from - g.n0) * tile_chunk(B);
     float v[32];
-    unpack_e2m1(q.x, s, v);
-    unpack_e2m1(q.y, s, v + 8);
-    unpack_e2m1(q.z, s, v + 16);
-    unpack_e2m1(q.w, s, v + 24);
+    unpack32(ld_global_nc_v4(ch + code_off(o, j, B * 32)), scale_value(ch[B * B / 2 + scale_off(o, j)]), v);
     store32(values + tile * B * B + o * B + j * kBlock, v);
   }
+}
+
+__global__ void __launch_bounds__(kThr) bell_mx_unpack_kernel(const TileGather g, int32_t B) { unpack_tiles(g, B); }
+
+// What a backward needs before its products, in one launch: gathered tiles,
+// rows, and zeros for the sums of the tile gradients.
+struct ExpandKernelArgs {
+  ExpandArgs e;
+  RowsArgs rows[2];
+};
+__global__ void __launch_bounds__(kThr) bell_mx_expand_kernel(const ExpandKernelArgs a) {
+  for (int i = 0; i < 2; ++i)
+    if (a.e.gather[i].tiles) unpack_tiles(a.e.gather[i], a.e.B);
+  for (int i = 0; i < 2; ++i)
+    if (a.e.rows[i].dst)
+      dequantize_rows(a.rows[i], static_cast<const uint8_t*>(a.e.rows[i].src), static_cast<__nv_bfloat16*>(a.e.rows[i].dst),
+                      a.e.rows[i].features);
+  for (int i = 0; i < 3; ++i)
+    for (int64_t k = int64_t(blockIdx.x) * kThr + threadIdx.x; k < a.e.zero[i].floats / 4; k += int64_t(gridDim.x) * kThr)
+      st_global_v4(a.e.zero[i].at + 4 * k, 0u, 0u, 0u, 0u);
+}
+
+// The fp32 sums of up to three tile gradients to bf16.
+__global__ void __launch_bounds__(kThr) bell_mx_round_kernel(const RoundArgs a) {
+  for (int i = 0; i < 3; ++i)
+    for (int64_t k = int64_t(blockIdx.x) * kThr + threadIdx.x; k < a.n[i] / 8; k += int64_t(gridDim.x) * kThr) {
+      const uint4 x = ld_global_v4(a.src[i] + 8 * k), y = ld_global_v4(a.src[i] + 8 * k + 4);
+      st_global_v4(static_cast<__nv_bfloat16*>(a.dst[i]) + 8 * k, pack_bf16x2(__uint_as_float(x.x), __uint_as_float(x.y)),
+                   pack_bf16x2(__uint_as_float(x.z), __uint_as_float(x.w)),
+                   pack_bf16x2(__uint_as_float(y.x), __uint_as_float(y.y)),
+                   pack_bf16x2(__uint_as_float(y.z), __uint_as_float(y.w)));
+    }
 }
 
 // Grid of grid-stride kernels: enough blocks for every SM's 2048 threads.
@@ -237,6 +282,34 @@ static RowsArgs rows_args(int64_t T, int32_t features, int32_t B) {
   a.col_groups = (features + 127) / 128;
   a.groups = (T + 7) / 8 * a.col_groups;
   return a;
+}
+
+int expand(const ExpandArgs& e, cudaStream_t s) {
+  ExpandKernelArgs a{};
+  a.e = e;
+  int64_t most = 0;
+  for (int i = 0; i < 2; ++i) {
+    most = std::max(most, e.gather[i].tiles * e.B * (e.B / kBlock));
+    if (e.rows[i].dst) {
+      a.rows[i] = rows_args(e.T, e.rows[i].features, e.B);
+      most = std::max(most, a.rows[i].groups * 32);
+    }
+  }
+  for (const Zeros& z : e.zero) most = std::max(most, z.floats / 4);
+  if (!most) return BELL_OK;
+  unsigned grid;
+  if (int rc = grid_for(most, &grid)) return rc;
+  bell_mx_expand_kernel<<<grid, kThr, 0, s>>>(a);
+  return check_launch("bell_mx_expand_kernel");
+}
+
+int round_sums(const RoundArgs& a, cudaStream_t s) {
+  const int64_t most = std::max({a.n[0], a.n[1], a.n[2]}) / 8;
+  if (!most) return BELL_OK;
+  unsigned grid;
+  if (int rc = grid_for(most, &grid)) return rc;
+  bell_mx_round_kernel<<<grid, kThr, 0, s>>>(a);
+  return check_launch("bell_mx_round_kernel");
 }
 
 }  // namespace mx
@@ -289,44 +362,46 @@ int bell_mx_dequantize_rows(int64_t T, int32_t features, int32_t B, const void* 
   return check_launch("bell_mx_dequantize_rows");
 }
 
-int bell_mx_pack_ell(const BellEll* w, int32_t dtype, void* chunks, void* plan, int32_t* status, void* stream) {
-  if (!w || !w->values || !w->col_indices || !chunks || !plan) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: NULL argument");
-  if (w->B != 64 && w->B != 128) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: tile size B must be 64 or 128");
-  if (w->R < 1 || w->C < 1 || w->K < 1) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R, C, K must be >= 1");
-  if (w->R > (1 << 23) || w->C > 65535 || w->K > 65535)
-    return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R must be <= 2^23, C and K <= 65535");
+int bell_mx_pack_ell(const BellEll* weights, int32_t n, int32_t dtype, void* const* chunks, void* const* plans,
+                     int32_t* status, void* stream) {
+  if (!weights || !chunks || !plans) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: NULL argument");
+  if (n < 1 || n > BELL_MX_PACK_MAX) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: 1 to BELL_MX_PACK_MAX weights");
   if (dtype != BELL_DTYPE_BF16 && dtype != BELL_DTYPE_F32)
     return fail(BELL_ERR_DTYPE, "bell_mx_pack_ell: dtype must be bf16 or f32");
-  if (w->layout != BELL_TILE_IN_OUT && w->layout != BELL_TILE_OUT_IN)
-    return fail(BELL_ERR_ARG, "bell_mx_pack_ell: unknown tile layout");
-  if (!aligned16(w->values) || !aligned16(chunks) || !aligned16(plan))
-    return fail(BELL_ERR_ALIGN, "bell_mx_pack_ell: values, chunks and plan must be 16-byte aligned");
-  if (int rc = require_sm100()) return rc;
-  int32_t* st = status ? status : default_status_ptr();
-  if (!st) return BELL_ERR_LAUNCH;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t tiles = int64_t(w->R) * w->K;
-  unsigned grid;
-  if (int rc = mx::grid_for(tiles * (w->B / 2) * (w->B / mx::kBlock), &grid)) return rc;
-  const mx::Plan p = mx::plan_of(plan, w->R, w->K);
   mx::PackArgs a{};
-  a.tiles = tiles;
-  a.B = w->B;
-  a.in_out = w->layout == BELL_TILE_IN_OUT;
-  a.cols = w->col_indices;
-  a.R = w->R;
-  a.C = w->C;
-  a.K = w->K;
-  a.entries = const_cast<uint32_t*>(p.entries);
-  a.counts = const_cast<int32_t*>(p.counts);
-  a.status = st;
-  a.plan_blocks = unsigned((w->R + mx::kThr / 32 - 1) / (mx::kThr / 32));
-  grid += a.plan_blocks;
-  uint8_t* dst = static_cast<uint8_t*>(chunks);
+  a.n = n;
+  int64_t most = 0;
+  unsigned plan_end = 0;
+  for (int i = 0; i < n; ++i) {
+    const BellEll& w = weights[i];
+    if (!w.values || !w.col_indices || !chunks[i] || !plans[i]) return fail(BELL_ERR_ARG, "bell_mx_pack_ell: NULL argument");
+    if (w.B != 64 && w.B != 128) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: tile size B must be 64 or 128");
+    if (w.R < 1 || w.C < 1 || w.K < 1) return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R, C, K must be >= 1");
+    if (w.R > (1 << 23) || w.C > 65535 || w.K > 65535)
+      return fail(BELL_ERR_SHAPE, "bell_mx_pack_ell: R must be <= 2^23, C and K <= 65535");
+    if (w.layout != BELL_TILE_IN_OUT && w.layout != BELL_TILE_OUT_IN)
+      return fail(BELL_ERR_ARG, "bell_mx_pack_ell: unknown tile layout");
+    if (!aligned16(w.values) || !aligned16(chunks[i]) || !aligned16(plans[i]))
+      return fail(BELL_ERR_ALIGN, "bell_mx_pack_ell: values, chunks and plans must be 16-byte aligned");
+    const mx::Plan p = mx::plan_of(plans[i], w.R, w.K);
+    const int64_t tiles = int64_t(w.R) * w.K;
+    plan_end += unsigned((w.R + mx::kThr / 32 - 1) / (mx::kThr / 32));
+    a.w[i] = mx::PackWeight{w.values, tiles, w.B, w.layout == BELL_TILE_IN_OUT, w.col_indices, w.R, w.C, w.K,
+                            static_cast<uint8_t*>(chunks[i]), const_cast<uint32_t*>(p.entries),
+                            const_cast<int32_t*>(p.counts), plan_end};
+    most = std::max(most, tiles * (w.B / 2) * (w.B / mx::kBlock));
+  }
+  if (int rc = require_sm100()) return rc;
+  a.status = status ? status : default_status_ptr();
+  if (!a.status) return BELL_ERR_LAUNCH;
+  unsigned grid;
+  if (int rc = mx::grid_for(most, &grid)) return rc;
+  grid += plan_end;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BELL_DTYPE_BF16)
-    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const __nv_bfloat16*>(w->values), a, dst);
+    mx::bell_mx_pack_kernel<__nv_bfloat16><<<grid, mx::kThr, 0, s>>>(a);
   else
-    mx::bell_mx_pack_kernel<<<grid, mx::kThr, 0, s>>>(static_cast<const float*>(w->values), a, dst);
+    mx::bell_mx_pack_kernel<float><<<grid, mx::kThr, 0, s>>>(a);
   return check_launch("bell_mx_pack_kernel");
 }
 
@@ -344,8 +419,7 @@ int bell_mx_unpack_tiles(const void* chunks0, int64_t tiles0, const void* chunks
   unsigned grid;
   if (int rc = mx::grid_for(tiles * B * (B / mx::kBlock), &grid)) return rc;
   mx::bell_mx_unpack_kernel<<<grid, mx::kThr, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint8_t*>(chunks0), tiles0, static_cast<const uint8_t*>(chunks1), tiles1, index, tiles, B,
-      static_cast<__nv_bfloat16*>(values));
+      mx::TileGather{chunks0, tiles0, chunks1, tiles1, index, tiles, values}, B);
   return check_launch("bell_mx_unpack_kernel");
 }
 

@@ -163,7 +163,8 @@ SIGNATURES = {
                                         C.c_void_p]),
     "bell_mx_dequantize_rows": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
                                           C.c_int64, C.c_void_p]),
-    "bell_mx_pack_ell": (C.c_int, [C.POINTER(BellEll), C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "bell_mx_pack_ell": (C.c_int, [C.POINTER(BellEll), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_void_p]),
     "bell_mx_unpack_tiles": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64,
                                        C.c_void_p, C.c_void_p]),
     "bell_linear_mx": (C.c_int, [C.POINTER(BellMxLinearDesc), C.c_void_p]),

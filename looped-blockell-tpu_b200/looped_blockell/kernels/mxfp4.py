@@ -184,22 +184,38 @@ def make_mxfp4(values: torch.Tensor, col_indices: torch.Tensor, C_blocks: int, l
     """Quantise the tiles of a Block-ELL weight (``values [R, K, B, B]`` bf16 or
     fp32, B 64 or 128) and list its live slots.  A column index of -1 is a dead
     slot; one outside [0, C_blocks) is dropped and sets the status word."""
-    dtype = values.dtype
+    return _pack(((values, col_indices, C_blocks),), layout)[0]
+
+
+def _pack(weights, layout: int):
+    """``make_mxfp4`` of several (values, col_indices, C_blocks), one launch for
+    those of one dtype."""
+    dtype = weights[0][0].dtype
+    if any(v.dtype != dtype for v, _, _ in weights):
+        return [_pack((w,), layout)[0] for w in weights]
     if dtype not in _DTYPES:
         raise RuntimeError("tiles must be bf16 or fp32")
-    v, cols = _prep_ell("weight", values, col_indices, dtype)
-    R, K, B, B2 = v.shape
-    _check_tile(B)
-    if B2 != B or tuple(cols.shape) != (R, K):
-        raise RuntimeError(f"values {tuple(v.shape)} and col_indices {tuple(cols.shape)} do not fit")
-    dev = v.device
-    if cols.device != dev:
-        raise RuntimeError("values and col_indices must be on one device")
-    n = _tiles_bytes(R, K, B)
-    data = _bytes(n + plan_bytes(0, 0, 0, R, K), dev)
-    w = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, int(C_blocks), K, B, layout, 0)
-    _call("bell_mx_pack_ell", dev, C.byref(w), _DTYPES[dtype], data.data_ptr(), data.data_ptr() + n, None)
-    return MXBlockELL(data, cols, R, K, int(C_blocks), B)
+    n, dev, out = len(weights), weights[0][0].device, []
+    abi, chunks, plans = (_lib.BellEll * n)(), (C.c_void_p * n)(), (C.c_void_p * n)()
+    held = []  # copies that must outlive the launch's enqueueing
+    for i, (values, col_indices, C_blocks) in enumerate(weights):
+        v, cols = _prep_ell("weight", values, col_indices, dtype)
+        R, K, B, B2 = v.shape
+        _check_tile(B)
+        if B2 != B or tuple(cols.shape) != (R, K):
+            raise RuntimeError(f"values {tuple(v.shape)} and col_indices {tuple(cols.shape)} do not fit")
+        if v.device != dev or cols.device != dev:
+            raise RuntimeError("values and col_indices must be on one device")
+        if v.data_ptr() % 16:
+            v = v.clone()
+        size = _tiles_bytes(R, K, B)
+        data = _bytes(size + plan_bytes(0, 0, 0, R, K), dev)
+        abi[i] = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, int(C_blocks), K, B, layout, 0)
+        chunks[i], plans[i] = data.data_ptr(), data.data_ptr() + size
+        held.append(v)
+        out.append(MXBlockELL(data, cols, R, K, int(C_blocks), B))
+    _call("bell_mx_pack_ell", dev, abi, n, _DTYPES[dtype], chunks, plans, None)
+    return out
 
 
 def _check_weight(w: MXBlockELL, dev: torch.device) -> None:
@@ -379,8 +395,7 @@ class MXSwiGLUFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, v_gate, ci_gate, v_up, ci_up, v_down, ci_down, add_residual, layout):
         C_model, R_ff = x.shape[1] // v_gate.shape[2], v_gate.shape[0]
-        gate, up = make_mxfp4(v_gate, ci_gate, C_model, layout), make_mxfp4(v_up, ci_up, C_model, layout)
-        down = make_mxfp4(v_down, ci_down, R_ff, layout)
+        gate, up, down = _pack(((v_gate, ci_gate, C_model), (v_up, ci_up, C_model), (v_down, ci_down, R_ff)), layout)
         out, ws = mxfp4_swiglu_fwd(x, gate, up, down, add_residual=add_residual, return_intermediates=True)
         ctx.weights = (gate, up, down)
         ctx.save_for_backward(ws["gate"], ws["up"], ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down, gate.data,

@@ -92,12 +92,13 @@ def test_pack_refusals():
     lib = L.load()
     ok = dict(values=1024, col_indices=1024, R=2, C=2, K=2, B=64, layout=0, flags=0)
 
-    def call(dtype=0, chunks=1024, plan=1024, **kw):
-        return lib.bell_mx_pack_ell(C.byref(L.BellEll(*{**ok, **kw}.values())), dtype, chunks, plan, None, None)
+    def call(dtype=0, chunks=1024, plan=1024, n=1, **kw):
+        return lib.bell_mx_pack_ell(C.byref(L.BellEll(*{**ok, **kw}.values())), n, dtype, (C.c_void_p * 1)(chunks),
+                                    (C.c_void_p * 1)(plan), None, None)
 
-    assert call(B=32) == -2 and call(K=0) == -2 and call(C=1 << 16) == -2
+    assert call(B=32) == -2 and call(K=0) == -2 and call(C=1 << 16) == -2 and call(R=1 << 24) == -2
     assert call(dtype=3) == -1 and call(layout=5) == -8 and call(values=None) == -8 and call(plan=None) == -8
-    assert call(values=1032) == -3
+    assert call(values=1032) == -3 and call(n=0) == -8 and call(n=4) == -8
     assert lib.bell_mx_unpack_tiles(1024, 2, None, 0, 64, None, 3, 1024, None) == -2
     assert lib.bell_mx_unpack_tiles(1024, 2, None, 0, 32, None, 2, 1024, None) == -2
 
@@ -171,7 +172,7 @@ def test_backward_refusals():
     assert lib.bell_linear_bwd_mx(C.byref(d), None) == -8
     d.grad_dtype, d.workspace = 0, None
     assert lib.bell_linear_bwd_mx(C.byref(d), None) == -3
-    d.K_t = 1
+    d.K_t, d.dx = 1, 1024
     # unpacked transpose [3, 1] tiles + plan + Q(x) + fp32 sums of [2, 2] tiles, each padded to 256 bytes
     assert lib.bell_linear_bwd_mx_workspace_bytes(C.byref(d)) == 3 * 64 * 64 * 2 + 256 + 4 * 192 * 2 + 4 * 64 * 64 * 4
     f = L.BellMxFFNBwdDesc()

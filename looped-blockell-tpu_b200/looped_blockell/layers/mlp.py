@@ -18,6 +18,11 @@ indices) is rebuilt only when the parameter or the topology buffers change,
 which in-place updates such as an optimizer step report through the tensor's
 version counter.  Writes through ``.data`` bypass that counter: call
 ``refresh()`` after them.
+
+``weight_format="mxfp4"`` (tile sizes 64 and 128) computes with MXFP4 weights
+and activations (``kernels.mxfp4``): quantised from the parameters on every
+training step, with the gradient passing straight through the quantisation,
+and once per parameter version without gradients.
 """
 
 from __future__ import annotations
@@ -37,9 +42,14 @@ class BlockELLLinear(nn.Module):
     """Single Block-ELL linear layer (reference mlp.py:28-95)."""
 
     def __init__(self, out_features: int, in_features: int, tile_size: int = 16, density: float = 1.0,
-                 dtype: torch.dtype = torch.bfloat16, bias: bool = True, device=None):
+                 dtype: torch.dtype = torch.bfloat16, bias: bool = True, device=None, weight_format: str = "native"):
         super().__init__()
         B = tile_size
+        if weight_format not in ("native", "mxfp4"):
+            raise ValueError(f"weight_format must be 'native' or 'mxfp4', got {weight_format!r}")
+        if weight_format == "mxfp4" and B not in (64, 128):
+            raise ValueError(f"weight_format 'mxfp4' needs tile_size 64 or 128, got {B}")
+        self.weight_format = weight_format
         if out_features % B or in_features % B:
             raise ValueError(f"features ({out_features}, {in_features}) must be divisible by tile_size {B}")
         self.out_features, self.in_features, self.tile_size, self.density = out_features, in_features, B, density
@@ -87,13 +97,26 @@ class BlockELLLinear(nn.Module):
         key = (v.data_ptr(), v._version, v.dtype)
         return self._cached("values", key, lambda: v.detach().to(self.dtype).contiguous())
 
+    def mxfp4_weight(self):
+        """The quantised weight (``kernels.MXBlockELL``) of the current parameters."""
+        from ..kernels.mxfp4 import make_mxfp4
+        v, cols = self.values, self.effective_col_indices()
+        key = (v.data_ptr(), v._version, v.dtype, cols.data_ptr(), cols._version)
+        return self._cached("mxfp4", key, lambda: make_mxfp4(v.detach(), cols, self.C))
+
     def as_block_ell(self) -> BlockELLTensor:
         return BlockELLTensor(values=self.kernel_values(), col_indices=self.effective_col_indices(), config=self.config)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.in_features).to(self.dtype)
-        if self.dtype == torch.bfloat16:
+        if self.weight_format == "mxfp4":
+            from ..kernels.mxfp4 import mxfp4_linear, mxfp4_linear_ad
+            if torch.is_grad_enabled() and (x2.requires_grad or self.values.requires_grad):
+                y = mxfp4_linear_ad(x2, self.values, self.effective_col_indices())
+            else:
+                y = mxfp4_linear(x2, self.mxfp4_weight())
+        elif self.dtype == torch.bfloat16:
             from ..kernels.autograd import block_ell_linear_ad
             y = block_ell_linear_ad(x2, self.values, self.effective_col_indices(), compute=self.kernel_values())
         else:  # fp32 accuracy path
@@ -112,11 +135,12 @@ class MLPBlock(nn.Module):
     """
 
     def __init__(self, d_model: int, d_ff: int, use_swiglu: bool = False, dropout: float = 0.0, tile_size: int = 16,
-                 density: float = 1.0, dtype: torch.dtype = torch.bfloat16, device=None):
+                 density: float = 1.0, dtype: torch.dtype = torch.bfloat16, device=None, weight_format: str = "native"):
         super().__init__()
+        self.weight_format = weight_format
         self.d_model, self.d_ff, self.use_swiglu, self.dropout = d_model, d_ff, use_swiglu, dropout
         self.tile_size, self.density, self.dtype = tile_size, density, dtype
-        kw = dict(tile_size=tile_size, density=density, dtype=dtype, device=device)
+        kw = dict(tile_size=tile_size, density=density, dtype=dtype, device=device, weight_format=weight_format)
         if use_swiglu:
             self.w_gate = BlockELLLinear(d_ff, d_model, bias=False, **kw)
             self.w_up = BlockELLLinear(d_ff, d_model, bias=False, **kw)
@@ -133,7 +157,15 @@ class MLPBlock(nn.Module):
             lead = x.shape[:-1]
             x2 = x.reshape(-1, self.d_model).to(self.dtype)
             g, u, d = self.w_gate, self.w_up, self.w_down
-            if self.dtype == torch.bfloat16:
+            if self.weight_format == "mxfp4":
+                from ..kernels.mxfp4 import mxfp4_swiglu, mxfp4_swiglu_fwd
+                if torch.is_grad_enabled() and (x2.requires_grad or any(w.values.requires_grad for w in (g, u, d))):
+                    out = mxfp4_swiglu(x2, g.values, g.effective_col_indices(), u.values, u.effective_col_indices(),
+                                       d.values, d.effective_col_indices(), add_residual=residual)
+                else:
+                    out = mxfp4_swiglu_fwd(x2, g.mxfp4_weight(), u.mxfp4_weight(), d.mxfp4_weight(),
+                                           add_residual=residual)
+            elif self.dtype == torch.bfloat16:
                 from ..kernels.autograd import block_ell_swiglu_ad
                 out = block_ell_swiglu_ad(x2, g.values, g.kernel_values(), g.effective_col_indices(), u.values,
                                           u.kernel_values(), u.effective_col_indices(), d.values, d.kernel_values(),

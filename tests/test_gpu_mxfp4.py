@@ -249,3 +249,226 @@ def test_swiglu_gradients(T, d, F, B, Kg, Kd, dead, layout, dtype):
         assert v.grad.dtype == dtype
         assert rel(f64(v.grad), M.tile_grads(ref, f64(c).astype(int), B, layout)) <= GRAD_TOL
     assert K.read_status() == 0
+
+
+# ------------------------------------------------------------ ways of calling
+
+
+def _ffn(rng, d=256, F=512, B=64, Kg=2, Kd=4, dead=0):
+    mats = [weight(rng, F // B, d // B, Kg, B, dead), weight(rng, F // B, d // B, Kg, B, dead),
+            weight(rng, d // B, F // B, Kd, B, dead)]
+    K = _K()
+    return mats, [K.make_mxfp4(v, c, n) for (v, c, _), n in zip(mats, (d // B, d // B, F // B))]
+
+
+@pytest.mark.parametrize("T", [3, 200])
+@pytest.mark.parametrize("B", [64, 128])
+def test_a_token_gets_the_same_result_in_any_batch(T, B):
+    """Sums run over the slots in one order whatever the batch (up to the number of CTAs sharing a row)."""
+    K = _K()
+    rng = np.random.default_rng(T)
+    _, packed = _ffn(rng, 512, 40960, B, 2, 3)  # more units than half of the SMs: whole units
+    x = rows(rng, T, 512)
+    whole = K.mxfp4_swiglu_fwd(x, *packed)
+    again = K.mxfp4_swiglu_fwd(x, *packed)
+    assert torch.equal(whole, again)
+    part = K.mxfp4_swiglu_fwd(x[1:2], *packed)
+    q_whole, q_part = (K.mxfp4_swiglu_fwd(t, *packed, return_intermediates=True)[1]["q_h"].dequantize() for t in (x, x[1:2]))
+    assert torch.equal(q_whole[1:2], q_part)
+    np.testing.assert_allclose(f64(part), f64(whole[1:2]), rtol=2.0 ** -7, atol=1e-5)
+
+
+def test_graph_replay_two_graphs_and_other_streams():
+    """Captured calls own their workspaces: two graphs and an eager call run at once, each with its own result."""
+    K = _K()
+    rng = np.random.default_rng(7)
+    _, packed = _ffn(rng)
+    xs = [rows(rng, T, 256) for T in (1, 70)]
+    want = [K.mxfp4_swiglu_fwd(x, *packed, add_residual=True) for x in xs]
+    graphs, outs, bufs = [], [], [torch.zeros_like(x) for x in xs]
+    for b in bufs:
+        K.mxfp4_swiglu_fwd(b, *packed, add_residual=True)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(K.mxfp4_swiglu_fwd(b, *packed, add_residual=True))
+        graphs.append(g)
+    for b, x in zip(bufs, xs):
+        b.copy_(x)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            graphs[0].replay()
+        with torch.cuda.stream(s2):
+            graphs[1].replay()
+        eager = K.mxfp4_swiglu_fwd(xs[1], *packed, add_residual=True)
+    torch.cuda.synchronize()
+    for got, ref in zip(outs + [eager], want + [want[1]]):
+        assert torch.equal(got, ref)
+    assert K.read_status() == 0
+
+
+def test_side_stream_inputs_and_producers_ahead():
+    """The call runs on the current stream, after what made its inputs there (x, weights and residual included)."""
+    K = _K()
+    rng = np.random.default_rng(8)
+    v, cols, _ = weight(rng, 4, 4, 3, 64)
+    x, res = rows(rng, 50, 256), rows(rng, 50, 256)
+    want = K.mxfp4_linear(x, K.make_mxfp4(v, cols, 4), residual=res)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        for T in (50, 5):
+            busy = torch.randn(2000, 2000, device="cuda")
+            for _ in range(20):
+                busy = busy @ busy * 1e-3
+            late = [t.clone() + 0 * busy[0, 0].to(t.dtype).nan_to_num() for t in (x, res)]
+            w = K.make_mxfp4(v.clone(), cols.clone(), 4)
+            y = K.mxfp4_linear(late[0][:T], w, residual=late[1][:T])
+            q = K.mxfp4_linear(K.mxfp4_quantize(late[0][:T], 64), w, residual=late[1][:T])
+            s.synchronize()
+            if T == 50:
+                assert torch.equal(y, want) and torch.equal(q, want)
+            else:
+                assert torch.equal(y, q)
+
+
+@pytest.mark.parametrize("T", [2, 33, 400])
+def test_nan_and_infinite_rows_stay_in_their_rows(T):
+    K = _K()
+    rng = np.random.default_rng(9)
+    _, packed = _ffn(rng, 256, 1024, 64, 3, 6)
+    x = rows(rng, T, 256)
+    clean = K.mxfp4_swiglu_fwd(x, *packed)
+    x[1, :] = float("nan")
+    x[T - 1, 200] = float("inf")
+    got = K.mxfp4_swiglu_fwd(x, *packed)
+    assert got[1].isnan().all()
+    keep = [t for t in range(T) if t not in (1, T - 1)]
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_rows_behind_the_last_token_are_left_alone():
+    K = _K()
+    rng = np.random.default_rng(10)
+    _, packed = _ffn(rng)
+    for T in (1, 37, 130):
+        out = torch.full((T + 3, 256), 7.0, dtype=BF16, device="cuda")
+        x = rows(rng, T, 256)
+        h = rows(rng, T, 512)
+        K.mxfp4_linear(h, packed[2], out=out[:T])
+        assert (out[T:] == 7).all()
+        dq = torch.full((T + 2, 256), 3.0, dtype=F32, device="cuda")
+        K.mxfp4_dequantize(K.mxfp4_quantize(x, 64), F32, out=dq[:T])
+        assert (dq[T:] == 3).all()
+
+
+def test_no_tokens_dead_weights_and_bad_columns():
+    K = _K()
+    rng = np.random.default_rng(11)
+    mats, packed = _ffn(rng)
+    empty = torch.empty(0, 256, dtype=BF16, device="cuda")
+    assert K.mxfp4_swiglu_fwd(empty, *packed, add_residual=True).shape == (0, 256)
+    assert K.mxfp4_dequantize(K.mxfp4_quantize(empty, 64)).shape == (0, 256)
+    leaves = [m[0].clone().requires_grad_(True) for m in mats]
+    xe = empty.clone().requires_grad_(True)
+    y = K.mxfp4_swiglu(xe, leaves[0], mats[0][1], leaves[1], mats[1][1], leaves[2], mats[2][1])
+    y.sum().backward()
+    assert xe.grad.shape == (0, 256) and all((t.grad == 0).all() for t in leaves)
+    # every slot dead: zeros, or the residual alone
+    dead = torch.full_like(mats[0][1], -1)
+    x = rows(rng, 40, 256)
+    w = K.make_mxfp4(mats[0][0], dead, 4)
+    assert (K.mxfp4_linear(x, w) == 0).all()
+    res = rows(rng, 40, 512)
+    assert torch.equal(K.mxfp4_linear(x, w, residual=res), res)
+    assert torch.equal(K.mxfp4_swiglu_fwd(x, w, w, packed[2], add_residual=True), x)
+    assert K.read_status() == 0
+    # an index outside the columns is dropped and reported
+    bad = mats[0][1].clone()
+    bad[1, 0] = 99
+    gone = mats[0][1].clone()
+    gone[1, 0] = -1
+    y1, y2 = (K.mxfp4_linear(x, K.make_mxfp4(mats[0][0], c, 4)) for c in (bad, gone))
+    assert torch.equal(y1, y2)
+    assert K.read_status() == 1
+
+
+def test_refusals_on_the_device():
+    K = _K()
+    rng = np.random.default_rng(12)
+    mats, packed = _ffn(rng)
+    x = rows(rng, 5, 256)
+    for call, text in [
+            (lambda: K.mxfp4_linear(x[:, :128], packed[0]), "features"),
+            (lambda: K.mxfp4_linear(x.half(), packed[0]), "bf16 or fp32"),
+            (lambda: K.mxfp4_linear(x[0], packed[0]), "2D"),
+            (lambda: K.mxfp4_linear(x, packed[0], residual=x), "residual"),
+            (lambda: K.mxfp4_linear(x, packed[0], out=torch.empty(5, 512, device="cuda")), "out must be"),
+            (lambda: K.mxfp4_linear(K.mxfp4_quantize(x, 128), packed[0]), "tile"),
+            (lambda: K.mxfp4_swiglu_fwd(x, packed[0], packed[1], packed[0]), "down"),
+            (lambda: K.mxfp4_swiglu_fwd(K.mxfp4_quantize(x, 64), *packed, add_residual=True), "needs the residual"),
+            (lambda: K.mxfp4_quantize(x, 96), "tile size"),
+            (lambda: K.mxfp4_quantize(x[:, :192], 128), "multiple"),
+            (lambda: K.make_mxfp4(mats[0][0][:, :, :32, :32].contiguous(), mats[0][1], 4), "tile size"),
+            (lambda: K.make_mxfp4(mats[0][0], mats[0][1].long(), 4), "int32"),
+            (lambda: K.make_mxfp4(mats[0][0], mats[0][1][:1], 4), "do not fit")]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+@pytest.mark.parametrize("swiglu", [True, False])
+def test_mlp_block_trains_and_serves_in_mxfp4(swiglu):
+    """The layers: a training step, the packed weight followed through the update, pruned tiles, serving."""
+    from looped_blockell.layers import MLPBlock
+    torch.manual_seed(0)
+    m = MLPBlock(256, 512, use_swiglu=swiglu, tile_size=64, density=0.5, device="cuda", weight_format="mxfp4")
+    lin = m.w_gate if swiglu else m.fc1
+    lin.alive_mask[0, 0] = False
+    x = torch.randn(2, 65, 256, device="cuda", dtype=BF16, requires_grad=True)
+    y = m(x, residual=True)
+    y.backward(torch.randn_like(y))
+    assert x.grad.isfinite().all() and (lin.values.grad[0, 0] == 0).all() and lin.values.grad[0, 1].abs().sum() > 0
+    with torch.no_grad():
+        before = m(x, residual=True)
+        assert torch.equal(before, y)  # the packed weight gives what the step computed
+        torch.optim.SGD(m.parameters(), lr=1.0).step()
+        after = m(x, residual=True)
+    assert torch.equal(after, m(x, residual=True).detach()) and not torch.equal(before, after)
+    with pytest.raises(ValueError, match="tile_size"):
+        MLPBlock(256, 512, tile_size=16, weight_format="mxfp4")
+    with pytest.raises(ValueError, match="weight_format"):
+        MLPBlock(256, 512, tile_size=64, weight_format="int3")
+
+
+def test_training_captured_in_a_graph():
+    """Forward and backward of one step captured, replayed on new data; no eager graph of the leaves is alive."""
+    K = _K()
+    rng = np.random.default_rng(13)
+    mats, _ = _ffn(rng)
+    x0, dy = rows(rng, 60, 256), rows(rng, 60, 256)
+    leaves = [x0.clone()] + [m[0].clone() for m in mats]
+
+    def step():
+        ls = [t.detach().requires_grad_(True) for t in leaves]
+        y = K.mxfp4_swiglu(ls[0], ls[1], mats[0][1], ls[2], mats[1][1], ls[3], mats[2][1], add_residual=True)
+        return (y.detach(), *torch.autograd.grad(y, ls, dy))
+
+    want = step()  # also builds the transposed topologies
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    leaves[0].copy_(rows(rng, 60, 256))
+    g.replay()
+    leaves[0].copy_(x0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in zip(got[2:], want[2:]):  # tile sums meet in arrival order: fp32 sums of 60 terms, then bf16
+        np.testing.assert_allclose(f64(a), f64(b), rtol=2.0 ** -7, atol=1e-4)

@@ -14,21 +14,8 @@ namespace mx {
 static constexpr int kThr = 256;
 
 // Q(v) is a 2-bit significand times a power of two: exact in bf16 and fp32.
-__device__ __forceinline__ void store32(__nv_bfloat16* p, const float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st_global_v4(p + 8 * i, pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                 pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-}
-__device__ __forceinline__ void store32(float* p, const float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    st_global_v4(p + 4 * i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                 __float_as_uint(v[4 * i + 3]));
-}
 
-// A warp takes 8 rows x 4 scale blocks: lane -> row l & 7, block l >> 3.  Its
-// 16-byte code stores fill whole core matrices (128 bytes each).
+// Rows: a warp takes groups of 8 rows x 128 columns.
 struct RowsArgs {
   int64_t T;
   int32_t features, C, B;
@@ -36,42 +23,45 @@ struct RowsArgs {
   int32_t col_groups;
 };
 
-__device__ __forceinline__ bool locate(const RowsArgs& a, int64_t w, int lane, int64_t& t, int32_t& f, int64_t& chunk,
-                                       int& n, int& j) {
-  const int64_t rg = w / a.col_groups;
-  const int32_t cg = int32_t(w - rg * a.col_groups);
-  t = rg * 8 + (lane & 7);
-  f = cg * 128 + (lane >> 3) * kBlock;
-  n = int(t & (kRows - 1));
-  const int32_t c = f / a.B;
-  j = (f - c * a.B) / kBlock;
-  chunk = ((t / kRows) * a.C + c) * row_chunk(a.B);
-  return t < a.T && f < a.features;
+struct Group {
+  int64_t t0;      // first row
+  int32_t f0;      // first column
+  int64_t chunks;  // offset of the chunks of the rows' 128
+};
+__device__ __forceinline__ Group group_of(const RowsArgs& a, int64_t w) {
+  // a 64-bit division costs more than a group's other arithmetic
+  const int64_t rg = a.groups <= 0xFFFFFFFFll ? int64_t(uint32_t(w) / uint32_t(a.col_groups)) : w / a.col_groups;
+  const int64_t t0 = rg * 8;
+  return {t0, int32_t(w - rg * a.col_groups) * 128, t0 / kRows * a.C * row_chunk(a.B)};
 }
 
+// Quantise: lane -> row l & 7, scale block l >> 3.  A warp's 16-byte code
+// stores fill whole core matrices (128 bytes each).
 template <class E>
 __global__ void __launch_bounds__(kThr) bell_mx_quantize_kernel(RowsArgs a, const E* __restrict__ src, int64_t ld,
                                                                uint8_t* __restrict__ dst) {
   griddep_launch();
   const int lane = threadIdx.x & 31;
   for (int64_t w = (int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5; w < a.groups; w += int64_t(gridDim.x) * (kThr / 32)) {
-    int64_t t, chunk;
-    int32_t f;
-    int n, j;
-    const bool ok = locate(a, w, lane, t, f, chunk, n, j);
+    const Group g = group_of(a, w);
+    const int64_t t = g.t0 + (lane & 7);
+    const int32_t f = g.f0 + (lane >> 3) * kBlock;
+    const int n = int(t & (kRows - 1)), c = f / a.B, j = (f - c * a.B) / kBlock;
+    uint8_t* chunk = dst + g.chunks + int64_t(c) * row_chunk(a.B);
+    const bool ok = t < a.T && f < a.features;
     uint32_t byte = 0;
     if (ok) {
       float v[32];
       load32(src + t * ld + f, v);
       const uint4 q = quantize32(v, byte);
-      st_global_v4(dst + chunk + code_off(n, j, kRows * 32), q.x, q.y, q.z, q.w);
+      st_global_v4(chunk + code_off(n, j, kRows * 32), q.x, q.y, q.z, q.w);
     }
     // the scales of one row and column block are adjacent bytes: two (B = 64)
     // or four (B = 128) lanes' bytes leave as one store
     uint32_t word = byte | (__shfl_xor_sync(0xffffffffu, byte, 8) << 8);
     if (a.B == 128) word |= __shfl_xor_sync(0xffffffffu, word, 16) << 16;
     if (ok && j == 0) {
-      uint8_t* p = dst + chunk + a.B * (kRows / 2) + scale_off(n, 0);
+      uint8_t* p = chunk + a.B * (kRows / 2) + scale_off(n, 0);
       if (a.B == 128)
         *reinterpret_cast<uint32_t*>(p) = word;
       else
@@ -80,26 +70,41 @@ __global__ void __launch_bounds__(kThr) bell_mx_quantize_kernel(RowsArgs a, cons
   }
 }
 
-__device__ __forceinline__ void unpack32(uint4 q, float s, float (&v)[32]) {
-  unpack_e2m1(q.x, s, v);
-  unpack_e2m1(q.y, s, v + 8);
-  unpack_e2m1(q.z, s, v + 16);
-  unpack_e2m1(q.w, s, v + 24);
+// Back: a lane's values fill one 16-byte store, and a warp's stores whole rows
+// of 128 columns (256 or 512 contiguous bytes).
+__device__ __forceinline__ void put_values(__nv_bfloat16* p, const uint8_t* codes, float s) {
+  float v[8];
+  unpack_e2m1(__ldg(reinterpret_cast<const unsigned*>(codes)), s, v);
+  st_global_v4(p, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+__device__ __forceinline__ void put_values(float* p, const uint8_t* codes, float s) {
+  // four codes: half of an aligned word
+  const uintptr_t at = reinterpret_cast<uintptr_t>(codes);
+  const uint32_t w = __ldg(reinterpret_cast<const unsigned*>(at & ~uintptr_t(3))) >> ((at & 2u) * 8u);
+  float v[8];
+  unpack_e2m1(w, s, v);
+  st_global_v4(p, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
 }
 
 template <class E>
 __device__ __forceinline__ void dequantize_rows(const RowsArgs& a, const uint8_t* __restrict__ src, E* __restrict__ dst,
                                                 int64_t ld) {
+  constexpr int V = 16 / int(sizeof(E)), LANES = 128 / V, PASS = 32 / LANES;  // values a lane, lanes a row, rows a pass
   const int lane = threadIdx.x & 31;
   for (int64_t w = (int64_t(blockIdx.x) * kThr + threadIdx.x) >> 5; w < a.groups; w += int64_t(gridDim.x) * (kThr / 32)) {
-    int64_t t, chunk;
-    int32_t f;
-    int n, j;
-    if (!locate(a, w, lane, t, f, chunk, n, j)) continue;
-    float v[32];
-    unpack32(ld_global_nc_v4(src + chunk + code_off(n, j, kRows * 32)),
-             scale_value(src[chunk + a.B * (kRows / 2) + scale_off(n, j)]), v);
-    store32(dst + t * ld + f, v);
+    const Group g = group_of(a, w);
+    const int32_t f = g.f0 + lane % LANES * V;
+    if (f >= a.features) continue;
+    const int c = f / a.B, j = (f - c * a.B) / kBlock, in = f % kBlock / 2;
+    const uint8_t* chunk = src + g.chunks + int64_t(c) * row_chunk(a.B);
+#pragma unroll
+    for (int i = 0; i < 8; i += PASS) {
+      const int64_t t = g.t0 + i + lane / LANES;
+      const int n = int(t & (kRows - 1));
+      if (t < a.T)
+        put_values(dst + t * ld + f, chunk + code_off(n, j, kRows * 32) + in,
+                   scale_value(chunk[a.B * (kRows / 2) + scale_off(n, j)]));
+    }
   }
 }
 
@@ -203,19 +208,18 @@ __global__ void __launch_bounds__(kThr) bell_mx_pack_kernel(const PackArgs a) {
   }
 }
 
-// Tiles back to bf16 [B_out, B_in].
+// Tiles back to bf16 [B_out, B_in], eight values a thread.
 __device__ __forceinline__ void unpack_tiles(const TileGather& g, int32_t B) {
-  const int blocks = B / kBlock, per_tile = B * blocks;
+  const int per_row = B / 8, per_tile = B * per_row;
   __nv_bfloat16* values = static_cast<__nv_bfloat16*>(g.values);
   for (int64_t i = int64_t(blockIdx.x) * kThr + threadIdx.x; i < g.tiles * per_tile; i += int64_t(gridDim.x) * kThr) {
     const int64_t tile = i / per_tile;
-    const int e = int(i - tile * per_tile), j = e % blocks, o = e / blocks;
+    const int e = int(i - tile * per_tile), o = e / per_row, k = e % per_row * 8, j = k / kBlock;
     const int64_t from = g.index ? g.index[tile] : tile;
     if (from < 0 || from >= g.n0 + g.n1) continue;
     const uint8_t* ch = static_cast<const uint8_t*>(from < g.n0 ? g.c0 : g.c1) + (from < g.n0 ? from : from - g.n0) * tile_chunk(B);
-    float v[32];
-    unpack32(ld_global_nc_v4(ch + code_off(o, j, B * 32)), scale_value(ch[B * B / 2 + scale_off(o, j)]), v);
-    store32(values + tile * B * B + o * B + j * kBlock, v);
+    put_values(values + tile * B * B + o * B + k, ch + code_off(o, j, B * 32) + k % kBlock / 2,
+               scale_value(ch[B * B / 2 + scale_off(o, j)]));
   }
 }
 
@@ -289,7 +293,7 @@ int expand(const ExpandArgs& e, cudaStream_t s) {
   a.e = e;
   int64_t most = 0;
   for (int i = 0; i < 2; ++i) {
-    most = std::max(most, e.gather[i].tiles * e.B * (e.B / kBlock));
+    most = std::max(most, e.gather[i].tiles * e.B * (e.B / 8));
     if (e.rows[i].dst) {
       a.rows[i] = rows_args(e.T, e.rows[i].features, e.B);
       most = std::max(most, a.rows[i].groups * 32);
@@ -417,7 +421,7 @@ int bell_mx_unpack_tiles(const void* chunks0, int64_t tiles0, const void* chunks
   if (int rc = require_sm100()) return rc;
   if (tiles == 0) return BELL_OK;
   unsigned grid;
-  if (int rc = mx::grid_for(tiles * B * (B / mx::kBlock), &grid)) return rc;
+  if (int rc = mx::grid_for(tiles * B * (B / 8), &grid)) return rc;
   mx::bell_mx_unpack_kernel<<<grid, mx::kThr, 0, static_cast<cudaStream_t>(stream)>>>(
       mx::TileGather{chunks0, tiles0, chunks1, tiles1, index, tiles, values}, B);
   return check_launch("bell_mx_unpack_kernel");

@@ -418,11 +418,10 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
 
 // ---------------------------------------------------------------- epilogue
 
-// h = silu(g) u = g u / (1 + e^-g) in fp32, two at a time (about 1e-6
-// relative): the hardware tanh form of the bf16 kernels (2^-11) would move one
+// silu(g) = g / (1 + e^-g) in fp32, two at a time (about 1e-6 relative): the hardware tanh form of the bf16 kernels (2^-11) would move one
 // in a few hundred of h's 4-bit codes to a neighbour.  Subnormal intermediates
 // are flushed: e^-g below 2^-126 next to 1, and 1 / (1 + e^-g) below 2^-126.
-__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+__device__ __forceinline__ float2 silu2(float2 g) {
   const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
   float2 e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
@@ -430,7 +429,30 @@ __device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
   const float2 a = add2(e, make_float2(1.f, 1.f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
-  return mul2(mul2(g, r), u);
+  return mul2(g, r);
+}
+
+// This warp has read accumulator `acc`.
+__device__ __forceinline__ void release(const Smem& s, uint32_t acc) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&s.acc_empty[acc]);
+}
+
+// A projection without a live slot is zero.
+__device__ __forceinline__ void clear16(uint32_t (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0u;
+}
+
+__device__ __forceinline__ void put_bf16(__nv_bfloat16* o, const uint32_t (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    uint32_t a[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = pack_bf16x2(__uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
+    st_global_v4(o + i, a[0], a[1], a[2], a[3]);
+  }
 }
 
 // Eight outputs of a linear at element `at`: the residual, one rounding, the store.
@@ -570,49 +592,68 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
     if constexpr (GATED) {
       const uint32_t a0 = acc, a1 = acc + 1 == uint32_t(G::ACCS) ? 0u : acc + 1;
       const uint32_t use1 = a1 ? use : use + 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
-      tc_fence_after();
+      const uint32_t col = tmem + lanes + uint32_t(j * 32);
       float h[32];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t col = tmem + lanes + uint32_t(j * 32 + half * 16);
-        uint32_t gr[16], ur[16];
-        tmem_ld16x2_sync(col + a0 * B, gr, col + a1 * B, ur);
-        if (half) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&s.acc_empty[a0]);
-            mbar_arrive(&s.acc_empty[a1]);
-          }
-        }
-        if (!live0 || !live1) {  // a projection without a live slot is zero
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (!live0) gr[i] = 0u;
-            if (!live1) ur[i] = 0u;
-          }
-        }
-        if (p.gate && t < p.T) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t a[4], c[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              a[e] = pack_bf16x2(__uint_as_float(gr[8 * i + 2 * e]), __uint_as_float(gr[8 * i + 2 * e + 1]));
-              c[e] = pack_bf16x2(__uint_as_float(ur[8 * i + 2 * e]), __uint_as_float(ur[8 * i + 2 * e + 1]));
-            }
-            st_global_v4(p.gate + at + half * 16 + 8 * i, a[0], a[1], a[2], a[3]);
-            st_global_v4(p.up + at + half * 16 + 8 * i, c[0], c[1], c[2], c[3]);
-          }
-        }
+      auto gates = [&](int k, uint32_t (&v)[16]) {  // h[k..k+16) = silu of the gate's columns
+        if (!live0) clear16(v);
+        if (p.gate && t < p.T) put_bf16(p.gate + at + k, v);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float2 v = silu_mul2(make_float2(__uint_as_float(gr[i]), __uint_as_float(gr[i + 1])),
-                                     make_float2(__uint_as_float(ur[i]), __uint_as_float(ur[i + 1])));
-          h[half * 16 + i] = v.x;
-          h[half * 16 + i + 1] = v.y;
+          const float2 x = silu2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+          h[k + i] = x.x;
+          h[k + i + 1] = x.y;
+        }
+      };
+      auto ups = [&](int k, uint32_t (&v)[16]) {  // times the up columns
+        if (!live1) clear16(v);
+        if (p.gate && t < p.T) put_bf16(p.up + at + k, v);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float2 x = mul2(make_float2(h[k + i], h[k + i + 1]),
+                                make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+          h[k + i] = x.x;
+          h[k + i + 1] = x.y;
+        }
+      };
+      // 16 columns at a time: 32 spill.  B = 128: the gate half is freed as soon
+      // as it is read, so that the next unit's jobs wait less for one of the
+      // three accumulators (gate/up at T = 16384, d = 4096, d_ff = 16384: 305 us
+      // against 345 with both halves read together).  B = 64, two units in turn
+      // on the epilogue's two groups, is bound by the epilogue's instructions
+      // and gains from fewer waits (124 us together, 138 one after the other;
+      // d = 2048, d_ff = 8192).
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
+      if constexpr (B == 128) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 32; k += 16) {
+          uint32_t v[16];
+          tmem_ld16_sync(col + a0 * B + k, v);
+          if (k) release(s, a0);
+          gates(k, v);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 32; k += 16) {
+          uint32_t v[16];
+          tmem_ld16_sync(col + a1 * B + k, v);
+          if (k) release(s, a1);
+          ups(k, v);
+        }
+      } else {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 32; k += 16) {
+          uint32_t v[16], w[16];
+          tmem_ld16x2_sync(col + a0 * B + k, v, col + a1 * B + k, w);
+          if (k) {
+            release(s, a0);
+            release(s, a1);
+          }
+          gates(k, v);
+          ups(k, w);
         }
       }
       uint32_t byte;
@@ -627,9 +668,7 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       tc_fence_after();
       uint32_t a[32];
       tmem_ld32_sync(tmem + lanes + acc * B + j * 32, a);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.acc_empty[acc]);
+      release(s, acc);
       if (t < p.T) {
         float f[32];
 #pragma unroll

@@ -408,8 +408,8 @@ size_t bell_linear_bwd_mx_workspace_bytes(const BellMxLinearBwdDesc* desc);
 int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
 
 /*
- * Straight-through backward of bell_swiglu_fwd_mx: gate_pre and up_out are its
- * bf16 projections, x and h its quantised rows.  cols_t_down / index_t_down:
+ * Straight-through backward of bell_swiglu_fwd_mx: x and h are its quantised
+ * rows; the projections are computed again.  cols_t_down / index_t_down:
  * transposed topology of down [d_ff/B, K_t_down]; cols_t_gate_up /
  * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
  * of up, and its tiles, counted after gate's).  Results that are NULL are not
@@ -420,8 +420,6 @@ typedef struct BellMxFFNBwdDesc {
   int32_t add_residual;
   int32_t layout;              /* of the tile gradients                      */
   const void* grad_out;        /* bf16 [T, d_model]                          */
-  const void* gate_pre;        /* bf16 [T, d_ff]                             */
-  const void* up_out;
   const void* x;               /* quantised rows                             */
   const void* h;
   BellMxEll gate, up, down;

@@ -6,6 +6,13 @@
 // y[t, rB + o] = sum over live slots k of row r, i < B, of
 //                Q(x)[t, c(r,k) B + i] Q(W)[r, k, i, o]
 //
+// The backward of the gated part is the same kernel with another epilogue: it
+// computes the projections g and u again, exactly as the forward had them, and
+// turns d_h into d_gate and d_up.  That costs the products a second time and
+// saves keeping g and u: writing them in bf16 made the forward's kernel 401 us
+// instead of 160 at T = 8192, d = 4096, d_ff = 16384, and their rounding was a
+// third of the tile gradients' error.
+//
 // A job is one accumulator: 128 tokens x one block-row of one matrix.  A unit
 // is one job (linear) or a gate job and an up job (gated).  A slot of a job
 // takes one activation chunk and one weight chunk (codes and scales, bulk
@@ -83,9 +90,12 @@ struct Params {
   Plan p0, p1;
   uint8_t* h;                     // gated: [mtiles, R] chunks
   __nv_bfloat16 *gate, *up;       // gated, optional [T, R*B]
+  const float* dh;                // backward: [T, R*B]
+  __nv_bfloat16* dgu;             // backward: [T, 2*R*B], d_gate then d_up
   void* out;                      // linear [T, R*B]
   const void* residual;           // linear, optional, out's type
   int32_t out_f32;
+  int32_t wide;                   // out, residual, gate and up are 32-byte aligned
   int32_t split;                  // linear: CTAs sharing a unit (0: persistent, whole units)
   int32_t early;                  // weights, plan and residual were complete before the kernel ahead
   int32_t* status;
@@ -445,50 +455,75 @@ __device__ __forceinline__ void clear16(uint32_t (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = 0u;
 }
 
-__device__ __forceinline__ void put_bf16(__nv_bfloat16* o, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void put_bf16(__nv_bfloat16* o, const uint32_t (&v)[16], bool wide) {
+  uint32_t a[8];
 #pragma unroll
-  for (int i = 0; i < 16; i += 8) {
-    uint32_t a[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = pack_bf16x2(__uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
-    st_global_v4(o + i, a[0], a[1], a[2], a[3]);
+  for (int e = 0; e < 8; ++e) a[e] = pack_bf16x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+  if (wide) {
+    st_global_v8(o, a);
+  } else {
+    st_global_v4(o, a[0], a[1], a[2], a[3]);
+    st_global_v4(o + 8, a[4], a[5], a[6], a[7]);
   }
 }
 
-// Eight outputs of a linear at element `at`: the residual, one rounding, the store.
-__device__ __forceinline__ void put8(const Params& p, int64_t at, const float* v) {
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = v[i];
-  if (p.out_f32) {
-    if (p.residual) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const uint4 r = ld_global_v4(static_cast<const float*>(p.residual) + at + i);
-        f[i] += __uint_as_float(r.x);
-        f[i + 1] += __uint_as_float(r.y);
-        f[i + 2] += __uint_as_float(r.z);
-        f[i + 3] += __uint_as_float(r.w);
-      }
+// Sixteen outputs of a linear at element `at`: the residual, one rounding, the
+// stores.  A lane's outputs lie 2 or 4 KB and more from the next lane's, so its
+// accesses fill sectors only if they are 32 bytes (p.wide: the buffers are
+// aligned so; else two of 16).
+__device__ __forceinline__ void put8(const Params& p, int64_t at, float* f) {  // fp32: 8 values are 32 bytes
+  uint32_t r[8];
+  if (p.residual) {
+    const float* from = static_cast<const float*>(p.residual) + at;
+    if (p.wide) {
+      ld_global_v8(from, r);
+    } else {
+      const uint4 a = ld_global_v4(from), b = ld_global_v4(from + 4);
+      r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w, r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
     }
-    float* o = static_cast<float*>(p.out) + at;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4)
-      st_global_v4(o + i, __float_as_uint(f[i]), __float_as_uint(f[i + 1]), __float_as_uint(f[i + 2]),
-                   __float_as_uint(f[i + 3]));
+    for (int i = 0; i < 8; ++i) f[i] += __uint_as_float(r[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(f[i]);
+  float* o = static_cast<float*>(p.out) + at;
+  if (p.wide) {
+    st_global_v8(o, r);
   } else {
-    if (p.residual) {
-      const uint4 r = ld_global_v4(static_cast<const __nv_bfloat16*>(p.residual) + at);
-      const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x2 = unpack_bf16x2(rw[i]);
-        f[2 * i] += x2.x;
-        f[2 * i + 1] += x2.y;
-      }
+    st_global_v4(o, r[0], r[1], r[2], r[3]);
+    st_global_v4(o + 4, r[4], r[5], r[6], r[7]);
+  }
+}
+__device__ __forceinline__ void put16(const Params& p, int64_t at, float* f) {
+  if (p.out_f32) {
+    put8(p, at, f);
+    put8(p, at + 8, f + 8);
+    return;
+  }
+  uint32_t r[8];
+  if (p.residual) {
+    const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(p.residual) + at;
+    if (p.wide) {
+      ld_global_v8(from, r);
+    } else {
+      const uint4 a = ld_global_v4(from), b = ld_global_v4(from + 8);
+      r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w, r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
     }
-    st_global_v4(static_cast<__nv_bfloat16*>(p.out) + at, pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                 pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = unpack_bf16x2(r[i]);
+      f[2 * i] += x.x;
+      f[2 * i + 1] += x.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
+  if (p.wide) {
+    st_global_v8(o, r);
+  } else {
+    st_global_v4(o, r[0], r[1], r[2], r[3]);
+    st_global_v4(o + 8, r[4], r[5], r[6], r[7]);
   }
 }
 
@@ -536,17 +571,17 @@ template <int B>
 __device__ void split_join(const Params& p, const Smem& s) {
   const int u = int(blockIdx.x) / p.split, rank = int(blockIdx.x) % p.split, m = u / p.R, r = u - m * p.R;
   const int rows = int(min(int64_t(kRows), p.T - int64_t(m) * kRows));
-  const int cols = B / p.split, per_row = cols / 8;
+  const int cols = B / p.split, per_row = cols / 16;
   const uint32_t base = smem_u32(s.stages);
   for (int i = threadIdx.x; i < rows * per_row; i += kThreads) {
-    const int n = i / per_row, c = rank * cols + (i - n * per_row) * 8;
-    float f[8];
+    const int n = i / per_row, c = rank * cols + (i - n * per_row) * 16;
+    float f[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    for (int e = 0; e < 16; ++e) f[e] = 0.f;
     for (int k = 0; k < p.split; ++k) {
       const uint32_t from = mapa_shared(base + uint32_t(n * Partial<B>::LD + c) * 4u, uint32_t(k));
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
+      for (int e = 0; e < 16; e += 4) {
         float4 v;
         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
@@ -558,12 +593,32 @@ __device__ void split_join(const Params& p, const Smem& s) {
         f[e + 3] += v.w;
       }
     }
-    put8(p, (int64_t(m) * kRows + n) * (int64_t(p.R) * B) + int64_t(r) * B + c, f);
+    put16(p, (int64_t(m) * kRows + n) * (int64_t(p.R) * B) + int64_t(r) * B + c, f);
   }
 }
 
-template <int B, bool GATED>
+// d_gate = d_h u silu'(g) and d_up = d_h silu(g), two at a time, fp32:
+// silu' = s + silu (1 - s), s = 1 / (1 + e^-g).
+__device__ __forceinline__ void silu_backward2(float2 dh, float2 g, float2 u, float2& dg, float2& du) {
+  const float2 t = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 a = add2(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(a.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(a.y));
+  const float2 f = mul2(g, r);
+  const float2 slope = add2(r, mul2(f, make_float2(1.f - r.x, 1.f - r.y)));
+  dg = mul2(mul2(dh, u), slope);
+  du = mul2(dh, f);
+}
+
+// What a kernel's epilogue does with its accumulators.
+enum Mode : int { kLinear, kGated, kGatedBackward };
+
+template <int B, Mode MODE>
 __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
+  constexpr bool GATED = MODE != kLinear;
   using G = Geo<B>;
   constexpr int NB = B / 32;             // scale blocks (32 features) of a unit
   constexpr int GROUPS = kEpiWarps / (4 * NB);
@@ -589,14 +644,57 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
     const bool live0 = c0 > 0, live1 = c1 > 0;
     if (u + step < units) counts(u + step);
     const int64_t at = t * ld + int64_t(r) * B + j * 32;
-    if constexpr (GATED) {
+    if constexpr (MODE == kGatedBackward) {
+      const uint32_t a0 = acc, a1 = acc + 1 == uint32_t(G::ACCS) ? 0u : acc + 1;
+      const uint32_t use1 = a1 ? use : use + 1;
+      const uint32_t col = tmem + lanes + uint32_t(j * 32);
+      const bool row = t < p.T;
+      uint32_t dh[2][8] = {};  // 16 columns of d_h, on their way while the products run
+      auto fetch = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (row) ld_global_v8(p.dh + at + k + 8 * i, dh[i]);
+      };
+      fetch(0);
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < 32; k += 16) {
+        uint32_t g[16], u[16];
+        tmem_ld16x2_sync(col + a0 * B + k, g, col + a1 * B + k, u);
+        if (k) {
+          release(s, a0);
+          release(s, a1);
+        }
+        if (!live0) clear16(g);
+        if (!live1) clear16(u);
+        uint32_t og[8], ou[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t* d = dh[i >> 2] + 2 * (i & 3);
+          float2 x, y;
+          silu_backward2(make_float2(__uint_as_float(d[0]), __uint_as_float(d[1])),
+                         make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
+                         make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), x, y);
+          og[i] = pack_bf16x2(x.x, x.y);
+          ou[i] = pack_bf16x2(y.x, y.y);
+        }
+        if (!k) fetch(16);
+        if (row) {
+          __nv_bfloat16* o = p.dgu + t * 2 * ld + int64_t(r) * B + j * 32 + k;
+          st_global_v8(o, og);
+          st_global_v8(o + ld, ou);
+        }
+      }
+    } else if constexpr (MODE == kGated) {
       const uint32_t a0 = acc, a1 = acc + 1 == uint32_t(G::ACCS) ? 0u : acc + 1;
       const uint32_t use1 = a1 ? use : use + 1;
       const uint32_t col = tmem + lanes + uint32_t(j * 32);
       float h[32];
       auto gates = [&](int k, uint32_t (&v)[16]) {  // h[k..k+16) = silu of the gate's columns
         if (!live0) clear16(v);
-        if (p.gate && t < p.T) put_bf16(p.gate + at + k, v);
+        if (p.gate && t < p.T) put_bf16(p.gate + at + k, v, p.wide);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float2 x = silu2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
@@ -606,7 +704,7 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       };
       auto ups = [&](int k, uint32_t (&v)[16]) {  // times the up columns
         if (!live1) clear16(v);
-        if (p.gate && t < p.T) put_bf16(p.up + at + k, v);
+        if (p.gate && t < p.T) put_bf16(p.up + at + k, v, p.wide);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float2 x = mul2(make_float2(h[k + i], h[k + i + 1]),
@@ -673,8 +771,8 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         float f[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) put8(p, at + i, f + i);
+        put16(p, at, f);
+        put16(p, at + 16, f + 16);
       }
     }
     acc += GROUPS * JOBS;
@@ -685,8 +783,9 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
   }
 }
 
-template <int B, bool GATED>
+template <int B, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
+  constexpr bool GATED = MODE != kLinear;
   using G = Geo<B>;
   extern __shared__ uint8_t smem_raw[];
   const Smem s = carve<B>(smem_raw);
@@ -726,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
     if constexpr (!GATED) {
       if (split) split_partial<B>(p, s, tmem, ctl);
     }
-    if (!split) epilogue<B, GATED>(p, s, tmem, ctl);
+    if (!split) epilogue<B, MODE>(p, s, tmem, ctl);
   } else {
     issue<B, GATED>(p, s, tmem, warp - kIssuer, ctl);
   }
@@ -747,17 +846,18 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
 
 // CTAs that share a unit of a linear: where whole units would leave more than
 // half of the SMs without one, as many as fit (a power of two, at most the
-// portable cluster of 8), while every ring gets a stage.
-static int split_of(int64_t units, int stages, int sms) {
+// portable cluster of 8 and 16 columns each to join), while every ring gets a
+// stage.
+static int split_of(int64_t units, int stages, int sms, int B) {
   if (units * 2 > sms) return 0;
   int split = 1;
-  while (split < 8 && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
+  while (split < std::min(8, B / 16) && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
   return split;
 }
 
-template <int B, bool GATED>
+template <int B, Mode MODE>
 static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
-  auto kern = bell_mx_kernel<B, GATED>;
+  auto kern = bell_mx_kernel<B, MODE>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
   int dev = 0, sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
@@ -768,7 +868,7 @@ static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   }
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
   const int64_t units = int64_t(p.mtiles) * p.R;
-  p.split = GATED ? 0 : split_of(units, (p.K0 + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS, sms);
+  p.split = MODE != kLinear ? 0 : split_of(units, (p.K0 + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS, sms, B);
   const int64_t grid = p.split ? units * p.split : std::min<int64_t>(units, sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));
@@ -851,7 +951,21 @@ static int linear(Params p, const BellMxEll& w, const void* residual, void* out,
   p.out = out;
   p.residual = residual;
   p.out_f32 = out_dtype == BELL_DTYPE_F32;
-  return w.B == 128 ? launch<128, false>(p, max_ctas, s) : launch<64, false>(p, max_ctas, s);
+  p.wide = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) & 31u) == 0;
+  return w.B == 128 ? launch<128, kLinear>(p, max_ctas, s) : launch<64, kLinear>(p, max_ctas, s);
+}
+
+int gated_backward(int64_t T, const void* x, const BellMxEll& gate, const BellMxEll& up, const float* dh, void* dgu,
+                   int32_t* status, cudaStream_t s) {
+  if (int rc = check_ell(gate, "gate")) return rc;
+  if (int rc = check_ell(up, "up")) return rc;
+  if (int rc = check_size(T, gate.R)) return rc;
+  if (!status) status = default_status_ptr();
+  if (!status) return BELL_ERR_LAUNCH;
+  Params p = base_params(T, gate, &up, x, status);
+  p.dh = dh;
+  p.dgu = static_cast<__nv_bfloat16*>(dgu);
+  return gate.B == 128 ? launch<128, kGatedBackward>(p, 0, s) : launch<64, kGatedBackward>(p, 0, s);
 }
 
 }  // namespace mx
@@ -913,8 +1027,9 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   p.h = static_cast<uint8_t*>(d->h);
   p.gate = static_cast<__nv_bfloat16*>(d->gate_pre);
   p.up = static_cast<__nv_bfloat16*>(d->up_out);
+  p.wide = ((reinterpret_cast<uintptr_t>(d->gate_pre) | reinterpret_cast<uintptr_t>(d->up_out)) & 31u) == 0;
   p.early = d->x && d->x_src;
-  if (int rc = g.B == 128 ? mx::launch<128, true>(p, d->max_ctas, s) : mx::launch<64, true>(p, d->max_ctas, s)) return rc;
+  if (int rc = g.B == 128 ? mx::launch<128, mx::kGated>(p, d->max_ctas, s) : mx::launch<64, mx::kGated>(p, d->max_ctas, s)) return rc;
   mx::Params q = mx::base_params(d->T, w, nullptr, d->h, status);
   q.early = d->x_src != nullptr;  // a plain launch (the quantisation, or gate/up from the caller's rows) came before
   return mx::linear(q, w, d->residual, d->out, d->out_dtype, d->max_ctas, s);

@@ -79,6 +79,19 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
+// 32 bytes of one thread: a whole sector of global memory (p 32-byte aligned).
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void ld_global_v8(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
 // Two fp32 products or sums in one instruction, each rounded as alone.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
@@ -277,6 +290,11 @@ struct RoundArgs {
   int64_t n[3];
 };
 int round_sums(const RoundArgs& a, cudaStream_t s);
+
+// [d_gate | d_up] (bf16 [T, 2 R B]) from d_h (fp32 [T, R B]) and the gated
+// block's quantised rows and weights (bell_mx.cu).
+int gated_backward(int64_t T, const void* x, const BellMxEll& gate, const BellMxEll& up, const float* dh, void* dgu,
+                   int32_t* status, cudaStream_t s);
 
 // Argument checks of rows [T, features], ld elements apart (bell_mx_quant.cu).
 int check_rows(int64_t T, int32_t features, int32_t B, int32_t dtype, const void* rows, const void* chunks, int64_t ld);

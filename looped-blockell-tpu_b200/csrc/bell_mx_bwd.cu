@@ -3,16 +3,17 @@
 // whose values are exact in bf16.  Each entry point is the sequence of launches
 // on the caller's stream and one workspace:
 //
-//   unpack    the gathered tiles of W_down^T and [W_gate ; W_up]^T, Q(x) and
-//             (at B = 64) Q(h), and zeros for the tile gradients: one launch
-//   [d_gate | d_up] from d_h = dy Q(W_down) and the SiLU backward (one kernel at
-//             B = 64, two at B = 128, as the bf16 backward measured faster)
+//   unpack    the gathered tiles of W_down^T and [W_gate ; W_up]^T, Q(x), and
+//             zeros for the tile gradients: one launch
+//   d_h = dy Q(W_down), fp32
+//   [d_gate | d_up] from d_h and the projections, computed again (bell_mx.cu)
 //   dx = [d_gate | d_up] Q([W_gate ; W_up]) (+ dy)
 //   the three tile gradients, summed in fp32; one launch rounds them to bf16
 //
-// The unpacked operands live in the workspace only during the call: they add 2
-// bytes a value to the traffic and nothing to what training keeps.  At B = 128
-// Q(h) takes the place of d_h once that has been read.
+// d_h stays in fp32: rounded to bf16, its error and that of d_gate and d_up
+// together made the tile gradients' 1.7 times that of one rounding.  The
+// unpacked operands live in the workspace only during the call; Q(h) takes the
+// place of d_h once that has been read.
 #include <algorithm>
 #include <string>
 
@@ -24,7 +25,7 @@ namespace mx {
 static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Offsets of the workspace: the unpacked transposes (of down, and of gate and
-// up or the one weight), a plan, the unpacked rows, d_h and Q(h), fp32 sums
+// up or the one weight), a plan, the unpacked rows, d_h then Q(h), fp32 sums
 // whose result is bf16, [d_gate | d_up].
 struct BwdWs {
   size_t tiles_down, tiles, plan, rows, mid, grads[3], dgu, total;
@@ -63,7 +64,7 @@ static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
   o.tiles = l.take(size_t(g.C) * d.K_t_gate_up * BB * 2);
   o.plan = l.take(std::max(bell_plan_bytes(0, 0, 0, g.R, d.K_t_down), bell_plan_bytes(0, 0, 0, g.C, d.K_t_gate_up)));
   o.rows = l.take(T * g.C * g.B * 2);
-  o.mid = l.take(T * F * 2);
+  o.mid = l.take(T * F * 4);
   o.grads[0] = l.take(sums_bytes(d.gate, d.d_gate != nullptr, d.gate_dtype));
   o.grads[1] = l.take(sums_bytes(d.up, d.d_up != nullptr, d.up_dtype));
   o.grads[2] = l.take(sums_bytes(d.down, d.d_down != nullptr, d.down_dtype));
@@ -117,11 +118,12 @@ static int round_all(const Grad (&g)[3], cudaStream_t s) {
   return round_sums(a, s);
 }
 
-static int product(int64_t T, const void* x, const BellEll& w, const void* residual, void* out, void* plan,
-                   int32_t* status, void* stream) {
+static int product(int64_t T, const void* x, const BellEll& w, const void* residual, void* out, int32_t out_dtype,
+                   void* plan, int32_t* status, void* stream) {
   BellLinearDesc d{};
   d.T = T;
-  d.dtype = d.out_dtype = BELL_DTYPE_BF16;
+  d.dtype = BELL_DTYPE_BF16;
+  d.out_dtype = out_dtype;
   d.add_residual = residual != nullptr;
   d.x = x;
   d.residual = residual;
@@ -179,7 +181,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dx) {
     const BellEll wt{ws + o.tiles, d->cols_t, w.C, w.R, d->K_t, w.B, BELL_TILE_IN_OUT, 0};
-    if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, ws + o.plan, d->status, stream)) return rc;
+    if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream)) return rc;
   }
   if (int rc = mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, grads[0],
                              d->status, stream))
@@ -203,8 +205,8 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   if (g.R != u.R || g.C != u.C || g.B != u.B || w.B != g.B || w.C != g.R || w.R != g.C)
     return fail(BELL_ERR_SHAPE, "gate, up and down do not fit");
   if (d->T < 0 || d->T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "T must be in [0, 2^31 - 256)");
-  if (d->T > 0 && (!d->grad_out || !d->gate_pre || !d->up_out || !d->x || !d->h))
-    return fail(BELL_ERR_ARG, "grad_out, gate_pre, up_out, x and h must be non-NULL");
+  if (d->T > 0 && (!d->grad_out || !d->x || !d->h)) return fail(BELL_ERR_ARG, "grad_out, x and h must be non-NULL");
+  if (!g.plan || !u.plan) return fail(BELL_ERR_ARG, "gate and up need their plans");
   if (!d->cols_t_down || !d->index_t_down || d->K_t_down < 1 || !d->cols_t_gate_up || !d->index_t_gate_up ||
       d->K_t_gate_up < 1)
     return fail(BELL_ERR_ARG, "the transposed topologies must be given");
@@ -234,31 +236,16 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     e.gather[1] = {g.chunks, int64_t(g.R) * g.K, u.chunks, int64_t(u.R) * u.K, d->index_t_gate_up,
                    int64_t(g.C) * d->K_t_gate_up, ws + o.tiles};
   if (T > 0 && (d->d_gate || d->d_up)) e.rows[0] = {d->x, D, ws + o.rows};
-  if (T > 0 && d->d_down && g.B == 64) e.rows[1] = {d->h, F, mid};
   for (int i = 0; i < 3; ++i) e.zero[i] = {grads[i].sums, grads[i].n};
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dgu) {
     const BellEll wt{ws + o.tiles_down, d->cols_t_down, g.R, w.R, d->K_t_down, g.B, BELL_TILE_IN_OUT, 0};
-    if (g.B == 64) {
-      BellDownBwdDesc b{};
-      b.T = T;
-      b.grad_out = d->grad_out;
-      b.gate_pre = d->gate_pre;
-      b.up_out = d->up_out;
-      b.d_gate_up = dgu;
-      b.plan = ws + o.plan;
-      b.w_t = wt;
-      b.status = d->status;
-      if (int rc = bell_down_silu_bwd_bf16(&b, stream)) return rc;
-    } else {
-      if (int rc = mx::product(T, d->grad_out, wt, nullptr, mid, ws + o.plan, d->status, stream)) return rc;
-      if (int rc = bell_silu_mul_bwd_bf16(T, F, mid, d->gate_pre, d->up_out, dgu, dgu + size_t(F) * 2, int64_t(F) * 2, stream))
-        return rc;
-    }
+    if (int rc = mx::product(T, d->grad_out, wt, nullptr, mid, BELL_DTYPE_F32, ws + o.plan, d->status, stream)) return rc;
+    if (int rc = mx::gated_backward(T, d->x, g, u, reinterpret_cast<const float*>(mid), dgu, d->status, s)) return rc;
   }
   if (want_dx) {
     const BellEll wt{ws + o.tiles, d->cols_t_gate_up, g.C, 2 * g.R, d->K_t_gate_up, g.B, BELL_TILE_IN_OUT, 0};
-    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, ws + o.plan, d->status, stream))
+    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream))
       return rc;
   }
   if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads[0], d->status, stream))
@@ -266,7 +253,7 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   if (int rc = mx::tile_grad(T, ws + o.rows, dgu + size_t(F) * 2, int64_t(F) * 2, d->cols_up, u, d->layout, grads[1],
                              d->status, stream))
     return rc;
-  if (T > 0 && d->d_down && g.B == 128)
+  if (T > 0 && d->d_down)
     if (int rc = bell_mx_dequantize_rows(T, F, g.B, d->h, BELL_DTYPE_BF16, mid, F, stream)) return rc;
   if (int rc = mx::tile_grad(T, mid, d->grad_out, D, d->cols_down, w, d->layout, grads[2], d->status, stream)) return rc;
   return mx::round_all(grads, s);

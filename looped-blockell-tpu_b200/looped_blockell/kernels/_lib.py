@@ -120,7 +120,7 @@ class BellMxLinearBwdDesc(C.Structure):
 
 class BellMxFFNBwdDesc(C.Structure):
     _fields_ = [("T", C.c_int64), ("add_residual", C.c_int32), ("layout", C.c_int32), ("grad_out", C.c_void_p),
-                ("gate_pre", C.c_void_p), ("up_out", C.c_void_p), ("x", C.c_void_p), ("h", C.c_void_p),
+                ("x", C.c_void_p), ("h", C.c_void_p),
                 ("gate", BellMxEll), ("up", BellMxEll), ("down", BellMxEll), ("cols_gate", C.c_void_p),
                 ("cols_up", C.c_void_p), ("cols_down", C.c_void_p), ("cols_t_down", C.c_void_p),
                 ("index_t_down", C.c_void_p), ("cols_t_gate_up", C.c_void_p), ("index_t_gate_up", C.c_void_p),

@@ -293,6 +293,12 @@ def mxfp4_swiglu_fwd(x: Union[torch.Tensor, MXRows], gate: MXBlockELL, up: MXBlo
     ``add_residual``).  ``return_intermediates`` returns ``(out, ws)``, ``ws``
     with the quantised rows ``q_x`` and ``q_h`` (``MXRows``) and the bf16
     projections ``gate`` and ``up``."""
+    out, ws = _swiglu(x, gate, up, down, add_residual, residual, return_intermediates, return_intermediates, max_ctas)
+    return (out, ws) if return_intermediates else out
+
+
+def _swiglu(x, gate, up, down, add_residual=False, residual=None, keep_rows=False, keep_projections=False, max_ctas=0):
+    """The forward; with ``keep_rows`` also its quantised rows (and projections)."""
     quantised = isinstance(x, MXRows)
     if not quantised:
         x = _rows_2d("x", x)
@@ -314,21 +320,21 @@ def mxfp4_swiglu_fwd(x: Union[torch.Tensor, MXRows], gate: MXBlockELL, up: MXBlo
             residual = x
         residual = _check_residual(residual, (T, D), dtype, dev)
     out = torch.empty((T, D), dtype=dtype, device=dev)
-    direct = not quantised and not return_intermediates and _direct(T, B)
+    direct = not quantised and not keep_rows and _direct(T, B)
     n_x, n_h = 0 if quantised or direct else _rows_bytes(T, D, B), _rows_bytes(T, F, B)
     ws = _bytes(n_x + n_h, dev)  # the quantised rows of x, then of h
     at = ws.data_ptr()
     g = u = None
-    if return_intermediates:
+    if keep_projections:
         g, u = (torch.empty((T, F), dtype=torch.bfloat16, device=dev) for _ in range(2))
     d = _lib.BellMxFFNDesc(T, _DTYPES[dtype], int(max_ctas), x.data.data_ptr() if quantised else None if direct else at, src, ld, src_type, 0,
                            None if residual is None else residual.data_ptr(), at + n_x,
                            None if g is None else g.data_ptr(), None if u is None else u.data_ptr(), out.data_ptr(),
                            gate._abi, up._abi, down._abi, None)
     _call("bell_swiglu_fwd_mx", dev, C.byref(d))
-    if return_intermediates:
-        return out, dict(q_x=x if quantised else MXRows(ws[:n_x], T, D, B), q_h=MXRows(ws[n_x:], T, F, B), gate=g, up=u)
-    return out
+    if not keep_rows:
+        return out, None
+    return out, dict(q_x=x if quantised else MXRows(ws[:n_x], T, D, B), q_h=MXRows(ws[n_x:], T, F, B), gate=g, up=u)
 
 
 # ----------------------------------------------------------------- training
@@ -396,17 +402,16 @@ class MXSwiGLUFn(torch.autograd.Function):
     def forward(ctx, x, v_gate, ci_gate, v_up, ci_up, v_down, ci_down, add_residual, layout):
         C_model, R_ff = x.shape[1] // v_gate.shape[2], v_gate.shape[0]
         gate, up, down = _pack(((v_gate, ci_gate, C_model), (v_up, ci_up, C_model), (v_down, ci_down, R_ff)), layout)
-        out, ws = mxfp4_swiglu_fwd(x, gate, up, down, add_residual=add_residual, return_intermediates=True)
+        out, ws = _swiglu(x, gate, up, down, add_residual, keep_rows=True)
         ctx.weights = (gate, up, down)
-        ctx.save_for_backward(ws["gate"], ws["up"], ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down, gate.data,
-                              up.data, down.data)
+        ctx.save_for_backward(ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down, gate.data, up.data, down.data)
         ctx.add_residual, ctx.layout = bool(add_residual), layout
         ctx.dtypes = (x.dtype, v_gate.dtype, v_up.dtype, v_down.dtype)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        g, u, q_x, q_h, ci_gate, ci_up, ci_down, *_ = ctx.saved_tensors
+        q_x, q_h, ci_gate, ci_up, ci_down, *_ = ctx.saved_tensors
         gate, up, down = ctx.weights
         dy = grad_out.to(torch.bfloat16).contiguous()
         T, dev = dy.shape[0], dy.device
@@ -417,7 +422,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         cols = (gate.col_indices, up.col_indices, down.col_indices)
         grads = [_grad(n, c, gate.B, t) for n, c, t in zip((need[1], need[3], need[5]), cols, ctx.dtypes[1:])]
         d = _lib.BellMxFFNBwdDesc(
-            T, int(ctx.add_residual), ctx.layout, dy.data_ptr(), g.data_ptr(), u.data_ptr(), q_x.data_ptr(),
+            T, int(ctx.add_residual), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
             q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
             td_cols.data_ptr(), td_index.data_ptr(), tg_cols.data_ptr(), tg_index.data_ptr(), td_cols.shape[1],
             tg_cols.shape[1], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
@@ -437,8 +442,10 @@ def mxfp4_swiglu(x: torch.Tensor, v_gate: torch.Tensor, ci_gate: torch.Tensor, v
     fp32, quantised on every call), with the arguments of ``block_ell_swiglu``.
 
     The backward is that of the bf16 block at the quantised operands Q(x),
-    Q(W), Q(h), the gradient passing straight through Q; tile gradients are
-    summed in fp32 and come back in the tiles' dtype."""
+    Q(W), Q(h), the gradient passing straight through Q; the projections are
+    computed again rather than kept, so a step keeps 4.25 bits a value of x
+    and h.  Tile gradients are summed in fp32 and come back in the tiles'
+    dtype."""
     if x.dim() != 2 or v_gate.dim() != 4 or v_up.dim() != 4 or v_down.dim() != 4:
         raise RuntimeError("x must be 2D [N, d_model] and the tiles 4D [R, K, B, B]")
     if x.shape[1] % v_gate.shape[2]:

@@ -177,7 +177,7 @@ def test_backward_refusals():
     assert lib.bell_linear_bwd_mx_workspace_bytes(C.byref(d)) == 3 * 64 * 64 * 2 + 256 + 4 * 192 * 2 + 4 * 64 * 64 * 4
     f = L.BellMxFFNBwdDesc()
     f.T, f.gate, f.up, f.down = 4, _mx(L, 4, 2), _mx(L, 4, 2), _mx(L, 2, 4)
-    f.grad_out = f.gate_pre = f.up_out = f.x = f.h = f.workspace = 1024
+    f.grad_out = f.x = f.h = f.workspace = 1024
     assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -8 and "topologies" in L.last_error()
     assert lib.bell_swiglu_bwd_mx_workspace_bytes(C.byref(f)) == 0
     f.up = _mx(L, 4, 3)

@@ -9,9 +9,9 @@
 // The backward of the gated part is the same kernel with another epilogue: it
 // computes the projections g and u again, exactly as the forward had them, and
 // turns d_h into d_gate and d_up.  That costs the products a second time and
-// saves keeping g and u: writing them in bf16 made the forward's kernel 401 us
-// instead of 160 at T = 8192, d = 4096, d_ff = 16384, and their rounding was a
-// third of the tile gradients' error.
+// saves keeping g and u: in bf16 their writes cost 74 us of the forward's 289
+// at T = 8192, d = 4096, d_ff = 16384, their reads as much in the backward, and
+// their rounding was a third of the tile gradients' error.
 //
 // A job is one accumulator: 128 tokens x one block-row of one matrix.  A unit
 // is one job (linear) or a gate job and an up job (gated).  A slot of a job
@@ -655,6 +655,13 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         for (int i = 0; i < 2; ++i)
           if (row) ld_global_v8(p.dh + at + k + 8 * i, dh[i]);
       };
+      // a lane's 32 columns are one line of d_h: the next unit's is called into L2
+      // now (this kernel waits for memory, not for its rate; without it 405 us
+      // at T = 8192, d = 4096, d_ff = 16384)
+      const int un = u + step, mn = un / p.R;
+      const int64_t tn = int64_t(mn) * kRows + n;
+      if (un < units && tn < p.T)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.dh + tn * ld + int64_t(un - mn * p.R) * B + j * 32));
       fetch(0);
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;

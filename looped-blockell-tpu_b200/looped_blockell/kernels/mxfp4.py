@@ -18,7 +18,9 @@ saturates.  A block that holds an infinity or a NaN is NaN throughout.
   from the gate/up kernel to the down projection.
 * ``mxfp4_linear_ad``, ``mxfp4_swiglu``: the same, differentiable.  The
   gradient passes straight through Q: the backward is the bf16 one at the
-  quantised operands (their values are exact in bf16).
+  quantised operands (their values are exact in bf16).  A weight's first
+  backward builds its transposed topology and waits for the device once: run a
+  step before capturing one in a graph.
 
 Where ``ternary`` keeps 2 bits a weight and int8 activations, this keeps
 4.25 bits of both, at tile sizes 64 and 128.  Stream-ordered on torch's
@@ -32,6 +34,7 @@ from dataclasses import dataclass
 from typing import Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .backward import transposed_topology
@@ -360,6 +363,7 @@ class MXLinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         w, (cols, _, rows) = ctx.w, ctx.saved_tensors
         x_dtype, v_dtype = ctx.dtypes
@@ -410,6 +414,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         q_x, q_h, ci_gate, ci_up, ci_down, *_ = ctx.saved_tensors
         gate, up, down = ctx.weights

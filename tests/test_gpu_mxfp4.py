@@ -489,3 +489,37 @@ def test_buffers_aligned_to_16_bytes_only(dtype):
         want = K.mxfp4_linear(x, packed[2], residual=res.clone())
         assert torch.equal(K.mxfp4_linear(x, packed[2], residual=res, out=out), want)
         assert (flat[:per16] == 5).all() and (flat[per16 + T * 256:] == 5).all()
+
+
+def test_gradients_of_fp32_layers_and_of_some_inputs_only():
+    """fp32 rows and tiles: dy is rounded to bf16 once more (2^-8).  Inputs that need no gradient get none, and the
+    others' do not change."""
+    K = _K()
+    rng = np.random.default_rng(15)
+    mats = [weight(rng, 8, 4, 2, 64, 1, F32), weight(rng, 8, 4, 3, 64, 0, F32), weight(rng, 4, 8, 5, 64, 0, F32)]
+    x, dy = rows(rng, 70, 256, F32, 1.0), rows(rng, 70, 256, F32)
+    everything = None
+    for which in ([0, 1, 2, 3], [0], [2], [3], [1, 3]):
+        leaves = [t.detach().clone().requires_grad_(i in which) for i, t in enumerate([x] + [m[0] for m in mats])]
+        y = K.mxfp4_swiglu(leaves[0], leaves[1], mats[0][1], leaves[2], mats[1][1], leaves[3], mats[2][1])
+        assert y.dtype == F32
+        y.backward(dy)
+        if everything is None:
+            everything = [t.grad for t in leaves]
+            _, ws = K.mxfp4_swiglu_fwd(x, *(K.make_mxfp4(m[0], m[1], n) for m, n in zip(mats, (4, 4, 8))),
+                                       return_intermediates=True)
+            refs = M.swiglu_backward(M.quantize(f64(x)), *(m[2] for m in mats), f64(ws["q_h"].dequantize(F32)), f64(dy),
+                                     False)
+            assert rel(f64(leaves[0].grad), refs[0]) <= GRAD_TOL + 2.0 ** -8
+            for t, (_, c, _), ref in zip(leaves[1:], mats, refs[1:]):
+                assert t.grad.dtype == F32
+                assert rel(f64(t.grad), M.tile_grads(ref, f64(c).astype(int), 64)) <= GRAD_TOL + 2.0 ** -8
+        for i, t in enumerate(leaves):
+            assert (t.grad is None) == (i not in which)
+            if i in which:  # tile sums meet in arrival order
+                np.testing.assert_allclose(f64(t.grad), f64(everything[i]), rtol=1e-4, atol=1e-4)
+    with pytest.raises(RuntimeError):  # no second derivative
+        xg = x.detach().requires_grad_(True)
+        y = K.mxfp4_linear_ad(xg, mats[0][0], mats[0][1])
+        (g,) = torch.autograd.grad(y.sum(), xg, create_graph=True)
+        torch.autograd.grad(g.sum(), xg)

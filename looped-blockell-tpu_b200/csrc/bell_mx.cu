@@ -221,72 +221,67 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   uint32_t* count = s.count + ring * G::NR;
   uint8_t* stages = s.stages + ring * (G::NR * G::STAGE);
   int job = 0, part = sub, left = rw.stages > 0 ? rw.jobs : 0;  // of the next use
-  auto settle = [&] {
-    while (part >= rw.stages && job < left) {
-      part -= rw.stages;
-      ++job;
-    }
-  };
-  settle();
-  // A use's entries (lane i: slot i of the stage) and where its chunks are.
+  while (part >= rw.stages && job < left) {
+    part -= rw.stages;
+    ++job;
+  }
+  // Lanes 2i and 2i + 1 bring slot i of a stage, its rows and its weights: one
+  // copy instruction for all of a stage's copies.  (One lane after another's
+  // took 700 cycles a stage, which the stages spend empty: the ring's bytes in
+  // flight, not the L2's rate, bound the kernel.)
+  const int slot = lane >> 1;
+  const bool is_w = lane & 1;
   struct Use {
-    uint32_t e;
-    const uint8_t *x, *w;
+    uint32_t e;           // this lane's slot's entry
+    const uint8_t* base;  // of its chunks
   };
+  // units advance by a fixed step: block-row and token tile without divisions
+  const int step = job_unit<GATED>(p, 1, ring) - job_unit<GATED>(p, 0, ring), dm = step / p.R, dr = step - dm * p.R;
+  int m = job_unit<GATED>(p, job, ring) / p.R, r = job_unit<GATED>(p, job, ring) - m * p.R;
   auto fetch = [&]() -> Use {
-    const int u = job_unit<GATED>(p, job, ring);
-    const int m = u / p.R, r = u - m * p.R;
-    const int k = (rw.first + part) * G::SLOTS + lane;
-    const uint32_t e = lane < G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
-    return {e, p.x + int64_t(m) * p.C * G::A, w + int64_t(r) * K * G::W};
+    const int k = (rw.first + part) * G::SLOTS + slot;
+    const uint32_t e = lane < 2 * G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
+    return {e, is_w ? w + int64_t(r) * K * G::W : p.x + int64_t(m) * p.C * G::A};
   };
   auto advance = [&] {
     part += 2;
-    settle();
+    while (part >= rw.stages && job < left) {
+      part -= rw.stages;
+      ++job;
+      m += dm;
+      r += dr;
+      if (r >= p.R) {
+        r -= p.R;
+        ++m;
+      }
+    }
   };
   auto copies = [&](const Use& use, uint32_t stage, bool weights, bool rows) {
-    const int cnt = __popc(__ballot_sync(0xffffffffu, use.e != kNoSlot));
-    uint32_t ent[G::SLOTS];
-#pragma unroll
-    for (int i = 0; i < G::SLOTS; ++i) ent[i] = __shfl_sync(0xffffffffu, use.e, i);
+    const bool live = use.e != kNoSlot;
+    const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, live)) / 2u;
     uint8_t* st = stages + stage * uint32_t(G::STAGE);
-    if (!p.x) {  // direct rows: this warp's, or with `rows` false already on their way
-      if (elect_one()) {
-        count[stage] = uint32_t(cnt);
-        mbar_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::W));
-#pragma unroll
-        for (int i = 0; i < G::SLOTS; ++i)
-          if (i < cnt)
-            bulk_load(st + i * G::SLOT + G::A, use.w + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
+    uint8_t* to = st + slot * G::SLOT + (is_w ? G::A : 0);
+    const uint8_t* from = use.base + (is_w ? int64_t(use.e >> 16) * G::W : int64_t(use.e & 0xFFFFu) * G::A);
+    if (weights && elect_one()) {
+      count[stage] = cnt;
+      if (!p.x)
+        mbar_expect_tx(&full[stage], cnt * uint32_t(G::W));
+      else if (cnt)
+        mbar_arrive_expect_tx(&full[stage], cnt * uint32_t(G::SLOT));
+      else
+        mbar_arrive(&full[stage]);
+    }
+    __syncwarp();
+    if (live && (is_w ? weights : rows && p.x != nullptr))
+      bulk_load(to, from, is_w ? G::W : G::A, &full[stage], is_w ? keep : pass);
+    if (!p.x && rows) {  // direct rows, this warp's (with `rows` false they are already on their way)
+      for (int i = 0; i < int(cnt); ++i) {
+        const int c = int(__shfl_sync(0xffffffffu, use.e, 2 * i) & 0xFFFFu);
+        for (int n0 = 0; n0 < int(p.T); n0 += DirectRows<B>::N) DirectRows<B>::put(p, c, n0, st + i * G::SLOT);
       }
-      __syncwarp();
-      if (!rows) return;
-#pragma unroll
-      for (int i = 0; i < G::SLOTS; ++i)
-        for (int n0 = 0; i < cnt && n0 < int(p.T); n0 += DirectRows<B>::N)
-          DirectRows<B>::put(p, int(ent[i] & 0xFFFFu), n0, st + i * G::SLOT);
       fence_proxy_async_smem();
       __syncwarp();
       if (elect_one()) mbar_arrive(&full[stage]);
-      __syncwarp();
-      return;
-    }
-    if (elect_one()) {
-      if (weights) {
-        count[stage] = uint32_t(cnt);
-        if (cnt)
-          mbar_arrive_expect_tx(&full[stage], uint32_t(cnt) * uint32_t(G::SLOT));
-        else
-          mbar_arrive(&full[stage]);
-      }
-#pragma unroll
-      for (int i = 0; i < G::SLOTS; ++i) {
-        if (i < cnt) {
-          if (rows) bulk_load(st + i * G::SLOT, use.x + int64_t(ent[i] & 0xFFFFu) * G::A, G::A, &full[stage], pass);
-          if (weights)
-            bulk_load(st + i * G::SLOT + G::A, use.w + int64_t(ent[i] >> 16) * G::W, G::W, &full[stage], keep);
-        }
-      }
     }
     __syncwarp();
   };
@@ -331,7 +326,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     __syncwarp();
   }
   // from here each use's entries travel while the one before is issued
-  Use next{kNoSlot, nullptr, nullptr};
+  Use next{kNoSlot, nullptr};
   if (job < left) next = fetch();
   bool ok = true;
   while (job < left) {

@@ -331,10 +331,11 @@ typedef struct BellMxEll {
 } BellMxEll;
 
 /* Rows that a product quantises itself: for T up to this, x may be NULL (with
- * x_src), which saves a launch. */
+ * x_src), which saves a launch; out must then not overlap x_src. */
 #define BELL_MX_DIRECT_ROWS 32
 
-/* out = Q(x) Q(W)^T (+ residual): fp32 sums, one rounding. */
+/* out = Q(x) Q(W)^T (+ residual): fp32 sums, one rounding.  out may be
+ * residual itself, and must not overlap it otherwise. */
 typedef struct BellMxLinearDesc {
   int64_t T;
   int32_t out_dtype;           /* BELL_DTYPE_BF16 / BELL_DTYPE_F32           */
@@ -385,6 +386,7 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* desc, void* stream);
  * on the live slots (zero in dead ones), in bf16 products with fp32 sums.
  * The transposed topology [C, K_t]: cols_t lists, for each column block, the
  * block-rows that use it (-1 pads), index_t those tiles' positions r * K + k.
+ * K_t is at most 254 (where dx is asked for).
  */
 typedef struct BellMxLinearBwdDesc {
   int64_t T;
@@ -412,8 +414,8 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
  * rows; the projections are computed again.  cols_t_down / index_t_down:
  * transposed topology of down [d_ff/B, K_t_down]; cols_t_gate_up /
  * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
- * of up, and its tiles, counted after gate's).  Results that are NULL are not
- * computed.  With add_residual, dx includes grad_out.
+ * of up, and its tiles, counted after gate's); each K_t at most 254.  Results
+ * that are NULL are not computed.  With add_residual, dx includes grad_out.
  */
 typedef struct BellMxFFNBwdDesc {
   int64_t T;

@@ -141,6 +141,14 @@ static int check_weight(const BellMxEll& w, const char* name) {
   return BELL_OK;
 }
 
+// the bf16 products' rows have at most 254 slots
+static int check_k_t(int32_t k_t, const char* name) {
+  if (k_t > 254)
+    return fail(BELL_ERR_SHAPE, std::string(name) + ": a column block is used by " + std::to_string(k_t) +
+                                    " block-rows; the backward takes at most 254");
+  return BELL_OK;
+}
+
 static bool grad_type(int32_t t) { return t == BELL_DTYPE_BF16 || t == BELL_DTYPE_F32; }
 
 }  // namespace mx
@@ -161,6 +169,8 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   if (d->T < 0 || d->T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "T must be in [0, 2^31 - 256)");
   if (d->T > 0 && (!d->grad_out || !d->x)) return fail(BELL_ERR_ARG, "grad_out and x must be non-NULL");
   if (d->dx && (!d->cols_t || !d->index_t || d->K_t < 1)) return fail(BELL_ERR_ARG, "dx needs the transposed topology");
+  if (d->dx)
+    if (int rc = mx::check_k_t(d->K_t, "weight")) return rc;
   if (d->dw && (!d->col_indices || !mx::grad_type(d->grad_dtype)))
     return fail(BELL_ERR_ARG, "dw needs col_indices and a bf16 or f32 grad_dtype");
   if (!d->workspace || !aligned16(d->workspace)) return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned");
@@ -210,6 +220,10 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   if (!d->cols_t_down || !d->index_t_down || d->K_t_down < 1 || !d->cols_t_gate_up || !d->index_t_gate_up ||
       d->K_t_gate_up < 1)
     return fail(BELL_ERR_ARG, "the transposed topologies must be given");
+  if (d->dx || d->d_gate || d->d_up)
+    if (int rc = mx::check_k_t(d->K_t_down, "down")) return rc;
+  if (d->dx)
+    if (int rc = mx::check_k_t(d->K_t_gate_up, "gate and up")) return rc;
   if ((d->d_gate && (!d->cols_gate || !mx::grad_type(d->gate_dtype))) ||
       (d->d_up && (!d->cols_up || !mx::grad_type(d->up_dtype))) ||
       (d->d_down && (!d->cols_down || !mx::grad_type(d->down_dtype))))

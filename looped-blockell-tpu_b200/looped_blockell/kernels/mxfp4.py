@@ -18,9 +18,11 @@ saturates.  A block that holds an infinity or a NaN is NaN throughout.
   from the gate/up kernel to the down projection.
 * ``mxfp4_linear_ad``, ``mxfp4_swiglu``: the same, differentiable.  The
   gradient passes straight through Q: the backward is the bf16 one at the
-  quantised operands (their values are exact in bf16).  A weight's first
-  backward builds its transposed topology and waits for the device once: run a
-  step before capturing one in a graph.
+  quantised operands (their values are exact in bf16).  Tile
+  gradients are fp32 sums of token ranges that meet in arrival order: their
+  last bits may differ from run to run.  A weight's first backward builds its
+  transposed topology and waits for the device once: before a step is captured
+  in a graph, run one, and let no autograd graph of the same leaves live on.
 
 Where ``ternary`` keeps 2 bits a weight and int8 activations, this keeps
 4.25 bits of both, at tile sizes 64 and 128.  Stream-ordered on torch's
@@ -93,9 +95,25 @@ class MXBlockELL:
     C: int                     # input column blocks
     B: int
 
-    def __post_init__(self):
-        at = self.data.data_ptr()
-        self._abi = _lib.BellMxEll(at, at + _tiles_bytes(self.R, self.K, self.B), self.R, self.C, self.K, self.B)
+    _key = None  # what _struct was made from
+
+    @property
+    def _abi(self):
+        """The library's view of this weight, made again when a field has changed."""
+        key = (self.data.data_ptr(), self.R, self.K, self.C, self.B)
+        if key != self._key:
+            _check_cuda("quantised weight", self.data)
+            _check_tile(self.B)
+            size = _tiles_bytes(self.R, self.K, self.B)
+            if self.R < 1 or self.K < 1 or self.data.dtype != torch.uint8 or not self.data.is_contiguous() or \
+                    self.data.numel() < size + plan_bytes(0, 0, 0, self.R, self.K):
+                raise RuntimeError("MXBlockELL.data does not hold R x K quantised tiles and their plan")
+            self._struct = _lib.BellMxEll(key[0], key[0] + size, self.R, self.C, self.K, self.B)
+            self._key = key
+        return self._struct
+
+    def __getstate__(self):  # a copy has other addresses
+        return {k: v for k, v in self.__dict__.items() if k not in ("_key", "_struct")}
 
     @property
     def in_features(self) -> int:
@@ -240,6 +258,14 @@ def _source(x, tile: int, features: int):
     return x.shape[0], x.device, x.dtype, x.data_ptr(), _ld(x), _DTYPES[x.dtype]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two 2-D tensors of rows share addresses (the ranges they span)."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _check_residual(residual, shape, dtype, dev) -> torch.Tensor:
     _check_cuda("residual", residual)
     if tuple(residual.shape) != shape or residual.dtype != dtype or residual.device != dev:
@@ -257,7 +283,8 @@ def mxfp4_linear(x: Union[torch.Tensor, MXRows], w: MXBlockELL, residual: Option
     ``x`` is ``[T, in_features]`` bf16 or fp32, or rows quantised before
     (``mxfp4_quantize``).  The output has ``out_dtype`` (default: x's, bf16 for
     quantised rows); ``residual`` has the output's shape and dtype.
-    ``max_ctas`` caps the persistent grid (0 = every SM)."""
+    ``out`` may be ``residual`` or ``x`` itself.  ``max_ctas`` caps the
+    persistent grid (0 = every SM)."""
     return _linear(x, w, residual, out_dtype, out, max_ctas)[0]
 
 
@@ -270,12 +297,17 @@ def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0, keep_rows
     dtype = out_dtype or dtype
     if dtype not in _DTYPES:
         raise RuntimeError("out_dtype must be bf16 or fp32")
+    if residual is not None:
+        residual = _check_residual(residual, (T, out_f), dtype, dev)
     if out is None:
         out = torch.empty((T, out_f), dtype=dtype, device=dev)
     else:
         _check_out("out", out, (T, out_f), dtype, dev)
-    if residual is not None:
-        residual = _check_residual(residual, (T, out_f), dtype, dev)
+        # one CTA writes its outputs while others still read x (direct) or
+        # residual elements other than those they replace
+        keep_rows = keep_rows or src is not None and _overlap(out, x)
+        if residual is not None and residual.data_ptr() != out.data_ptr() and _overlap(out, residual):
+            residual = residual.clone()
     if src is None:
         rows = x.data
     else:  # a few rows are quantised by the product itself
@@ -395,7 +427,8 @@ def mxfp4_linear_ad(x: torch.Tensor, values: torch.Tensor, cols: torch.Tensor, r
 
     The backward passes the gradient straight through Q:
     ``dx = dy Q(W)``, ``dW = dy^T Q(x)`` on the live tiles (zero in dead slots),
-    in bf16 products with fp32 sums."""
+    in bf16 products with fp32 sums.  A column block of W may be used by at most
+    254 block-rows."""
     if x.dim() != 2 or values.dim() != 4 or x.shape[1] % values.shape[2]:
         raise RuntimeError("x must be 2D [N, C*B] and values [R, K, B, B]")
     return MXLinearFn.apply(x, values, cols, residual, layout)
@@ -424,10 +457,12 @@ class MXSwiGLUFn(torch.autograd.Function):
         td_cols, td_index = transposed_topology([ci_down], gate.R)
         tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
         dx = torch.empty_like(dy) if need[0] else None
+        # fp32 rows: the residual's gradient is added to theirs in fp32
+        late = ctx.add_residual and ctx.dtypes[0] == torch.float32
         cols = (gate.col_indices, up.col_indices, down.col_indices)
         grads = [_grad(n, c, gate.B, t) for n, c, t in zip((need[1], need[3], need[5]), cols, ctx.dtypes[1:])]
         d = _lib.BellMxFFNBwdDesc(
-            T, int(ctx.add_residual), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
+            T, int(ctx.add_residual and not late), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
             q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
             td_cols.data_ptr(), td_index.data_ptr(), tg_cols.data_ptr(), tg_index.data_ptr(), td_cols.shape[1],
             tg_cols.shape[1], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
@@ -436,7 +471,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         d.workspace = ws.data_ptr()
         _call("bell_swiglu_bwd_mx", dev, C.byref(d))
         if dx is not None:
-            dx = dx.to(ctx.dtypes[0])
+            dx = dx + grad_out if late else dx.to(ctx.dtypes[0])
         return dx, grads[0][0], None, grads[1][0], None, grads[2][0], None, None, None
 
 
@@ -450,7 +485,8 @@ def mxfp4_swiglu(x: torch.Tensor, v_gate: torch.Tensor, ci_gate: torch.Tensor, v
     Q(W), Q(h), the gradient passing straight through Q; the projections are
     computed again rather than kept, so a step keeps 4.25 bits a value of x
     and h.  Tile gradients are summed in fp32 and come back in the tiles'
-    dtype."""
+    dtype.  A column block may be used by at most 254 block-rows of down, and by
+    254 of gate and up together."""
     if x.dim() != 2 or v_gate.dim() != 4 or v_up.dim() != 4 or v_down.dim() != 4:
         raise RuntimeError("x must be 2D [N, d_model] and the tiles 4D [R, K, B, B]")
     if x.shape[1] % v_gate.shape[2]:

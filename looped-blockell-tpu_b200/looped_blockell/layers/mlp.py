@@ -79,8 +79,15 @@ class BlockELLLinear(nn.Module):
         hit = cache.get(name)
         if hit is None or hit[0] != key:
             hit = (key, make())
-            cache[name] = hit
+            # made during a capture it holds nothing until a replay
+            if not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+                cache[name] = hit
         return hit[1]
+
+    def __getstate__(self):  # copies and pickles make their own kernel copies
+        state = self.__dict__.copy()
+        state.pop("_kcache", None)
+        return state
 
     def effective_col_indices(self) -> torch.Tensor:
         """col_indices with dead slots set to -1 (skipped by the kernel)."""
@@ -98,11 +105,28 @@ class BlockELLLinear(nn.Module):
         return self._cached("values", key, lambda: v.detach().to(self.dtype).contiguous())
 
     def mxfp4_weight(self):
-        """The quantised weight (``kernels.MXBlockELL``) of the current parameters."""
+        """The quantised weight (``kernels.MXBlockELL``) of the current parameters.
+
+        While a graph is captured it is made anew, inside the graph: replays
+        then follow the parameters.  A graph that should not quantise again
+        takes a weight made before its capture (``kernels.mxfp4_linear``,
+        ``kernels.mxfp4_swiglu_fwd``)."""
         from ..kernels.mxfp4 import make_mxfp4
         v, cols = self.values, self.effective_col_indices()
+        if not v.is_cuda or torch.cuda.is_current_stream_capturing():
+            return make_mxfp4(v.detach(), cols, self.C)
         key = (v.data_ptr(), v._version, v.dtype, cols.data_ptr(), cols._version)
-        return self._cached("mxfp4", key, lambda: make_mxfp4(v.detach(), cols, self.C))
+        stream = torch.cuda.current_stream(v.device)
+
+        def make():  # with the tensors that the key's addresses belong to
+            w = make_mxfp4(v.detach(), cols, self.C)
+            return w, stream, stream.record_event(), v.detach(), cols
+
+        w, made_on, ready, *_ = self._cached("mxfp4", key, make)
+        if stream != made_on:
+            stream.wait_event(ready)
+            w.data.record_stream(stream)
+        return w
 
     def as_block_ell(self) -> BlockELLTensor:
         return BlockELLTensor(values=self.kernel_values(), col_indices=self.effective_col_indices(), config=self.config)

@@ -523,3 +523,131 @@ def test_gradients_of_fp32_layers_and_of_some_inputs_only():
         y = K.mxfp4_linear_ad(xg, mats[0][0], mats[0][1])
         (g,) = torch.autograd.grad(y.sum(), xg, create_graph=True)
         torch.autograd.grad(g.sum(), xg)
+
+
+@pytest.mark.parametrize("T", [5, 100])
+@pytest.mark.parametrize("B", [64, 128])
+def test_outputs_that_overlap_inputs(T, B):
+    """out may be x or the residual; a residual that starts a row later is read before it is overwritten."""
+    K = _K()
+    rng = np.random.default_rng(16)
+    v, cols, _ = weight(rng, 512 // B, 512 // B, 2, B)
+    w = K.make_mxfp4(v, cols, 512 // B)
+    x, res = rows(rng, T, 512), rows(rng, T, 512)
+    want, want_res = K.mxfp4_linear(x, w), K.mxfp4_linear(x, w, residual=res)
+    for _ in range(5):
+        buf = x.clone()
+        assert K.mxfp4_linear(buf, w, out=buf) is buf and torch.equal(buf, want)
+        buf = res.clone()
+        K.mxfp4_linear(x, w, residual=buf, out=buf)
+        assert torch.equal(buf, want_res)
+        buf = torch.cat([torch.zeros_like(res[:1]), res])
+        K.mxfp4_linear(x, w, residual=buf[1:], out=buf[:T])
+        assert torch.equal(buf[:T], want_res)
+        buf = torch.cat([x, torch.zeros_like(x[:1])])
+        K.mxfp4_linear(buf[:T], w, out=buf[1:])
+        assert torch.equal(buf[1:], want)
+
+
+def test_a_weight_whose_fields_change():
+    """The library sees the fields of the call, not those of the weight's making."""
+    import copy
+    K = _K()
+    rng = np.random.default_rng(17)
+    v, cols, _ = weight(rng, 3, 4, 2, 64)
+    w = K.make_mxfp4(v, cols, 4)
+    x = rows(rng, 9, 256)
+    want = K.mxfp4_linear(x, w)
+    other = copy.deepcopy(w)
+    w.data = w.data.clone()
+    assert torch.equal(K.mxfp4_linear(x, w), want) and torch.equal(K.mxfp4_linear(x, other), want)
+    for bad in (dict(R=4), dict(data=w.data[:-16]), dict(data=w.data.view(torch.int8)), dict(B=32),
+                dict(data=w.data.cpu())):
+        broken = copy.copy(w)
+        for k, f in bad.items():
+            setattr(broken, k, f)
+        with pytest.raises(RuntimeError):
+            K.mxfp4_linear(x, broken)
+        with pytest.raises(RuntimeError):
+            broken.dequantize()
+
+
+def _block():
+    from looped_blockell.layers import MLPBlock
+    torch.manual_seed(1)
+    return MLPBlock(256, 512, use_swiglu=True, tile_size=64, density=0.5, device="cuda", weight_format="mxfp4")
+
+
+@torch.no_grad()
+def test_a_captured_layer_follows_its_parameters():
+    """Captured before any eager call: replays see updates, and the eager call after it has a weight of its own."""
+    m, ref = _block(), _block()
+    x = torch.randn(40, 256, device="cuda", dtype=BF16)
+    ref(x)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        y = m(x)
+    assert torch.equal(m(x), ref(x))  # the graph has not run yet
+    g.replay()
+    assert torch.equal(y, ref(x))
+    for b in (m, ref):
+        b.w_down.values.mul_(-3)
+        b.w_up.alive_mask[0, 0] = False
+        b.w_up.values[0, 0] = 0  # the graph's topology is that of its capture
+    g.replay()
+    assert torch.equal(y, ref(x)) and torch.equal(m(x), ref(x))
+
+
+@torch.no_grad()
+def test_a_layer_used_on_two_streams():
+    """The weight quantised on one stream is ready on the next one that uses it, and outlives its replacement there."""
+    x = torch.randn(40, 256, device="cuda", dtype=BF16)
+    want = [_block()(x)]
+    m = _block()
+    m.w_down.values.mul_(2)
+    want.append(m(x))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        m = _block()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            busy = torch.randn(2000, 2000, device="cuda")
+            for _ in range(20):
+                busy = busy @ busy * 1e-3
+            m.w_down.mxfp4_weight(), m.w_up.mxfp4_weight(), m.w_gate.mxfp4_weight()
+        y0 = m(x)
+        m.w_down.values.mul_(2)
+        y1 = m(x)
+        junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(y0, want[0]) and torch.equal(y1, want[1])
+        del junk
+
+
+def test_residual_gradient_of_fp32_rows_is_not_rounded():
+    K = _K()
+    rng = np.random.default_rng(18)
+    mats, _ = _ffn(rng)
+    x0, dy = rows(rng, 33, 256, F32), rows(rng, 33, 256, F32)
+    dx = []
+    for add in (False, True):
+        x = x0.clone().requires_grad_(True)
+        y = K.mxfp4_swiglu(x, mats[0][0], mats[0][1], mats[1][0], mats[1][1], mats[2][0], mats[2][1], add_residual=add)
+        dx.append(torch.autograd.grad(y, x, dy)[0])
+    assert torch.equal(dx[1], dx[0] + dy)
+
+
+def test_more_slots_than_the_backward_takes():
+    """A column block that 255 block-rows use: the forward and the tile gradients run, dx is refused before it starts."""
+    K = _K()
+    rng = np.random.default_rng(19)
+    cols = torch.zeros(255, 1, dtype=torch.int32, device="cuda")
+    v = torch.randn(255, 1, 64, 64, device="cuda").to(BF16).requires_grad_(True)
+    x = rows(rng, 3, 64).requires_grad_(True)
+    y = K.mxfp4_linear_ad(x.detach(), v, cols)
+    assert torch.autograd.grad(y.sum(), v)[0].isfinite().all()
+    y = K.mxfp4_linear_ad(x, v, cols)
+    with pytest.raises(RuntimeError, match="254"):
+        y.sum().backward()

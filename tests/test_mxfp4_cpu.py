@@ -175,6 +175,9 @@ def test_backward_refusals():
     d.K_t, d.dx = 1, 1024
     # unpacked transpose [3, 1] tiles + plan + Q(x) + fp32 sums of [2, 2] tiles, each padded to 256 bytes
     assert lib.bell_linear_bwd_mx_workspace_bytes(C.byref(d)) == 3 * 64 * 64 * 2 + 256 + 4 * 192 * 2 + 4 * 64 * 64 * 4
+    d.cols_t = d.index_t = d.workspace = 1024
+    d.K_t = 255
+    assert lib.bell_linear_bwd_mx(C.byref(d), None) == -2 and "254" in L.last_error()
     f = L.BellMxFFNBwdDesc()
     f.T, f.gate, f.up, f.down = 4, _mx(L, 4, 2), _mx(L, 4, 2), _mx(L, 2, 4)
     f.grad_out = f.x = f.h = f.workspace = 1024
@@ -182,3 +185,20 @@ def test_backward_refusals():
     assert lib.bell_swiglu_bwd_mx_workspace_bytes(C.byref(f)) == 0
     f.up = _mx(L, 4, 3)
     assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -2
+    f.up, f.dx = _mx(L, 4, 2), 1024
+    f.cols_t_down = f.index_t_down = f.cols_t_gate_up = f.index_t_gate_up = 1024
+    for kd, kg, name in [(255, 1, "down"), (1, 255, "gate and up")]:
+        f.K_t_down, f.K_t_gate_up = kd, kg
+        assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -2 and "254" in L.last_error() and name in L.last_error()
+
+
+def test_a_copied_layer_makes_its_own_kernel_copies():
+    """A copy or a pickle holds no buffer that was derived for the original."""
+    import copy
+    import pickle
+    from looped_blockell.layers import MLPBlock
+    m = MLPBlock(128, 256, use_swiglu=True, tile_size=64, weight_format="mxfp4")
+    m.w_gate.effective_col_indices()
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert "_kcache" not in other.w_gate.__dict__ and torch.equal(other.w_gate.values, m.w_gate.values)
+    assert "_kcache" in m.w_gate.__dict__

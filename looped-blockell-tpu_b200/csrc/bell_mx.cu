@@ -22,17 +22,26 @@
 // dead row's are empty), so that every warp knows the order of the stages
 // without reading the plan first.
 //
-// The issuing warp's wait, commit and bookkeeping cost about 300 cycles a
-// stage, more than a slot's MMAs (B = 128: 128 cycles at the fp4 rate).  Hence
-// the multi-slot stages, and two issuers: job j of the CTA belongs to issuer
-// j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
+// The issuing warp's wait, commit and bookkeeping cost about 170 cycles a
+// stage, as much as a slot's MMAs (B = 128: 120 cycles and 20 for its scales).
+// Hence the multi-slot stages, and two issuers: job j of the CTA belongs to
+// issuer j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
 //
-// Warps: 0-3 producers (ring w / 2; stage use h of a ring belongs to its
-// producer h & 1), 4-19 epilogue (a warp takes the TMEM lane quadrant w % 4 and
-// one 32-column block of a unit; at B = 64, two blocks, two groups of eight
-// warps take the CTA's units in turn), 20 and 21 issuers (20 owns TMEM).
-// Accumulators form a ring of ACCS in job order, so the issuers run ahead of the
-// epilogue.
+// What bounds it: B = 128, the way from the L2 into the SM.  A slot is 17.4 KB
+// and takes 300 cycles of the 140 that its MMAs need (T = 16384, 16384 -> 4096:
+// 143 us, 3.8 PFLOP/s, 16 TB/s out of the L2; with a quarter of the bytes left
+// out 132).  B = 64, gated: the epilogue, 16 instructions an output
+// (T = 16384, d = 2048, d_ff = 8192: 125 us; without the SiLU's exponential and
+// reciprocal 104).
+//
+// Warps: 0-5 producers (ring w / 3; stage use h of a ring belongs to its
+// producer h % 3, since a producer's turn, from a stage's release to its copies'
+// issue, is on the ring's path: one producer a ring 156 us where two or three
+// take 146 to 143, gated B = 64 128 us with two, 125 with three), 6-21 epilogue
+// (a warp takes the TMEM lane quadrant warp % 4 and one 32-column block of a
+// unit; at B = 64, two blocks, two groups of eight warps take the CTA's units in
+// turn), 22 and 23 issuers (22 owns TMEM).  Accumulators form a ring of ACCS in
+// job order, so the issuers run ahead of the epilogue.
 //
 // Few units (a linear of few tokens): split mode.  A cluster of `split` CTAs
 // shares one unit, each ring of each CTA takes an equal range of the stages
@@ -56,9 +65,10 @@
 namespace bell {
 namespace mx {
 
-static constexpr int kProducers = 4;  // two to a ring
+static constexpr int kPer = 3;       // producers of a ring
+static constexpr int kProducers = 2 * kPer;
 static constexpr int kEpiWarps = 16;
-static constexpr int kIssuer = kProducers + kEpiWarps;  // 20, 21
+static constexpr int kIssuer = kProducers + kEpiWarps;  // 22, 23
 static constexpr int kThreads = 32 * (kIssuer + 2);
 
 template <int B>
@@ -73,8 +83,9 @@ struct Geo {
   static constexpr int SF_COL = ACCS * B;        // 8 scale columns per slot of a stage from here
   static constexpr int SMEM = NS * STAGE + 1024 + 1024;
   // a producer's wait for the release of use h - NR must not meet the parity of
-  // use h - 2 NR: that one is released before h - 2 - NR, which it waited for
-  static_assert(NR > 2, "mbarrier parity");
+  // use h - 2 NR: that one is released no later than h - kPer - NR, which it
+  // waited for
+  static_assert(NR >= kPer, "mbarrier parity");
   static_assert(SF_COL + NS * SLOTS * 8 <= 512, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -227,8 +238,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   }
   // Lanes 2i and 2i + 1 bring slot i of a stage, its rows and its weights: one
   // copy instruction for all of a stage's copies.  (One lane after another's
-  // took 700 cycles a stage, which the stages spend empty: the ring's bytes in
-  // flight, not the L2's rate, bound the kernel.)
+  // took 700 cycles a stage, which the stages spend empty.)
   const int slot = lane >> 1;
   const bool is_w = lane & 1;
   struct Use {
@@ -244,7 +254,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     return {e, is_w ? w + int64_t(r) * K * G::W : p.x + int64_t(m) * p.C * G::A};
   };
   auto advance = [&] {
-    part += 2;
+    part += kPer;
     while (part >= rw.stages && job < left) {
       part -= rw.stages;
       ++job;
@@ -289,7 +299,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   int64_t filled = 0;
   auto turn = [&] {
     ++filled;
-    stage += 2;
+    stage += kPer;
     if (stage >= uint32_t(G::NR)) {
       stage -= G::NR;
       phase ^= 1u;
@@ -298,14 +308,14 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   // The ring's first filling: the weights need not wait for the rows, which the
   // kernel ahead or the epilogue's warps make.
   if (p.early || !p.x) {
-    Use first[(G::NR + 1) / 2];
+    Use first[(G::NR + kPer - 1) / kPer];
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < (G::NR + 1) / 2; ++i) {
-      if (sub + 2 * i < G::NR && job < left) {
+    for (int i = 0; i < (G::NR + kPer - 1) / kPer; ++i) {
+      if (sub + kPer * i < G::NR && job < left) {
         first[i] = fetch();
         advance();
-        copies(first[i], uint32_t(sub + 2 * i), true, false);
+        copies(first[i], uint32_t(sub + kPer * i), true, false);
         n = i + 1;
       }
     }
@@ -314,12 +324,12 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     else
       direct_barrier();
 #pragma unroll
-    for (int i = 0; i < (G::NR + 1) / 2; ++i) {
+    for (int i = 0; i < (G::NR + kPer - 1) / kPer; ++i) {
       if (i < n) {
         if (p.x)
-          copies(first[i], uint32_t(sub + 2 * i), false, true);
+          copies(first[i], uint32_t(sub + kPer * i), false, true);
         else if (elect_one())
-          mbar_arrive(&full[sub + 2 * i]);
+          mbar_arrive(&full[sub + kPer * i]);
         turn();
       }
     }
@@ -340,11 +350,11 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   }
   if (!ok && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
     for (int i = 0; i < G::NR && filled > 0; ++i, --filled) {
-      if (stage < 2u) {
+      if (stage < uint32_t(kPer)) {
         stage += G::NR;
         phase ^= 1u;
       }
-      stage -= 2;
+      stage -= kPer;
       const uint32_t a = smem_u32(&full[stage]);
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(a, phase) && globaltimer_ns() - t0 < 100000000ull) {
@@ -536,7 +546,7 @@ template <int B>
 __device__ void split_partial(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
   using G = Geo<B>;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
-  const int q = w & 3, j = w >> 2;
+  const int q = int(threadIdx.x >> 5) & 3, j = w >> 2;
   if (j >= B / 32) return;  // one unit: the second group of B = 64 has none
   const int u = int(blockIdx.x) / p.split, m = u / p.R, r = u - m * p.R;
   const int n = q * 32 + lane;
@@ -619,25 +629,35 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
   constexpr int GROUPS = kEpiWarps / (4 * NB);
   constexpr int JOBS = GATED ? 2 : 1;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
-  const int q = w & 3, j = (w >> 2) % NB, group = (w >> 2) / NB;
+  const int q = int(threadIdx.x >> 5) & 3, j = (w >> 2) % NB, group = (w >> 2) / NB;
   const int units = p.mtiles * p.R;
   const int64_t ld = int64_t(p.R) * B;
   const uint32_t lanes = uint32_t(q * 32) << 16;
   const int step = GROUPS * int(gridDim.x);
   uint32_t acc = uint32_t(group * JOBS), use = 0;  // accumulator of this unit's first job
   int c0 = 0, c1 = 0;  // live slots of the next unit's rows, read a unit ahead
-  auto counts = [&](int u) {
-    c0 = __ldg(p.p0.counts + u % p.R);
-    if (GATED) c1 = __ldg(p.p1.counts + u % p.R);
+  auto counts = [&](int r) {
+    c0 = __ldg(p.p0.counts + r);
+    if (GATED) c1 = __ldg(p.p1.counts + r);
   };
   int u = int(blockIdx.x) + group * int(gridDim.x);
-  if (u < units) counts(u);
+  // the next unit's token tile and block-row, advanced without divisions
+  const int dm = step / p.R, dr = step - dm * p.R;
+  int mn = u / p.R, rn = u - mn * p.R;
+  if (u < units) counts(rn);
   for (; u < units; u += step) {
-    const int m = u / p.R, r = u - m * p.R;
+    const int m = mn, r = rn;
     const int n = q * 32 + lane;
     const int64_t t = int64_t(m) * kRows + n;
     const bool live0 = c0 > 0, live1 = c1 > 0;
-    if (u + step < units) counts(u + step);
+    mn += dm;
+    rn += dr;
+    if (rn >= p.R) {
+      rn -= p.R;
+      ++mn;
+    }
+    const bool more = u + step < units;
+    if (more) counts(rn);
     const int64_t at = t * ld + int64_t(r) * B + j * 32;
     if constexpr (MODE == kGatedBackward) {
       const uint32_t a0 = acc, a1 = acc + 1 == uint32_t(G::ACCS) ? 0u : acc + 1;
@@ -653,10 +673,9 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       // a lane's 32 columns are one line of d_h: the next unit's is called into L2
       // now (this kernel waits for memory, not for its rate; without it 405 us
       // at T = 8192, d = 4096, d_ff = 16384)
-      const int un = u + step, mn = un / p.R;
       const int64_t tn = int64_t(mn) * kRows + n;
-      if (un < units && tn < p.T)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.dh + tn * ld + int64_t(un - mn * p.R) * B + j * 32));
+      if (more && tn < p.T)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.dh + tn * ld + int64_t(rn) * B + j * 32));
       fetch(0);
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a1], use1 & 1u, ctl))) return;
@@ -717,11 +736,11 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       };
       // 16 columns at a time: 32 spill.  B = 128: the gate half is freed as soon
       // as it is read, so that the next unit's jobs wait less for one of the
-      // three accumulators (gate/up at T = 16384, d = 4096, d_ff = 16384: 305 us
+      // three accumulators (gate/up at T = 16384, d = 4096, d_ff = 16384: 307 us
       // against 345 with both halves read together).  B = 64, two units in turn
-      // on the epilogue's two groups, is bound by the epilogue's instructions
-      // and gains from fewer waits (124 us together, 138 one after the other;
-      // d = 2048, d_ff = 8192).
+      // on the epilogue's two groups, is bound by the epilogue and gains from
+      // fewer waits (125 us together, 138 one after the other; d = 2048,
+      // d_ff = 8192).
       if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[a0], use & 1u, ctl))) return;
       if constexpr (B == 128) {
         tc_fence_after();
@@ -821,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   if (!p.early || warp >= kProducers) griddep_wait();
   const bool split = !GATED && p.split;
   if (warp < kProducers) {
-    produce<B, GATED>(p, s, warp >> 1, warp & 1, ctl);
+    produce<B, GATED>(p, s, warp / kPer, warp % kPer, ctl);
   } else if (warp < kIssuer) {
     if (!p.x) direct_first<B, GATED>(p, s);
     if constexpr (!GATED) {

@@ -75,8 +75,10 @@ struct EightOf<float> {
 // scale block.  (One lane to a block, its loads 64 bytes apart from the next
 // lane's, read fp32 at 4.6 TB/s instead of 6.4.)  The four lanes then exchange
 // their words, so that lane k has all 16 bytes of pass k, and eight rows' stores
-// fill a core matrix (128 bytes).  bf16 is bound by the arithmetic, 15
-// instructions a value (72 % of the issue slots at T = 8192, d = 16384, 71 us).
+// fill a core matrix (128 bytes).  T = 8192, d = 16384: 67 us, 5.1 TB/s (T = 16384
+// 126 us, 5.4 TB/s), where dequantisation, which computes little, reaches 5.5
+// (5.7); the ALU is 74 % busy with 13 instructions a value, and without the
+// maxima it took 65 us, so that memory is the nearer bound.
 template <class E>
 __global__ void __launch_bounds__(kThr) bell_mx_quantize_kernel(RowsArgs a, const E* __restrict__ src, int64_t ld,
                                                                uint8_t* __restrict__ dst) {

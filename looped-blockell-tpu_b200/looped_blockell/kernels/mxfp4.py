@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import cached_property, lru_cache
 from typing import Optional, Union
 
 import torch
@@ -85,7 +86,7 @@ class MXRows:
         return mxfp4_dequantize(self, dtype)
 
 
-@dataclass
+@dataclass(frozen=True)
 class MXBlockELL:
     """A quantised Block-ELL weight (``make_mxfp4``)."""
     data: torch.Tensor         # uint8: the quantised tiles, operand layout, then the plan of the live slots
@@ -95,25 +96,21 @@ class MXBlockELL:
     C: int                     # input column blocks
     B: int
 
-    _key = None  # what _struct was made from
+    @cached_property
+    def _abi(self):  # the library's view of this weight
+        data = self.data
+        _check_cuda("quantised weight", data)
+        _check_tile(self.B)
+        if self.R < 1 or self.K < 1 or data.dtype != torch.uint8 or not data.is_contiguous() or \
+                data.numel() < _tiles_bytes(self.R, self.K, self.B) + _plan_bytes(self.R, self.K):
+            raise RuntimeError("MXBlockELL.data does not hold R x K quantised tiles and their plan")
+        return self._view(data.data_ptr())
 
-    @property
-    def _abi(self):
-        """The library's view of this weight, made again when a field has changed."""
-        key = (self.data.data_ptr(), self.R, self.K, self.C, self.B)
-        if key != self._key:
-            _check_cuda("quantised weight", self.data)
-            _check_tile(self.B)
-            size = _tiles_bytes(self.R, self.K, self.B)
-            if self.R < 1 or self.K < 1 or self.data.dtype != torch.uint8 or not self.data.is_contiguous() or \
-                    self.data.numel() < size + plan_bytes(0, 0, 0, self.R, self.K):
-                raise RuntimeError("MXBlockELL.data does not hold R x K quantised tiles and their plan")
-            self._struct = _lib.BellMxEll(key[0], key[0] + size, self.R, self.C, self.K, self.B)
-            self._key = key
-        return self._struct
+    def _view(self, at: int):
+        return _lib.BellMxEll(at, at + _tiles_bytes(self.R, self.K, self.B), self.R, self.C, self.K, self.B)
 
     def __getstate__(self):  # a copy has other addresses
-        return {k: v for k, v in self.__dict__.items() if k not in ("_key", "_struct")}
+        return {k: v for k, v in self.__dict__.items() if k != "_abi"}
 
     @property
     def in_features(self) -> int:
@@ -131,6 +128,11 @@ class MXBlockELL:
         return v if layout == TILE_OUT_IN else v.transpose(-1, -2).contiguous()
 
 
+@lru_cache(maxsize=256)
+def _plan_bytes(R: int, K: int) -> int:
+    return plan_bytes(0, 0, 0, R, K)
+
+
 def _tiles_bytes(R: int, K: int, B: int) -> int:
     return R * K * (B * B // 2 + 512)
 
@@ -143,6 +145,8 @@ def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
         raise RuntimeError(f"{name} must be 2D [N, features]")
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"{name} must be bf16 or fp32")
+    if x.is_contiguous() and x.data_ptr() % 16 == 0 and x.shape[1] % 8 == 0:
+        return x
     per16 = 16 // x.element_size()
     T, f = x.shape
     ok = x.data_ptr() % 16 == 0 and x.stride(1) == 1 and \
@@ -229,12 +233,13 @@ def _pack(weights, layout: int):
             raise RuntimeError("values and col_indices must be on one device")
         if v.data_ptr() % 16:
             v = v.clone()
-        size = _tiles_bytes(R, K, B)
-        data = _bytes(size + plan_bytes(0, 0, 0, R, K), dev)
-        abi[i] = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, int(C_blocks), K, B, layout, 0)
-        chunks[i], plans[i] = data.data_ptr(), data.data_ptr() + size
+        data = _bytes(_tiles_bytes(R, K, B) + _plan_bytes(R, K), dev)
+        w = MXBlockELL(data, cols, R, K, int(C_blocks), B)
+        view = w.__dict__["_abi"] = w._view(data.data_ptr())
+        abi[i] = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, w.C, K, B, layout, 0)
+        chunks[i], plans[i] = view.chunks, view.plan
         held.append(v)
-        out.append(MXBlockELL(data, cols, R, K, int(C_blocks), B))
+        out.append(w)
     _call("bell_mx_pack_ell", dev, abi, n, _DTYPES[dtype], chunks, plans, None)
     return out
 
@@ -300,7 +305,7 @@ def _linear(x, w, residual=None, out_dtype=None, out=None, max_ctas=0, keep_rows
     if residual is not None:
         residual = _check_residual(residual, (T, out_f), dtype, dev)
     if out is None:
-        out = torch.empty((T, out_f), dtype=dtype, device=dev)
+        out = w.data.new_empty((T, out_f), dtype=dtype)
     else:
         _check_out("out", out, (T, out_f), dtype, dev)
         # one CTA writes its outputs while others still read x (direct) or
@@ -354,7 +359,7 @@ def _swiglu(x, gate, up, down, add_residual=False, residual=None, keep_rows=Fals
                 raise RuntimeError("add_residual on quantised rows needs the residual")
             residual = x
         residual = _check_residual(residual, (T, D), dtype, dev)
-    out = torch.empty((T, D), dtype=dtype, device=dev)
+    out = gate.data.new_empty((T, D), dtype=dtype)
     direct = not quantised and not keep_rows and _direct(T, B)
     n_x, n_h = 0 if quantised or direct else _rows_bytes(T, D, B), _rows_bytes(T, F, B)
     ws = _bytes(n_x + n_h, dev)  # the quantised rows of x, then of h

@@ -549,23 +549,23 @@ def test_outputs_that_overlap_inputs(T, B):
         assert torch.equal(buf[1:], want)
 
 
-def test_a_weight_whose_fields_change():
-    """The library sees the fields of the call, not those of the weight's making."""
+def test_a_weight_with_other_fields():
+    """A weight's fields are fixed; one made from others, or copied, is checked and used as it is."""
     import copy
+    from dataclasses import FrozenInstanceError, replace
     K = _K()
     rng = np.random.default_rng(17)
     v, cols, _ = weight(rng, 3, 4, 2, 64)
     w = K.make_mxfp4(v, cols, 4)
     x = rows(rng, 9, 256)
     want = K.mxfp4_linear(x, w)
-    other = copy.deepcopy(w)
-    w.data = w.data.clone()
-    assert torch.equal(K.mxfp4_linear(x, w), want) and torch.equal(K.mxfp4_linear(x, other), want)
+    with pytest.raises(FrozenInstanceError):
+        w.data = w.data.clone()
+    for other in (copy.deepcopy(w), replace(w, data=w.data.clone())):
+        assert torch.equal(K.mxfp4_linear(x, other), want) and torch.equal(other.dequantize(), w.dequantize())
     for bad in (dict(R=4), dict(data=w.data[:-16]), dict(data=w.data.view(torch.int8)), dict(B=32),
                 dict(data=w.data.cpu())):
-        broken = copy.copy(w)
-        for k, f in bad.items():
-            setattr(broken, k, f)
+        broken = replace(w, **bad)
         with pytest.raises(RuntimeError):
             K.mxfp4_linear(x, broken)
         with pytest.raises(RuntimeError):

@@ -27,17 +27,28 @@
 // Hence the multi-slot stages, and two issuers: job j of the CTA belongs to
 // issuer j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
 //
-// What bounds it: B = 128, the way from the L2 into the SM.  A slot is 17.4 KB
-// and takes 300 cycles of the 140 that its MMAs need (T = 16384, 16384 -> 4096:
-// 143 us, 3.8 PFLOP/s, 16 TB/s out of the L2; with a quarter of the bytes left
-// out 132).  B = 64, gated: the epilogue, 16 instructions an output
+// A linear at B = 128 with units enough takes two token tiles to a unit (kPairs):
+// one ring, whose stages hold the rows of both tiles and the weights once, and
+// issuer k takes tile k from every stage; a stage is free when both have
+// committed it, so neither is more than the ring ahead of the other.  13 KB for
+// a tile's slot instead of 17.4: 16384 -> 4096 at T = 16384 148 -> 133 us.  The
+// gated kernel gains nothing that way (313 us with a tile, 322 with two):
+// two gates and two ups need four accumulators and TMEM holds three, so the next
+// unit's gates wait for most of an epilogue.
+//
+// What bounds it: B = 128, the way from the L2 into the SM, 60 bytes a cycle, and
+// the ring's latency.  Of the linear's 133 us (4.2 PFLOP/s) the copies and the
+// epilogue without MMAs take 102, the MMAs and the epilogue without copies 102,
+// the MMAs alone 76 (120 cycles a slot; its scales 20), copies and MMAs without
+// the output 109.  B = 64, gated: the epilogue, 16 instructions an output
 // (T = 16384, d = 2048, d_ff = 8192: 125 us; without the SiLU's exponential and
 // reciprocal 104).
 //
 // Warps: 0-5 producers (ring w / 3; stage use h of a ring belongs to its
 // producer h % 3, since a producer's turn, from a stage's release to its copies'
-// issue, is on the ring's path: one producer a ring 156 us where two or three
-// take 146 to 143, gated B = 64 128 us with two, 125 with three), 6-21 epilogue
+// issue, is on the ring's path: with one tile to a unit 156 us with one producer
+// a ring, 147 with two or three; gated B = 64 128 us with two, 125 with three;
+// kPairs leaves 3-5 idle), 6-21 epilogue
 // (a warp takes the TMEM lane quadrant warp % 4 and one 32-column block of a
 // unit; at B = 64, two blocks, two groups of eight warps take the CTA's units in
 // turn), 22 and 23 issuers (22 owns TMEM).  Accumulators form a ring of ACCS in
@@ -65,28 +76,37 @@
 namespace bell {
 namespace mx {
 
-static constexpr int kPer = 3;       // producers of a ring
-static constexpr int kProducers = 2 * kPer;
+static constexpr int kProducers = 6;
 static constexpr int kEpiWarps = 16;
 static constexpr int kIssuer = kProducers + kEpiWarps;  // 22, 23
 static constexpr int kThreads = 32 * (kIssuer + 2);
 
-template <int B>
+// What a kernel's epilogue does with its accumulators; kPairs: a linear whose
+// two issuers take two token tiles of one unit from one ring.
+enum Mode : int { kLinear, kPairs, kGated, kGatedBackward };
+
+template <int B, Mode MODE>
 struct Geo {
+  static constexpr bool GATED = MODE == kGated || MODE == kGatedBackward, PAIRS = MODE == kPairs;
   static constexpr int A = row_chunk(B), W = tile_chunk(B);
-  static constexpr int SLOT = A + W;             // 17408 / 7168 bytes, multiples of 256
+  static constexpr int TILES = PAIRS ? 2 : 1;    // token tiles of a unit
+  static constexpr int SLOT = TILES * A + W;     // 17408 / 7168 / 26112 bytes, multiples of 256
   static constexpr int SLOTS = B == 128 ? 2 : 4;
   static constexpr int STAGE = SLOTS * SLOT;
-  static constexpr int NR = B == 128 ? 3 : 4;    // stages of a ring
-  static constexpr int NS = 2 * NR;
+  static constexpr int RINGS = PAIRS ? 1 : 2;
+  static constexpr int NR = B == 64 || PAIRS ? 4 : 3;  // stages of a ring
+  static constexpr int NS = RINGS * NR;
+  static constexpr int PER = kProducers / 2;      // producers of a ring
   static constexpr int ACCS = B == 128 ? 3 : 4;
-  static constexpr int SF_COL = ACCS * B;        // 8 scale columns per slot of a stage from here
+  // TMEM: the accumulators, then 8 scale columns for each slot that an issuer
+  // takes from a stage
+  static constexpr int SF_COL = ACCS * B, SF_STAGE = SLOTS * 8;
   static constexpr int SMEM = NS * STAGE + 1024 + 1024;
   // a producer's wait for the release of use h - NR must not meet the parity of
-  // use h - 2 NR: that one is released no later than h - kPer - NR, which it
+  // use h - 2 NR: that one is released no later than h - PER - NR, which it
   // waited for
-  static_assert(NR >= kPer, "mbarrier parity");
-  static_assert(SF_COL + NS * SLOTS * 8 <= 512, "TMEM columns");
+  static_assert(NR >= PER && RINGS * PER <= kProducers, "mbarrier parity");
+  static_assert(SF_COL + 2 * NR * SF_STAGE <= 512, "TMEM columns");
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -120,9 +140,8 @@ struct Smem {
   volatile int* abort_flag;
 };
 
-template <int B>
+template <class G>
 __device__ __forceinline__ Smem carve(uint8_t* raw) {
-  using G = Geo<B>;
   Smem s;
   s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ctl = s.stages + G::NS * G::STAGE;
@@ -137,28 +156,33 @@ __device__ __forceinline__ Smem carve(uint8_t* raw) {
   return s;
 }
 
-// The CTA's units are blockIdx.x + i * gridDim.x; ring k's job i is unit i of
-// matrix k (gated) or unit 2i + k (linear).  In split mode a ring has one job,
-// stages [first, first + stages) of the cluster's unit.
+// The CTA's units are blockIdx.x + i * gridDim.x, a unit being a block-row of a
+// token tile (kPairs: of two).  Issuer k's job i is unit i of matrix k (gated),
+// of tile k of the two, or unit 2i + k (linear).  In split mode a ring has one
+// job, stages [first, first + stages) of the cluster's unit.
 struct RingWork {
   int jobs, first, stages;
 };
-template <int B, bool GATED>
+template <class G>
+__device__ __forceinline__ int all_units(const Params& p) {
+  return (p.mtiles + G::TILES - 1) / G::TILES * p.R;
+}
+template <class G>
 __device__ __forceinline__ RingWork ring_work(const Params& p, int k) {
-  const int K = GATED && k ? p.K1 : p.K0;
-  const int all = (K + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS;
-  if (!GATED && p.split) {
+  const int K = G::GATED && k ? p.K1 : p.K0;
+  const int all = (K + G::SLOTS - 1) / G::SLOTS;
+  if (!G::GATED && p.split) {
     const int part = int(blockIdx.x) % p.split * 2 + k, each = (all + 2 * p.split - 1) / (2 * p.split);
     return {1, part * each, max(0, min(each, all - part * each))};
   }
-  const int units = p.mtiles * p.R, grid = int(gridDim.x);
+  const int units = all_units<G>(p), grid = int(gridDim.x);
   const int mine = int(blockIdx.x) < units ? (units - int(blockIdx.x) + grid - 1) / grid : 0;
-  return {GATED ? mine : (mine - k + 1) / 2, 0, all};
+  return {G::GATED || G::PAIRS ? mine : (mine - k + 1) / 2, 0, all};
 }
-template <bool GATED>
+template <class G>
 __device__ __forceinline__ int job_unit(const Params& p, int i, int k) {
-  if (!GATED && p.split) return int(blockIdx.x) / p.split;
-  return int(blockIdx.x) + (GATED ? i : 2 * i + k) * int(gridDim.x);
+  if (!G::GATED && p.split) return int(blockIdx.x) / p.split;
+  return int(blockIdx.x) + (G::GATED || G::PAIRS ? i : 2 * i + k) * int(gridDim.x);
 }
 
 // ------------------------------------------------------------- direct rows
@@ -195,19 +219,18 @@ __device__ __forceinline__ void direct_barrier() {
   asm volatile("bar.sync 1, %0;" ::"n"(32 * (kProducers + kEpiWarps)) : "memory");
 }
 
-template <int B, bool GATED>
+template <int B, class G>
 __device__ void direct_first(const Params& p, const Smem& s) {
-  using G = Geo<B>;
   const int w = (threadIdx.x >> 5) - kProducers;
   const int groups = (int(p.T) + DirectRows<B>::N - 1) / DirectRows<B>::N;
   for (int item = w; item < G::NS * G::SLOTS * groups; item += kEpiWarps) {
     const int n0 = item % groups * DirectRows<B>::N, at = item / groups;
     const int i = at % G::SLOTS, use = at / G::SLOTS % G::NR, ring = at / (G::SLOTS * G::NR);
-    const RingWork rw = ring_work<B, GATED>(p, ring);
+    const RingWork rw = ring_work<G>(p, ring);
     const int job = rw.stages > 0 ? use / rw.stages : rw.jobs;
     if (job >= rw.jobs) continue;
-    const int u = job_unit<GATED>(p, job, ring), r = u % p.R;
-    const int mat = GATED ? ring : 0, K = mat ? p.K1 : p.K0, k = (rw.first + use - job * rw.stages) * G::SLOTS + i;
+    const int u = job_unit<G>(p, job, ring), r = u % p.R;
+    const int mat = G::GATED ? ring : 0, K = mat ? p.K1 : p.K0, k = (rw.first + use - job * rw.stages) * G::SLOTS + i;
     const uint32_t e = k < K ? __ldg((mat ? p.p1 : p.p0).entries + int64_t(r) * K + k) : kNoSlot;
     if (e != kNoSlot) DirectRows<B>::put(p, int(e & 0xFFFFu), n0, s.stages + (ring * G::NR + use) * G::STAGE + i * G::SLOT);
   }
@@ -217,16 +240,15 @@ __device__ void direct_first(const Params& p, const Smem& s) {
 
 // ---------------------------------------------------------------- producer
 
-template <int B, bool GATED>
+template <int B, class G>
 __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const Ctl& ctl) {
-  using G = Geo<B>;
   const int lane = threadIdx.x & 31;
   const uint64_t keep = policy_evict_last(), pass = policy_evict_normal();
-  const int mat = GATED ? ring : 0;
+  const int mat = G::GATED ? ring : 0;
   const int K = mat ? p.K1 : p.K0;
   const uint8_t* w = mat ? p.w1 : p.w0;
   const uint32_t* entries = (mat ? p.p1 : p.p0).entries;
-  const RingWork rw = ring_work<B, GATED>(p, ring);
+  const RingWork rw = ring_work<G>(p, ring);
   uint64_t* full = s.full + ring * G::NR;
   uint64_t* empty = s.empty + ring * G::NR;
   uint32_t* count = s.count + ring * G::NR;
@@ -236,25 +258,28 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     part -= rw.stages;
     ++job;
   }
-  // Lanes 2i and 2i + 1 bring slot i of a stage, its rows and its weights: one
-  // copy instruction for all of a stage's copies.  (One lane after another's
+  // Two lanes (kPairs: three) bring a slot of a stage, its rows and its weights:
+  // one copy instruction for all of a stage's copies.  (One lane after another's
   // took 700 cycles a stage, which the stages spend empty.)
-  const int slot = lane >> 1;
-  const bool is_w = lane & 1;
+  constexpr int LANES = G::TILES + 1;
+  const int slot = lane / LANES, piece = lane - slot * LANES;
+  const bool is_w = piece == G::TILES;
   struct Use {
     uint32_t e;           // this lane's slot's entry
     const uint8_t* base;  // of its chunks
   };
   // units advance by a fixed step: block-row and token tile without divisions
-  const int step = job_unit<GATED>(p, 1, ring) - job_unit<GATED>(p, 0, ring), dm = step / p.R, dr = step - dm * p.R;
-  int m = job_unit<GATED>(p, job, ring) / p.R, r = job_unit<GATED>(p, job, ring) - m * p.R;
+  const int step = job_unit<G>(p, 1, ring) - job_unit<G>(p, 0, ring), dm = step / p.R, dr = step - dm * p.R;
+  int m = job_unit<G>(p, job, ring) / p.R, r = job_unit<G>(p, job, ring) - m * p.R;
   auto fetch = [&]() -> Use {
     const int k = (rw.first + part) * G::SLOTS + slot;
-    const uint32_t e = lane < 2 * G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
-    return {e, is_w ? w + int64_t(r) * K * G::W : p.x + int64_t(m) * p.C * G::A};
+    const uint32_t e = lane < LANES * G::SLOTS && k < K ? __ldg(entries + int64_t(r) * K + k) : kNoSlot;
+    // an odd last tile is its own neighbour (the epilogue stores it once)
+    const int mt = G::PAIRS ? min(2 * m + piece, p.mtiles - 1) : m;
+    return {e, is_w ? w + int64_t(r) * K * G::W : p.x + int64_t(mt) * p.C * G::A};
   };
   auto advance = [&] {
-    part += kPer;
+    part += G::PER;
     while (part >= rw.stages && job < left) {
       part -= rw.stages;
       ++job;
@@ -268,9 +293,9 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   };
   auto copies = [&](const Use& use, uint32_t stage, bool weights, bool rows) {
     const bool live = use.e != kNoSlot;
-    const uint32_t cnt = __popc(__ballot_sync(0xffffffffu, live)) / 2u;
+    const uint32_t cnt = uint32_t(__popc(__ballot_sync(0xffffffffu, live))) / uint32_t(LANES);
     uint8_t* st = stages + stage * uint32_t(G::STAGE);
-    uint8_t* to = st + slot * G::SLOT + (is_w ? G::A : 0);
+    uint8_t* to = st + slot * G::SLOT + piece * G::A;
     const uint8_t* from = use.base + (is_w ? int64_t(use.e >> 16) * G::W : int64_t(use.e & 0xFFFFu) * G::A);
     if (weights && elect_one()) {
       count[stage] = cnt;
@@ -286,7 +311,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
       bulk_load(to, from, is_w ? G::W : G::A, &full[stage], is_w ? keep : pass);
     if (!p.x && rows) {  // direct rows, this warp's (with `rows` false they are already on their way)
       for (int i = 0; i < int(cnt); ++i) {
-        const int c = int(__shfl_sync(0xffffffffu, use.e, 2 * i) & 0xFFFFu);
+        const int c = int(__shfl_sync(0xffffffffu, use.e, LANES * i) & 0xFFFFu);
         for (int n0 = 0; n0 < int(p.T); n0 += DirectRows<B>::N) DirectRows<B>::put(p, c, n0, st + i * G::SLOT);
       }
       fence_proxy_async_smem();
@@ -299,7 +324,7 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   int64_t filled = 0;
   auto turn = [&] {
     ++filled;
-    stage += kPer;
+    stage += G::PER;
     if (stage >= uint32_t(G::NR)) {
       stage -= G::NR;
       phase ^= 1u;
@@ -308,14 +333,14 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   // The ring's first filling: the weights need not wait for the rows, which the
   // kernel ahead or the epilogue's warps make.
   if (p.early || !p.x) {
-    Use first[(G::NR + kPer - 1) / kPer];
+    Use first[(G::NR + G::PER - 1) / G::PER];
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < (G::NR + kPer - 1) / kPer; ++i) {
-      if (sub + kPer * i < G::NR && job < left) {
+    for (int i = 0; i < (G::NR + G::PER - 1) / G::PER; ++i) {
+      if (sub + G::PER * i < G::NR && job < left) {
         first[i] = fetch();
         advance();
-        copies(first[i], uint32_t(sub + kPer * i), true, false);
+        copies(first[i], uint32_t(sub + G::PER * i), true, false);
         n = i + 1;
       }
     }
@@ -324,12 +349,12 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
     else
       direct_barrier();
 #pragma unroll
-    for (int i = 0; i < (G::NR + kPer - 1) / kPer; ++i) {
+    for (int i = 0; i < (G::NR + G::PER - 1) / G::PER; ++i) {
       if (i < n) {
         if (p.x)
-          copies(first[i], uint32_t(sub + kPer * i), false, true);
+          copies(first[i], uint32_t(sub + G::PER * i), false, true);
         else if (elect_one())
-          mbar_arrive(&full[sub + kPer * i]);
+          mbar_arrive(&full[sub + G::PER * i]);
         turn();
       }
     }
@@ -350,11 +375,11 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
   }
   if (!ok && lane == 0) {  // let this producer's copies land before the CTA exits (bounded)
     for (int i = 0; i < G::NR && filled > 0; ++i, --filled) {
-      if (stage < uint32_t(kPer)) {
+      if (stage < uint32_t(G::PER)) {
         stage += G::NR;
         phase ^= 1u;
       }
-      stage -= kPer;
+      stage -= G::PER;
       const uint32_t a = smem_u32(&full[stage]);
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(a, phase) && globaltimer_ns() - t0 < 100000000ull) {
@@ -365,17 +390,19 @@ __device__ void produce(const Params& p, const Smem& s, int ring, int sub, const
 
 // ------------------------------------------------------------------ issuer
 
-template <int B, bool GATED>
-__device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, const Ctl& ctl) {
-  using G = Geo<B>;
+template <int B, class G>
+__device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int k, const Ctl& ctl) {
   const bool leader = elect_one();
+  const int ring = G::PAIRS ? 0 : k;
+  constexpr uint32_t w_at = G::TILES * G::A;          // of a slot: its weights
+  const uint32_t a_at = G::PAIRS ? uint32_t(k * G::A) : 0u;  // and this issuer's rows
   const uint32_t a0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 128);
   const uint32_t sf0 = sdesc_lo(smem_u32(s.stages) + ring * (G::NR * G::STAGE), 16);
-  const RingWork rw = ring_work<B, GATED>(p, ring);
+  const RingWork rw = ring_work<G>(p, k);
   uint64_t* full = s.full + ring * G::NR;
   uint64_t* empty = s.empty + ring * G::NR;
   uint32_t stage = 0, phase = 0;
-  uint32_t acc = uint32_t(ring), use = 0;  // job 2i + ring of the CTA: accumulator (2i + ring) % ACCS
+  uint32_t acc = uint32_t(k), use = 0;  // job 2i + k of the CTA: accumulator (2i + k) % ACCS
   bool ok = true;
   for (int i = 0; i < rw.jobs && ok; ++i) {
     ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_empty[acc], (use & 1u) ^ 1u, ctl));
@@ -390,16 +417,16 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
       const int n = int(s.count[ring * G::NR + stage]);
       if (leader) {
         const uint32_t st = stage * uint32_t(G::STAGE >> 4);
-        const uint32_t sf = tmem + G::SF_COL + (ring * G::NR + stage) * (G::SLOTS * 8);
+        const uint32_t sf = tmem + G::SF_COL + (uint32_t(k) * G::NR + stage) * G::SF_STAGE;
 #pragma unroll
         for (int j = 0; j < G::SLOTS; ++j) {
           if (j < n) {
             const uint32_t at = st + j * (G::SLOT >> 4);
-            copy_scales(sf + j * 8, sf0 + at + ((G::A - kScaleBytes) >> 4));
+            copy_scales(sf + j * 8, sf0 + at + ((a_at + G::A - kScaleBytes) >> 4));
             copy_scales(sf + j * 8 + 4, sf0 + at + ((G::SLOT - kScaleBytes) >> 4));
 #pragma unroll
             for (int kk = 0; kk < B / 64; ++kk)
-              mma_mxf4(d, a0 + at + kk * (kRows * 32 >> 4), a0 + at + ((G::A + kk * B * 32) >> 4),
+              mma_mxf4(d, a0 + at + ((a_at + kk * kRows * 32) >> 4), a0 + at + ((w_at + kk * B * 32) >> 4),
                        idesc_mxf4(kRows, B, kk * 2), sf + j * 8, sf + j * 8 + 4, j > 0 || kk > 0 ? 1u : more);
           }
         }
@@ -422,8 +449,8 @@ __device__ void issue(const Params& p, const Smem& s, uint32_t tmem, int ring, c
     }
   }
   if (leader) {  // every MMA has completed before TMEM is released
-    mma_commit(&s.drain[ring]);
-    const uint32_t a = smem_u32(&s.drain[ring]);
+    mma_commit(&s.drain[k]);
+    const uint32_t a = smem_u32(&s.drain[k]);
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(a, 0) && globaltimer_ns() - t0 < 100000000ull) {
     }
@@ -539,12 +566,12 @@ __device__ __forceinline__ void put16(const Params& p, int64_t at, float* f) {
 template <int B>
 struct Partial {
   static constexpr int LD = B + 4;
-  static_assert(kRows * LD * 4 <= Geo<B>::NS * Geo<B>::STAGE, "the partial sums fit the ring");
+  static_assert(kRows * LD * 4 <= Geo<B, kLinear>::NS * Geo<B, kLinear>::STAGE, "the partial sums fit the ring");
 };
 
 template <int B>
 __device__ void split_partial(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
-  using G = Geo<B>;
+  using G = Geo<B, kLinear>;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
   const int q = int(threadIdx.x >> 5) & 3, j = w >> 2;
   if (j >= B / 32) return;  // one unit: the second group of B = 64 has none
@@ -560,7 +587,7 @@ __device__ void split_partial(const Params& p, const Smem& s, uint32_t tmem, con
     tc_fence_after();
     uint32_t a[32];
     tmem_ld32_sync(tmem + (uint32_t(q * 32) << 16) + uint32_t(k * B + j * 32), a);
-    const RingWork rw = ring_work<B, false>(p, k);
+    const RingWork rw = ring_work<G>(p, k);
     if (rw.stages > 0 && live > rw.first * G::SLOTS) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) f[i] += __uint_as_float(a[i]);
@@ -618,19 +645,16 @@ __device__ __forceinline__ void silu_backward2(float2 dh, float2 g, float2 u, fl
   du = mul2(dh, f);
 }
 
-// What a kernel's epilogue does with its accumulators.
-enum Mode : int { kLinear, kGated, kGatedBackward };
-
 template <int B, Mode MODE>
 __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ctl& ctl) {
-  constexpr bool GATED = MODE != kLinear;
-  using G = Geo<B>;
+  using G = Geo<B, MODE>;
+  constexpr bool GATED = G::GATED;
   constexpr int NB = B / 32;             // scale blocks (32 features) of a unit
   constexpr int GROUPS = kEpiWarps / (4 * NB);
   constexpr int JOBS = GATED ? 2 : 1;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kProducers;
   const int q = int(threadIdx.x >> 5) & 3, j = (w >> 2) % NB, group = (w >> 2) / NB;
-  const int units = p.mtiles * p.R;
+  const int units = all_units<G>(p);
   const int64_t ld = int64_t(p.R) * B;
   const uint32_t lanes = uint32_t(q * 32) << 16;
   const int step = GROUPS * int(gridDim.x);
@@ -640,13 +664,20 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
     c0 = __ldg(p.p0.counts + r);
     if (GATED) c1 = __ldg(p.p1.counts + r);
   };
+  auto next = [&] {  // this group's next accumulator (the first of two)
+    acc += GROUPS * JOBS;
+    while (acc >= uint32_t(G::ACCS)) {
+      acc -= G::ACCS;
+      ++use;
+    }
+  };
   int u = int(blockIdx.x) + group * int(gridDim.x);
   // the next unit's token tile and block-row, advanced without divisions
   const int dm = step / p.R, dr = step - dm * p.R;
   int mn = u / p.R, rn = u - mn * p.R;
   if (u < units) counts(rn);
   for (; u < units; u += step) {
-    const int m = mn, r = rn;
+    const int m = mn * G::TILES, r = rn;
     const int n = q * 32 + lane;
     const int64_t t = int64_t(m) * kRows + n;
     const bool live0 = c0 > 0, live1 = c1 > 0;
@@ -783,38 +814,36 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         ch[kRows * B / 2 + scale_off(n, j)] = uint8_t(byte);
       }
     } else {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
-      tc_fence_after();
-      uint32_t a[32];
-      tmem_ld32_sync(tmem + lanes + acc * B + j * 32, a);
-      release(s, acc);
-      if (t < p.T) {
-        float f[32];
+      for (int k = 0; k < G::TILES; ++k) {
+        if (k) next();
+        if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
+        tc_fence_after();
+        uint32_t a[32];
+        tmem_ld32_sync(tmem + lanes + acc * B + j * 32, a);
+        release(s, acc);
+        if (t + k * kRows < p.T) {
+          float f[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
-        put16(p, at, f);
-        put16(p, at + 16, f + 16);
+          for (int i = 0; i < 32; ++i) f[i] = live0 ? __uint_as_float(a[i]) : 0.f;
+          put16(p, at + k * kRows * ld, f);
+          put16(p, at + k * kRows * ld + 16, f + 16);
+        }
       }
     }
-    acc += GROUPS * JOBS;
-    while (acc >= uint32_t(G::ACCS)) {
-      acc -= G::ACCS;
-      ++use;
-    }
+    next();
   }
 }
 
 template <int B, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
-  constexpr bool GATED = MODE != kLinear;
-  using G = Geo<B>;
+  using G = Geo<B, MODE>;
   extern __shared__ uint8_t smem_raw[];
-  const Smem s = carve<B>(smem_raw);
+  const Smem s = carve<G>(smem_raw);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < G::NS; ++i) {
       mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.empty[i], 2 / G::RINGS);  // the issuers that take from it
     }
     for (int i = 0; i < G::ACCS; ++i) {
       mbar_init(&s.acc_full[i], 1);
@@ -838,21 +867,23 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   // Rows, and possibly weights, come from the kernel ahead.  With p.early only
   // the rows do, and the producers start the weights before they wait.
   if (!p.early || warp >= kProducers) griddep_wait();
-  const bool split = !GATED && p.split;
+  const bool split = MODE == kLinear && p.split;
   if (warp < kProducers) {
-    produce<B, GATED>(p, s, warp / kPer, warp % kPer, ctl);
+    if (warp < G::RINGS * G::PER) produce<B, G>(p, s, warp / G::PER, warp % G::PER, ctl);
   } else if (warp < kIssuer) {
-    if (!p.x) direct_first<B, GATED>(p, s);
-    if constexpr (!GATED) {
+    if constexpr (!G::PAIRS) {
+      if (!p.x) direct_first<B, G>(p, s);
+    }
+    if constexpr (MODE == kLinear) {
       if (split) split_partial<B>(p, s, tmem, ctl);
     }
     if (!split) epilogue<B, MODE>(p, s, tmem, ctl);
   } else {
-    issue<B, GATED>(p, s, tmem, warp - kIssuer, ctl);
+    issue<B, G>(p, s, tmem, warp - kIssuer, ctl);
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (!GATED) {
+  if constexpr (MODE == kLinear) {
     if (split) {
       cluster_sync();  // every partial sum is in place
       split_join<B>(p, s);
@@ -878,23 +909,24 @@ static int split_of(int64_t units, int stages, int sms, int B) {
 
 template <int B, Mode MODE>
 static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
+  using G = Geo<B, MODE>;
   auto kern = bell_mx_kernel<B, MODE>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
   int dev = 0, sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(BELL_ERR_LAUNCH, "cudaGetDevice");
   if (!(ready.load() >> dev & 1)) {
-    if (int rc = set_smem(reinterpret_cast<const void*>(kern), Geo<B>::SMEM)) return rc;
+    if (int rc = set_smem(reinterpret_cast<const void*>(kern), G::SMEM)) return rc;
     ready.fetch_or(uint64_t(1) << dev);
   }
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
-  const int64_t units = int64_t(p.mtiles) * p.R;
-  p.split = MODE != kLinear ? 0 : split_of(units, (p.K0 + Geo<B>::SLOTS - 1) / Geo<B>::SLOTS, sms, B);
+  const int64_t units = (int64_t(p.mtiles) + G::TILES - 1) / G::TILES * p.R;
+  p.split = MODE != kLinear ? 0 : split_of(units, (p.K0 + G::SLOTS - 1) / G::SLOTS, sms, B);
   const int64_t grid = p.split ? units * p.split : std::min<int64_t>(units, sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Geo<B>::SMEM;
+  cfg.dynamicSmemBytes = G::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -973,7 +1005,16 @@ static int linear(Params p, const BellMxEll& w, const void* residual, void* out,
   p.residual = residual;
   p.out_f32 = out_dtype == BELL_DTYPE_F32;
   p.wide = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) & 31u) == 0;
-  return w.B == 128 ? launch<128, kLinear>(p, max_ctas, s) : launch<64, kLinear>(p, max_ctas, s);
+  if (w.B == 64) return launch<64, kLinear>(p, max_ctas, s);
+  // Two token tiles to a unit where that leaves a unit for three of four SMs.
+  // 16384 -> 4096, K = 32, us with one tile and with two: 160 units (80 pairs)
+  // 12.5, 13.4; 256: 15.2, 13.4; 320: 19.8, 19.8; 512: 24.8, 21.3; 1024: 40, 36;
+  // 4096: 148, 133.
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
+  const bool pairs = p.x && int64_t(p.mtiles + 1) / 2 * p.R * 4 >= int64_t(sms) * 3;
+  return pairs ? launch<128, kPairs>(p, max_ctas, s) : launch<128, kLinear>(p, max_ctas, s);
 }
 
 int gated_backward(int64_t T, const void* x, const BellMxEll& gate, const BellMxEll& up, const float* dh, void* dgu,

@@ -188,7 +188,7 @@ def mxfp4_dequantize(q: MXRows, dtype: torch.dtype = torch.bfloat16, out: Option
         raise RuntimeError("dtype must be bf16 or fp32")
     dev = q.data.device
     if out is None:
-        out = torch.empty((q.T, q.features), dtype=dtype, device=dev)
+        out = q.data.new_empty((q.T, q.features), dtype=dtype)
     else:
         _check_out("out", out, (q.T, q.features), dtype, dev)
     _call("bell_mx_dequantize_rows", dev, q.T, q.features, q.tile, q.data.data_ptr(), _DTYPES[dtype], out.data_ptr(),
@@ -366,7 +366,7 @@ def _swiglu(x, gate, up, down, add_residual=False, residual=None, keep_rows=Fals
     at = ws.data_ptr()
     g = u = None
     if keep_projections:
-        g, u = (torch.empty((T, F), dtype=torch.bfloat16, device=dev) for _ in range(2))
+        g, u = (ws.new_empty((T, F), dtype=torch.bfloat16) for _ in range(2))
     d = _lib.BellMxFFNDesc(T, _DTYPES[dtype], int(max_ctas), x.data.data_ptr() if quantised else None if direct else at, src, ld, src_type, 0,
                            None if residual is None else residual.data_ptr(), at + n_x,
                            None if g is None else g.data_ptr(), None if u is None else u.data_ptr(), out.data_ptr(),
@@ -385,7 +385,7 @@ def _grad(need: bool, cols: torch.Tensor, B: int, dtype: torch.dtype):
     if not need:
         return None, None, _BF16
     kind = torch.bfloat16 if dtype == torch.bfloat16 else torch.float32
-    g = torch.empty((*cols.shape, B, B), dtype=kind, device=cols.device)
+    g = cols.new_empty((*cols.shape, B, B), dtype=kind)
     return g, g.data_ptr(), _DTYPES[kind]
 
 
@@ -395,14 +395,14 @@ class MXLinearFn(torch.autograd.Function):
         w = make_mxfp4(values, cols, x.shape[1] // values.shape[2], layout)
         y, rows = _linear(x, w, residual, keep_rows=True)
         ctx.w, ctx.layout = w, layout
-        ctx.save_for_backward(cols, w.data, rows)
+        ctx.save_for_backward(cols, rows)
         ctx.dtypes = (x.dtype, values.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w, (cols, _, rows) = ctx.w, ctx.saved_tensors
+        w, (cols, rows) = ctx.w, ctx.saved_tensors
         x_dtype, v_dtype = ctx.dtypes
         dyb = dy.to(torch.bfloat16).contiguous()
         T, dev = dyb.shape[0], dyb.device
@@ -412,7 +412,7 @@ class MXLinearFn(torch.autograd.Function):
         if need[0]:
             cols_t, index_t = transposed_topology([cols], w.C)
             K_t = cols_t.shape[1]
-            dx = torch.empty((T, w.C * w.B), dtype=torch.bfloat16, device=dev)
+            dx = dyb.new_empty((T, w.C * w.B))
             dx_at = dx.data_ptr()
         dw, dw_at, kind = _grad(need[1], w.col_indices, w.B, v_dtype)
         d = _lib.BellMxLinearBwdDesc(T, dyb.data_ptr(), rows.data_ptr(), w._abi, w.col_indices.data_ptr(),
@@ -446,7 +446,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         gate, up, down = _pack(((v_gate, ci_gate, C_model), (v_up, ci_up, C_model), (v_down, ci_down, R_ff)), layout)
         out, ws = _swiglu(x, gate, up, down, add_residual, keep_rows=True)
         ctx.weights = (gate, up, down)
-        ctx.save_for_backward(ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down, gate.data, up.data, down.data)
+        ctx.save_for_backward(ws["q_x"].data, ws["q_h"].data, ci_gate, ci_up, ci_down)
         ctx.add_residual, ctx.layout = bool(add_residual), layout
         ctx.dtypes = (x.dtype, v_gate.dtype, v_up.dtype, v_down.dtype)
         return out
@@ -454,7 +454,7 @@ class MXSwiGLUFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q_x, q_h, ci_gate, ci_up, ci_down, *_ = ctx.saved_tensors
+        q_x, q_h, ci_gate, ci_up, ci_down = ctx.saved_tensors
         gate, up, down = ctx.weights
         dy = grad_out.to(torch.bfloat16).contiguous()
         T, dev = dy.shape[0], dy.device

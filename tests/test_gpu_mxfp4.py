@@ -651,3 +651,43 @@ def test_more_slots_than_the_backward_takes():
     y = K.mxfp4_linear_ad(x, v, cols)
     with pytest.raises(RuntimeError, match="254"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("T", [128 * 74, 128 * 74 - 5, 128 * 73])
+@pytest.mark.parametrize("B,dtype", [(64, BF16), (128, BF16), (128, F32)])
+def test_many_tokens_equal_the_same_tokens_in_parts(T, B, dtype):
+    """The kernels for many tokens (two token tiles to a unit, odd and even numbers of tiles) against those for few."""
+    K = _K()
+    rng = np.random.default_rng(20)
+    v, cols, _ = weight(rng, 8, 4, 3, B, dead=5, dead_row=4)
+    w = K.make_mxfp4(v, cols, 4)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(T, 4 * B, generator=g, device="cuda").to(dtype)
+    res = torch.randn(T, 8 * B, generator=g, device="cuda").to(dtype)
+    big = torch.full((T + 130, 8 * B), 7.0, device="cuda", dtype=dtype)
+    y = K.mxfp4_linear(x, w, residual=res, out=big[:T])
+    parts = torch.cat([K.mxfp4_linear(a, w, residual=b) for a, b in zip(x.split(1000), res.split(1000))])
+    assert torch.equal(y, parts) and (big[T:] == 7).all()
+    assert torch.equal(y[:, 4 * B:5 * B], res[:, 4 * B:5 * B])
+    assert torch.equal(K.mxfp4_linear(x, w, max_ctas=5), K.mxfp4_linear(x, w))
+
+
+@pytest.mark.parametrize("T", [128 * 74, 128 * 74 - 5, 128 * 73])
+@pytest.mark.parametrize("B,Kg,Ku,Kd", [(64, 2, 3, 5), (128, 1, 5, 8), (128, 2, 7, 8), (128, 19, 3, 8), (128, 18, 20, 1)])
+def test_many_tokens_of_a_block_equal_the_same_tokens_in_parts(T, B, Kg, Ku, Kd):
+    """As above for the gated block: unequal numbers of slots, dead rows, several stages and units of each CTA."""
+    K = _K()
+    rng = np.random.default_rng(21)
+    C = 20
+    mats = [weight(rng, 8, C, Kg, B, dead=4, dead_row=3), weight(rng, 8, C, Ku, B, dead=4, dead_row=5),
+            weight(rng, C, 8, Kd, B)]
+    packed = [K.make_mxfp4(v, c, n) for (v, c, _), n in zip(mats, (C, C, 8))]
+    x = torch.randn(T, C * B, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(BF16)
+    y = K.mxfp4_swiglu_fwd(x, *packed, add_residual=True)
+    parts = torch.cat([K.mxfp4_swiglu_fwd(a, *packed, add_residual=True) for a in x.split(1000)])
+    assert torch.equal(y, parts)
+    y2, ws = K.mxfp4_swiglu_fwd(x, *packed, add_residual=True, return_intermediates=True)
+    assert torch.equal(y, y2) and (ws["gate"][:, 3 * B:4 * B] == 0).all() and (ws["up"][:, 5 * B:6 * B] == 0).all()
+    for _ in range(3):
+        assert torch.equal(K.mxfp4_swiglu_fwd(x, *packed, add_residual=True), y)
+    assert K.read_status() == 0

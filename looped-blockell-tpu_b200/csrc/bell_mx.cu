@@ -80,6 +80,7 @@ static constexpr int kProducers = 6;
 static constexpr int kEpiWarps = 16;
 static constexpr int kIssuer = kProducers + kEpiWarps;  // 22, 23
 static constexpr int kThreads = 32 * (kIssuer + 2);
+static constexpr int kMaxSplit = 8;  // CTAs that share a unit: the portable cluster
 
 // What a kernel's epilogue does with its accumulators; kPairs: a linear whose
 // two issuers take two token tiles of one unit from one ring.
@@ -599,33 +600,49 @@ __device__ void split_partial(const Params& p, const Smem& s, uint32_t tmem, con
   for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
 }
 
+// Four outputs of a linear at element `at`.
+__device__ __forceinline__ void put4(const Params& p, int64_t at, float4 f) {
+  if (p.out_f32) {
+    if (p.residual) {
+      const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at);
+      f.x += r.x, f.y += r.y, f.z += r.z, f.w += r.w;
+    }
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = f;
+    return;
+  }
+  if (p.residual) {
+    const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.residual) + at);
+    const float2 a = unpack_bf16x2(r.x), b = unpack_bf16x2(r.y);
+    f.x += a.x, f.y += a.y, f.z += b.x, f.w += b.y;
+  }
+  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+      make_uint2(pack_bf16x2(f.x, f.y), pack_bf16x2(f.z, f.w));
+}
+
+// A thread joins four columns of a row: the loads of all ranks first, then the
+// sum in rank order.
 template <int B>
 __device__ void split_join(const Params& p, const Smem& s) {
   const int u = int(blockIdx.x) / p.split, rank = int(blockIdx.x) % p.split, m = u / p.R, r = u - m * p.R;
   const int rows = int(min(int64_t(kRows), p.T - int64_t(m) * kRows));
-  const int cols = B / p.split, per_row = cols / 16;
+  const int cols = B / p.split, per_row = cols / 4;
   const uint32_t base = smem_u32(s.stages);
   for (int i = threadIdx.x; i < rows * per_row; i += kThreads) {
-    const int n = i / per_row, c = rank * cols + (i - n * per_row) * 16;
-    float f[16];
+    const int n = i / per_row, c = rank * cols + (i - n * per_row) * 4;
+    float4 v[kMaxSplit];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = 0.f;
-    for (int k = 0; k < p.split; ++k) {
-      const uint32_t from = mapa_shared(base + uint32_t(n * Partial<B>::LD + c) * 4u, uint32_t(k));
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        float4 v;
+    for (int k = 0; k < kMaxSplit; ++k) {
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < p.split)
         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                     : "r"(from + e * 4)
+                     : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
+                     : "r"(mapa_shared(base + uint32_t(n * Partial<B>::LD + c) * 4u, uint32_t(k)))
                      : "memory");
-        f[e] += v.x;
-        f[e + 1] += v.y;
-        f[e + 2] += v.z;
-        f[e + 3] += v.w;
-      }
     }
-    put16(p, (int64_t(m) * kRows + n) * (int64_t(p.R) * B) + int64_t(r) * B + c, f);
+    float4 f = v[0];
+#pragma unroll
+    for (int k = 1; k < kMaxSplit; ++k) f.x += v[k].x, f.y += v[k].y, f.z += v[k].z, f.w += v[k].w;
+    put4(p, (int64_t(m) * kRows + n) * (int64_t(p.R) * B) + int64_t(r) * B + c, f);
   }
 }
 
@@ -896,14 +913,17 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   }
 }
 
-// CTAs that share a unit of a linear: where whole units would leave more than
-// half of the SMs without one, as many as fit (a power of two, at most the
-// portable cluster of 8 and 16 columns each to join), while every ring gets a
-// stage.
-static int split_of(int64_t units, int stages, int sms, int B) {
-  if (units * 2 > sms) return 0;
-  int split = 1;
-  while (split < std::min(8, B / 16) && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
+// CTAs that share a unit of a linear.  The cluster's launch and the join cost
+// 2.6 us and 1 to 3 for 128 rows, a slot 0.14 us (B = 128) or 0.08 (B = 64), so
+// whole units serve short rows better.  us whole and split, by CTAs as many as
+// fit: B = 128, R = 32, K = 16: 6.0, 6.9 (T = 1), 6.8, 9.9 (T = 128); K = 32: 8.4,
+// 7.8 (T = 1), 8.4, 8.7 (T = 32), 9.1, 10.9 (T = 128); K = 64: 13.0, 9.2 (T = 1),
+// 13.6, 12.2 (T = 128).  B = 64, R = 16, K = 16: 4.7, 5.8 (T = 1); K = 64: 8.5, 6.5
+// (T = 1), 8.9, 8.5 (T = 128).
+static int split_of(int64_t units, int64_t T, int K, int stages, int sms, int B) {
+  if (units * 2 > sms || K * B < (T > BELL_MX_DIRECT_ROWS ? 8192 : 4096)) return 0;
+  int split = 1;  // a power of two, 16 columns each to join, a stage for every ring
+  while (split < std::min(kMaxSplit, B / 16) && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
   return split;
 }
 
@@ -921,7 +941,7 @@ static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   }
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
   const int64_t units = (int64_t(p.mtiles) + G::TILES - 1) / G::TILES * p.R;
-  p.split = MODE != kLinear ? 0 : split_of(units, (p.K0 + G::SLOTS - 1) / G::SLOTS, sms, B);
+  p.split = MODE != kLinear ? 0 : split_of(units, p.T, p.K0, (p.K0 + G::SLOTS - 1) / G::SLOTS, sms, B);
   const int64_t grid = p.split ? units * p.split : std::min<int64_t>(units, sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));

@@ -691,3 +691,21 @@ def test_many_tokens_of_a_block_equal_the_same_tokens_in_parts(T, B, Kg, Ku, Kd)
     for _ in range(3):
         assert torch.equal(K.mxfp4_swiglu_fwd(x, *packed, add_residual=True), y)
     assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 32, 33, 128, 300])
+@pytest.mark.parametrize("R,C,Kk,B,dead,dtype", [
+    (2, 40, 33, 128, 0, BF16), (5, 70, 64, 128, 9, F32), (1, 140, 129, 64, 3, BF16), (12, 80, 64, 64, 0, F32)])
+def test_long_rows_shared_by_a_cluster(T, R, C, Kk, B, dead, dtype):
+    """Few units of many slots: CTAs of a cluster share each (up to the largest cluster; fewer tokens, more of them)."""
+    K = _K()
+    rng = np.random.default_rng(22)
+    v, cols, w = weight(rng, R, C, Kk, B, dead, dead_row=R - 1 if R > 1 else None)
+    x, res = rows(rng, T, C * B, dtype), rows(rng, T, R * B, dtype)
+    p = K.make_mxfp4(v, cols, C)
+    xq = M.quantize(f64(x))
+    check_linear(K.mxfp4_linear(x, p), xq, w, Kk * B // 64)
+    y = K.mxfp4_linear(x, p, residual=res)
+    check_linear(y, xq, w, Kk * B // 64, f64(res))
+    assert torch.equal(y, K.mxfp4_linear(x, p, residual=res))
+    assert K.read_status() == 0

@@ -46,6 +46,7 @@ from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _prep_ell, p
 _BF16, _F32 = _lib.BELL_DTYPE_BF16, _lib.BELL_DTYPE_F32
 _DTYPES = {torch.bfloat16: _BF16, torch.float32: _F32}
 _ROWS = 128  # tokens of one chunk of quantised rows
+_ELLS = {n: (_lib.BellEll * n, C.c_void_p * n) for n in (1, 2, 3)}  # array types of a pack of n weights
 
 
 def _call(name: str, dev: torch.device, *args) -> None:
@@ -157,9 +158,9 @@ def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
 def _direct(T: int, tile: int) -> bool:
     """Whether a product of T rows quantises them itself, which saves a launch
     (about 5 us of the host's time).  On the device alone, graph replays of the
-    gated block: tile 64, d_model 1024: 11.1 us either way at 1 token, 12.4
-    against 11.1 at 24; tile 128, d_model 4096: 15.1 against 15.4 at 1, 16.6
-    against 15.8 at 8, 21.3 against 16.6 at 24."""
+    gated block, on the way and quantised first: tile 64, d_model 1024: 9.5 us
+    and 9.4 at 1 token, 10.7 and 9.5 at 24; tile 128, d_model 4096: 15.2 and
+    15.4 at 1, 16.4 and 15.5 at 8, 21.0 and 16.4 at 24."""
     return T <= (_lib.BELL_MX_DIRECT_ROWS if tile == 64 else 8)
 
 
@@ -221,7 +222,8 @@ def _pack(weights, layout: int):
     if dtype not in _DTYPES:
         raise RuntimeError("tiles must be bf16 or fp32")
     n, dev, out = len(weights), weights[0][0].device, []
-    abi, chunks, plans = (_lib.BellEll * n)(), (C.c_void_p * n)(), (C.c_void_p * n)()
+    ells, pointers = _ELLS[n]
+    abi, chunks, plans = ells(), pointers(), pointers()
     held = []  # copies that must outlive the launch's enqueueing
     for i, (values, col_indices, C_blocks) in enumerate(weights):
         v, cols = _prep_ell("weight", values, col_indices, dtype)

@@ -709,3 +709,60 @@ def test_long_rows_shared_by_a_cluster(T, R, C, Kk, B, dead, dtype):
     check_linear(y, xq, w, Kk * B // 64, f64(res))
     assert torch.equal(y, K.mxfp4_linear(x, p, residual=res))
     assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("B", [64, 128])
+def test_a_column_block_twice_in_a_row(B):
+    """Slots of one block-row may share a column block: both count, in the sums and in each one's gradient."""
+    K = _K()
+    rng = np.random.default_rng(23)
+    cols = torch.tensor([[1, 1, 0], [2, -1, 2], [0, 0, 0]], dtype=torch.int32, device="cuda")
+    v = torch.from_numpy((rng.standard_normal((3, 3, B, B)) * 0.02).astype(np.float32)).to(BF16).cuda()
+    w = M.dense(M.quantize_tiles(f64(v), 0), cols.cpu().numpy(), 3, 0)
+    x, dy = rows(rng, 77, 3 * B), rows(rng, 77, 3 * B)
+    xq = M.quantize(f64(x))
+    leaves = [t.clone().requires_grad_(True) for t in (x, v)]
+    y = K.mxfp4_linear_ad(*leaves, cols)
+    check_linear(y, xq, w, 3 * B // 64)
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    ref = f64(dy) @ w
+    assert np.linalg.norm(f64(dx) - ref) <= 2.1 * 2.0 ** -8 * np.linalg.norm(ref)
+    full = f64(dy).T @ xq  # [out, in]
+    for r in range(3):
+        for k, c in enumerate(cols[r].tolist()):
+            want = full[r * B:(r + 1) * B, c * B:(c + 1) * B].T if c >= 0 else np.zeros((B, B))
+            assert np.linalg.norm(f64(dw[r, k]) - want) <= 2.1 * 2.0 ** -8 * np.linalg.norm(want), (r, k)
+
+
+def test_offsets_past_32_bits():
+    """Rows, chunks, hidden states and gradients of more than 2^32 values: the last tokens as in a call of their own."""
+    K = _K()
+    rng = np.random.default_rng(24)
+    T, n, d, F, B = 270336, 1000, 2048, 16384, 128
+    x = torch.zeros(T, d, dtype=BF16, device="cuda")
+    dy = torch.zeros(T, d, dtype=BF16, device="cuda")
+    x[:n], x[-n:], dy[-n:] = rows(rng, n, d), rows(rng, n, d), rows(rng, n, d)
+    mats = [weight(rng, F // B, d // B, 1, B)[:2] for _ in range(2)] + [weight(rng, d // B, F // B, 2, B)[:2]]
+    packed = [K.make_mxfp4(v, c, C) for (v, c), C in zip(mats, (d // B, d // B, F // B))]
+    y, ws = K.mxfp4_swiglu_fwd(x, *packed, return_intermediates=True)
+    y2, ws2 = K.mxfp4_swiglu_fwd(x[-n:].clone(), *packed, return_intermediates=True)
+    assert ws["gate"].numel() > 2 ** 32 and ws["q_h"].data.numel() > 2 ** 31
+    assert torch.equal(y[-n:], y2) and torch.equal(ws["gate"][-n:], ws2["gate"]) and torch.equal(ws["up"][-n:], ws2["up"])
+    h = ws["q_h"].dequantize()
+    assert torch.equal(h[-n:], ws2["q_h"].dequantize())
+    q = K.mxfp4_quantize(h, B)  # quantising is idempotent
+    assert torch.equal(K.mxfp4_dequantize(q)[-n:], h[-n:])
+    assert torch.equal(K.mxfp4_linear(q, packed[2])[-n:], y2)
+    del ws, h, q, y
+
+    def grads(a, g):
+        leaves = [a.requires_grad_(True)] + [v.clone().requires_grad_(True) for v, _ in mats]
+        out = K.mxfp4_swiglu(leaves[0], leaves[1], mats[0][1], leaves[2], mats[1][1], leaves[3], mats[2][1])
+        return torch.autograd.grad(out, leaves, g)
+
+    many, few = grads(x, dy), grads(x[-n:].detach().clone(), dy[-n:].clone())
+    # both are within one rounding and an fp32 sum's order of the same value
+    for a, b in zip((many[0][-n:], *many[1:]), few):
+        assert torch.linalg.norm(a.float() - b.float()) <= 2.0 ** -7 * torch.linalg.norm(b.float())
+    assert (many[0][:-n] == 0).all()
+    assert K.read_status() == 0

@@ -27,11 +27,12 @@
 // Hence the multi-slot stages, and two issuers: job j of the CTA belongs to
 // issuer j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
 //
-// A linear at B = 128 with units enough takes two token tiles to a unit (kPairs):
+// A linear with units enough takes two token tiles to a unit (kPairs):
 // one ring, whose stages hold the rows of both tiles and the weights once, and
 // issuer k takes tile k from every stage; a stage is free when both have
-// committed it, so neither is more than the ring ahead of the other.  13 KB for
-// a tile's slot instead of 17.4: 16384 -> 4096 at T = 16384 148 -> 133 us.  The
+// committed it, so neither is more than the ring ahead of the other.  At B = 128
+// 13 KB for a tile's slot instead of 17.4 (16384 -> 4096 at T = 16384 148 -> 133
+// us), at B = 64 fewer stages too (2048 -> 8192, 84 -> 72 us).  The
 // gated kernel gains nothing that way (313 us with a tile, 322 with two):
 // two gates and two ups need four accumulators and TMEM holds three, so the next
 // unit's gates wait for most of an epilogue.
@@ -675,14 +676,14 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
   const int64_t ld = int64_t(p.R) * B;
   const uint32_t lanes = uint32_t(q * 32) << 16;
   const int step = GROUPS * int(gridDim.x);
-  uint32_t acc = uint32_t(group * JOBS), use = 0;  // accumulator of this unit's first job
+  uint32_t acc = uint32_t(group * JOBS * G::TILES), use = 0;  // accumulator of this unit's first job
   int c0 = 0, c1 = 0;  // live slots of the next unit's rows, read a unit ahead
   auto counts = [&](int r) {
     c0 = __ldg(p.p0.counts + r);
     if (GATED) c1 = __ldg(p.p1.counts + r);
   };
-  auto next = [&] {  // this group's next accumulator (the first of two)
-    acc += GROUPS * JOBS;
+  auto next = [&](int jobs) {
+    acc += jobs;
     while (acc >= uint32_t(G::ACCS)) {
       acc -= G::ACCS;
       ++use;
@@ -832,7 +833,7 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
       }
     } else {
       for (int k = 0; k < G::TILES; ++k) {
-        if (k) next();
+        if (k) next(1);
         if (!__all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], use & 1u, ctl))) return;
         tc_fence_after();
         uint32_t a[32];
@@ -847,7 +848,7 @@ __device__ void epilogue(const Params& p, const Smem& s, uint32_t tmem, const Ct
         }
       }
     }
-    next();
+    next(GROUPS * JOBS * G::TILES - (G::TILES - 1));  // this group's next unit
   }
 }
 
@@ -1025,15 +1026,16 @@ static int linear(Params p, const BellMxEll& w, const void* residual, void* out,
   p.residual = residual;
   p.out_f32 = out_dtype == BELL_DTYPE_F32;
   p.wide = ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) & 31u) == 0;
-  if (w.B == 64) return launch<64, kLinear>(p, max_ctas, s);
   // Two token tiles to a unit where that leaves a unit for three of four SMs.
   // 16384 -> 4096, K = 32, us with one tile and with two: 160 units (80 pairs)
   // 12.5, 13.4; 256: 15.2, 13.4; 320: 19.8, 19.8; 512: 24.8, 21.3; 1024: 40, 36;
-  // 4096: 148, 133.
+  // 4096: 148, 133.  B = 64, 2048 -> 8192, K = 4: 1024 units 9.8, 9.6; 2048: 14.6,
+  // 13.2; 4224: 25.7, 22.1; 16384: 84, 72.
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
   const bool pairs = p.x && int64_t(p.mtiles + 1) / 2 * p.R * 4 >= int64_t(sms) * 3;
+  if (w.B == 64) return pairs ? launch<64, kPairs>(p, max_ctas, s) : launch<64, kLinear>(p, max_ctas, s);
   return pairs ? launch<128, kPairs>(p, max_ctas, s) : launch<128, kLinear>(p, max_ctas, s);
 }
 

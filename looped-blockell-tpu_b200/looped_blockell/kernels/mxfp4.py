@@ -355,12 +355,12 @@ def _swiglu(x, gate, up, down, add_residual=False, residual=None, keep_rows=Fals
         _check_weight(w, dev)
     if not add_residual:
         residual = None
-    else:
-        if residual is None:
-            if quantised:
-                raise RuntimeError("add_residual on quantised rows needs the residual")
-            residual = x
+    elif residual is not None:
         residual = _check_residual(residual, (T, D), dtype, dev)
+    elif quantised:
+        raise RuntimeError("add_residual on quantised rows needs the residual")
+    else:  # x is [T, D] of the output's dtype, aligned
+        residual = x.contiguous()
     out = gate.data.new_empty((T, D), dtype=dtype)
     direct = not quantised and not keep_rows and _direct(T, B)
     n_x, n_h = 0 if quantised or direct else _rows_bytes(T, D, B), _rows_bytes(T, F, B)

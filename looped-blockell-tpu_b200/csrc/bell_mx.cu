@@ -881,10 +881,13 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   tc_fence_after();
   const uint32_t tmem = *s.tmem_slot;
   const Ctl ctl{s.abort_flag, p.status, p.timeout_ns};
-  griddep_launch();
   // Rows, and possibly weights, come from the kernel ahead.  With p.early only
-  // the rows do, and the producers start the weights before they wait.
+  // the rows do, and the producers start the weights before they wait.  A kernel
+  // on the caller's rows lets the next one start only when all before it is
+  // complete: the next one's p.early rests on that.
+  if (p.x) griddep_launch();
   if (!p.early || warp >= kProducers) griddep_wait();
+  if (!p.x) griddep_launch();
   const bool split = MODE == kLinear && p.split;
   if (warp < kProducers) {
     if (warp < G::RINGS * G::PER) produce<B, G>(p, s, warp / G::PER, warp % G::PER, ctl);
@@ -955,9 +958,8 @@ static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(p.split);
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  // direct rows may come from any kernel ahead: a plain launch waits for it
-  cfg.attrs = attr + (p.x ? 0 : 1);
-  cfg.numAttrs = (p.x ? 1 : 0) + (p.split ? 1 : 0);
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -1115,7 +1117,9 @@ int bell_swiglu_fwd_mx(const BellMxFFNDesc* d, void* stream) {
   p.early = d->x && d->x_src;
   if (int rc = g.B == 128 ? mx::launch<128, mx::kGated>(p, d->max_ctas, s) : mx::launch<64, mx::kGated>(p, d->max_ctas, s)) return rc;
   mx::Params q = mx::base_params(d->T, w, nullptr, d->h, status);
-  q.early = d->x_src != nullptr;  // a plain launch (the quantisation, or gate/up from the caller's rows) came before
+  // what came before the quantisation (a plain launch) or before gate/up on the
+  // caller's rows is complete when the kernel ahead of this one lets it start
+  q.early = d->x_src != nullptr;
   return mx::linear(q, w, d->residual, d->out, d->out_dtype, d->max_ctas, s);
 }
 

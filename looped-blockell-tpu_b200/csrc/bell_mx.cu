@@ -27,15 +27,15 @@
 // Hence the multi-slot stages, and two issuers: job j of the CTA belongs to
 // issuer j & 1 (gated: gate jobs and up jobs), each with a ring of its own.
 //
-// A linear with units enough takes two token tiles to a unit (kPairs):
-// one ring, whose stages hold the rows of both tiles and the weights once, and
-// issuer k takes tile k from every stage; a stage is free when both have
-// committed it, so neither is more than the ring ahead of the other.  At B = 128
-// 13 KB for a tile's slot instead of 17.4 (16384 -> 4096 at T = 16384 148 -> 133
-// us), at B = 64 fewer stages too (2048 -> 8192, 84 -> 72 us).  The
-// gated kernel gains nothing that way (313 us with a tile, 322 with two):
-// two gates and two ups need four accumulators and TMEM holds three, so the next
-// unit's gates wait for most of an epilogue.
+// A linear with units enough takes two token tiles to a unit (kPairs): one ring,
+// whose stages hold the rows of both tiles and the weights once, and issuer k
+// takes tile k from every stage; a stage is free when both have committed it, so
+// neither is more than the ring ahead of the other.  At B = 128 13 KB for a tile's
+// slot instead of 17.4 (16384 -> 4096 at T = 16384 148 -> 133 us), at B = 64 fewer
+// stages too (2048 -> 8192, 84 -> 72 us).  The gated kernel gains nothing that way
+// (313 us with a tile, 322 with two): two gates and two ups need four
+// accumulators and TMEM holds three, so the next unit's gates wait for most of an
+// epilogue.
 //
 // What bounds it: B = 128, the way from the L2 into the SM, 60 bytes a cycle, and
 // the ring's latency.  Of the linear's 133 us (4.2 PFLOP/s) the copies and the
@@ -45,25 +45,25 @@
 // (T = 16384, d = 2048, d_ff = 8192: 125 us; without the SiLU's exponential and
 // reciprocal 104).
 //
-// Warps: 0-5 producers (ring w / 3; stage use h of a ring belongs to its
-// producer h % 3, since a producer's turn, from a stage's release to its copies'
-// issue, is on the ring's path: with one tile to a unit 156 us with one producer
-// a ring, 147 with two or three; gated B = 64 128 us with two, 125 with three;
-// kPairs leaves 3-5 idle), 6-21 epilogue
-// (a warp takes the TMEM lane quadrant warp % 4 and one 32-column block of a
-// unit; at B = 64, two blocks, two groups of eight warps take the CTA's units in
-// turn), 22 and 23 issuers (22 owns TMEM).  Accumulators form a ring of ACCS in
-// job order, so the issuers run ahead of the epilogue.
+// Warps: 0-5 producers (ring w / 3; stage use h of a ring belongs to its producer
+// h % 3; kPairs leaves 3-5 idle), 6-21 epilogue (a warp takes the TMEM lane
+// quadrant warp % 4 and one 32-column block of a unit; at B = 64, two blocks, two
+// groups of eight warps take the CTA's units in turn), 22 and 23 issuers (22 owns
+// TMEM).  A producer's turn, from a stage's release to its copies' issue, is on
+// the ring's path: with one tile to a unit 156 us with one producer a ring, 147
+// with two or three; gated B = 64 128 us with two, 125 with three.  Accumulators
+// form a ring of ACCS in job order, so the issuers run ahead of the epilogue.
 //
-// Few units (a linear of few tokens): split mode.  A cluster of `split` CTAs
-// shares one unit, each ring of each CTA takes an equal range of the stages
-// into an accumulator of its own, and the partial sums meet in distributed
-// shared memory, in a fixed order.  The TMEM scale
-// columns belong to the stage: a stage is refilled only after its MMAs have
-// completed, so the scales of MMAs in flight are never overwritten.
-// Token-major, because a lane of the epilogue then holds 32 consecutive
-// features of its token: one scale block, quantised without talking to another
-// lane and stored as 16 bytes.
+// Few units (a linear of few tokens with long rows): split mode.  A cluster of
+// `split` CTAs shares one unit, each ring of each CTA takes an equal range of the
+// stages into an accumulator of its own, and the partial sums meet in distributed
+// shared memory, in a fixed order.
+//
+// The TMEM scale columns belong to the stage: a stage is refilled only after its
+// MMAs have completed, so the scales of MMAs in flight are never overwritten.
+// Token-major, because a lane of the epilogue then holds 32 consecutive features
+// of its token: one scale block, quantised without talking to another lane and
+// stored as 16 bytes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -158,9 +158,9 @@ def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
 def _direct(T: int, tile: int) -> bool:
     """Whether a product of T rows quantises them itself, which saves a launch
     (about 5 us of the host's time).  On the device alone, graph replays of the
-    gated block, on the way and quantised first: tile 64, d_model 1024: 9.5 us
-    and 9.4 at 1 token, 10.7 and 9.5 at 24; tile 128, d_model 4096: 15.2 and
-    15.4 at 1, 16.4 and 15.5 at 8, 21.0 and 16.4 at 24."""
+    gated block, on the way and quantised first: tile 64, d_model 1024: 8.9 us
+    and 9.3 at 1 token, 10.1 and 9.5 at 24; tile 128, d_model 4096: 14.7 and
+    15.5 at 1, 15.7 and 15.6 at 8, 20.2 and 16.4 at 24."""
     return T <= (_lib.BELL_MX_DIRECT_ROWS if tile == 64 else 8)
 
 

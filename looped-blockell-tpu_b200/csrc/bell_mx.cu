@@ -1032,11 +1032,12 @@ static int linear(Params p, const BellMxEll& w, const void* residual, void* out,
   // 16384 -> 4096, K = 32, us with one tile and with two: 160 units (80 pairs)
   // 12.5, 13.4; 256: 15.2, 13.4; 320: 19.8, 19.8; 512: 24.8, 21.3; 1024: 40, 36;
   // 4096: 148, 133.  B = 64, 2048 -> 8192, K = 4: 1024 units 9.8, 9.6; 2048: 14.6,
-  // 13.2; 4224: 25.7, 22.1; 16384: 84, 72.
+  // 13.2; 4224: 25.7, 22.1; 16384: 84, 72.  A tile alone (128 units, B = 128, K = 8)
+  // 6.1, 7.3; three of them 9.9, 9.9; five 13.7, 13.5.
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
-  const bool pairs = p.x && int64_t(p.mtiles + 1) / 2 * p.R * 4 >= int64_t(sms) * 3;
+  const bool pairs = p.x && p.mtiles > 1 && int64_t(p.mtiles + 1) / 2 * p.R * 4 >= int64_t(sms) * 3;
   if (w.B == 64) return pairs ? launch<64, kPairs>(p, max_ctas, s) : launch<64, kLinear>(p, max_ctas, s);
   return pairs ? launch<128, kPairs>(p, max_ctas, s) : launch<128, kLinear>(p, max_ctas, s);
 }

@@ -1,5 +1,5 @@
 """MXFP4 Block-ELL in float64 NumPy, from the definition (OCP Microscaling
-Formats 1.0): the checker of the GPU operators, not a fast path.
+Formats 1.0): what the GPU operators are tested against, not a fast path.
 
 Blocks of 32 values along the last axis share s = 2^max(floor(log2 a) - 2, -127),
 a the block's largest magnitude; codes are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6),

@@ -290,7 +290,10 @@ def mxfp4_linear(x: Union[torch.Tensor, MXRows], w: MXBlockELL, residual: Option
     ``x`` is ``[T, in_features]`` bf16 or fp32, or rows quantised before
     (``mxfp4_quantize``).  The output has ``out_dtype`` (default: x's, bf16 for
     quantised rows); ``residual`` has the output's shape and dtype.
-    ``out`` may be ``residual`` or ``x`` itself.  ``max_ctas`` caps the
+    Where there are few units of many slots, parts of a row are summed first, so
+    the order of its fp32 sum may depend on the number of tokens (and on the
+    device's SMs); it is the same on every run.  ``out`` may be ``residual`` or
+    ``x`` itself.  ``max_ctas`` caps the
     persistent grid (0 = every SM)."""
     return _linear(x, w, residual, out_dtype, out, max_ctas)[0]
 

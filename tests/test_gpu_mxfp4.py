@@ -766,3 +766,36 @@ def test_offsets_past_32_bits():
         assert torch.linalg.norm(a.float() - b.float()) <= 2.0 ** -7 * torch.linalg.norm(b.float())
     assert (many[0][:-n] == 0).all()
     assert K.read_status() == 0
+
+
+def test_two_host_threads():
+    """Calls from two threads, each on a stream of its own, do not see one another's arguments or errors."""
+    import threading
+    K = _K()
+    rng = np.random.default_rng(25)
+    _, packed = _ffn(rng)
+    xs = [rows(rng, T, 256) for T in (3, 150)]
+    want = [K.mxfp4_swiglu_fwd(x, *packed, add_residual=True) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                y = K.mxfp4_swiglu_fwd(xs[i], *packed, add_residual=True)
+                try:
+                    K.mxfp4_linear(xs[i], packed[0], out=y)
+                    wrong.append("not refused")
+                except RuntimeError as e:
+                    if "out must be" not in str(e):
+                        wrong.append(str(e))
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(y, want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and K.read_status() == 0

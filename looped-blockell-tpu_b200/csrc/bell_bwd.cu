@@ -17,7 +17,9 @@
 //     row's b features M and the two slots' a features N = 256.  Either way
 //     one b chunk serves every slot of the unit.  Tokens
 //     run in ranges sized to stay in L2; each CTA takes an equal share of a
-//     range and adds its fp32 partial tiles into the gradient with atomics.
+//     range and adds its fp32 partial tiles into the gradient with atomics
+//     (or, for the MXFP4 backward, so that their order is fixed; see seg_next).
+#include <algorithm>
 #include <string>
 
 #include "bell_bf16.cuh"
@@ -100,6 +102,8 @@ struct SddmmParams {
   int64_t split_chunks;      // 64-token chunks per token range
   const int32_t* cols;       // [R, K]
   float* grad;               // [R, K, B, B] fp32, accumulated
+  int32_t own;               // one CTA to a sum (see seg_next): grad is written, not added to
+  float* parts;              // with it: [gridDim.x, SLOTS, B, B]
   int32_t out_in;            // tile layout of grad: 0 [B_in, B_out], 1 [B_out, B_in]
   int32_t* status;
   uint64_t timeout_ns;
@@ -107,6 +111,20 @@ struct SddmmParams {
 
 __device__ __forceinline__ void red_add_v4(float* p, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// Sums leave as stores (`put`, uniform) or additions.
+__device__ __forceinline__ void add_v4(float* p, const uint32_t* v, bool put) {
+  if (put)
+    st_global_v4(p, v[0], v[1], v[2], v[3]);
+  else
+    red_add_v4(p, __uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+}
+__device__ __forceinline__ void add_1(float* p, uint32_t v, bool put) {
+  if (put)
+    *p = __uint_as_float(v);
+  else
+    atomicAdd(p, __uint_as_float(v));
 }
 
 struct Unit {
@@ -149,7 +167,12 @@ __device__ __forceinline__ Unit unit_of(int u, const SddmmParams& p) {
 // per CTA, so every CTA streams the same tokens at the same time (the
 // activation tiles are shared through L2) and no CTA waits on a longer share.
 // A share may start or end inside a unit: each piece (segment) adds its
-// partial tiles into the gradient like a whole unit.
+// partial tiles into the gradient like a whole unit.  With p.own only the
+// piece with the unit's first chunk does; a share that starts inside a unit
+// (its first segment, the same one in every range) sums that segment's tiles in
+// the CTA's own part instead.  Every sum then has one CTA, whose threads write
+// the first range and add the others in order, and whoever adds the parts in CTA
+// order (sddmm_cuts) has a gradient that does not depend on the order of arrival.
 struct SegIt {
   int s;
   int64_t L, L1, Ws;
@@ -169,10 +192,11 @@ __device__ __forceinline__ SegIt seg_begin(const SddmmParams& p) {
 }
 
 // Next segment of this CTA: unit `x`, chunks [a0, a1) (empty when a1 <= a0),
-// `head` when it starts at the unit's first chunk of split 0.  False at the end.
+// `head` when it starts at the unit's first chunk of split 0, `cut` when it
+// starts behind the first chunk of its split.  False at the end.
 template <int SLOTS>
 __device__ __forceinline__ bool seg_next(const SddmmParams& p, SegIt& it, Unit& x, int64_t& a0, int64_t& a1,
-                                         bool& head) {
+                                         bool& head, bool& cut) {
   while (it.L >= it.L1) {
     if (++it.s >= p.n_split) return false;
     seg_share(p, it);
@@ -186,6 +210,7 @@ __device__ __forceinline__ bool seg_next(const SddmmParams& p, SegIt& it, Unit& 
   a0 = x.ch0 + c_lo;
   a1 = min(x.ch0 + c_hi, x.ch1);
   head = it.s == 0 && c_lo == 0;
+  cut = c_lo != 0;
   return true;
 }
 
@@ -240,8 +265,8 @@ __global__ void __launch_bounds__(kThr, 1)
       SegIt it = seg_begin(p);
       Unit x;
       int64_t a0, a1;
-      bool head;
-      while (alive && seg_next<SLOTS>(p, it, x, a0, a1, head)) {
+      bool head, cut;
+      while (alive && seg_next<SLOTS>(p, it, x, a0, a1, head, cut)) {
         if (head) {  // once per unit: report indices outside [-1, C)
 #pragma unroll
           for (int j = 0; j < SLOTS; ++j) {
@@ -312,8 +337,8 @@ __global__ void __launch_bounds__(kThr, 1)
     SegIt it = seg_begin(p);
     Unit x;
     int64_t a0, a1;
-    bool head;
-    while (seg_next<SLOTS>(p, it, x, a0, a1, head)) {
+    bool head, cut;
+    while (seg_next<SLOTS>(p, it, x, a0, a1, head, cut)) {
       if (!x.any || a1 <= a0) continue;
       const int buf = i & 1;
       const uint32_t use = uint32_t(i >> 1);
@@ -367,8 +392,8 @@ __global__ void __launch_bounds__(kThr, 1)
     SegIt it = seg_begin(p);
     Unit x;
     int64_t a0, a1;
-    bool head;
-    while (seg_next<SLOTS>(p, it, x, a0, a1, head)) {
+    bool head, cut;
+    while (seg_next<SLOTS>(p, it, x, a0, a1, head, cut)) {
       if (!x.any || a1 <= a0) continue;
       const int buf = i & 1;
       const uint32_t use = uint32_t(i >> 1);
@@ -376,6 +401,8 @@ __global__ void __launch_bounds__(kThr, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], use & 1u, ctl))) break;
       tc_fence_after();
       const uint32_t tb = tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * C::NACC * C::N);
+      const bool part = p.own && cut, put = p.own && it.s == 0;
+      float* own = p.parts + size_t(blockIdx.x) * SLOTS * B * B;
       if constexpr (!C::TR) {
         // B = 64: accumulator ac, row = a feature; rows 0-63 slot 2ac, 64-127
         // slot 2ac+1; columns = the row's 64 b (output) features
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(kThr, 1)
           const int ac = jj / (B / 32), j = jj % (B / 32);
           const int sl = 2 * ac + (q >= 2 ? 1 : 0);
           const int k = pick4(x.k, sl), c = pick4(x.c, sl);
-          float* tile = p.grad + (size_t(x.r) * p.K + (k >= 0 ? k : 0)) * B * B;
+          float* tile = part ? own + sl * B * B : p.grad + (size_t(x.r) * p.K + (k >= 0 ? k : 0)) * B * B;
           uint32_t v[32];
           tmem_ld32_sync(tb + uint32_t(ac * C::N) + j * 32, v);
           if (c < 0) continue;
@@ -393,11 +420,10 @@ __global__ void __launch_bounds__(kThr, 1)
             float* dst = tile + size_t(fin) * B + j * 32;
 #pragma unroll
             for (int t = 0; t < 8; ++t)
-              red_add_v4(dst + 4 * t, __uint_as_float(v[4 * t]), __uint_as_float(v[4 * t + 1]),
-                         __uint_as_float(v[4 * t + 2]), __uint_as_float(v[4 * t + 3]));
+              add_v4(dst + 4 * t, v + 4 * t, put);
           } else {  // [B_out, B_in]: consecutive lanes hit consecutive addresses
 #pragma unroll
-            for (int t = 0; t < 32; ++t) atomicAdd(tile + size_t(j * 32 + t) * B + fin, __uint_as_float(v[t]));
+            for (int t = 0; t < 32; ++t) add_1(tile + size_t(j * 32 + t) * B + fin, v[t], put);
           }
         }
       } else {
@@ -408,20 +434,19 @@ __global__ void __launch_bounds__(kThr, 1)
           const int k = pick4(x.k, sl);
           const int c = pick4(x.c, sl);
           if (c < 0) continue;  // warp-uniform
-          float* tile = p.grad + (size_t(x.r) * p.K + k) * B * B;
+          float* tile = part ? own + sl * B * B : p.grad + (size_t(x.r) * p.K + k) * B * B;
 #pragma unroll 1
           for (int j = 0; j < B / 32; ++j) {
             uint32_t v[32];
             tmem_ld32_sync(tb + sl * B + j * 32, v);
             if (!p.out_in) {  // [B_in, B_out]: consecutive lanes hit consecutive addresses
 #pragma unroll
-              for (int t = 0; t < 32; ++t) atomicAdd(tile + size_t(j * 32 + t) * B + row, __uint_as_float(v[t]));
+              for (int t = 0; t < 32; ++t) add_1(tile + size_t(j * 32 + t) * B + row, v[t], put);
             } else {  // [B_out, B_in]: this row's 32 inputs are contiguous
               float* dst = tile + size_t(row) * B + j * 32;
 #pragma unroll
               for (int t = 0; t < 8; ++t)
-                red_add_v4(dst + 4 * t, __uint_as_float(v[4 * t]), __uint_as_float(v[4 * t + 1]),
-                           __uint_as_float(v[4 * t + 2]), __uint_as_float(v[4 * t + 3]));
+                add_v4(dst + 4 * t, v + 4 * t, put);
             }
           }
         }
@@ -451,7 +476,7 @@ int grid_for(int64_t n8, int sms) {
 }
 
 template <int B>
-int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sms) {
+int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sms, bool own, float* parts) {
   using C = SCfg<B>;
   CUtensorMap ma, mb;
   if (int rc = make_map_2d(&ma, d->a, MapType::BF16, uint64_t(d->C) * B, uint64_t(d->T), uint64_t(d->lda) * 2, 64,
@@ -460,39 +485,95 @@ int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sm
   if (int rc = make_map_2d(&mb, d->b, MapType::BF16, uint64_t(d->R) * B, uint64_t(d->T), uint64_t(d->ldb) * 2, 64,
                            kTok, Swz::B128))
     return rc;
+  const SddmmCuts cuts = sddmm_cuts(d->T, d->R, d->C, d->K, B, own ? std::min(sms, kMaxParts) : sms);
   SddmmParams p{};
   p.T = d->T;
   p.R = d->R;
   p.K = d->K;
-  p.KP = (d->K + C::SLOTS - 1) / C::SLOTS;
+  p.KP = cuts.KP;
   p.C = d->C;
-  const int64_t chunks = (d->T + kTok - 1) / kTok;
-  const int64_t per = int64_t(p.R) * p.KP;
-  // token ranges whose operands (a and b rows, bf16) fit in ~96 MB of the
-  // 126 MB L2, so every unit of the range re-reads them from L2; 16..128
-  // chunks (1024..8192 tokens) keep each CTA's partial-tile additions small
-  // next to its loads
-  const int64_t row_bytes = 2 * (int64_t(d->C) + d->R) * B;
-  int64_t range = (int64_t(96) << 20) / (row_bytes * kTok);
-  range = range < 16 ? 16 : (range > 128 ? 128 : range);
-  p.split_chunks = chunks < range ? chunks : range;
-  p.n_split = int32_t((chunks + p.split_chunks - 1) / p.split_chunks);
+  p.split_chunks = cuts.chunks;
+  p.n_split = int32_t(((d->T + kTok - 1) / kTok + cuts.chunks - 1) / cuts.chunks);
   p.cols = d->col_indices;
   p.grad = d->grad;
+  p.own = own;
+  p.parts = parts;
   p.out_in = d->layout == BELL_TILE_OUT_IN;
   p.status = status;
   p.timeout_ns = wait_budget_ns();
-  if (per * p.n_split > INT32_MAX) return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: too many work units");
+  if (int64_t(p.R) * p.KP * p.n_split > INT32_MAX) return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: too many work units");
   auto kern = bell_sddmm_kernel<B>;
   if (int rc = set_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
-  const int64_t share = per * p.split_chunks;  // chunk-steps of one range
-  const int grid = int(share < sms ? share : sms);
-  kern<<<grid, kThr, C::SMEM, s>>>(ma, mb, p);
+  kern<<<cuts.grid, kThr, C::SMEM, s>>>(ma, mb, p);
   return check_launch("bell_sddmm_kernel");
 }
 
 }  // namespace
 }  // namespace bwd
+
+SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas) {
+  SddmmCuts c{};
+  c.slots = B == 128 ? bwd::SCfg<128>::SLOTS : bwd::SCfg<64>::SLOTS;
+  c.KP = (K + c.slots - 1) / c.slots;
+  const int64_t chunks = (T + bwd::kTok - 1) / bwd::kTok;
+  // token ranges whose operands (a and b rows, bf16) fit in ~96 MB of the
+  // 126 MB L2, so every unit of the range re-reads them from L2; 16..128
+  // chunks (1024..8192 tokens) keep each CTA's partial-tile additions small
+  // next to its loads
+  const int64_t row_bytes = 2 * (int64_t(C) + R) * B;
+  int64_t range = (int64_t(96) << 20) / (row_bytes * bwd::kTok);
+  range = range < 16 ? 16 : (range > 128 ? 128 : range);
+  c.chunks = chunks < range ? chunks : range;
+  c.steps = int64_t(R) * c.KP * c.chunks;  // chunk-steps of one range
+  c.grid = int32_t(c.steps < ctas ? c.steps : ctas);
+  return c;
+}
+
+int sddmm_bf16(const BellSddmmDesc* d, bool own, float* parts, void* stream) {
+  if (!d) return fail(BELL_ERR_ARG, "bell_sddmm_bf16: NULL descriptor");
+  if (!d->col_indices || !d->grad || (d->T > 0 && (!d->a || !d->b)))
+    return fail(BELL_ERR_ARG, "bell_sddmm_bf16: NULL pointer");
+  if (d->B != 16 && d->B != 32 && d->B != 64 && d->B != 128)
+    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: tile size must be 16, 32, 64 or 128");
+  if (d->T < 0 || d->R <= 0 || d->C <= 0 || d->K <= 0)
+    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: need T >= 0 and R, C, K > 0");
+  if (d->T > INT32_MAX - 64) return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: T too large");
+  if (d->lda < int64_t(d->C) * d->B || d->ldb < int64_t(d->R) * d->B)
+    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: row pitch smaller than the row");
+  if (d->layout != BELL_TILE_IN_OUT && d->layout != BELL_TILE_OUT_IN)
+    return fail(BELL_ERR_ARG, "bell_sddmm_bf16: unknown tile layout");
+  if (!aligned16(d->grad) || (d->grad_bf16 && !aligned16(d->grad_bf16)))
+    return fail(BELL_ERR_ALIGN, "bell_sddmm_bf16: gradient buffers must be 16-byte aligned");
+  if (int rc = require_sm100()) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int32_t* status = d->status ? d->status : default_status_ptr();
+  if (!status) return BELL_ERR_LAUNCH;
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  const size_t n = size_t(d->R) * d->K * d->B * d->B;
+  if (!d->accumulate && !own) {
+    cudaError_t e = cudaMemsetAsync(d->grad, 0, n * sizeof(float), s);
+    if (e != cudaSuccess) return fail(BELL_ERR_LAUNCH, std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+  }
+  if (d->T > 0) {
+    const int rc = d->B < 64     ? launch_sddmm_ffma(d, false, status, s)
+                   : d->B == 64 ? bwd::launch_sddmm<64>(d, status, s, sms, own, parts)
+                                : bwd::launch_sddmm<128>(d, status, s, sms, own, parts);
+    if (rc) return rc;
+  }
+  if (d->grad_bf16) {
+    const int64_t n8 = int64_t(n / 8);
+    bwd::bell_f32_to_bf16_kernel<<<bwd::grid_for(n8, sms), 256, 0, s>>>(d->grad, static_cast<__nv_bfloat16*>(d->grad_bf16), n8);
+    return check_launch("bell_f32_to_bf16_kernel");
+  }
+  return BELL_OK;
+}
+
+size_t sddmm_parts_bytes(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B) {
+  const SddmmCuts c = sddmm_cuts(T, R, C, K, B, kMaxParts);
+  return c.chunks > 1 ? size_t(c.grid) * c.slots * B * B * 4 : 0;
+}
+
 }  // namespace bell
 
 using namespace bell;
@@ -520,45 +601,7 @@ int bell_silu_mul_bwd_bf16(int64_t T, int32_t d_ff, const void* d_h, const void*
   return check_launch("bell_silu_mul_bwd_kernel");
 }
 
-int bell_sddmm_bf16(const BellSddmmDesc* d, void* stream) {
-  if (!d) return fail(BELL_ERR_ARG, "bell_sddmm_bf16: NULL descriptor");
-  if (!d->col_indices || !d->grad || (d->T > 0 && (!d->a || !d->b)))
-    return fail(BELL_ERR_ARG, "bell_sddmm_bf16: NULL pointer");
-  if (d->B != 16 && d->B != 32 && d->B != 64 && d->B != 128)
-    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: tile size must be 16, 32, 64 or 128");
-  if (d->T < 0 || d->R <= 0 || d->C <= 0 || d->K <= 0)
-    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: need T >= 0 and R, C, K > 0");
-  if (d->T > INT32_MAX - 64) return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: T too large");
-  if (d->lda < int64_t(d->C) * d->B || d->ldb < int64_t(d->R) * d->B)
-    return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: row pitch smaller than the row");
-  if (d->layout != BELL_TILE_IN_OUT && d->layout != BELL_TILE_OUT_IN)
-    return fail(BELL_ERR_ARG, "bell_sddmm_bf16: unknown tile layout");
-  if (!aligned16(d->grad) || (d->grad_bf16 && !aligned16(d->grad_bf16)))
-    return fail(BELL_ERR_ALIGN, "bell_sddmm_bf16: gradient buffers must be 16-byte aligned");
-  if (int rc = require_sm100()) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int32_t* status = d->status ? d->status : default_status_ptr();
-  if (!status) return BELL_ERR_LAUNCH;
-  int sms = 0;
-  if (int rc = device_sm_count(&sms)) return rc;
-  const size_t n = size_t(d->R) * d->K * d->B * d->B;
-  if (!d->accumulate) {
-    cudaError_t e = cudaMemsetAsync(d->grad, 0, n * sizeof(float), s);
-    if (e != cudaSuccess) return fail(BELL_ERR_LAUNCH, std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
-  }
-  if (d->T > 0) {
-    const int rc = d->B < 64     ? launch_sddmm_ffma(d, false, status, s)
-                   : d->B == 64 ? launch_sddmm<64>(d, status, s, sms)
-                                : launch_sddmm<128>(d, status, s, sms);
-    if (rc) return rc;
-  }
-  if (d->grad_bf16) {
-    const int64_t n8 = int64_t(n / 8);
-    bell_f32_to_bf16_kernel<<<grid_for(n8, sms), 256, 0, s>>>(d->grad, static_cast<__nv_bfloat16*>(d->grad_bf16), n8);
-    return check_launch("bell_f32_to_bf16_kernel");
-  }
-  return BELL_OK;
-}
+int bell_sddmm_bf16(const BellSddmmDesc* d, void* stream) { return sddmm_bf16(d, false, nullptr, stream); }
 
 int bell_sddmm_f32(const BellSddmmDesc* d, void* stream) {
   if (!d) return fail(BELL_ERR_ARG, "bell_sddmm_f32: NULL descriptor");

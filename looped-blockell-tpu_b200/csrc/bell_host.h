@@ -68,6 +68,24 @@ int gate_up_bf16(const BellFFNDesc* d, int32_t* status, cudaStream_t s, bool pdl
                  int64_t h_parts = 0);
 int down_bf16(const BellFFNDesc* d, int32_t* status, cudaStream_t s, bool pdl = false);
 
+// Tile gradients (bell_bwd.cu) whose sums do not depend on the order of CTAs.
+// The chunk-steps [0, steps) of one token range, `chunks` to a unit (a group of
+// `slots` slots of a block-row, KP groups to a row), are cut into `grid` equal
+// shares, of which share b starts at steps * b / grid.  sddmm_bf16 with `own`
+// (T > 0, B 64 or 128; it takes sddmm_cuts() of at most kMaxParts CTAs) writes
+// into d->grad, for each unit, the sums of the share that holds its first chunk,
+// and into parts[b] ([slots, B, B]; sddmm_parts_bytes() bytes, 16-byte aligned,
+// NULL where that is 0) those of a share b that starts inside a unit: a tile's
+// gradient is its grad plus the parts of its unit.  Dead slots are not written.
+struct SddmmCuts {
+  int64_t steps, chunks;
+  int32_t grid, slots, KP;
+};
+static constexpr int kMaxParts = 160;  // a B200 has 148 SMs
+SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas);
+size_t sddmm_parts_bytes(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B);
+int sddmm_bf16(const BellSddmmDesc* d, bool own, float* parts, void* stream);
+
 // Workspace of the loop: per-tile counters, per-row partial sums of squares
 // and the gain-scaled gate/up tiles (tile size 64; other sizes need none).
 struct LoopWs {

@@ -270,26 +270,29 @@ struct RowsTo {  // quantised rows to bf16 [T, features]
   int32_t features;
   void* dst;
 };
-struct Zeros {
-  float* at;
-  int64_t floats;  // a multiple of 4
-};
-// Everything that a backward unpacks or clears before its products, one launch.
+// Everything that a backward unpacks before its products, one launch.
 struct ExpandArgs {
   int64_t T;
   int32_t B;
   TileGather gather[2];
   RowsTo rows[2];
-  Zeros zero[3];
 };
 int expand(const ExpandArgs& e, cudaStream_t s);
-// n[i] fp32 sums (a multiple of 8) rounded to bf16.
-struct RoundArgs {
-  const float* src[3];
-  void* dst[3];
-  int64_t n[3];
+// A tile gradient [R, K, B, B]: its sums as sddmm_bf16 leaves them
+// (bell_host.h), completed by the parts of their units, zero in dead slots, and,
+// where `rounded` is given, written there in bf16.
+struct TileGrad {
+  float* sums;
+  void* rounded;
+  const float* parts;   // optional
+  const int32_t* cols;  // [R, K]: live in [0, C), C = 0 without tokens
+  int32_t R, C, K, B;
+  SddmmCuts cuts;
 };
-int round_sums(const RoundArgs& a, cudaStream_t s);
+struct FinishArgs {
+  TileGrad g[3];  // without sums: skipped
+};
+int finish_grads(const FinishArgs& a, cudaStream_t s);
 
 // [d_gate | d_up] (bf16 [T, 2 R B]) from d_h (fp32 [T, R B]) and the gated
 // block's quantised rows and weights (bell_mx.cu).

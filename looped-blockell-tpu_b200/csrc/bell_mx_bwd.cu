@@ -3,12 +3,13 @@
 // whose values are exact in bf16.  Each entry point is the sequence of launches
 // on the caller's stream and one workspace:
 //
-//   unpack    the gathered tiles of W_down^T and [W_gate ; W_up]^T, Q(x), and
-//             zeros for the tile gradients: one launch
+//   unpack    the gathered tiles of W_down^T and [W_gate ; W_up]^T, and Q(x):
+//             one launch
 //   d_h = dy Q(W_down), fp32
 //   [d_gate | d_up] from d_h and the projections, computed again (bell_mx.cu)
 //   dx = [d_gate | d_up] Q([W_gate ; W_up]) (+ dy)
-//   the three tile gradients, summed in fp32; one launch rounds them to bf16
+//   the three tile gradients, summed in fp32; one launch completes the sums
+//   that CTAs shared, in a fixed order, and rounds them to bf16
 //
 // d_h stays in fp32: rounded to bf16, its error and that of d_gate and d_up
 // together made the tile gradients' 1.7 times that of one rounding.  The
@@ -26,9 +27,9 @@ static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Offsets of the workspace: the unpacked transposes (of down, and of gate and
 // up or the one weight), a plan, the unpacked rows, d_h then Q(h), fp32 sums
-// whose result is bf16, [d_gate | d_up].
+// whose result is bf16, the parts of sums that CTAs share, [d_gate | d_up].
 struct BwdWs {
-  size_t tiles_down, tiles, plan, rows, mid, grads[3], dgu, total;
+  size_t tiles_down, tiles, plan, rows, mid, grads[3], parts[3], dgu, total;
 };
 
 struct Layout {
@@ -44,6 +45,10 @@ static size_t sums_bytes(const BellMxEll& w, bool wanted, int32_t dtype) {
   return wanted && dtype == BELL_DTYPE_BF16 ? size_t(w.R) * w.K * w.B * w.B * 4 : 0;
 }
 
+static size_t parts_bytes(const BellMxEll& w, bool wanted, int64_t T) {
+  return wanted ? sddmm_parts_bytes(T, w.R, w.C, w.K, w.B) : 0;
+}
+
 static BwdWs linear_ws(const BellMxLinearBwdDesc& d) {
   BwdWs o{};
   Layout l;
@@ -51,6 +56,7 @@ static BwdWs linear_ws(const BellMxLinearBwdDesc& d) {
   o.plan = l.take(d.dx ? bell_plan_bytes(0, 0, 0, d.w.C, d.K_t) : 0);
   o.rows = l.take(d.dw ? size_t(d.T) * d.w.C * d.w.B * 2 : 0);
   o.grads[0] = l.take(sums_bytes(d.w, d.dw != nullptr, d.grad_dtype));
+  o.parts[0] = l.take(parts_bytes(d.w, d.dw != nullptr, d.T));
   o.total = std::max<size_t>(l.at, 256);
   return o;
 }
@@ -68,28 +74,35 @@ static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
   o.grads[0] = l.take(sums_bytes(d.gate, d.d_gate != nullptr, d.gate_dtype));
   o.grads[1] = l.take(sums_bytes(d.up, d.d_up != nullptr, d.up_dtype));
   o.grads[2] = l.take(sums_bytes(d.down, d.d_down != nullptr, d.down_dtype));
+  o.parts[0] = l.take(parts_bytes(d.gate, d.d_gate != nullptr, d.T));
+  o.parts[1] = l.take(parts_bytes(d.up, d.d_up != nullptr, d.T));
+  o.parts[2] = l.take(parts_bytes(d.down, d.d_down != nullptr, d.T));
   o.dgu = l.take(T * 2 * F * 2);
   o.total = l.at;
   return o;
 }
 
-// One tile gradient's place: its fp32 sums (the result itself, or workspace) and
-// its bf16 result.
-struct Grad {
-  float* sums = nullptr;
-  void* rounded = nullptr;
-  int64_t n = 0;
-};
-static Grad grad_of(const BellMxEll& w, void* out, int32_t dtype, char* ws) {
-  if (!out) return Grad{};
+// One tile gradient's place: its fp32 sums (the result itself, or workspace),
+// the parts of those that CTAs share, and its bf16 result.
+static TileGrad grad_of(int64_t T, const BellMxEll& w, const int32_t* cols, void* out, int32_t dtype, char* ws,
+                        size_t sums, size_t parts) {
+  TileGrad g{};
+  if (!out) return g;
   const bool half = dtype == BELL_DTYPE_BF16;
-  return Grad{half ? reinterpret_cast<float*>(ws) : static_cast<float*>(out), half ? out : nullptr,
-              int64_t(w.R) * w.K * w.B * w.B};
+  g.sums = half ? reinterpret_cast<float*>(ws + sums) : static_cast<float*>(out);
+  g.rounded = half ? out : nullptr;
+  g.cols = cols;
+  g.R = w.R, g.C = T > 0 ? w.C : 0, g.K = w.K, g.B = w.B;
+  int sms = 0;
+  if (!parts_bytes(w, true, T) || device_sm_count(&sms)) return g;
+  g.parts = reinterpret_cast<float*>(ws + parts);
+  g.cuts = sddmm_cuts(T, w.R, w.C, w.K, w.B, std::min(sms, kMaxParts));
+  return g;
 }
 
 static int tile_grad(int64_t T, const void* a, const void* b, int64_t ldb, const int32_t* cols, const BellMxEll& w,
-                     int32_t layout, const Grad& g, int32_t* status, void* stream) {
-  if (!g.sums) return BELL_OK;
+                     int32_t layout, const TileGrad& g, int32_t* status, void* stream) {
+  if (!g.sums || T == 0) return BELL_OK;
   BellSddmmDesc s{};
   s.T = T;
   s.a = a;
@@ -102,20 +115,9 @@ static int tile_grad(int64_t T, const void* a, const void* b, int64_t ldb, const
   s.K = w.K;
   s.B = w.B;
   s.layout = layout;
-  s.accumulate = 1;  // onto the zeros written with the unpacked operands
   s.grad = g.sums;
   s.status = status;
-  return bell_sddmm_bf16(&s, stream);
-}
-
-static int round_all(const Grad (&g)[3], cudaStream_t s) {
-  RoundArgs a{};
-  for (int i = 0; i < 3; ++i) {
-    a.src[i] = g[i].sums;
-    a.dst[i] = g[i].rounded;
-    a.n[i] = g[i].rounded ? g[i].n : 0;
-  }
-  return round_sums(a, s);
+  return sddmm_bf16(&s, true, const_cast<float*>(g.parts), stream);
 }
 
 static int product(int64_t T, const void* x, const BellEll& w, const void* residual, void* out, int32_t out_dtype,
@@ -180,23 +182,22 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   const mx::BwdWs o = mx::linear_ws(*d);
   const bool want_dx = d->dx && d->T > 0;
   const int32_t in_f = w.C * w.B;
-  const mx::Grad grads[3] = {mx::grad_of(w, d->dw, d->grad_dtype, ws + o.grads[0]), {}, {}};
+  const mx::FinishArgs grads{{mx::grad_of(d->T, w, d->col_indices, d->dw, d->grad_dtype, ws, o.grads[0], o.parts[0]), {}, {}}};
   mx::ExpandArgs e{};
   e.T = d->T;
   e.B = w.B;
   if (want_dx)
     e.gather[0] = {w.chunks, int64_t(w.R) * w.K, nullptr, 0, d->index_t, int64_t(w.C) * d->K_t, ws + o.tiles};
   if (d->dw && d->T > 0) e.rows[0] = {d->x, in_f, ws + o.rows};
-  e.zero[0] = {grads[0].sums, grads[0].n};
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dx) {
     const BellEll wt{ws + o.tiles, d->cols_t, w.C, w.R, d->K_t, w.B, BELL_TILE_IN_OUT, 0};
     if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream)) return rc;
   }
-  if (int rc = mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, grads[0],
+  if (int rc = mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, grads.g[0],
                              d->status, stream))
     return rc;
-  return mx::round_all(grads, s);
+  return mx::finish_grads(grads, s);
 }
 
 size_t bell_swiglu_bwd_mx_workspace_bytes(const BellMxFFNBwdDesc* d) {
@@ -237,9 +238,9 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   const int64_t T = d->T;
   const bool want_dgu = T > 0 && (d->dx || d->d_gate || d->d_up), want_dx = T > 0 && d->dx;
   char *dgu = ws + o.dgu, *mid = ws + o.mid;
-  const mx::Grad grads[3] = {mx::grad_of(g, d->d_gate, d->gate_dtype, ws + o.grads[0]),
-                             mx::grad_of(u, d->d_up, d->up_dtype, ws + o.grads[1]),
-                             mx::grad_of(w, d->d_down, d->down_dtype, ws + o.grads[2])};
+  const mx::FinishArgs grads{{mx::grad_of(T, g, d->cols_gate, d->d_gate, d->gate_dtype, ws, o.grads[0], o.parts[0]),
+                              mx::grad_of(T, u, d->cols_up, d->d_up, d->up_dtype, ws, o.grads[1], o.parts[1]),
+                              mx::grad_of(T, w, d->cols_down, d->d_down, d->down_dtype, ws, o.grads[2], o.parts[2])}};
   mx::ExpandArgs e{};
   e.T = T;
   e.B = g.B;
@@ -250,7 +251,6 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     e.gather[1] = {g.chunks, int64_t(g.R) * g.K, u.chunks, int64_t(u.R) * u.K, d->index_t_gate_up,
                    int64_t(g.C) * d->K_t_gate_up, ws + o.tiles};
   if (T > 0 && (d->d_gate || d->d_up)) e.rows[0] = {d->x, D, ws + o.rows};
-  for (int i = 0; i < 3; ++i) e.zero[i] = {grads[i].sums, grads[i].n};
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dgu) {
     const BellEll wt{ws + o.tiles_down, d->cols_t_down, g.R, w.R, d->K_t_down, g.B, BELL_TILE_IN_OUT, 0};
@@ -262,15 +262,15 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream))
       return rc;
   }
-  if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads[0], d->status, stream))
+  if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads.g[0], d->status, stream))
     return rc;
-  if (int rc = mx::tile_grad(T, ws + o.rows, dgu + size_t(F) * 2, int64_t(F) * 2, d->cols_up, u, d->layout, grads[1],
+  if (int rc = mx::tile_grad(T, ws + o.rows, dgu + size_t(F) * 2, int64_t(F) * 2, d->cols_up, u, d->layout, grads.g[1],
                              d->status, stream))
     return rc;
   if (T > 0 && d->d_down)
     if (int rc = bell_mx_dequantize_rows(T, F, g.B, d->h, BELL_DTYPE_BF16, mid, F, stream)) return rc;
-  if (int rc = mx::tile_grad(T, mid, d->grad_out, D, d->cols_down, w, d->layout, grads[2], d->status, stream)) return rc;
-  return mx::round_all(grads, s);
+  if (int rc = mx::tile_grad(T, mid, d->grad_out, D, d->cols_down, w, d->layout, grads.g[2], d->status, stream)) return rc;
+  return mx::finish_grads(grads, s);
 }
 
 }  // extern "C"

@@ -19,8 +19,9 @@ saturates.  A block that holds an infinity or a NaN is NaN throughout.
 * ``mxfp4_linear_ad``, ``mxfp4_swiglu``: the same, differentiable.  The
   gradient passes straight through Q: the backward is the bf16 one at the
   quantised operands (their values are exact in bf16).  Tile
-  gradients are fp32 sums of token ranges that meet in arrival order: their
-  last bits may differ from run to run.  A weight's first backward builds its
+  gradients are fp32 sums of token ranges added in a fixed order, which
+  depends on the sizes and the device's SMs: they are the same on every run.
+  A weight's first backward builds its
   transposed topology and waits for the device once: before a step is captured
   in a graph, run one, and let no autograd graph of the same leaves live on.
 

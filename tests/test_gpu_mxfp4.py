@@ -799,3 +799,50 @@ def test_two_host_threads():
     for t in threads:
         t.join()
     assert not wrong and K.read_status() == 0
+
+
+def tile_errors(grad, ref, cols, B, layout):
+    """Each live tile's error norm over its reference's; ref is the dense gradient on the device, float64."""
+    R, Kk = cols.shape
+    dense = ref.reshape(R, B, -1, B).permute(0, 2, 3, 1)  # [R, C, B_in, B_out]
+    want = dense[torch.arange(R, device="cuda")[:, None], cols.clamp(min=0).long()]
+    got = grad.double() if layout == 0 else grad.double().transpose(-1, -2)
+    e = (torch.linalg.vector_norm(got - want, dim=(-1, -2)) / torch.linalg.vector_norm(want, dim=(-1, -2)))
+    return e[cols >= 0]
+
+
+@pytest.mark.parametrize("T,R,C,Kk,B,dead,layout,dtype", [
+    (64, 8, 4, 3, 64, 1, 0, BF16), (777, 16, 16, 4, 64, 3, 0, BF16), (777, 16, 16, 7, 64, 3, 1, F32),
+    (5000, 128, 32, 2, 64, 9, 0, BF16), (1000, 8, 8, 3, 128, 2, 0, BF16), (1000, 8, 8, 5, 128, 2, 1, F32),
+    (2600, 128, 32, 3, 128, 9, 1, BF16), (2047, 1, 2, 1, 128, 0, 0, BF16), (2047, 1, 3, 2, 64, 0, 1, BF16)])
+def test_tile_gradients_repeat_exactly(T, R, C, Kk, B, dead, layout, dtype):
+    K = _K()
+    rng = np.random.default_rng(T + B)
+    v, cols, _ = weight(rng, R, C, Kk, B, dead, dtype=dtype, layout=layout)
+    x, dy = rows(rng, T, C * B), rows(rng, T, R * B)
+    v.requires_grad_(True)
+    y = K.mxfp4_linear_ad(x, v, cols, layout=layout)
+    grads = [torch.autograd.grad(y, v, dy, retain_graph=True)[0] for _ in range(8)]
+    for g in grads[1:]:
+        assert torch.equal(g, grads[0])
+    xq = K.mxfp4_dequantize(K.mxfp4_quantize(x, B), F32).double()
+    assert tile_errors(grads[0], dy.double().T @ xq, cols, B, layout).max() <= GRAD_TOL
+    assert (grads[0][cols < 0] == 0).all()
+    assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("T,d,F,B,Kg,Kd", [(777, 1024, 4096, 64, 4, 16), (1000, 1024, 4096, 128, 3, 6)])
+def test_a_training_step_repeats_exactly(T, d, F, B, Kg, Kd):
+    K = _K()
+    rng = np.random.default_rng(T)
+    mats, _ = _ffn(rng, d, F, B, Kg, Kd, 3)
+    x, dy = rows(rng, T, d), rows(rng, T, d)
+    leaves = [x] + [m[0] for m in mats]
+    for t in leaves:
+        t.requires_grad_(True)
+    first = None
+    for _ in range(6):
+        y = K.mxfp4_swiglu(x, *(a for m in mats for a in m[:2]), add_residual=True)
+        got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))

@@ -416,6 +416,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
  * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
  * of up, and its tiles, counted after gate's); each K_t at most 254.  Results
  * that are NULL are not computed.  With add_residual, dx includes grad_out.
+ * The workspace is 32-byte aligned.
  */
 typedef struct BellMxFFNBwdDesc {
   int64_t T;

@@ -16,6 +16,7 @@
 // unpacked operands live in the workspace only during the call; Q(h) takes the
 // place of d_h once that has been read.
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 
 #include "bell_mx.cuh"
@@ -139,7 +140,8 @@ static int product(int64_t T, const void* x, const BellEll& w, const void* resid
 static int check_weight(const BellMxEll& w, const char* name) {
   if (!w.chunks) return fail(BELL_ERR_ARG, std::string(name) + ": NULL chunks");
   if (w.B != 64 && w.B != 128) return fail(BELL_ERR_SHAPE, std::string(name) + ": tile size B must be 64 or 128");
-  if (w.R < 1 || w.C < 1 || w.K < 1) return fail(BELL_ERR_SHAPE, std::string(name) + ": R, C, K must be >= 1");
+  if (w.R < 1 || w.C < 1 || w.K < 1 || w.R > (1 << 23) || w.C > 65535 || w.K > 65535)
+    return fail(BELL_ERR_SHAPE, std::string(name) + ": R, C, K must be >= 1, R <= 2^23 and C, K <= 65535");
   return BELL_OK;
 }
 
@@ -149,6 +151,26 @@ static int check_k_t(int32_t k_t, const char* name) {
     return fail(BELL_ERR_SHAPE, std::string(name) + ": a column block is used by " + std::to_string(k_t) +
                                     " block-rows; the backward takes at most 254");
   return BELL_OK;
+}
+
+// The kernels' widest accesses: 32 bytes in the gated backward's workspace, 16 in
+// rows, chunks and results, and each index's own size.
+static bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+static int check_aligned(std::initializer_list<const void*> by16, std::initializer_list<const void*> by8,
+                         std::initializer_list<const void*> by4, const void* workspace, uintptr_t n) {
+  if (!workspace || !aligned_to(workspace, n))
+    return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned to " + std::to_string(n) + " bytes");
+  for (const void* p : by16)
+    if (!aligned16(p)) return fail(BELL_ERR_ALIGN, "rows, chunks, plans and results must be 16-byte aligned");
+  for (const void* p : by8)
+    if (!aligned_to(p, 8)) return fail(BELL_ERR_ALIGN, "index_t must be 8-byte aligned");
+  for (const void* p : by4)
+    if (!aligned_to(p, 4)) return fail(BELL_ERR_ALIGN, "column indices must be 4-byte aligned");
+  return BELL_OK;
+}
+
+static int check_layout(int32_t layout) {
+  return layout == BELL_TILE_IN_OUT || layout == BELL_TILE_OUT_IN ? BELL_OK : fail(BELL_ERR_ARG, "unknown tile layout");
 }
 
 static bool grad_type(int32_t t) { return t == BELL_DTYPE_BF16 || t == BELL_DTYPE_F32; }
@@ -175,7 +197,10 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
     if (int rc = mx::check_k_t(d->K_t, "weight")) return rc;
   if (d->dw && (!d->col_indices || !mx::grad_type(d->grad_dtype)))
     return fail(BELL_ERR_ARG, "dw needs col_indices and a bf16 or f32 grad_dtype");
-  if (!d->workspace || !aligned16(d->workspace)) return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned");
+  if (int rc = mx::check_layout(d->layout)) return rc;
+  if (int rc = mx::check_aligned({d->grad_out, d->x, w.chunks, d->dx, d->dw}, {d->index_t}, {d->col_indices, d->cols_t},
+                                 d->workspace, 16))
+    return rc;
   if (int rc = require_sm100()) return rc;
   char* ws = static_cast<char*>(d->workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -229,7 +254,13 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
       (d->d_up && (!d->cols_up || !mx::grad_type(d->up_dtype))) ||
       (d->d_down && (!d->cols_down || !mx::grad_type(d->down_dtype))))
     return fail(BELL_ERR_ARG, "a tile gradient needs its col_indices and a bf16 or f32 type");
-  if (!d->workspace || !aligned16(d->workspace)) return fail(BELL_ERR_ALIGN, "workspace must be non-NULL and aligned");
+  if (int rc = mx::check_layout(d->layout)) return rc;
+  if (int rc = mx::check_aligned({d->grad_out, d->x, d->h, g.chunks, u.chunks, w.chunks, g.plan, u.plan, d->dx, d->d_gate,
+                                  d->d_up, d->d_down},
+                                 {d->index_t_down, d->index_t_gate_up},
+                                 {d->cols_gate, d->cols_up, d->cols_down, d->cols_t_down, d->cols_t_gate_up},
+                                 d->workspace, 32))
+    return rc;
   if (int rc = require_sm100()) return rc;
   char* ws = static_cast<char*>(d->workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

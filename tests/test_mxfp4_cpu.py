@@ -202,3 +202,47 @@ def test_a_copied_layer_makes_its_own_kernel_copies():
     for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
         assert "_kcache" not in other.w_gate.__dict__ and torch.equal(other.w_gate.values, m.w_gate.values)
     assert "_kcache" in m.w_gate.__dict__
+
+
+def test_backward_refuses_misaligned_buffers():
+    """Every pointer of both backwards is checked before anything is launched: the gated one's workspace for 32 bytes."""
+    L = _L()
+    lib = L.load()
+    d = L.BellMxLinearBwdDesc()
+
+    def lin(**kw):
+        d.T, d.grad_out, d.x, d.w, d.K_t = 4, 1024, 1024, _mx(L, 2, 3), 1
+        d.workspace = d.dx = d.dw = d.col_indices = d.cols_t = d.index_t = 1024
+        d.layout = d.grad_dtype = 0
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return lib.bell_linear_bwd_mx(C.byref(d), None)
+
+    for name in ("grad_out", "x", "dx", "dw", "workspace"):
+        assert lin(**{name: 1032}) == -3, name
+    assert lin(w=_mx(L, 2, 3, chunks=1032)) == -3 and lin(index_t=1028) == -3
+    assert lin(col_indices=1026) == -3 and lin(cols_t=1026) == -3
+    assert lin(layout=2) == -8 and lin(w=_mx(L, 2, 1 << 16)) == -2
+    f = L.BellMxFFNBwdDesc()
+
+    def ffn(**kw):
+        f.T, f.gate, f.up, f.down = 4, _mx(L, 4, 2), _mx(L, 4, 2), _mx(L, 2, 4)
+        for n in ("grad_out", "x", "h", "workspace", "cols_gate", "cols_up", "cols_down", "cols_t_down", "index_t_down",
+                  "cols_t_gate_up", "index_t_gate_up", "dx", "d_gate", "d_up", "d_down"):
+            setattr(f, n, 1024)
+        f.K_t_down = f.K_t_gate_up = 1
+        f.layout = 0
+        for k, v in kw.items():
+            setattr(f, k, v)
+        return lib.bell_swiglu_bwd_mx(C.byref(f), None)
+
+    assert ffn(workspace=1024 + 16) == -3 and "32" in L.last_error()
+    for name in ("grad_out", "x", "h", "dx", "d_gate", "d_up", "d_down", "workspace"):
+        assert ffn(**{name: 1032}) == -3, name
+    for name, m in (("gate", _mx(L, 4, 2, chunks=1032)), ("up", _mx(L, 4, 2, plan=1032)), ("down", _mx(L, 2, 4, chunks=1032))):
+        assert ffn(**{name: m}) == -3, name
+    for name in ("index_t_down", "index_t_gate_up"):
+        assert ffn(**{name: 1028}) == -3, name
+    for name in ("cols_gate", "cols_up", "cols_down", "cols_t_down", "cols_t_gate_up"):
+        assert ffn(**{name: 1026}) == -3, name
+    assert ffn(layout=-1) == -8

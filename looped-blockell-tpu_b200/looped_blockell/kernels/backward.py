@@ -35,10 +35,11 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
+from ..made import Made, capturing
 from . import _lib
 from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _ell, _stream, block_ell_linear, plan_bytes
 
-# (C_blocks, ids of the column-index tensors) -> (weak references, versions, result).
+# (C_blocks, ids of the column-index tensors) -> (weak references, versions, result, Made).
 # A hit needs the very same tensor objects (alive) at the same version: a new
 # tensor that happens to reuse a freed tensor's memory or id never matches.
 _TOPO_CACHE: "OrderedDict[tuple, tuple]" = OrderedDict()
@@ -50,9 +51,10 @@ def _topo_lookup(mats: Sequence[torch.Tensor], C_blocks: int):
     hit = _TOPO_CACHE.get(key)
     if hit is None:
         return key, None
-    refs, versions, result = hit
+    refs, versions, result, made = hit
     if all(r() is m for r, m in zip(refs, mats)) and versions == tuple(m._version for m in mats):
         _TOPO_CACHE.move_to_end(key)
+        made.use()
         return key, result
     del _TOPO_CACHE[key]
     return key, None
@@ -102,13 +104,14 @@ def transposed_topology(mats: Sequence[torch.Tensor], C_blocks: int) -> Tuple[to
     tile_idx = torch.zeros((C_blocks, K_t), dtype=torch.long, device=dev)
     cols_t[grp_s[keep], pos[keep]] = r_s[keep].to(torch.int32)
     tile_idx[grp_s[keep], pos[keep]] = t_s[keep]
-    _TOPO_CACHE[key] = (tuple(weakref.ref(m) for m in mats), tuple(m._version for m in mats), (cols_t, tile_idx))
+    _TOPO_CACHE[key] = (tuple(weakref.ref(m) for m in mats), tuple(m._version for m in mats), (cols_t, tile_idx),
+                        Made(cols_t, tile_idx))
     while len(_TOPO_CACHE) > _TOPO_CACHE_MAX:
         _TOPO_CACHE.popitem(last=False)
     return cols_t, tile_idx
 
 
-# (ids of the value and column tensors, C_blocks) -> (weak refs, versions, values_t):
+# (ids of the value and column tensors, C_blocks) -> (weak refs, versions, values_t, Made):
 # the gathered tiles of a transposed weight, reused while the same tensors
 # keep the same contents (the optimizer bumps the version of what it updates)
 _TILE_CACHE: "OrderedDict[tuple, tuple]" = OrderedDict()
@@ -131,15 +134,18 @@ def transpose_ell(values: Sequence[torch.Tensor], cols: Sequence[torch.Tensor], 
     key = (C_blocks,) + tuple(id(m) for m in mats)
     hit = _TILE_CACHE.get(key)
     if hit is not None:
-        refs, versions, values_t = hit
+        refs, versions, values_t, made = hit
         if all(r() is m for r, m in zip(refs, mats)) and versions == tuple(m._version for m in mats):
             _TILE_CACHE.move_to_end(key)
+            made.use()
             return values_t, cols_t, lay_t
         del _TILE_CACHE[key]
     B = values[0].shape[-1]
     flat = torch.cat([v.reshape(-1, B, B) for v in values]) if len(values) > 1 else values[0].reshape(-1, B, B)
     values_t = flat.index_select(0, tile_idx.reshape(-1)).view(cols_t.shape[0], cols_t.shape[1], B, B)
-    _TILE_CACHE[key] = (tuple(weakref.ref(m) for m in mats), tuple(m._version for m in mats), values_t)
+    if capturing(values_t):
+        return values_t, cols_t, lay_t
+    _TILE_CACHE[key] = (tuple(weakref.ref(m) for m in mats), tuple(m._version for m in mats), values_t, Made(values_t))
     while len(_TILE_CACHE) > _TILE_CACHE_MAX:
         _TILE_CACHE.popitem(last=False)
     return values_t, cols_t, lay_t

@@ -1,0 +1,38 @@
+"""Device tensors that a cache hands out, on whatever stream asks for them."""
+
+from __future__ import annotations
+
+import torch
+
+
+def capturing(t: torch.Tensor) -> bool:
+    """Whether work on ``t`` is being captured: what is made then holds nothing until a replay."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+class Made:
+    """The tensors of one cache entry, made by work on the current stream (not
+    while it is captured).  ``use`` before each further use: another stream
+    waits for that work, and the memory is not reused before that stream's own.
+    In a capture it does neither: a graph cannot wait for work outside it, so a
+    capture begins after what was made before it (``torch.cuda.graph``
+    synchronises first)."""
+
+    __slots__ = ("tensors", "stream", "event")
+
+    def __init__(self, *tensors: torch.Tensor):
+        self.tensors = tensors if tensors[0].is_cuda else ()
+        if self.tensors:
+            s = torch.cuda.current_stream(tensors[0].device)
+            self.stream, self.event = s.cuda_stream, s.record_event()
+
+    def use(self) -> None:
+        if not self.tensors:
+            return
+        dev = self.tensors[0].device
+        if torch._C._cuda_getCurrentRawStream(dev.index) == self.stream or torch.cuda.is_current_stream_capturing():
+            return
+        s = torch.cuda.current_stream(dev)
+        s.wait_event(self.event)
+        for t in self.tensors:
+            t.record_stream(s)

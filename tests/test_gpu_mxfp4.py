@@ -846,3 +846,45 @@ def test_a_training_step_repeats_exactly(T, d, F, B, Kg, Kd):
         got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+def _busy():
+    a = torch.randn(4000, 4000, device="cuda")
+    for _ in range(30):
+        a = a @ a * 1e-3
+    return a
+
+
+def test_gradients_on_a_second_stream():
+    """A topology that is still being written on one stream is whole on the next stream that uses it."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    K = _K()
+    rng = np.random.default_rng(30)
+    mats, _ = _ffn(rng, 1024, 2048, 64, 4, 16)
+    x, dy = rows(rng, 60, 1024), rows(rng, 60, 1024)
+
+    class BehindOtherWork(TorchDispatchMode):  # the topology's last kernels
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func is torch.ops.aten.index_put_.default:
+                _busy()
+            return func(*args, **(kwargs or {}))
+
+    def step(cols):
+        ls = [t.detach().requires_grad_(True) for t in [x] + [m[0] for m in mats]]
+        y = K.mxfp4_swiglu(ls[0], ls[1], cols[0], ls[2], cols[1], ls[3], cols[2])
+        return torch.autograd.grad(y, ls, dy)
+
+    want = step([m[1] for m in mats])
+    _busy()
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        cols = [m[1].clone() for m in mats]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s), BehindOtherWork():
+            K.transposed_topology([cols[2]], 32)
+            K.transposed_topology(cols[:2], 16)
+        with torch.cuda.stream(t):
+            got = step(cols)
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))

@@ -31,6 +31,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..made import Made, capturing
 from .block_ell import BlockELLConfig, BlockELLTensor, create_random_topology
 
 
@@ -74,15 +75,19 @@ class BlockELLLinear(nn.Module):
         """Drop the cached kernel copies (after writes through ``.data``)."""
         self._kcache = {}
 
-    def _cached(self, name, key, make):
+    def _cached(self, name, key, make, device_tensor=lambda value: value):
+        """``make()``, kept until ``key`` changes and ordered before its use on other streams; ``device_tensor`` of it
+        is what the device wrote."""
         cache = self.__dict__.setdefault("_kcache", {})
         hit = cache.get(name)
-        if hit is None or hit[0] != key:
-            hit = (key, make())
-            # made during a capture it holds nothing until a replay
-            if not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
-                cache[name] = hit
-        return hit[1]
+        if hit is not None and hit[0] == key:
+            hit[2].use()
+            return hit[1]
+        value = make()
+        t = device_tensor(value)
+        if not capturing(t):
+            cache[name] = (key, value, Made(t))
+        return value
 
     def __getstate__(self):  # copies and pickles make their own kernel copies
         state = self.__dict__.copy()
@@ -116,17 +121,9 @@ class BlockELLLinear(nn.Module):
         if not v.is_cuda or torch.cuda.is_current_stream_capturing():
             return make_mxfp4(v.detach(), cols, self.C)
         key = (v.data_ptr(), v._version, v.dtype, cols.data_ptr(), cols._version)
-        stream = torch.cuda.current_stream(v.device)
-
-        def make():  # with the tensors that the key's addresses belong to
-            w = make_mxfp4(v.detach(), cols, self.C)
-            return w, stream, stream.record_event(), v.detach(), cols
-
-        w, made_on, ready, *_ = self._cached("mxfp4", key, make)
-        if stream != made_on:
-            stream.wait_event(ready)
-            w.data.record_stream(stream)
-        return w
+        # kept with the tensors that the key's addresses belong to
+        return self._cached("mxfp4", key, lambda: (make_mxfp4(v.detach(), cols, self.C), v.detach(), cols),
+                            lambda value: value[0].data)[0]
 
     def as_block_ell(self) -> BlockELLTensor:
         return BlockELLTensor(values=self.kernel_values(), col_indices=self.effective_col_indices(), config=self.config)

@@ -888,3 +888,39 @@ def test_gradients_on_a_second_stream():
             got = step(cols)
         torch.cuda.synchronize()
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_a_layers_columns_on_a_second_stream(train):
+    """Masked columns made behind queued work on one stream, used on another by a layer whose weight changed."""
+    x = torch.randn(40, 256, device="cuda", dtype=BF16)
+    dy = torch.randn(40, 256, device="cuda", dtype=BF16)
+
+    def run(m):
+        if not train:
+            with torch.no_grad():
+                return [m(x)]
+        y = m(x)
+        return [y.detach(), *torch.autograd.grad(y, [m.w_gate.values, m.w_down.values], dy)]
+
+    ref = _block()
+    with torch.no_grad():
+        ref.w_up.alive_mask[1:, 0] = False
+        ref.w_gate.alive_mask[1:, 1] = False
+    want = run(ref)
+    s = torch.cuda.Stream()
+    for _ in range(5):
+        m = _block()
+        with torch.no_grad():
+            m.w_up.alive_mask[1:, 0] = False
+            m.w_gate.alive_mask[1:, 1] = False
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            keep = _busy()
+            for w in (m.w_gate, m.w_up, m.w_down):
+                w.effective_col_indices()
+        got = run(m)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        del keep

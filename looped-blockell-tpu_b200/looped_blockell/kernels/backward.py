@@ -41,9 +41,10 @@ from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _ell, _strea
 
 # (C_blocks, ids of the column-index tensors) -> (weak references, versions, result, Made).
 # A hit needs the very same tensor objects (alive) at the same version: a new
-# tensor that happens to reuse a freed tensor's memory or id never matches.
-_TOPO_CACHE: "OrderedDict[tuple, tuple]" = OrderedDict()
-_TOPO_CACHE_MAX = 16
+# tensor that happens to reuse a freed tensor's memory or id never matches.  An
+# entry lives as long as its column-index tensors, so however many weights a
+# model has, a step after the first builds none.
+_TOPO_CACHE: dict = {}
 
 
 def _topo_lookup(mats: Sequence[torch.Tensor], C_blocks: int):
@@ -53,10 +54,9 @@ def _topo_lookup(mats: Sequence[torch.Tensor], C_blocks: int):
         return key, None
     refs, versions, result, made = hit
     if all(r() is m for r, m in zip(refs, mats)) and versions == tuple(m._version for m in mats):
-        _TOPO_CACHE.move_to_end(key)
         made.use()
         return key, result
-    del _TOPO_CACHE[key]
+    _TOPO_CACHE.pop(key, None)
     return key, None
 
 
@@ -70,7 +70,8 @@ def transposed_topology(mats: Sequence[torch.Tensor], C_blocks: int) -> Tuple[to
     kept), and ``tile_idx`` the position of that tile in the concatenation of
     the flattened value tensors.  Padding slots hold column -1 and tile 0.
     Dead slots (-1) and indices outside [0, C_blocks) are left out.  One
-    device-to-host read (the maximum column count) sizes K_t.
+    device-to-host read (the largest and the sum of the column counts) sizes
+    K_t.  Kept while the ``mats`` live and stay as they are.
     """
     key, hit = _topo_lookup(mats, C_blocks)
     if hit is not None:
@@ -96,18 +97,21 @@ def transposed_topology(mats: Sequence[torch.Tensor], C_blocks: int) -> Tuple[to
     order = torch.argsort(grp * max(n, 1) + t)
     grp_s, r_s, t_s = grp[order], r[order], t[order]
     counts = torch.zeros(C_blocks + 1, dtype=torch.long, device=dev).scatter_add_(0, grp, torch.ones_like(grp))
-    K_t = max(1, int(counts[:C_blocks].max().item())) if C_blocks > 0 and n > 0 else 1
+    K_t, used = torch.stack((counts[:C_blocks].max(), counts[:C_blocks].sum())).tolist() if C_blocks > 0 else (0, 0)
+    K_t = max(1, K_t)
     starts = torch.cumsum(counts, 0) - counts
     pos = torch.arange(n, device=dev, dtype=torch.long) - starts[grp_s]
-    keep = grp_s < C_blocks
     cols_t = torch.full((C_blocks, K_t), -1, dtype=torch.int32, device=dev)
     tile_idx = torch.zeros((C_blocks, K_t), dtype=torch.long, device=dev)
-    cols_t[grp_s[keep], pos[keep]] = r_s[keep].to(torch.int32)
-    tile_idx[grp_s[keep], pos[keep]] = t_s[keep]
-    _TOPO_CACHE[key] = (tuple(weakref.ref(m) for m in mats), tuple(m._version for m in mats), (cols_t, tile_idx),
-                        Made(cols_t, tile_idx))
-    while len(_TOPO_CACHE) > _TOPO_CACHE_MAX:
-        _TOPO_CACHE.popitem(last=False)
+    at = (grp_s[:used], pos[:used])  # what is left out was sorted last
+    cols_t[at] = r_s[:used].to(torch.int32)
+    tile_idx[at] = t_s[:used]
+
+    def forget(_, key=key, pop=_TOPO_CACHE.pop):
+        pop(key, None)
+
+    _TOPO_CACHE[key] = (tuple(weakref.ref(m, forget) for m in mats), tuple(m._version for m in mats),
+                        (cols_t, tile_idx), Made(cols_t, tile_idx))
     return cols_t, tile_idx
 
 

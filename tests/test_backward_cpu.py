@@ -115,3 +115,27 @@ def test_transpose_ell_caches_tiles_per_weight_version():
     d = transpose_ell([v], [c], 3)
     assert d[0] is not a[0]
     assert torch.equal(d[0], a[0] * 2.0)
+
+
+def test_topologies_live_as_long_as_their_columns():
+    """However many weights there are, a second look-up builds nothing; an entry goes with its tensors."""
+    import gc
+    K = _K()
+    from looped_blockell.kernels.backward import _TOPO_CACHE
+    mats = [torch.tensor([[0, 1], [1, i % 2]], dtype=torch.int32) for i in range(60)]
+    before = len(_TOPO_CACHE)
+    first = [K.transposed_topology([a, b], 2)[0] for a, b in zip(mats, mats[1:])]
+    assert len(_TOPO_CACHE) == before + 59
+    assert all(K.transposed_topology([a, b], 2)[0] is t for a, b, t in zip(mats, mats[1:], first))
+    del mats[30:]
+    a = b = None
+    gc.collect()
+    assert len(_TOPO_CACHE) == before + 29
+
+
+def test_transposed_topology_of_nothing():
+    K = _K()
+    for cols, C in ((torch.full((2, 2), -1, dtype=torch.int32), 3), (torch.zeros(0, 2, dtype=torch.int32), 2),
+                    (torch.tensor([[7]], dtype=torch.int32), 2)):
+        ct, idx = K.transposed_topology([cols], C)
+        assert ct.tolist() == [[-1]] * C and idx.tolist() == [[0]] * C

@@ -924,3 +924,30 @@ def test_a_layers_columns_on_a_second_stream(train):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
         del keep
+
+
+def test_twelve_blocks_train_from_a_graph():
+    """The topologies of many blocks stay: a second step builds none, and can be captured."""
+    K = _K()
+    rng = np.random.default_rng(31)
+    blocks = [_ffn(rng)[0] for _ in range(12)]
+    x, dy = rows(rng, 40, 256, spread=0.5), rows(rng, 40, 256)
+    leaves = [x] + [m[0] for b in blocks for m in b]
+
+    def step():
+        ls = [t.detach().requires_grad_(True) for t in leaves]
+        y = ls[0]
+        for i, b in enumerate(blocks):
+            vs = ls[1 + 3 * i:4 + 3 * i]
+            y = K.mxfp4_swiglu(y, vs[0], b[0][1], vs[1], b[1][1], vs[2], b[2][1], add_residual=True)
+        return (y.detach(), *torch.autograd.grad(y, ls, dy))
+
+    want = step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -415,8 +415,9 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
  * transposed topology of down [d_ff/B, K_t_down]; cols_t_gate_up /
  * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
  * of up, and its tiles, counted after gate's); each K_t at most 254.  Results
- * that are NULL are not computed.  With add_residual, dx includes grad_out.
- * The workspace is 32-byte aligned.
+ * that are NULL are not computed: d_down alone needs neither topology, the
+ * gradients of tiles alone not that of gate and up.  With add_residual, dx
+ * includes grad_out.  The workspace is 32-byte aligned.
  */
 typedef struct BellMxFFNBwdDesc {
   int64_t T;

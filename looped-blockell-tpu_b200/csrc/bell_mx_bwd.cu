@@ -46,6 +46,11 @@ static size_t sums_bytes(const BellMxEll& w, bool wanted, int32_t dtype) {
   return wanted && dtype == BELL_DTYPE_BF16 ? size_t(w.R) * w.K * w.B * w.B * 4 : 0;
 }
 
+// Which transposed topologies a call needs: down's for d_gate and d_up, that of
+// gate and up for dx.
+static bool needs_down_t(const BellMxFFNBwdDesc& d) { return d.dx || d.d_gate || d.d_up || !d.d_down; }
+static bool needs_gate_up_t(const BellMxFFNBwdDesc& d) { return d.dx || !(d.d_gate || d.d_up || d.d_down); }
+
 static size_t parts_bytes(const BellMxEll& w, bool wanted, int64_t T) {
   return wanted ? sddmm_parts_bytes(T, w.R, w.C, w.K, w.B) : 0;
 }
@@ -67,9 +72,10 @@ static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
   const size_t BB = size_t(g.B) * g.B, F = size_t(g.R) * g.B, T = size_t(d.T);
   BwdWs o{};
   Layout l;
-  o.tiles_down = l.take(size_t(g.R) * d.K_t_down * BB * 2);
-  o.tiles = l.take(size_t(g.C) * d.K_t_gate_up * BB * 2);
-  o.plan = l.take(std::max(bell_plan_bytes(0, 0, 0, g.R, d.K_t_down), bell_plan_bytes(0, 0, 0, g.C, d.K_t_gate_up)));
+  const int32_t kd = needs_down_t(d) ? d.K_t_down : 0, kg = needs_gate_up_t(d) ? d.K_t_gate_up : 0;
+  o.tiles_down = l.take(size_t(g.R) * kd * BB * 2);
+  o.tiles = l.take(size_t(g.C) * kg * BB * 2);
+  o.plan = l.take(std::max(bell_plan_bytes(0, 0, 0, g.R, kd), bell_plan_bytes(0, 0, 0, g.C, kg)));
   o.rows = l.take(T * g.C * g.B * 2);
   o.mid = l.take(T * F * 4);
   o.grads[0] = l.take(sums_bytes(d.gate, d.d_gate != nullptr, d.gate_dtype));
@@ -227,7 +233,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
 
 size_t bell_swiglu_bwd_mx_workspace_bytes(const BellMxFFNBwdDesc* d) {
   if (!d || mx::check_weight(d->gate, "gate") || mx::check_weight(d->up, "up") || mx::check_weight(d->down, "down") ||
-      d->T < 0 || d->K_t_down < 1 || d->K_t_gate_up < 1)
+      d->T < 0 || (mx::needs_down_t(*d) && d->K_t_down < 1) || (mx::needs_gate_up_t(*d) && d->K_t_gate_up < 1))
     return 0;
   return mx::swiglu_ws(*d).total;
 }
@@ -243,8 +249,8 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   if (d->T < 0 || d->T > (int64_t(1) << 31) - 256) return fail(BELL_ERR_SHAPE, "T must be in [0, 2^31 - 256)");
   if (d->T > 0 && (!d->grad_out || !d->x || !d->h)) return fail(BELL_ERR_ARG, "grad_out, x and h must be non-NULL");
   if (!g.plan || !u.plan) return fail(BELL_ERR_ARG, "gate and up need their plans");
-  if (!d->cols_t_down || !d->index_t_down || d->K_t_down < 1 || !d->cols_t_gate_up || !d->index_t_gate_up ||
-      d->K_t_gate_up < 1)
+  if ((mx::needs_down_t(*d) && (!d->cols_t_down || !d->index_t_down || d->K_t_down < 1)) ||
+      (mx::needs_gate_up_t(*d) && (!d->cols_t_gate_up || !d->index_t_gate_up || d->K_t_gate_up < 1)))
     return fail(BELL_ERR_ARG, "the transposed topologies must be given");
   if (d->dx || d->d_gate || d->d_up)
     if (int rc = mx::check_k_t(d->K_t_down, "down")) return rc;

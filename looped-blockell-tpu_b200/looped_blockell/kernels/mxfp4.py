@@ -465,8 +465,14 @@ class MXSwiGLUFn(torch.autograd.Function):
         dy = grad_out.to(torch.bfloat16).contiguous()
         T, dev = dy.shape[0], dy.device
         need = ctx.needs_input_grad
-        td_cols, td_index = transposed_topology([ci_down], gate.R)
-        tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
+        # transposed topologies: of down for d_gate and d_up, of gate and up for dx (the address, the address, slots)
+        td = tg = (None, None, 1)
+        if need[0] or need[1] or need[3]:
+            td_cols, td_index = transposed_topology([ci_down], gate.R)
+            td = td_cols.data_ptr(), td_index.data_ptr(), td_cols.shape[1]
+        if need[0]:
+            tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
+            tg = tg_cols.data_ptr(), tg_index.data_ptr(), tg_cols.shape[1]
         dx = torch.empty_like(dy) if need[0] else None
         # fp32 rows: the residual's gradient is added to theirs in fp32
         late = ctx.add_residual and ctx.dtypes[0] == torch.float32
@@ -475,8 +481,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         d = _lib.BellMxFFNBwdDesc(
             T, int(ctx.add_residual and not late), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
             q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
-            td_cols.data_ptr(), td_index.data_ptr(), tg_cols.data_ptr(), tg_index.data_ptr(), td_cols.shape[1],
-            tg_cols.shape[1], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
+            *td[:2], *tg[:2], td[2], tg[2], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
             grads[1][2], grads[2][2], 0, None, None)
         ws = _bytes(_lib.load().bell_swiglu_bwd_mx_workspace_bytes(C.byref(d)), dev)
         d.workspace = ws.data_ptr()

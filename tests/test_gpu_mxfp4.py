@@ -951,3 +951,23 @@ def test_twelve_blocks_train_from_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_only_the_wanted_gradients_build_topologies(monkeypatch):
+    """d_down needs none, d_gate and d_up that of down, dx both; the gradients are the same."""
+    K = _K()
+    from looped_blockell.kernels import mxfp4
+    rng = np.random.default_rng(38)
+    mats, _ = _ffn(rng)
+    x, dy = rows(rng, 70, 256), rows(rng, 70, 256)
+    built = []
+    real = mxfp4.transposed_topology
+    monkeypatch.setattr(mxfp4, "transposed_topology", lambda m, n: built.append(len(m)) or real(m, n))
+    every = None
+    for which, want in (([0, 1, 2, 3], [1, 2]), ([3], []), ([1], [1]), ([2, 3], [1]), ([0], [1, 2])):
+        ls = [t.detach().requires_grad_(i in which) for i, t in enumerate([x] + [m[0] for m in mats])]
+        built.clear()
+        y = K.mxfp4_swiglu(ls[0], ls[1], mats[0][1], ls[2], mats[1][1], ls[3], mats[2][1], add_residual=True)
+        got = dict(zip(which, torch.autograd.grad(y, [ls[i] for i in which], dy)))
+        every = every or got
+        assert built == want and all(torch.equal(g, every[i]) for i, g in got.items())

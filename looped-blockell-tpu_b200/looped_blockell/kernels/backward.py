@@ -39,11 +39,12 @@ from ..made import Made, capturing
 from . import _lib
 from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _ell, _stream, block_ell_linear, plan_bytes
 
-# (C_blocks, ids of the column-index tensors) -> (weak references, versions, result, Made).
+# (C_blocks, ids of the column-index tensors) -> (weak references, versions, result, Made, captured ones before).
 # A hit needs the very same tensor objects (alive) at the same version: a new
 # tensor that happens to reuse a freed tensor's memory or id never matches.  An
 # entry lives as long as its column-index tensors, so however many weights a
-# model has, a step after the first builds none.
+# model has, a step after the first builds none; one that a graph has captured
+# stays for that time too when they change (its replays keep that topology).
 _TOPO_CACHE: dict = {}
 
 
@@ -52,11 +53,13 @@ def _topo_lookup(mats: Sequence[torch.Tensor], C_blocks: int):
     hit = _TOPO_CACHE.get(key)
     if hit is None:
         return key, None
-    refs, versions, result, made = hit
-    if all(r() is m for r, m in zip(refs, mats)) and versions == tuple(m._version for m in mats):
-        made.use()
-        return key, result
-    _TOPO_CACHE.pop(key, None)
+    refs, versions, result, made, _ = hit
+    if all(r() is m for r, m in zip(refs, mats)):
+        if versions == tuple(m._version for m in mats):
+            made.use()
+            return key, result
+    else:
+        _TOPO_CACHE.pop(key, None)
     return key, None
 
 
@@ -110,8 +113,10 @@ def transposed_topology(mats: Sequence[torch.Tensor], C_blocks: int) -> Tuple[to
     def forget(_, key=key, pop=_TOPO_CACHE.pop):
         pop(key, None)
 
+    old = _TOPO_CACHE.get(key)  # of the same tensors, before they changed
+    captured = () if old is None else old[4] + ((old[3],) if old[3].captured else ())
     _TOPO_CACHE[key] = (tuple(weakref.ref(m, forget) for m in mats), tuple(m._version for m in mats),
-                        (cols_t, tile_idx), Made(cols_t, tile_idx))
+                        (cols_t, tile_idx), Made(cols_t, tile_idx), captured)
     return cols_t, tile_idx
 
 

@@ -73,6 +73,9 @@ class BlockELLLinear(nn.Module):
 
     def refresh(self) -> None:
         """Drop the cached kernel copies (after writes through ``.data``)."""
+        for _, _, made in self.__dict__.get("_kcache", {}).values():
+            if made.captured:
+                self.__dict__.setdefault("_kcaptured", []).append(made)
         self._kcache = {}
 
     def _cached(self, name, key, make, device_tensor=lambda value: value):
@@ -83,6 +86,8 @@ class BlockELLLinear(nn.Module):
         if hit is not None and hit[0] == key:
             hit[2].use()
             return hit[1]
+        if hit is not None and hit[2].captured:  # a graph's replays still read it
+            self.__dict__.setdefault("_kcaptured", []).append(hit[2])
         value = make()
         t = device_tensor(value)
         if not capturing(t):
@@ -92,14 +97,18 @@ class BlockELLLinear(nn.Module):
     def __getstate__(self):  # copies and pickles make their own kernel copies
         state = self.__dict__.copy()
         state.pop("_kcache", None)
+        state.pop("_kcaptured", None)
         return state
 
     def effective_col_indices(self) -> torch.Tensor:
         """col_indices with dead slots set to -1 (skipped by the kernel)."""
         ci, am = self.col_indices, self.alive_mask
         key = (ci.data_ptr(), ci._version, am.data_ptr(), am._version)
-        return self._cached("cols", key, lambda: torch.where(am, ci, torch.full_like(ci, -1)).to(torch.int32)
-                            .contiguous())
+        return self._cached("cols", key, self._masked_col_indices)
+
+    def _masked_col_indices(self) -> torch.Tensor:
+        ci = self.col_indices
+        return torch.where(self.alive_mask, ci, torch.full_like(ci, -1)).to(torch.int32).contiguous()
 
     def kernel_values(self) -> torch.Tensor:
         """The tiles the kernels read (``values`` in the compute dtype)."""
@@ -113,13 +122,14 @@ class BlockELLLinear(nn.Module):
         """The quantised weight (``kernels.MXBlockELL``) of the current parameters.
 
         While a graph is captured it is made anew, inside the graph: replays
-        then follow the parameters.  A graph that should not quantise again
+        then follow the parameters and the topology.  A graph that should not quantise again
         takes a weight made before its capture (``kernels.mxfp4_linear``,
         ``kernels.mxfp4_swiglu_fwd``)."""
         from ..kernels.mxfp4 import make_mxfp4
-        v, cols = self.values, self.effective_col_indices()
+        v = self.values
         if not v.is_cuda or torch.cuda.is_current_stream_capturing():
-            return make_mxfp4(v.detach(), cols, self.C)
+            return make_mxfp4(v.detach(), self._masked_col_indices(), self.C)
+        cols = self.effective_col_indices()
         key = (v.data_ptr(), v._version, v.dtype, cols.data_ptr(), cols._version)
         # kept with the tensors that the key's addresses belong to
         return self._cached("mxfp4", key, lambda: (make_mxfp4(v.detach(), cols, self.C), v.detach(), cols),

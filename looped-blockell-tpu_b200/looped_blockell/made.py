@@ -16,12 +16,14 @@ class Made:
     waits for that work, and the memory is not reused before that stream's own.
     In a capture it does neither: a graph cannot wait for work outside it, so a
     capture begins after what was made before it (``torch.cuda.graph``
-    synchronises first)."""
+    synchronises first).  Its replays read the memory again: what a graph has
+    ``captured`` must outlive the entry."""
 
-    __slots__ = ("tensors", "stream", "event")
+    __slots__ = ("tensors", "stream", "event", "captured")
 
     def __init__(self, *tensors: torch.Tensor):
         self.tensors = tensors if tensors[0].is_cuda else ()
+        self.captured = False
         if self.tensors:
             s = torch.cuda.current_stream(tensors[0].device)
             self.stream, self.event = s.cuda_stream, s.record_event()
@@ -29,8 +31,11 @@ class Made:
     def use(self) -> None:
         if not self.tensors:
             return
+        if torch.cuda.is_current_stream_capturing():
+            self.captured = True
+            return
         dev = self.tensors[0].device
-        if torch._C._cuda_getCurrentRawStream(dev.index) == self.stream or torch.cuda.is_current_stream_capturing():
+        if torch._C._cuda_getCurrentRawStream(dev.index) == self.stream:
             return
         s = torch.cuda.current_stream(dev)
         s.wait_event(self.event)

@@ -971,3 +971,61 @@ def test_only_the_wanted_gradients_build_topologies(monkeypatch):
         got = dict(zip(which, torch.autograd.grad(y, [ls[i] for i in which], dy)))
         every = every or got
         assert built == want and all(torch.equal(g, every[i]) for i, g in got.items())
+
+
+def _junk():
+    """Buffers of the sizes that a layer caches, filled, so that freed ones hold something else."""
+    return [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (8, 16, 32, 64, 128) for _ in range(64)]
+
+
+@torch.no_grad()
+def test_a_captured_layer_follows_its_topology():
+    """Captured with its caches filled: replays follow the mask, whatever the eager calls between have replaced."""
+    m, ref = _block(), _block()
+    x = torch.randn(40, 256, device="cuda", dtype=BF16)
+    m(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = m(x)
+    for b in (m, ref):
+        b.w_up.alive_mask[0, 0] = False
+        b.w_down.alive_mask[1, 1] = False
+    assert torch.equal(m(x), ref(x))
+    junk = _junk()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ref(x))
+    del junk
+
+
+def test_a_captured_training_step_keeps_its_topology():
+    """The columns and transposed topologies that a graph reads stay when the layer's are replaced."""
+    m = _block()
+    x, dy = (torch.randn(40, 256, device="cuda", dtype=BF16) for _ in range(2))
+    leaf = x.clone().requires_grad_(True)
+
+    def step():
+        y = m(leaf)
+        return (y.detach(), *torch.autograd.grad(y, [leaf, m.w_gate.values, m.w_up.values, m.w_down.values], dy))
+
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for how in range(3):
+        with torch.no_grad():
+            if how == 0:
+                m.w_up.alive_mask[0, 0] = False
+            elif how == 1:
+                m.w_down.alive_mask[1, 1] = False
+            else:
+                for w in (m.w_gate, m.w_up, m.w_down):
+                    w.refresh()
+        step()
+        junk = _junk()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del junk

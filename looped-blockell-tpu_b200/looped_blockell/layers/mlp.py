@@ -42,6 +42,8 @@ def _topology_seed(out_features: int, in_features: int) -> int:
 class BlockELLLinear(nn.Module):
     """Single Block-ELL linear layer (reference mlp.py:28-95)."""
 
+    weight_format = "native"  # of modules pickled before there was a choice
+
     def __init__(self, out_features: int, in_features: int, tile_size: int = 16, density: float = 1.0,
                  dtype: torch.dtype = torch.bfloat16, bias: bool = True, device=None, weight_format: str = "native"):
         super().__init__()
@@ -164,6 +166,8 @@ class MLPBlock(nn.Module):
     SwiGLU: ``w_down(silu(w_gate(x)) * w_up(x))`` as one fused forward;
     otherwise the GELU MLP ``fc2(gelu(fc1(x)))``.
     """
+
+    weight_format = "native"  # of modules pickled before there was a choice
 
     def __init__(self, d_model: int, d_ff: int, use_swiglu: bool = False, dropout: float = 0.0, tile_size: int = 16,
                  density: float = 1.0, dtype: torch.dtype = torch.bfloat16, device=None, weight_format: str = "native"):

@@ -246,3 +246,16 @@ def test_backward_refuses_misaligned_buffers():
     for name in ("cols_gate", "cols_up", "cols_down", "cols_t_down", "cols_t_gate_up"):
         assert ffn(**{name: 1026}) == -3, name
     assert ffn(layout=-1) == -8
+
+
+@pytest.mark.parametrize("swiglu", [True, False])
+def test_a_module_pickled_without_a_weight_format(swiglu):
+    """Modules from before the choice hold no such attribute: they compute as they did, in the native format."""
+    import pickle
+    from looped_blockell.layers import MLPBlock
+    m = MLPBlock(128, 256, use_swiglu=swiglu, tile_size=64)
+    for part in m.modules():
+        part.__dict__.pop("weight_format", None)
+    other = pickle.loads(pickle.dumps(m))
+    with pytest.raises(RuntimeError, match="CUDA"):  # the forward reaches the kernels, which need a GPU
+        other(torch.zeros(1, 128))

@@ -336,9 +336,12 @@ def mxfp4_swiglu_fwd(x: Union[torch.Tensor, MXRows], gate: MXBlockELL, up: MXBlo
 
     ``x`` is ``[T, d_model]`` bf16 or fp32 (the output's dtype too), or
     quantised rows (bf16 output; a ``residual`` must then be given for
-    ``add_residual``).  ``return_intermediates`` returns ``(out, ws)``, ``ws``
+    ``add_residual``).  ``residual`` stands for x there and needs
+    ``add_residual``.  ``return_intermediates`` returns ``(out, ws)``, ``ws``
     with the quantised rows ``q_x`` and ``q_h`` (``MXRows``) and the bf16
     projections ``gate`` and ``up``."""
+    if residual is not None and not add_residual:
+        raise RuntimeError("a residual needs add_residual=True")
     out, ws = _swiglu(x, gate, up, down, add_residual, residual, return_intermediates, return_intermediates, max_ctas)
     return (out, ws) if return_intermediates else out
 

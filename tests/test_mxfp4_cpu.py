@@ -259,3 +259,12 @@ def test_a_module_pickled_without_a_weight_format(swiglu):
     other = pickle.loads(pickle.dumps(m))
     with pytest.raises(RuntimeError, match="CUDA"):  # the forward reaches the kernels, which need a GPU
         other(torch.zeros(1, 128))
+
+
+def test_a_residual_needs_add_residual():
+    """It was dropped without a word."""
+    _L()
+    from looped_blockell import kernels as K
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="add_residual"):
+        K.mxfp4_swiglu_fwd(x, None, None, None, residual=x)

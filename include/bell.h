@@ -398,10 +398,10 @@ typedef struct BellMxLinearBwdDesc {
   const int64_t* index_t;
   int32_t K_t;
   int32_t layout;              /* of dw                                      */
-  void* dx;                    /* optional bf16 [T, C*B]                     */
+  void* dx;                    /* optional [T, C*B]                          */
   void* dw;                    /* optional [R, K, B, B]                      */
   int32_t grad_dtype;          /* of dw: BELL_DTYPE_BF16 / BELL_DTYPE_F32    */
-  int32_t reserved;
+  int32_t dx_dtype;
   void* workspace;
   int32_t* status;
 } BellMxLinearBwdDesc;
@@ -435,12 +435,13 @@ typedef struct BellMxFFNBwdDesc {
   const int32_t* cols_t_gate_up;
   const int64_t* index_t_gate_up;
   int32_t K_t_down, K_t_gate_up;
-  void* dx;                    /* optional bf16 [T, d_model]                 */
+  void* dx;                    /* optional [T, d_model]                      */
   void* d_gate;                /* optional tile gradients, each of its type  */
   void* d_up;
   void* d_down;
   int32_t gate_dtype, up_dtype, down_dtype;
-  int32_t reserved;
+  int16_t dx_dtype;
+  int16_t reserved;
   void* workspace;
   int32_t* status;
 } BellMxFFNBwdDesc;

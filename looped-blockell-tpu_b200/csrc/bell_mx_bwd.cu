@@ -201,6 +201,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   if (d->dx && (!d->cols_t || !d->index_t || d->K_t < 1)) return fail(BELL_ERR_ARG, "dx needs the transposed topology");
   if (d->dx)
     if (int rc = mx::check_k_t(d->K_t, "weight")) return rc;
+  if (d->dx && !mx::grad_type(d->dx_dtype)) return fail(BELL_ERR_DTYPE, "dx_dtype must be bf16 or f32");
   if (d->dw && (!d->col_indices || !mx::grad_type(d->grad_dtype)))
     return fail(BELL_ERR_ARG, "dw needs col_indices and a bf16 or f32 grad_dtype");
   if (int rc = mx::check_layout(d->layout)) return rc;
@@ -223,7 +224,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dx) {
     const BellEll wt{ws + o.tiles, d->cols_t, w.C, w.R, d->K_t, w.B, BELL_TILE_IN_OUT, 0};
-    if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream)) return rc;
+    if (int rc = mx::product(d->T, d->grad_out, wt, nullptr, d->dx, d->dx_dtype, ws + o.plan, d->status, stream)) return rc;
   }
   if (int rc = mx::tile_grad(d->T, ws + o.rows, d->grad_out, int64_t(w.R) * w.B, d->col_indices, w, d->layout, grads.g[0],
                              d->status, stream))
@@ -256,6 +257,7 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     if (int rc = mx::check_k_t(d->K_t_down, "down")) return rc;
   if (d->dx)
     if (int rc = mx::check_k_t(d->K_t_gate_up, "gate and up")) return rc;
+  if (d->dx && !mx::grad_type(d->dx_dtype)) return fail(BELL_ERR_DTYPE, "dx_dtype must be bf16 or f32");
   if ((d->d_gate && (!d->cols_gate || !mx::grad_type(d->gate_dtype))) ||
       (d->d_up && (!d->cols_up || !mx::grad_type(d->up_dtype))) ||
       (d->d_down && (!d->cols_down || !mx::grad_type(d->down_dtype))))
@@ -296,7 +298,7 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
   }
   if (want_dx) {
     const BellEll wt{ws + o.tiles, d->cols_t_gate_up, g.C, 2 * g.R, d->K_t_gate_up, g.B, BELL_TILE_IN_OUT, 0};
-    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, BELL_DTYPE_BF16, ws + o.plan, d->status, stream))
+    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, d->dx_dtype, ws + o.plan, d->status, stream))
       return rc;
   }
   if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads.g[0], d->status, stream))

@@ -115,7 +115,7 @@ class BellMxLinearBwdDesc(C.Structure):
     _fields_ = [("T", C.c_int64), ("grad_out", C.c_void_p), ("x", C.c_void_p), ("w", BellMxEll),
                 ("col_indices", C.c_void_p), ("cols_t", C.c_void_p), ("index_t", C.c_void_p), ("K_t", C.c_int32),
                 ("layout", C.c_int32), ("dx", C.c_void_p), ("dw", C.c_void_p), ("grad_dtype", C.c_int32),
-                ("reserved", C.c_int32), ("workspace", C.c_void_p), ("status", C.c_void_p)]
+                ("dx_dtype", C.c_int32), ("workspace", C.c_void_p), ("status", C.c_void_p)]
 
 
 class BellMxFFNBwdDesc(C.Structure):
@@ -126,7 +126,7 @@ class BellMxFFNBwdDesc(C.Structure):
                 ("index_t_down", C.c_void_p), ("cols_t_gate_up", C.c_void_p), ("index_t_gate_up", C.c_void_p),
                 ("K_t_down", C.c_int32), ("K_t_gate_up", C.c_int32), ("dx", C.c_void_p), ("d_gate", C.c_void_p),
                 ("d_up", C.c_void_p), ("d_down", C.c_void_p), ("gate_dtype", C.c_int32), ("up_dtype", C.c_int32),
-                ("down_dtype", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p),
+                ("down_dtype", C.c_int32), ("dx_dtype", C.c_int16), ("reserved", C.c_int16), ("workspace", C.c_void_p),
                 ("status", C.c_void_p)]
 
 

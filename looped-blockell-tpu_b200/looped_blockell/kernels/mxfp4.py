@@ -421,17 +421,17 @@ class MXLinearFn(torch.autograd.Function):
         if need[0]:
             cols_t, index_t = transposed_topology([cols], w.C)
             K_t = cols_t.shape[1]
-            dx = dyb.new_empty((T, w.C * w.B))
+            dx = dyb.new_empty((T, w.C * w.B), dtype=x_dtype)
             dx_at = dx.data_ptr()
         dw, dw_at, kind = _grad(need[1], w.col_indices, w.B, v_dtype)
         d = _lib.BellMxLinearBwdDesc(T, dyb.data_ptr(), rows.data_ptr(), w._abi, w.col_indices.data_ptr(),
                                      None if cols_t is None else cols_t.data_ptr(),
                                      None if index_t is None else index_t.data_ptr(), K_t, ctx.layout, dx_at, dw_at,
-                                     kind, 0, None, None)
+                                     kind, _DTYPES[x_dtype], None, None)
         ws = _bytes(_lib.load().bell_linear_bwd_mx_workspace_bytes(C.byref(d)), dev)
         d.workspace = ws.data_ptr()
         _call("bell_linear_bwd_mx", dev, C.byref(d))
-        return (None if dx is None else dx.to(x_dtype)), dw, None, dy if need[3] else None, None
+        return dx, dw, None, dy if need[3] else None, None
 
 
 def mxfp4_linear_ad(x: torch.Tensor, values: torch.Tensor, cols: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -441,7 +441,8 @@ def mxfp4_linear_ad(x: torch.Tensor, values: torch.Tensor, cols: torch.Tensor, r
 
     The backward passes the gradient straight through Q:
     ``dx = dy Q(W)``, ``dW = dy^T Q(x)`` on the live tiles (zero in dead slots),
-    in bf16 products with fp32 sums.  A column block of W may be used by at most
+    in bf16 products with fp32 sums, in the dtypes of x and values.  The
+    operands are bf16: an fp32 dy is rounded to it first.  A column block of W may be used by at most
     254 block-rows."""
     if x.dim() != 2 or values.dim() != 4 or x.shape[1] % values.shape[2]:
         raise RuntimeError("x must be 2D [N, C*B] and values [R, K, B, B]")
@@ -476,7 +477,7 @@ class MXSwiGLUFn(torch.autograd.Function):
         if need[0]:
             tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
             tg = tg_cols.data_ptr(), tg_index.data_ptr(), tg_cols.shape[1]
-        dx = torch.empty_like(dy) if need[0] else None
+        dx = torch.empty_like(dy, dtype=ctx.dtypes[0]) if need[0] else None
         # fp32 rows: the residual's gradient is added to theirs in fp32
         late = ctx.add_residual and ctx.dtypes[0] == torch.float32
         cols = (gate.col_indices, up.col_indices, down.col_indices)
@@ -485,12 +486,12 @@ class MXSwiGLUFn(torch.autograd.Function):
             T, int(ctx.add_residual and not late), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
             q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
             *td[:2], *tg[:2], td[2], tg[2], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
-            grads[1][2], grads[2][2], 0, None, None)
+            grads[1][2], grads[2][2], _DTYPES[ctx.dtypes[0]], 0, None, None)
         ws = _bytes(_lib.load().bell_swiglu_bwd_mx_workspace_bytes(C.byref(d)), dev)
         d.workspace = ws.data_ptr()
         _call("bell_swiglu_bwd_mx", dev, C.byref(d))
-        if dx is not None:
-            dx = dx + grad_out if late else dx.to(ctx.dtypes[0])
+        if dx is not None and late:
+            dx += grad_out
         return dx, grads[0][0], None, grads[1][0], None, grads[2][0], None, None, None
 
 
@@ -503,8 +504,10 @@ def mxfp4_swiglu(x: torch.Tensor, v_gate: torch.Tensor, ci_gate: torch.Tensor, v
     The backward is that of the bf16 block at the quantised operands Q(x),
     Q(W), Q(h), the gradient passing straight through Q; the projections are
     computed again rather than kept, so a step keeps 4.25 bits a value of x
-    and h.  Tile gradients are summed in fp32 and come back in the tiles'
-    dtype.  A column block may be used by at most 254 block-rows of down, and by
+    and h.  Gradients are summed in fp32 and come back in the dtypes of x and
+    the tiles; the operands of the backward's products (dy, the gradients of
+    the projections) are bf16, an fp32 dy and its own are rounded to it first.
+    A column block may be used by at most 254 block-rows of down, and by
     254 of gate and up together."""
     if x.dim() != 2 or v_gate.dim() != 4 or v_up.dim() != 4 or v_down.dim() != 4:
         raise RuntimeError("x must be 2D [N, d_model] and the tiles 4D [R, K, B, B]")

@@ -1029,3 +1029,33 @@ def test_a_captured_training_step_keeps_its_topology():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         del junk
+
+
+def test_fp32_rows_get_fp32_gradients():
+    K = _K()
+    rng = np.random.default_rng(32)
+    v, cols, w = weight(rng, 4, 6, 3, 64, 1)
+    x = rows(rng, 70, 384, F32).requires_grad_(True)
+    dy = rows(rng, 70, 256).float()  # bf16 values: rounding dy costs nothing
+    (dx,) = torch.autograd.grad(K.mxfp4_linear_ad(x, v, cols), x, dy)
+    ref = f64(dy) @ w
+    bound = (16 + 4 * 64 * 4 // 16) * 2.0 ** -23 * (np.abs(f64(dy)) @ np.abs(w))
+    assert (np.abs(f64(dx) - ref) <= bound + HALF_STEP[F32] * np.abs(ref)).all()
+
+
+@pytest.mark.parametrize("B", [64, 128])
+def test_fp32_rows_of_a_block_get_fp32_gradients(B):
+    """dx is not rounded to bf16 on its way, with and without the residual; no tokens, one token."""
+    K = _K()
+    rng = np.random.default_rng(39)
+    mats, _ = _ffn(rng, 4 * B, 8 * B, B)
+    for T in (0, 1, 150):
+        x, dy = rows(rng, T, 4 * B, F32, 1.0), rows(rng, T, 4 * B, F32)
+        dx = []
+        for dtype in (F32, BF16):
+            leaf = x.to(dtype).requires_grad_(True)
+            y = K.mxfp4_swiglu(leaf, *(a for m in mats for a in m[:2]))
+            dx.append(torch.autograd.grad(y, leaf, dy.to(dtype))[0])
+        assert dx[0].dtype == F32 and dx[1].dtype == BF16 and dx[0].shape == x.shape
+        if T:  # bf16 rows of other values have other codes: only the type is compared
+            assert (dx[0] != dx[0].bfloat16().float()).float().mean() > 0.9

@@ -268,3 +268,20 @@ def test_a_residual_needs_add_residual():
     x = torch.zeros(4, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="add_residual"):
         K.mxfp4_swiglu_fwd(x, None, None, None, residual=x)
+
+
+def test_backward_refuses_other_types_of_dx():
+    L = _L()
+    lib = L.load()
+    d = L.BellMxLinearBwdDesc()
+    d.T, d.grad_out, d.x, d.w, d.K_t = 4, 1024, 1024, _mx(L, 2, 3), 1
+    d.workspace = d.dx = d.cols_t = d.index_t = 1024
+    d.dx_dtype = 2
+    assert lib.bell_linear_bwd_mx(C.byref(d), None) == -1 and "dx_dtype" in L.last_error()
+    f = L.BellMxFFNBwdDesc()
+    f.T, f.gate, f.up, f.down = 4, _mx(L, 4, 2), _mx(L, 4, 2), _mx(L, 2, 4)
+    f.grad_out = f.x = f.h = f.workspace = f.dx = 1024
+    f.cols_t_down = f.index_t_down = f.cols_t_gate_up = f.index_t_gate_up = 1024
+    f.K_t_down = f.K_t_gate_up = 1
+    f.dx_dtype = 2
+    assert lib.bell_swiglu_bwd_mx(C.byref(f), None) == -1 and "dx_dtype" in L.last_error()

@@ -414,7 +414,10 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* desc, void* stream);
  * rows; the projections are computed again.  cols_t_down / index_t_down:
  * transposed topology of down [d_ff/B, K_t_down]; cols_t_gate_up /
  * index_t_gate_up: of gate stacked on up [d_model/B, K_t_gate_up] (block-rows
- * of up, and its tiles, counted after gate's); each K_t at most 254.  Results
+ * of up, and its tiles, counted after gate's); each K_t at most 254.  Where a
+ * column block of gate and up together is used more often, their topology comes
+ * in gate_up_passes pieces, [passes, d_model/B, K_t_gate_up], whose products are
+ * summed in fp32.  Results
  * that are NULL are not computed: d_down alone needs neither topology, the
  * gradients of tiles alone not that of gate and up.  With add_residual, dx
  * includes grad_out.  The workspace is 32-byte aligned.
@@ -441,7 +444,7 @@ typedef struct BellMxFFNBwdDesc {
   void* d_down;
   int32_t gate_dtype, up_dtype, down_dtype;
   int16_t dx_dtype;
-  int16_t reserved;
+  int16_t gate_up_passes;      /* 0: one                                     */
   void* workspace;
   int32_t* status;
 } BellMxFFNBwdDesc;

@@ -293,6 +293,8 @@ struct FinishArgs {
   TileGrad g[3];  // without sums: skipped
 };
 int finish_grads(const FinishArgs& a, cudaStream_t s);
+// out = a + b, n fp32 values (a multiple of 8); out fp32 (a itself may be) or bf16.
+int add_sums(const float* a, const float* b, int64_t n, void* out, int32_t out_dtype, cudaStream_t s);
 
 // [d_gate | d_up] (bf16 [T, 2 R B]) from d_h (fp32 [T, R B]) and the gated
 // block's quantised rows and weights (bell_mx.cu).

@@ -28,9 +28,10 @@ static size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Offsets of the workspace: the unpacked transposes (of down, and of gate and
 // up or the one weight), a plan, the unpacked rows, d_h then Q(h), fp32 sums
-// whose result is bf16, the parts of sums that CTAs share, [d_gate | d_up].
+// whose result is bf16, the parts of sums that CTAs share, [d_gate | d_up], and
+// the sums of dx where it takes several passes.
 struct BwdWs {
-  size_t tiles_down, tiles, plan, rows, mid, grads[3], parts[3], dgu, total;
+  size_t tiles_down, tiles, plan, rows, mid, grads[3], parts[3], dgu, dx[2], total;
 };
 
 struct Layout {
@@ -50,6 +51,8 @@ static size_t sums_bytes(const BellMxEll& w, bool wanted, int32_t dtype) {
 // gate and up for dx.
 static bool needs_down_t(const BellMxFFNBwdDesc& d) { return d.dx || d.d_gate || d.d_up || !d.d_down; }
 static bool needs_gate_up_t(const BellMxFFNBwdDesc& d) { return d.dx || !(d.d_gate || d.d_up || d.d_down); }
+
+static int32_t passes_of(const BellMxFFNBwdDesc& d) { return d.gate_up_passes ? d.gate_up_passes : 1; }
 
 static size_t parts_bytes(const BellMxEll& w, bool wanted, int64_t T) {
   return wanted ? sddmm_parts_bytes(T, w.R, w.C, w.K, w.B) : 0;
@@ -74,7 +77,7 @@ static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
   Layout l;
   const int32_t kd = needs_down_t(d) ? d.K_t_down : 0, kg = needs_gate_up_t(d) ? d.K_t_gate_up : 0;
   o.tiles_down = l.take(size_t(g.R) * kd * BB * 2);
-  o.tiles = l.take(size_t(g.C) * kg * BB * 2);
+  o.tiles = l.take(size_t(g.C) * kg * passes_of(d) * BB * 2);
   o.plan = l.take(std::max(bell_plan_bytes(0, 0, 0, g.R, kd), bell_plan_bytes(0, 0, 0, g.C, kg)));
   o.rows = l.take(T * g.C * g.B * 2);
   o.mid = l.take(T * F * 4);
@@ -85,6 +88,10 @@ static BwdWs swiglu_ws(const BellMxFFNBwdDesc& d) {
   o.parts[1] = l.take(parts_bytes(d.up, d.d_up != nullptr, d.T));
   o.parts[2] = l.take(parts_bytes(d.down, d.d_down != nullptr, d.T));
   o.dgu = l.take(T * 2 * F * 2);
+  if (d.dx && passes_of(d) > 1) {
+    o.dx[0] = l.take(d.dx_dtype == BELL_DTYPE_F32 ? 0 : T * g.C * g.B * 4);
+    o.dx[1] = l.take(T * g.C * g.B * 4);
+  }
   o.total = l.at;
   return o;
 }
@@ -234,7 +241,7 @@ int bell_linear_bwd_mx(const BellMxLinearBwdDesc* d, void* stream) {
 
 size_t bell_swiglu_bwd_mx_workspace_bytes(const BellMxFFNBwdDesc* d) {
   if (!d || mx::check_weight(d->gate, "gate") || mx::check_weight(d->up, "up") || mx::check_weight(d->down, "down") ||
-      d->T < 0 || (mx::needs_down_t(*d) && d->K_t_down < 1) || (mx::needs_gate_up_t(*d) && d->K_t_gate_up < 1))
+      d->T < 0 || d->gate_up_passes < 0 || (mx::needs_down_t(*d) && d->K_t_down < 1) || (mx::needs_gate_up_t(*d) && d->K_t_gate_up < 1))
     return 0;
   return mx::swiglu_ws(*d).total;
 }
@@ -257,6 +264,7 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     if (int rc = mx::check_k_t(d->K_t_down, "down")) return rc;
   if (d->dx)
     if (int rc = mx::check_k_t(d->K_t_gate_up, "gate and up")) return rc;
+  if (d->gate_up_passes < 0) return fail(BELL_ERR_SHAPE, "gate_up_passes must be >= 0");
   if (d->dx && !mx::grad_type(d->dx_dtype)) return fail(BELL_ERR_DTYPE, "dx_dtype must be bf16 or f32");
   if ((d->d_gate && (!d->cols_gate || !mx::grad_type(d->gate_dtype))) ||
       (d->d_up && (!d->cols_up || !mx::grad_type(d->up_dtype))) ||
@@ -288,7 +296,7 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
                    ws + o.tiles_down};
   if (want_dx)
     e.gather[1] = {g.chunks, int64_t(g.R) * g.K, u.chunks, int64_t(u.R) * u.K, d->index_t_gate_up,
-                   int64_t(g.C) * d->K_t_gate_up, ws + o.tiles};
+                   int64_t(g.C) * d->K_t_gate_up * mx::passes_of(*d), ws + o.tiles};
   if (T > 0 && (d->d_gate || d->d_up)) e.rows[0] = {d->x, D, ws + o.rows};
   if (int rc = mx::expand(e, s)) return rc;
   if (want_dgu) {
@@ -296,10 +304,19 @@ int bell_swiglu_bwd_mx(const BellMxFFNBwdDesc* d, void* stream) {
     if (int rc = mx::product(T, d->grad_out, wt, nullptr, mid, BELL_DTYPE_F32, ws + o.plan, d->status, stream)) return rc;
     if (int rc = mx::gated_backward(T, d->x, g, u, reinterpret_cast<const float*>(mid), dgu, d->status, s)) return rc;
   }
-  if (want_dx) {
-    const BellEll wt{ws + o.tiles, d->cols_t_gate_up, g.C, 2 * g.R, d->K_t_gate_up, g.B, BELL_TILE_IN_OUT, 0};
-    if (int rc = mx::product(T, dgu, wt, d->add_residual ? d->grad_out : nullptr, d->dx, d->dx_dtype, ws + o.plan, d->status, stream))
+  const int32_t passes = mx::passes_of(*d);
+  for (int32_t p = 0; want_dx && p < passes; ++p) {
+    const int64_t tiles = int64_t(g.C) * d->K_t_gate_up;
+    const BellEll wt{ws + o.tiles + size_t(p * tiles) * g.B * g.B * 2, d->cols_t_gate_up + p * tiles, g.C, 2 * g.R,
+                     d->K_t_gate_up, g.B, BELL_TILE_IN_OUT, 0};
+    float* sums = d->dx_dtype == BELL_DTYPE_F32 ? static_cast<float*>(d->dx) : reinterpret_cast<float*>(ws + o.dx[0]);
+    float* more = reinterpret_cast<float*>(ws + o.dx[1]);
+    const bool whole = passes == 1, last = p == passes - 1;
+    if (int rc = mx::product(T, dgu, wt, d->add_residual && p == 0 ? d->grad_out : nullptr, whole ? d->dx : p ? more : sums,
+                             whole ? int32_t(d->dx_dtype) : BELL_DTYPE_F32, ws + o.plan, d->status, stream))
       return rc;
+    if (p)
+      if (int rc = mx::add_sums(sums, more, T * D, last ? d->dx : sums, last ? int32_t(d->dx_dtype) : BELL_DTYPE_F32, s)) return rc;
   }
   if (int rc = mx::tile_grad(T, ws + o.rows, dgu, int64_t(F) * 2, d->cols_gate, g, d->layout, grads.g[0], d->status, stream))
     return rc;

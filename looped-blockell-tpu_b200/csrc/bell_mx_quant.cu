@@ -385,6 +385,25 @@ __global__ void __launch_bounds__(kThr) bell_mx_finish_kernel(const FinishKernel
   }
 }
 
+__global__ void __launch_bounds__(kThr) bell_mx_add_kernel(const float* a, const float* b, int64_t n, void* out, bool bf16) {
+  for (int64_t i = (int64_t(blockIdx.x) * kThr + threadIdx.x) * 8; i < n; i += int64_t(gridDim.x) * kThr * 8) {
+    Eight x, y;
+    x.load(a + i);
+    y.load(b + i);
+    float v[8] = {};
+    x.add_to(v);
+    y.add_to(v);
+    if (bf16) {
+      st_global_v4(static_cast<__nv_bfloat16*>(out) + i, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                   pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+      float* o = static_cast<float*>(out) + i;
+      st_global_v4(o, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      st_global_v4(o + 4, __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    }
+  }
+}
+
 // Grid of grid-stride kernels: enough blocks for every SM's 2048 threads.
 static int grid_for(int64_t threads, unsigned* grid) {
   int sms = 0;
@@ -453,6 +472,13 @@ int finish_grads(const FinishArgs& a, cudaStream_t s) {
   else
     bell_mx_finish_kernel<uint64_t><<<grid, kThr, 0, s>>>(k);
   return check_launch("bell_mx_finish_kernel");
+}
+
+int add_sums(const float* a, const float* b, int64_t n, void* out, int32_t out_dtype, cudaStream_t s) {
+  unsigned grid;
+  if (int rc = grid_for(n / 8, &grid)) return rc;
+  bell_mx_add_kernel<<<grid, kThr, 0, s>>>(a, b, n, out, out_dtype == BELL_DTYPE_BF16);
+  return check_launch("bell_mx_add_kernel");
 }
 
 }  // namespace mx

@@ -126,7 +126,7 @@ class BellMxFFNBwdDesc(C.Structure):
                 ("index_t_down", C.c_void_p), ("cols_t_gate_up", C.c_void_p), ("index_t_gate_up", C.c_void_p),
                 ("K_t_down", C.c_int32), ("K_t_gate_up", C.c_int32), ("dx", C.c_void_p), ("d_gate", C.c_void_p),
                 ("d_up", C.c_void_p), ("d_down", C.c_void_p), ("gate_dtype", C.c_int32), ("up_dtype", C.c_int32),
-                ("down_dtype", C.c_int32), ("dx_dtype", C.c_int16), ("reserved", C.c_int16), ("workspace", C.c_void_p),
+                ("down_dtype", C.c_int32), ("dx_dtype", C.c_int16), ("gate_up_passes", C.c_int16), ("workspace", C.c_void_p),
                 ("status", C.c_void_p)]
 
 

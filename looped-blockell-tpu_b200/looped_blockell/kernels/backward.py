@@ -39,7 +39,7 @@ from ..made import Made, capturing
 from . import _lib
 from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _ell, _stream, block_ell_linear, plan_bytes
 
-# (C_blocks, ids of the column-index tensors) -> (weak references, versions, result, Made, captured ones before).
+# (what is kept, ids of the column-index tensors) -> (weak references, versions, result, Made, captured ones before).
 # A hit needs the very same tensor objects (alive) at the same version: a new
 # tensor that happens to reuse a freed tensor's memory or id never matches.  An
 # entry lives as long as its column-index tensors, so however many weights a
@@ -48,8 +48,8 @@ from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _ell, _strea
 _TOPO_CACHE: dict = {}
 
 
-def _topo_lookup(mats: Sequence[torch.Tensor], C_blocks: int):
-    key = (C_blocks,) + tuple(id(m) for m in mats)
+def _topo_lookup(mats: Sequence[torch.Tensor], what):
+    key = (what,) + tuple(id(m) for m in mats)
     hit = _TOPO_CACHE.get(key)
     if hit is None:
         return key, None
@@ -109,15 +109,41 @@ def transposed_topology(mats: Sequence[torch.Tensor], C_blocks: int) -> Tuple[to
     at = (grp_s[:used], pos[:used])  # what is left out was sorted last
     cols_t[at] = r_s[:used].to(torch.int32)
     tile_idx[at] = t_s[:used]
+    return _topo_keep(key, mats, (cols_t, tile_idx))
+
+
+def _topo_keep(key, mats, result):
+    if capturing(result[0]):
+        return result
 
     def forget(_, key=key, pop=_TOPO_CACHE.pop):
         pop(key, None)
 
     old = _TOPO_CACHE.get(key)  # of the same tensors, before they changed
     captured = () if old is None else old[4] + ((old[3],) if old[3].captured else ())
-    _TOPO_CACHE[key] = (tuple(weakref.ref(m, forget) for m in mats), tuple(m._version for m in mats),
-                        (cols_t, tile_idx), Made(cols_t, tile_idx), captured)
-    return cols_t, tile_idx
+    _TOPO_CACHE[key] = (tuple(weakref.ref(m, forget) for m in mats), tuple(m._version for m in mats), result,
+                        Made(*result), captured)
+    return result
+
+
+def topology_in_passes(mats: Sequence[torch.Tensor], C_blocks: int, most: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``transposed_topology`` in pieces of at most ``most`` slots a row: both
+    results ``[passes, C_blocks, K_t]``."""
+    cols_t, tile_idx = transposed_topology(mats, C_blocks)
+    K_t = cols_t.shape[1]
+    if K_t <= most:
+        return cols_t[None], tile_idx[None]
+    key, hit = _topo_lookup(mats, (C_blocks, most))
+    if hit is not None:
+        return hit
+    passes = -(-K_t // most)
+    width = -(-K_t // passes)
+
+    def cut(t, fill):
+        t = torch.nn.functional.pad(t, (0, passes * width - K_t), value=fill)
+        return t.view(C_blocks, passes, width).transpose(0, 1).contiguous()
+
+    return _topo_keep(key, mats, (cut(cols_t, -1), cut(tile_idx, 0)))
 
 
 # (ids of the value and column tensors, C_blocks) -> (weak refs, versions, values_t, Made):

@@ -41,11 +41,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .backward import transposed_topology
+from .backward import topology_in_passes, transposed_topology
 from .ops import TILE_IN_OUT, TILE_OUT_IN, _check_cuda, _check_out, _prep_ell, plan_bytes
 
 _BF16, _F32 = _lib.BELL_DTYPE_BF16, _lib.BELL_DTYPE_F32
 _DTYPES = {torch.bfloat16: _BF16, torch.float32: _F32}
+_SLOTS = 254  # of a row of the backward's bf16 products
 _ROWS = 128  # tokens of one chunk of quantised rows
 _ELLS = {n: (_lib.BellEll * n, C.c_void_p * n) for n in (1, 2, 3)}  # array types of a pack of n weights
 
@@ -471,12 +472,16 @@ class MXSwiGLUFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         # transposed topologies: of down for d_gate and d_up, of gate and up for dx (the address, the address, slots)
         td = tg = (None, None, 1)
+        passes = 1
         if need[0] or need[1] or need[3]:
             td_cols, td_index = transposed_topology([ci_down], gate.R)
             td = td_cols.data_ptr(), td_index.data_ptr(), td_cols.shape[1]
         if need[0]:
             tg_cols, tg_index = transposed_topology([ci_gate, ci_up], gate.C)
-            tg = tg_cols.data_ptr(), tg_index.data_ptr(), tg_cols.shape[1]
+            if tg_cols.shape[1] > _SLOTS:
+                tg_cols, tg_index = topology_in_passes([ci_gate, ci_up], gate.C, _SLOTS)
+                passes = tg_cols.shape[0]
+            tg = tg_cols.data_ptr(), tg_index.data_ptr(), tg_cols.shape[-1]
         dx = torch.empty_like(dy, dtype=ctx.dtypes[0]) if need[0] else None
         # fp32 rows: the residual's gradient is added to theirs in fp32
         late = ctx.add_residual and ctx.dtypes[0] == torch.float32
@@ -486,7 +491,7 @@ class MXSwiGLUFn(torch.autograd.Function):
             T, int(ctx.add_residual and not late), ctx.layout, dy.data_ptr(), q_x.data_ptr(),
             q_h.data_ptr(), gate._abi, up._abi, down._abi, cols[0].data_ptr(), cols[1].data_ptr(), cols[2].data_ptr(),
             *td[:2], *tg[:2], td[2], tg[2], None if dx is None else dx.data_ptr(), grads[0][1], grads[1][1], grads[2][1], grads[0][2],
-            grads[1][2], grads[2][2], _DTYPES[ctx.dtypes[0]], 0, None, None)
+            grads[1][2], grads[2][2], _DTYPES[ctx.dtypes[0]], passes, None, None)
         ws = _bytes(_lib.load().bell_swiglu_bwd_mx_workspace_bytes(C.byref(d)), dev)
         d.workspace = ws.data_ptr()
         _call("bell_swiglu_bwd_mx", dev, C.byref(d))
@@ -507,8 +512,8 @@ def mxfp4_swiglu(x: torch.Tensor, v_gate: torch.Tensor, ci_gate: torch.Tensor, v
     and h.  Gradients are summed in fp32 and come back in the dtypes of x and
     the tiles; the operands of the backward's products (dy, the gradients of
     the projections) are bf16, an fp32 dy and its own are rounded to it first.
-    A column block may be used by at most 254 block-rows of down, and by
-    254 of gate and up together."""
+    A column block may be used by at most 254 block-rows of down; of gate and
+    up together by any number (dx then takes several passes)."""
     if x.dim() != 2 or v_gate.dim() != 4 or v_up.dim() != 4 or v_down.dim() != 4:
         raise RuntimeError("x must be 2D [N, d_model] and the tiles 4D [R, K, B, B]")
     if x.shape[1] % v_gate.shape[2]:

@@ -139,3 +139,19 @@ def test_transposed_topology_of_nothing():
                     (torch.tensor([[7]], dtype=torch.int32), 2)):
         ct, idx = K.transposed_topology([cols], C)
         assert ct.tolist() == [[-1]] * C and idx.tolist() == [[0]] * C
+
+
+def test_topology_in_passes_lists_the_same_tiles():
+    from looped_blockell.kernels.backward import topology_in_passes
+    K = _K()
+    g = torch.Generator().manual_seed(1)
+    cols = torch.randint(-1, 3, (40, 4), generator=g, dtype=torch.int32)
+    whole, index = K.transposed_topology([cols], 3)
+    for most in (1, 7, 16, whole.shape[1] - 1, whole.shape[1], 254):
+        ct, it = topology_in_passes([cols], 3, most)
+        assert ct.shape == it.shape and ct.shape[2] <= most and ct.is_contiguous() and it.is_contiguous()
+        for c in range(3):
+            live = ct[:, c] >= 0
+            assert ct[:, c][live].tolist() == whole[c][whole[c] >= 0].tolist()
+            assert it[:, c][live].tolist() == index[c][whole[c] >= 0].tolist()
+        assert topology_in_passes([cols], 3, most)[0].data_ptr() == ct.data_ptr()

@@ -1059,3 +1059,38 @@ def test_fp32_rows_of_a_block_get_fp32_gradients(B):
         assert dx[0].dtype == F32 and dx[1].dtype == BF16 and dx[0].shape == x.shape
         if T:  # bf16 rows of other values have other codes: only the type is compared
             assert (dx[0] != dx[0].bfloat16().float()).float().mean() > 0.9
+
+
+@pytest.mark.parametrize("T,d,F,B,Kg,dtype,residual", [
+    (40, 128, 8192, 64, 2, BF16, True), (1, 128, 8192, 64, 2, F32, True), (200, 64, 20480, 64, 1, BF16, False),
+    (130, 256, 16640, 128, 2, F32, True)])
+def test_gate_and_up_on_more_than_254_slots(T, d, F, B, Kg, dtype, residual):
+    """Column blocks that 256, 640 and 260 block-rows of gate and up use: dx in several passes, also from a graph."""
+    K = _K()
+    rng = np.random.default_rng(33)
+    mats, _ = _ffn(rng, d, F, B, Kg, 3, 2)
+    x, dy = rows(rng, T, d, dtype, 1.0), rows(rng, T, d, dtype)
+    leaves = [x] + [m[0] for m in mats]
+    for t in leaves:
+        t.requires_grad_(True)
+
+    def step():
+        y = K.mxfp4_swiglu(x, *(a for m in mats for a in m[:2]), add_residual=residual)
+        return torch.autograd.grad(y, leaves, dy)
+
+    grads = step()
+    packed = [K.make_mxfp4(v.detach(), c, n) for (v, c, _), n in zip(mats, (d // B, d // B, F // B))]
+    _, ws = K.mxfp4_swiglu_fwd(x.detach(), *packed, add_residual=residual, return_intermediates=True)
+    refs = M.swiglu_backward(M.quantize(f64(x)), *(m[2] for m in mats), f64(ws["q_h"].dequantize(F32)), f64(dy), residual)
+    tol = GRAD_TOL + (2.0 ** -8 if dtype == F32 else 0)  # fp32: dy is rounded to bf16 once more
+    assert grads[0].dtype == dtype and rel(f64(grads[0]), refs[0]) <= tol
+    for g, (_, c, _), ref in zip(grads[1:], mats, refs[1:]):
+        assert rel(f64(g), M.tile_grads(ref, f64(c).astype(int), B)) <= tol
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, grads))
+    assert K.read_status() == 0

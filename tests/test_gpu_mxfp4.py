@@ -1094,3 +1094,37 @@ def test_gate_and_up_on_more_than_254_slots(T, d, F, B, Kg, dtype, residual):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(again, grads))
     assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("B", [64, 128])
+def test_gates_far_below_zero(B):
+    """Gates of -16 to -96.  silu's error: 1.25 |g| 2^-24 for the rounded exponent (2^-24 and 2^-26 of its constant) and
+    2^-21 for ex2, rcp, the sum and the products; flushed below -87.3, |g| e^g <= 2^-119.  u adds one rounding, 2^-24."""
+    K = _K()
+    rng = np.random.default_rng(37)
+    d, T = 4 * B, 150
+    cols = torch.arange(4, dtype=torch.int32, device="cuda")[:, None].contiguous()
+
+    def diagonal(values):  # exact in MXFP4
+        t = torch.zeros(4, 1, B, B, device="cuda")
+        t[:, 0] = torch.diag_embed(torch.from_numpy(values.astype(np.float32)).cuda().view(4, B))
+        return K.make_mxfp4(t, cols, 4)
+
+    wg = diagonal(np.full(d, 16.0))
+    wu = diagonal(rng.choice([1.0, 1.5, 2.0, 3.0, -4.0, 6.0], d) * 2.0 ** 60)
+    # a scale block has one gate: its h's differ by u alone
+    x = -np.repeat(rng.choice([1.0, 1.5, 2.0, 3.0, 4.0, 6.0], (T, d // 32)), 32, 1)
+    out, ws = K.mxfp4_swiglu_fwd(torch.from_numpy(x).to(BF16).cuda(), wg, wu, wg, return_intermediates=True)
+    g, u = f64(ws["gate"]), f64(ws["up"])
+    h = M.silu_mul(g, u)
+    tol = np.abs(h) * (1.25 * np.abs(g) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -24) + np.abs(u) * 2.0 ** -119
+    lo, hi = h - tol, h + tol
+    q = f64(ws["q_h"].dequantize(F32)).reshape(T, -1, 32)
+    mag, t3 = np.abs(h).reshape(T, -1, 32), tol.reshape(T, -1, 32)
+    fits = np.zeros(q.shape[:2], bool)
+    for s in (-1, 1):
+        sc = M.scales(np.repeat(np.maximum(mag + s * t3, 0).max(-1, keepdims=True), 32, -1))
+        a, b = (M.e2m1(v.reshape(T, -1, 32) / sc[..., :1]) * sc[..., :1] for v in (lo, hi))
+        fits |= ((q >= np.minimum(a, b)) & (q <= np.maximum(a, b))).all(-1)
+    assert fits.all()
+    assert K.read_status() == 0

@@ -1128,3 +1128,65 @@ def test_gates_far_below_zero(B):
         fits |= ((q >= np.minimum(a, b)) & (q <= np.maximum(a, b))).all(-1)
     assert fits.all()
     assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("B,T,d,F,Kg,Ku,Kd", [(64, 777, 1024, 4096, 4, 3, 16), (128, 1000, 1024, 8192, 2, 5, 8)])
+def test_backward_of_many_units_equals_the_same_tokens_in_parts(B, T, d, F, Kg, Ku, Kd):
+    """Several units for each CTA of the gated backward: dx and the sums of d_gate, d_up."""
+    K = _K()
+    rng = np.random.default_rng(35)
+    mats = [weight(rng, F // B, d // B, Kg, B, 5, dead_row=1), weight(rng, F // B, d // B, Ku, B, 2),
+            weight(rng, d // B, F // B, Kd, B, 3)]
+    x, dy = rows(rng, T, d, spread=1.0), rows(rng, T, d)
+
+    def grads(a, g):
+        ls = [a.detach().requires_grad_(True)] + [m[0].detach().requires_grad_(True) for m in mats]
+        y = K.mxfp4_swiglu(ls[0], ls[1], mats[0][1], ls[2], mats[1][1], ls[3], mats[2][1], add_residual=True)
+        return torch.autograd.grad(y, ls, g)
+
+    whole = grads(x, dy)
+    parts = [grads(x[i:i + 100], dy[i:i + 100]) for i in range(0, T, 100)]
+    assert torch.equal(whole[0], torch.cat([p[0] for p in parts]))
+    packed = [K.make_mxfp4(m[0], m[1], n) for m, n in zip(mats, (d // B, d // B, F // B))]
+    q = K.mxfp4_quantize(x, B)
+    _, ws = K.mxfp4_swiglu_fwd(q, *packed, return_intermediates=True)
+    xq, hq = K.mxfp4_dequantize(q, F32).double(), ws["q_h"].dequantize(F32).double()
+    wg, wu, wd = (torch.from_numpy(m[2]).cuda() for m in mats)
+    g, u = xq @ wg.T, xq @ wu.T
+    sig = torch.sigmoid(g)
+    dh = dy.double() @ wd
+    du, dg = dh * g * sig, dh * u * sig * (1 + g * (1 - sig))
+    for got, ref, m in zip(whole[1:], (dg.T @ xq, du.T @ xq, dy.double().T @ hq), mats):
+        e = tile_errors(got, ref, m[1], B, 0)
+        assert e[e.isfinite()].max() <= GRAD_TOL
+    assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("T", [9, 17, 32])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_direct_rows_of_several_groups(T, dtype):
+    """x = NULL at tile 128 up to BELL_MX_DIRECT_ROWS rows: what rows quantised before give."""
+    import ctypes as C
+    K = _K()
+    from looped_blockell.kernels import _lib as L
+    rng = np.random.default_rng(36)
+    lib = L.load()
+    kind = L.BELL_DTYPE_BF16 if dtype == BF16 else L.BELL_DTYPE_F32
+    mats, packed = _ffn(rng, 1024, 2560, 128, 5, 9, 2)
+    x = rows(rng, T, 2560, dtype)
+    stream = torch.cuda.current_stream().cuda_stream
+    for w, n in ((packed[2], 1024),):
+        out = torch.full((T, n), 7.0, dtype=dtype, device="cuda")
+        d = L.BellMxLinearDesc(T, kind, 0, None, x.data_ptr(), 2560, kind, 0, None, out.data_ptr(), w._abi, None)
+        assert lib.bell_linear_mx(C.byref(d), stream) == 0
+        assert torch.equal(out, K.mxfp4_linear(K.mxfp4_quantize(x, 128), w, out_dtype=dtype))
+    x = rows(rng, T, 1024, dtype)
+    out = torch.full((T, 1024), 7.0, dtype=dtype, device="cuda")
+    h = torch.empty(lib.bell_mx_rows_bytes(T, 2560, 128), dtype=torch.uint8, device="cuda")
+    d = L.BellMxFFNDesc(T, kind, 0, None, x.data_ptr(), 1024, kind, 0, None, h.data_ptr(), None, None, out.data_ptr(),
+                        *(p._abi for p in packed), None)
+    assert lib.bell_swiglu_fwd_mx(C.byref(d), stream) == 0
+    want = K.mxfp4_swiglu_fwd(K.mxfp4_quantize(x, 128), *packed) if dtype == BF16 else \
+        K.mxfp4_swiglu_fwd(x, *packed, return_intermediates=True)[0]
+    assert torch.equal(out, want)
+    assert K.read_status() == 0

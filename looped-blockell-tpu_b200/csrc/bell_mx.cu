@@ -925,18 +925,53 @@ __global__ void __launch_bounds__(kThreads, 1) bell_mx_kernel(const Params p) {
   }
 }
 
-// CTAs that share a unit of a linear.  The cluster's launch and the join cost
-// 2.6 us and 1 to 3 for 128 rows, a slot 0.14 us (B = 128) or 0.08 (B = 64), so
-// whole units serve short rows better.  us whole and split, by CTAs as many as
-// fit: B = 128, R = 32, K = 16: 6.0, 6.9 (T = 1), 6.8, 9.9 (T = 128); K = 32: 8.4,
-// 7.8 (T = 1), 8.4, 8.7 (T = 32), 9.1, 10.9 (T = 128); K = 64: 13.0, 9.2 (T = 1),
-// 13.6, 12.2 (T = 128).  B = 64, R = 16, K = 16: 4.7, 5.8 (T = 1); K = 64: 8.5, 6.5
-// (T = 1), 8.9, 8.5 (T = 128).
-static int split_of(int64_t units, int64_t T, int K, int stages, int sms, int B) {
-  if (units * 2 > sms || K * B < (T > BELL_MX_DIRECT_ROWS ? 8192 : 4096)) return 0;
-  int split = 1;  // a power of two, 16 columns each to join, a stage for every ring
-  while (split < std::min(kMaxSplit, B / 16) && units * split * 2 <= sms && split * 4 <= stages) split *= 2;
-  return split;
+// Slots of a row from which CTAs share a unit of a linear.  The cluster's launch
+// and the join cost 2 us, more with more rows to join; a slot takes a whole unit
+// 0.15 to 0.3 us, and 0.25 to 0.5 where it quantises its rows itself, which the
+// mxfp4.py calls have it do up to 8 tokens at B = 128 and 32 at B = 64.  us whole
+// and split (graph replays, quantisation included where it is a launch of its own):
+//   B = 128, R = 32   T = 1: K = 16 7.5, 6.9; 32 12.0, 7.4; R = 16, K = 12 6.1, 6.6
+//     T = 16: K = 24 8.7, 9.1; 28 9.2, 9.2; 32 9.9, 9.4   T = 32: 32 10.0, 10.2; 40 11.2, 10.9
+//     T = 64: K = 36 10.8, 11.2; 44 12.1, 11.5   T = 128: K = 40 12.4, 13.5; 48 13.6, 13.7; 64 16.1, 14.1
+//   B = 64, R = 16    T = 1: K = 16 5.2, 6.7; 24 7.3, 7.4; 32 9.3, 6.8   T = 32: K = 16 7.9, 8.9; 24 12.2, 10.4
+//     T = 33: K = 40 8.5, 8.8; 64 10.3, 8.8   T = 128: K = 48 9.6, 10.4; 64 10.7, 10.7; 96 13.6, 11.3
+static int split_from(int64_t T, int B) {
+  if (T <= (B == 64 ? BELL_MX_DIRECT_ROWS : 8)) return B == 64 ? 24 : 16;
+  return B == 64 ? 64 : 32 + int(std::min<int64_t>(std::max<int64_t>(T - 32, 0), 96) / 4);
+}
+
+// CTAs that share a unit: a power of two, 16 columns each to join, a stage for
+// every ring, and all clusters at once (of 16 clusters of eight some wait for the
+// others: B = 128, R = 16, K = 32, T = 1: 12.4 us with eight CTAs, 11.9 whole, 7.3
+// with four).  fit[i]: clusters of 2 << i CTAs that run together.
+static int split_of(int64_t units, int64_t T, int K, int stages, int sms, int B, const int (&fit)[3]) {
+  if (units * 2 > sms || K < split_from(T, B)) return 0;
+  int split = 1;
+  for (int i = 0; i < 3; ++i)
+    if (2 * split <= B / 16 && units * split * 2 <= sms && split * 4 <= stages && units <= fit[i]) split *= 2;
+    else break;
+  return split > 1 ? split : 0;
+}
+
+// Clusters of 2, 4 and 8 CTAs of `kern` that run at once on the current device.
+static int clusters_at_once(const void* kern, int threads, int smem, int (&fit)[3]) {
+  for (int i = 0; i < 3; ++i) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(2 << i);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(unsigned(2 << i));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&fit[i], kern, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return fail(BELL_ERR_LAUNCH, "cudaOccupancyMaxActiveClusters");
+    }
+  }
+  return BELL_OK;
 }
 
 template <int B, Mode MODE>
@@ -944,16 +979,23 @@ static int launch(Params p, int32_t max_ctas, cudaStream_t s) {
   using G = Geo<B, MODE>;
   auto kern = bell_mx_kernel<B, MODE>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
+  static std::atomic<int> fits[64][3];    // and there, clusters at once
   int dev = 0, sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(BELL_ERR_LAUNCH, "cudaGetDevice");
   if (!(ready.load() >> dev & 1)) {
     if (int rc = set_smem(reinterpret_cast<const void*>(kern), G::SMEM)) return rc;
+    if (MODE == kLinear) {
+      int fit[3];
+      if (int rc = clusters_at_once(reinterpret_cast<const void*>(kern), kThreads, G::SMEM, fit)) return rc;
+      for (int i = 0; i < 3; ++i) fits[dev][i] = fit[i];
+    }
     ready.fetch_or(uint64_t(1) << dev);
   }
   if (max_ctas > 0 && sms > max_ctas) sms = max_ctas;
   const int64_t units = (int64_t(p.mtiles) + G::TILES - 1) / G::TILES * p.R;
-  p.split = MODE != kLinear ? 0 : split_of(units, p.T, p.K0, (p.K0 + G::SLOTS - 1) / G::SLOTS, sms, B);
+  const int fit[3] = {fits[dev][0], fits[dev][1], fits[dev][2]};
+  p.split = MODE != kLinear ? 0 : split_of(units, p.T, p.K0, (p.K0 + G::SLOTS - 1) / G::SLOTS, sms, B, fit);
   const int64_t grid = p.split ? units * p.split : std::min<int64_t>(units, sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(grid));

@@ -1190,3 +1190,20 @@ def test_direct_rows_of_several_groups(T, dtype):
         K.mxfp4_swiglu_fwd(x, *packed, return_intermediates=True)[0]
     assert torch.equal(out, want)
     assert K.read_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 8, 9, 32, 33, 64, 128, 129])
+@pytest.mark.parametrize("R,Kk,B,dead,dtype", [
+    (3, 16, 128, 5, BF16), (16, 32, 128, 0, F32), (18, 44, 128, 9, BF16), (3, 24, 64, 7, BF16), (16, 64, 64, 3, F32),
+    (70, 33, 64, 0, BF16)])
+def test_rows_that_begin_to_be_shared(T, R, Kk, B, dead, dtype):
+    """Around the lengths from which clusters share a unit: dead slots, rows quantised before and on the way."""
+    K = _K()
+    rng = np.random.default_rng(T + Kk)
+    v, cols, w = weight(rng, R, 2 * Kk, Kk, B, dead, dead_row=1 if dead else None)
+    mw = K.make_mxfp4(v, cols, 2 * Kk)
+    x, res = rows(rng, T, 2 * Kk * B, dtype), rows(rng, T, R * B, dtype)
+    y = K.mxfp4_linear(x, mw, residual=res)
+    check_linear(y, M.quantize(f64(x)), w, Kk * B // 64, f64(res))
+    assert torch.equal(y, K.mxfp4_linear(K.mxfp4_quantize(x, B), mw, residual=res, out_dtype=dtype))
+    assert torch.equal(y, K.mxfp4_linear(x, mw, residual=res)) and K.read_status() == 0

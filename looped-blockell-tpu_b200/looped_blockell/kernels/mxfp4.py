@@ -159,11 +159,14 @@ def _rows_2d(name: str, x: torch.Tensor) -> torch.Tensor:
 
 def _direct(T: int, tile: int) -> bool:
     """Whether a product of T rows quantises them itself, which saves a launch
-    (about 5 us of the host's time).  On the device alone, graph replays of the
-    gated block, on the way and quantised first: tile 64, d_model 1024: 8.9 us
-    and 9.3 at 1 token, 10.1 and 9.5 at 24; tile 128, d_model 4096: 14.7 and
-    15.5 at 1, 15.7 and 15.6 at 8, 20.2 and 16.4 at 24."""
-    return T <= (_lib.BELL_MX_DIRECT_ROWS if tile == 64 else 8)
+    (about 5 us of the host's time, none in a graph).  On the device alone, graph
+    replays of the gated block, on the way and quantised first: tile 64, d_model
+    1024: 8.5 us and 9.1 at 1 token, 8.8 and 9.0 at 16, 9.6 and 9.1 at 24, 9.7
+    and 8.9 at 32; tile 128, d_model 4096: 14.6 and 15.6 at 1, 15.6 and 15.6 at
+    8, 17.1 and 15.6 at 9, 20.0 and 16.5 at 24.  Either way gives the same bits."""
+    if tile != 64:
+        return T <= 8
+    return T <= 16 or T <= _lib.BELL_MX_DIRECT_ROWS and not torch.cuda.is_current_stream_capturing()
 
 
 def _ld(x: torch.Tensor) -> int:

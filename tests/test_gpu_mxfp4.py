@@ -1207,3 +1207,20 @@ def test_rows_that_begin_to_be_shared(T, R, Kk, B, dead, dtype):
     check_linear(y, M.quantize(f64(x)), w, Kk * B // 64, f64(res))
     assert torch.equal(y, K.mxfp4_linear(K.mxfp4_quantize(x, B), mw, residual=res, out_dtype=dtype))
     assert torch.equal(y, K.mxfp4_linear(x, mw, residual=res)) and K.read_status() == 0
+
+
+@pytest.mark.parametrize("T", [16, 17, 32])
+def test_a_captured_call_gives_the_same_bits(T):
+    """Captured calls may quantise their rows first where eager ones do not."""
+    K = _K()
+    rng = np.random.default_rng(40)
+    _, packed = _ffn(rng, 512, 2048, 64, 4, 24, 3)
+    x, h = rows(rng, T, 512), rows(rng, T, 2048)
+    want = K.mxfp4_swiglu_fwd(x, *packed, add_residual=True), K.mxfp4_linear(h, packed[2])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = K.mxfp4_swiglu_fwd(x, *packed, add_residual=True), K.mxfp4_linear(h, packed[2])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

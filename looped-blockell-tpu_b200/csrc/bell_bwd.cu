@@ -485,7 +485,7 @@ int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sm
   if (int rc = make_map_2d(&mb, d->b, MapType::BF16, uint64_t(d->R) * B, uint64_t(d->T), uint64_t(d->ldb) * 2, 64,
                            kTok, Swz::B128))
     return rc;
-  const SddmmCuts cuts = sddmm_cuts(d->T, d->R, d->C, d->K, B, own ? std::min(sms, kMaxParts) : sms);
+  const SddmmCuts cuts = sddmm_cuts(d->T, d->R, d->C, d->K, B, own ? std::min(sms, kMaxParts) : sms, own);
   SddmmParams p{};
   p.T = d->T;
   p.R = d->R;
@@ -511,7 +511,7 @@ int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sm
 }  // namespace
 }  // namespace bwd
 
-SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas) {
+SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas, bool own) {
   SddmmCuts c{};
   c.slots = B == 128 ? bwd::SCfg<128>::SLOTS : bwd::SCfg<64>::SLOTS;
   c.KP = (K + c.slots - 1) / c.slots;
@@ -525,6 +525,14 @@ SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int 
   range = range < 16 ? 16 : (range > 128 ? 128 : range);
   c.chunks = chunks < range ? chunks : range;
   c.steps = int64_t(R) * c.KP * c.chunks;  // chunk-steps of one range
+  // With parts a cut costs their write and their read, so a few idle CTAs are
+  // cheaper than cuts inside units: as many CTAs to each unit, where that leaves a
+  // quarter idle at most.  us of a linear's step with dW, equal shares for every SM
+  // and as many CTAs to each unit: B = 64, 64 units, T = 777 28.2, 25.0; 120, T = 1000
+  // 34.4, 31.4; 128, T = 2047 48.3, 45.5; B = 128, 32 units, T = 777 32.2, 27.0; 128,
+  // T = 2047 61.1, 56.6.
+  const int64_t units = int64_t(R) * c.KP;
+  if (own && units <= ctas && ctas / units * units * 4 >= int64_t(ctas) * 3) ctas = int(ctas / units * units);
   c.grid = int32_t(c.steps < ctas ? c.steps : ctas);
   return c;
 }
@@ -570,8 +578,8 @@ int sddmm_bf16(const BellSddmmDesc* d, bool own, float* parts, void* stream) {
 }
 
 size_t sddmm_parts_bytes(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B) {
-  const SddmmCuts c = sddmm_cuts(T, R, C, K, B, kMaxParts);
-  return c.chunks > 1 ? size_t(c.grid) * c.slots * B * B * 4 : 0;
+  const SddmmCuts c = sddmm_cuts(T, R, C, K, B, kMaxParts, true);
+  return c.chunks > 1 ? size_t(std::min<int64_t>(c.steps, kMaxParts)) * c.slots * B * B * 4 : 0;
 }
 
 }  // namespace bell

@@ -72,7 +72,7 @@ int down_bf16(const BellFFNDesc* d, int32_t* status, cudaStream_t s, bool pdl = 
 // The chunk-steps [0, steps) of one token range, `chunks` to a unit (a group of
 // `slots` slots of a block-row, KP groups to a row), are cut into `grid` equal
 // shares, of which share b starts at steps * b / grid.  sddmm_bf16 with `own`
-// (T > 0, B 64 or 128; it takes sddmm_cuts() of at most kMaxParts CTAs) writes
+// (T > 0, B 64 or 128; it takes the sddmm_cuts() of at most kMaxParts CTAs) writes
 // into d->grad, for each unit, the sums of the share that holds its first chunk,
 // and into parts[b] ([slots, B, B]; sddmm_parts_bytes() bytes, 16-byte aligned,
 // NULL where that is 0) those of a share b that starts inside a unit: a tile's
@@ -82,7 +82,7 @@ struct SddmmCuts {
   int32_t grid, slots, KP;
 };
 static constexpr int kMaxParts = 160;  // a B200 has 148 SMs
-SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas);
+SddmmCuts sddmm_cuts(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B, int ctas, bool own);
 size_t sddmm_parts_bytes(int64_t T, int32_t R, int32_t C, int32_t K, int32_t B);
 int sddmm_bf16(const BellSddmmDesc* d, bool own, float* parts, void* stream);
 

@@ -110,7 +110,7 @@ static TileGrad grad_of(int64_t T, const BellMxEll& w, const int32_t* cols, void
   int sms = 0;
   if (!parts_bytes(w, true, T) || device_sm_count(&sms)) return g;
   g.parts = reinterpret_cast<float*>(ws + parts);
-  g.cuts = sddmm_cuts(T, w.R, w.C, w.K, w.B, std::min(sms, kMaxParts));
+  g.cuts = sddmm_cuts(T, w.R, w.C, w.K, w.B, std::min(sms, kMaxParts), true);
   return g;
 }
 

@@ -393,6 +393,13 @@ def _swiglu(x, gate, up, down, add_residual=False, residual=None, keep_rows=Fals
 # ----------------------------------------------------------------- training
 
 
+def _grad_rows(dy: torch.Tensor) -> torch.Tensor:
+    """An incoming gradient as the backward reads it: contiguous bf16 rows,
+    16-byte aligned (that of a slice may start anywhere)."""
+    dy = dy.to(torch.bfloat16).contiguous()
+    return dy if dy.data_ptr() % 16 == 0 else dy.clone()
+
+
 def _grad(need: bool, cols: torch.Tensor, B: int, dtype: torch.dtype):
     """Buffer of a tile gradient (bf16 for bf16 tiles, else fp32), its address and type."""
     if not need:
@@ -417,7 +424,7 @@ class MXLinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         w, (cols, rows) = ctx.w, ctx.saved_tensors
         x_dtype, v_dtype = ctx.dtypes
-        dyb = dy.to(torch.bfloat16).contiguous()
+        dyb = _grad_rows(dy)
         T, dev = dyb.shape[0], dyb.device
         need = ctx.needs_input_grad
         dx = dx_at = cols_t = index_t = None
@@ -470,7 +477,7 @@ class MXSwiGLUFn(torch.autograd.Function):
     def backward(ctx, grad_out):
         q_x, q_h, ci_gate, ci_up, ci_down = ctx.saved_tensors
         gate, up, down = ctx.weights
-        dy = grad_out.to(torch.bfloat16).contiguous()
+        dy = _grad_rows(grad_out)
         T, dev = dy.shape[0], dy.device
         need = ctx.needs_input_grad
         # transposed topologies: of down for d_gate and d_up, of gate and up for dx (the address, the address, slots)

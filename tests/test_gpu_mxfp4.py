@@ -1224,3 +1224,35 @@ def test_a_captured_call_gives_the_same_bits(T):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_gradients_that_start_anywhere():
+    """The output's gradient as a slice of a larger one, at any element, and as an expanded scalar."""
+    K = _K()
+    rng = np.random.default_rng(41)
+    mats, _ = _ffn(rng)
+    x, dy = rows(rng, 9, 256).requires_grad_(True), rows(rng, 9, 256)
+    vs = [m[0].requires_grad_(True) for m in mats]
+
+    def ffn():
+        return K.mxfp4_swiglu(x, vs[0], mats[0][1], vs[1], mats[1][1], vs[2], mats[2][1], add_residual=True)
+
+    def linear():
+        return K.mxfp4_linear_ad(x, vs[0], mats[0][1])[:, :256].contiguous()
+
+    for call, leaves in ((ffn, [x] + vs), (linear, [x, vs[0]])):
+        want = torch.autograd.grad(call(), leaves, dy)
+        for start in (1, 3, 4, 8):
+            y = torch.cat([torch.zeros(start, dtype=BF16, device="cuda"), call().reshape(-1)])
+            weights = torch.cat([torch.zeros(start, dtype=BF16, device="cuda"), dy.reshape(-1)])
+            got = torch.autograd.grad(y, leaves, weights)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        ones = torch.autograd.grad(call(), leaves, torch.ones_like(dy))
+        got = torch.autograd.grad(call().sum(), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, ones))
+    flat = torch.zeros(9 * 512 + 8, dtype=BF16, device="cuda")
+    for start in (0, 1, 4, 8):
+        g = flat[start:start + 9 * 512].view(9, 512).copy_(rows(np.random.default_rng(1), 9, 512))
+        got = torch.autograd.grad(K.mxfp4_linear_ad(x, vs[0], mats[0][1]), [x, vs[0]], g)
+        want = torch.autograd.grad(K.mxfp4_linear_ad(x, vs[0], mats[0][1]), [x, vs[0]], g.clone())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

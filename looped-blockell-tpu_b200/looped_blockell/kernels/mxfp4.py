@@ -91,7 +91,9 @@ class MXRows:
 
 @dataclass(frozen=True)
 class MXBlockELL:
-    """A quantised Block-ELL weight (``make_mxfp4``)."""
+    """A quantised Block-ELL weight (``make_mxfp4``).  One put together from
+    fields (``dataclasses.replace``) is checked on its first use, which waits
+    for the device: the kernels follow its plan into the rows and the tiles."""
     data: torch.Tensor         # uint8: the quantised tiles, operand layout, then the plan of the live slots
     col_indices: torch.Tensor  # int32 [R, K]
     R: int
@@ -107,7 +109,22 @@ class MXBlockELL:
         if self.R < 1 or self.K < 1 or data.dtype != torch.uint8 or not data.is_contiguous() or \
                 data.numel() < _tiles_bytes(self.R, self.K, self.B) + _plan_bytes(self.R, self.K):
             raise RuntimeError("MXBlockELL.data does not hold R x K quantised tiles and their plan")
+        if "_made" not in self.__dict__:
+            self._check_plan()
         return self._view(data.data_ptr())
+
+    def _check_plan(self):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("use an MXBlockELL made from fields once before a capture")
+        R, K = self.R, self.K
+        plan = self.data[_tiles_bytes(R, K, self.B):_tiles_bytes(R, K, self.B) + _plan_bytes(R, K)].clone().view(torch.int32)
+        e, counts = plan[:R * K].view(R, K), plan[-(-R * K // 4) * 4:][:R]
+        slots = torch.arange(K, device=e.device)
+        dead = e == -1
+        ok = ((e & 0xFFFF) < self.C) & ((e >> 16) & 0xFFFF < K)
+        ok = torch.where(dead, slots >= counts[:, None], ok & (slots < counts[:, None])).all() & (counts >= 0).all()
+        if not (0 < self.C <= 65535 and bool(ok)):
+            raise RuntimeError("MXBlockELL.data's plan does not fit R, K and C")
 
     def _view(self, at: int):
         return _lib.BellMxEll(at, at + _tiles_bytes(self.R, self.K, self.B), self.R, self.C, self.K, self.B)
@@ -242,6 +259,7 @@ def _pack(weights, layout: int):
             v = v.clone()
         data = _bytes(_tiles_bytes(R, K, B) + _plan_bytes(R, K), dev)
         w = MXBlockELL(data, cols, R, K, int(C_blocks), B)
+        w.__dict__["_made"] = True
         view = w.__dict__["_abi"] = w._view(data.data_ptr())
         abi[i] = _lib.BellEll(v.data_ptr(), cols.data_ptr(), R, w.C, K, B, layout, 0)
         chunks[i], plans[i] = view.chunks, view.plan

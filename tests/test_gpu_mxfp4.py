@@ -1256,3 +1256,38 @@ def test_gradients_that_start_anywhere():
         got = torch.autograd.grad(K.mxfp4_linear_ad(x, vs[0], mats[0][1]), [x, vs[0]], g)
         want = torch.autograd.grad(K.mxfp4_linear_ad(x, vs[0], mats[0][1]), [x, vs[0]], g.clone())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_weight_put_together_from_fields_is_checked():
+    """Fields that do not fit the plan are refused before a kernel follows it; those that do are used."""
+    import copy
+    import pickle
+    from dataclasses import replace
+    K = _K()
+    rng = np.random.default_rng(42)
+    v, cols, _ = weight(rng, 6, 5, 3, 64, 2)
+    cols[0, 0] = 4
+    w = K.make_mxfp4(v, cols, 5)
+    x = rows(rng, 9, 320)
+    want = K.mxfp4_linear(x, w)
+    for bad in (dict(C=4), dict(C=0), dict(C=1 << 16), dict(R=3, K=6), dict(R=9, K=2), dict(R=2, K=9), dict(R=1, K=18),
+                dict(data=torch.zeros_like(w.data)), dict(data=torch.full_like(w.data, 255))):
+        broken = replace(w, **bad)
+        with pytest.raises(RuntimeError):
+            K.mxfp4_linear(rows(rng, 9, 64 * max(1, min(broken.C, 16))), broken)
+        with pytest.raises(RuntimeError, match="plan"):
+            broken.dequantize()
+    fits = replace(w, C=7)  # columns 5 and 6 are not used
+    assert torch.equal(K.mxfp4_linear(torch.cat([x, x[:, :128]], 1), fits), want)
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w)), replace(w, data=w.data.clone())):
+        assert torch.equal(K.mxfp4_linear(x, other), want)
+    fresh, unused = copy.deepcopy(w), replace(w, data=w.data.clone())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = K.mxfp4_linear(x, fresh)  # a copy of a made weight needs no check
+        with pytest.raises(RuntimeError, match="capture"):
+            K.mxfp4_linear(x, unused)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and K.read_status() == 0

@@ -401,7 +401,7 @@ typedef struct BellMxLinearBwdDesc {
   void* dx;                    /* optional [T, C*B]                          */
   void* dw;                    /* optional [R, K, B, B]                      */
   int32_t grad_dtype;          /* of dw: BELL_DTYPE_BF16 / BELL_DTYPE_F32    */
-  int32_t dx_dtype;
+  int32_t dx_dtype;            /* of dx                                      */
   void* workspace;
   int32_t* status;
 } BellMxLinearBwdDesc;
@@ -443,7 +443,7 @@ typedef struct BellMxFFNBwdDesc {
   void* d_up;
   void* d_down;
   int32_t gate_dtype, up_dtype, down_dtype;
-  int16_t dx_dtype;
+  int16_t dx_dtype;            /* of dx: BELL_DTYPE_BF16 / BELL_DTYPE_F32    */
   int16_t gate_up_passes;      /* 0: one                                     */
   void* workspace;
   int32_t* status;

@@ -486,6 +486,7 @@ int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sm
                            kTok, Swz::B128))
     return rc;
   const SddmmCuts cuts = sddmm_cuts(d->T, d->R, d->C, d->K, B, own ? std::min(sms, kMaxParts) : sms, own);
+  if (own && cuts.chunks > 1 && !parts) return fail(BELL_ERR_ARG, "bell_sddmm_bf16: cut units need parts");
   SddmmParams p{};
   p.T = d->T;
   p.R = d->R;

@@ -102,8 +102,7 @@ struct SddmmParams {
   int64_t split_chunks;      // 64-token chunks per token range
   const int32_t* cols;       // [R, K]
   float* grad;               // [R, K, B, B] fp32, accumulated
-  int32_t own;               // one CTA to a sum (see seg_next): grad is written, not added to
-  float* parts;              // with it: [gridDim.x, SLOTS, B, B]
+  float* parts;              // own sums: [gridDim.x, SLOTS, B, B]
   int32_t out_in;            // tile layout of grad: 0 [B_in, B_out], 1 [B_out, B_in]
   int32_t* status;
   uint64_t timeout_ns;
@@ -167,7 +166,7 @@ __device__ __forceinline__ Unit unit_of(int u, const SddmmParams& p) {
 // per CTA, so every CTA streams the same tokens at the same time (the
 // activation tiles are shared through L2) and no CTA waits on a longer share.
 // A share may start or end inside a unit: each piece (segment) adds its
-// partial tiles into the gradient like a whole unit.  With p.own only the
+// partial tiles into the gradient like a whole unit.  With OWN only the
 // piece with the unit's first chunk does; a share that starts inside a unit
 // (its first segment, the same one in every range) sums that segment's tiles in
 // the CTA's own part instead.  Every sum then has one CTA, whose threads write
@@ -214,7 +213,8 @@ __device__ __forceinline__ bool seg_next(const SddmmParams& p, SegIt& it, Unit& 
   return true;
 }
 
-template <int B>
+// OWN: one CTA to a sum, the gradient is written and not added to (see seg_next).
+template <int B, bool OWN>
 __global__ void __launch_bounds__(kThr, 1)
     bell_sddmm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                       const SddmmParams p) {
@@ -401,8 +401,8 @@ __global__ void __launch_bounds__(kThr, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], use & 1u, ctl))) break;
       tc_fence_after();
       const uint32_t tb = tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * C::NACC * C::N);
-      const bool part = p.own && cut, put = p.own && it.s == 0;
-      float* own = p.parts + size_t(blockIdx.x) * SLOTS * B * B;
+      const bool part = OWN && cut, put = OWN && it.s == 0;
+      float* own = OWN ? p.parts + size_t(blockIdx.x) * SLOTS * B * B : nullptr;
       if constexpr (!C::TR) {
         // B = 64: accumulator ac, row = a feature; rows 0-63 slot 2ac, 64-127
         // slot 2ac+1; columns = the row's 64 b (output) features
@@ -497,13 +497,12 @@ int launch_sddmm(const BellSddmmDesc* d, int32_t* status, cudaStream_t s, int sm
   p.n_split = int32_t(((d->T + kTok - 1) / kTok + cuts.chunks - 1) / cuts.chunks);
   p.cols = d->col_indices;
   p.grad = d->grad;
-  p.own = own;
   p.parts = parts;
   p.out_in = d->layout == BELL_TILE_OUT_IN;
   p.status = status;
   p.timeout_ns = wait_budget_ns();
   if (int64_t(p.R) * p.KP * p.n_split > INT32_MAX) return fail(BELL_ERR_SHAPE, "bell_sddmm_bf16: too many work units");
-  auto kern = bell_sddmm_kernel<B>;
+  auto kern = own ? bell_sddmm_kernel<B, true> : bell_sddmm_kernel<B, false>;
   if (int rc = set_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
   kern<<<cuts.grid, kThr, C::SMEM, s>>>(ma, mb, p);
   return check_launch("bell_sddmm_kernel");

@@ -4,6 +4,9 @@ from __future__ import annotations
 
 import torch
 
+_capturing = torch.cuda.is_current_stream_capturing
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 
 def capturing(t: torch.Tensor) -> bool:
     """Whether work on ``t`` is being captured: what is made then holds nothing until a replay."""
@@ -19,25 +22,25 @@ class Made:
     synchronises first).  Its replays read the memory again: what a graph has
     ``captured`` must outlive the entry."""
 
-    __slots__ = ("tensors", "stream", "event", "captured")
+    __slots__ = ("tensors", "index", "stream", "event", "captured")
 
     def __init__(self, *tensors: torch.Tensor):
         self.tensors = tensors if tensors[0].is_cuda else ()
         self.captured = False
         if self.tensors:
             s = torch.cuda.current_stream(tensors[0].device)
-            self.stream, self.event = s.cuda_stream, s.record_event()
+            self.index, self.stream, self.event = s.device_index, s.cuda_stream, s.record_event()
 
     def use(self) -> None:
         if not self.tensors:
             return
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             self.captured = True
-            return
-        dev = self.tensors[0].device
-        if torch._C._cuda_getCurrentRawStream(dev.index) == self.stream:
-            return
-        s = torch.cuda.current_stream(dev)
+        elif _raw_stream(self.index) != self.stream:
+            self._order()
+
+    def _order(self) -> None:
+        s = torch.cuda.current_stream(self.index)
         s.wait_event(self.event)
         for t in self.tensors:
             t.record_stream(s)

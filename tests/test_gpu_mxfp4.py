@@ -1291,3 +1291,25 @@ def test_a_weight_put_together_from_fields_is_checked():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want) and K.read_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,F", [(64, 512), (128, 1024), (64, 8192)])
+def test_gradients_of_no_tokens(B, F, dtype):
+    """Empty dx, tile gradients that are zero whatever lay in their memory; 8192 features take dx in two passes."""
+    K = _K()
+    rng = np.random.default_rng(43)
+    mats, _ = _ffn(rng, 2 * B, F, B, 2, 3, 1)
+    x = torch.zeros(0, 2 * B, dtype=dtype, device="cuda", requires_grad=True)
+    vs = [m[0].to(dtype).requires_grad_(True) for m in mats]
+    for _ in range(2):
+        junk = [torch.full_like(v, 7.0) for v in vs]
+        del junk
+        y = K.mxfp4_swiglu(x, vs[0], mats[0][1], vs[1], mats[1][1], vs[2], mats[2][1], add_residual=True)
+        dx, *dws = torch.autograd.grad(y, [x] + vs, torch.zeros_like(y))
+        assert dx.shape == x.shape and dx.dtype == dtype
+        assert all(g.dtype == dtype and (g == 0).all() for g in dws)
+        y = K.mxfp4_linear_ad(x, vs[0], mats[0][1])
+        dx, dw = torch.autograd.grad(y, [x, vs[0]], torch.zeros_like(y))
+        assert dx.shape == x.shape and (dw == 0).all()
+    assert K.read_status() == 0
